@@ -74,6 +74,16 @@ SIGNATURES = {
     "ppo_linear_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, I, I, I]),
     "ppo_ssm_scan_fwd": (I, [P, I, P, P, P, P, P, P, I, I, I]),
     "ppo_ssm_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, I, I, I]),
+    "ppo_linear_attention_max_width": (I, []),
+    "ppo_linear_attention_workspace": (SZ, [I, I, I, I, I, I]),
+    "ppo_linear_attention_fwd": (I, [P, I, P, P, P, P, P, P, P, P, F, P, P, P, SZ, I, I, I, I, I, I]),
+    "ppo_linear_attention_bwd_workspace": (SZ, [I, I, I, I, I, I, I]),
+    "ppo_linear_attention_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, F, P, P, P, P, P, P, P, SZ, I, I, I, I, I, I]),
+    "ppo_linear_attention_step": (I, [P, I, P, P, P, P, P, P, P, P, P, F, I, I, I, I, I]),
+    "ppo_qk_norm_rotary_max_width": (I, []),
+    "ppo_qk_norm_rotary_fwd": (I, [P, I, P, P, P, P, P, P, P, F, I, P, P, I, I, I, I, I, I]),
+    "ppo_qk_norm_rotary_bwd_workspace": (SZ, [I]),
+    "ppo_qk_norm_rotary_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, F, I, P, P, P, P, P, SZ, I, I, I, I, I, I]),
     "ppo_gemm_f32": (I, [P, I, I, P, I64, P, P, I64, P, I64, I, I, I, I, I64, I, P, I, P, P, I64, P, I]),
     "ppo_gemm_f32_towers": (I, [P, I, I, I, P, I64, P, P, I64, P, I64, I, I, I, I, I64, I, P, I, P, P, I64, P, I,
                                 I64, I64, I64, I64, I64, I64, I64]),

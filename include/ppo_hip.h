@@ -362,6 +362,76 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
                      const void* carry, const void* cot, void* da, void* db, void* dcarry, int batch, int steps,
                      int features);
 
+/* ------------------------------------------------------ linear attention
+ * The scan's recurrence with a matrix for a state (no counterpart in the
+ * reference): per sequence b and head h, lam = exp(log_decay[h]),
+ *   S_t = lam (done_t ? 0 : S_{t-1}) + k_t v_t^T,  S_{-1} = carry
+ *   o_t = scale q_t S_t
+ * for t < lengths[b]; later rows of q, k, v are not read and those of the
+ * outputs and gradients are zeros.  dtype 0 = float32, 1 = bf16 storage of q,
+ * k, v, out and their gradients; the states are float32.
+ *   q [batch, steps, heads, key_width], k [batch, steps, kv_heads, key_width],
+ *   v [batch, steps, kv_heads, value_width]: columns side by side, element
+ *   strides of (batch, step, head) in the host array `strides`, 3 for each of
+ *   q, k, v (and dout in the backward); a step's stride is at most 2^23
+ *   and none is negative.
+ *   heads / kv_heads query heads in a row share a key head.  Widths are at most
+ *   ppo_linear_attention_max_width().
+ *   log_decay float [heads] (<= 0; -inf: no memory), carry / final float
+ *   [batch, heads, key_width, value_width] (carry may be NULL: zeros), done
+ *   uint8 [batch, steps] (NULL: none), lengths int32 [batch] (NULL: steps),
+ *   out [batch, steps, heads, value_width] contiguous.
+ * The workspace (4-byte aligned) holds the states between pieces of long
+ * sequences; the backward pass reads the forward's as fwd_workspace. */
+int ppo_linear_attention_max_width(void);
+size_t ppo_linear_attention_workspace(int dtype, int batch, int steps, int heads, int key_width, int value_width);
+int ppo_linear_attention_fwd(void* stream, int dtype, const void* q, const void* k, const void* v,
+                             const int64_t* strides, const float* log_decay, const float* carry, const uint8_t* done,
+                             const int32_t* lengths, float scale, void* out, float* final, void* workspace,
+                             size_t workspace_bytes, int batch, int steps, int heads, int kv_heads, int key_width,
+                             int value_width);
+/* From the cotangents of out (dout, strided as q) and final (dfinal, NULL:
+ * zeros): dq, dk, dv contiguous, shaped as q, k, v; dcarry (may be NULL). */
+size_t ppo_linear_attention_bwd_workspace(int dtype, int batch, int steps, int heads, int kv_heads, int key_width,
+                                          int value_width);
+int ppo_linear_attention_bwd(void* stream, int dtype, const void* q, const void* k, const void* v, const void* dout,
+                             const int64_t* strides, const float* log_decay, const float* carry, const uint8_t* done,
+                             const int32_t* lengths, float scale, const float* dfinal, const void* fwd_workspace,
+                             void* dq, void* dk, void* dv, float* dcarry, void* workspace, size_t workspace_bytes,
+                             int batch, int steps, int heads, int kv_heads, int key_width, int value_width);
+/* One step: q [batch, heads, key_width], k, v [batch, kv_heads, width] with
+ * element strides of (batch, head), 2 for each; done uint8 [batch] or NULL;
+ * final may be carry. */
+int ppo_linear_attention_step(void* stream, int dtype, const void* q, const void* k, const void* v,
+                              const int64_t* strides, const float* log_decay, const uint8_t* done, const float* carry,
+                              float* final, void* out, float scale, int batch, int heads, int kv_heads, int key_width,
+                              int value_width);
+
+/* Norms of queries and keys for each head with the position rotation (no
+ * counterpart in the reference).  Per row x of `width` columns at position p:
+ * y = x / sqrt(mean(x^2) + epsilon) * scale, then each of the `pairs` first
+ * pairs of columns (i, i + pairs) -- interleaved: (2 i, 2 i + 1) -- turned by
+ * the angle p * frequencies[i].  q [batch, steps, heads, width], k [batch,
+ * steps, kv_heads, width]: element strides of (batch, step, head) in the host
+ * array `strides`, 3 for each (the backward: for q, k, dq_out, dk_out);
+ * outputs and gradients contiguous.  scales float [width] (NULL: ones),
+ * frequencies double [pairs] in radians, positions int32 [batch, steps] (NULL:
+ * the step).  dtype 0 = float32, 1 = bf16 storage.  width at most
+ * ppo_qk_norm_rotary_max_width(). */
+int ppo_qk_norm_rotary_max_width(void);
+int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, const void* k, const int64_t* strides,
+                           const float* q_scale, const float* k_scale, const double* frequencies,
+                           const int32_t* positions, float epsilon, int interleaved, void* q_out, void* k_out,
+                           int batch, int steps, int heads, int kv_heads, int width, int pairs);
+/* dq_scale, dk_scale float [width] (may be NULL). */
+size_t ppo_qk_norm_rotary_bwd_workspace(int width);
+int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, const void* k, const void* dq_out,
+                           const void* dk_out, const int64_t* strides, const float* q_scale, const float* k_scale,
+                           const double* frequencies, const int32_t* positions, float epsilon, int interleaved,
+                           void* dq, void* dk, float* dq_scale, float* dk_scale, void* workspace,
+                           size_t workspace_bytes, int batch, int steps, int heads, int kv_heads, int width,
+                           int pairs);
+
 /* ------------------------------------------------------------------ GEMM
  * Dense layers of the torso and heads (flax.linen.Dense as composed in
  * hangar/recipes/*.py; forward at boonta/networks/network.py:38-49, backward

@@ -1,0 +1,112 @@
+"""What linear attention and the query / key norms refuse, on the host."""
+import ctypes
+
+import pytest
+import torch
+
+from boonta_amd import _lib
+from boonta_amd.kernels import linear_attention, linear_attention_step, qk_norm_rotary, rotary_frequencies
+
+
+def operands(B=2, T=3, H=4, G=2, K=8, V=6, dtype=torch.float32):
+    return [torch.zeros(B, T, H, K, dtype=dtype), torch.zeros(B, T, G, K, dtype=dtype),
+            torch.zeros(B, T, G, V, dtype=dtype), torch.zeros(H)]
+
+
+def refused(error, match, f, *args, **kw):
+    with pytest.raises(error, match=match):
+        f(*args, **kw)
+
+
+def test_linear_attention_refuses_what_it_does_not_take():
+    q, k, v, g = operands()
+    refused(TypeError, "device", linear_attention, q, k, v, g)
+    refused(TypeError, "float32 or bfloat16", linear_attention, q.half(), k.half(), v.half(), g)
+    refused(TypeError, "one dtype", linear_attention, q, k.bfloat16(), v, g)
+    refused(ValueError, "need q", linear_attention, q[0], k, v, g)
+    refused(ValueError, "need q", linear_attention, q, k[:, :2], v, g)
+    refused(ValueError, "need q", linear_attention, q, k, v[:, :, :1], g)
+    refused(ValueError, "evenly", linear_attention, q[:, :, :3], k, v, g[:3])
+    refused(ValueError, "up to 128", linear_attention, *operands(K=129))
+    refused(ValueError, "up to 128", linear_attention, *operands(V=129))
+    refused(ValueError, "log_decay", linear_attention, q, k, v, g[:2])
+    refused(ValueError, "log_decay", linear_attention, q, k, v, g.double())
+    refused(ValueError, "fixed schedule", linear_attention, q, k, v, g.clone().requires_grad_())
+    refused(ValueError, "carry", linear_attention, q, k, v, g, torch.zeros(2, 2, 8, 6))
+    refused(ValueError, "carry", linear_attention, q, k, v, g, torch.zeros(2, 4, 8, 6).bfloat16())
+    refused(ValueError, "done", linear_attention, q, k, v, g, done=torch.zeros(2, 4).bool())
+    refused(ValueError, "done", linear_attention, q, k, v, g, done=torch.zeros(2, 3))
+    refused(ValueError, "lengths", linear_attention, q, k, v, g, lengths=torch.zeros(2, dtype=torch.int64))
+    refused(ValueError, "lengths", linear_attention, q, k, v, g, lengths=torch.zeros(3, dtype=torch.int32))
+
+
+def test_linear_attention_step_refuses_what_it_does_not_take():
+    q, k, v, g = operands()
+    q, k, v, carry = q[:, 0], k[:, 0], v[:, 0], torch.zeros(2, 4, 8, 6)
+    refused(TypeError, "device", linear_attention_step, q, k, v, g, carry)
+    refused(ValueError, "need q", linear_attention_step, q[:, None], k, v, g, carry)
+    refused(ValueError, "carry", linear_attention_step, q, k, v, g, carry[:1])
+    refused(ValueError, "done", linear_attention_step, q, k, v, g, carry, torch.zeros(2, 1).bool())
+    refused(ValueError, "no gradients", linear_attention_step, q, k, v, g, carry.clone().requires_grad_())
+    refused(ValueError, "out_carry", linear_attention_step, q, k, v, g, carry, out_carry=carry.transpose(2, 3))
+
+
+def test_qk_norm_rotary_refuses_what_it_does_not_take():
+    q, k, _, _ = operands()
+    f = rotary_frequencies(8, device="cpu")
+    assert f.dtype == torch.float64 and f.shape == (4,) and f[0] == 1
+    refused(ValueError, "pairs", rotary_frequencies, 7, device="cpu")
+    refused(TypeError, "device", qk_norm_rotary, q, k)
+    refused(TypeError, "one dtype", qk_norm_rotary, q, k.bfloat16())
+    refused(ValueError, "need q", qk_norm_rotary, q, k[..., :4])
+    refused(ValueError, "up to 256", qk_norm_rotary, *operands(K=257)[:2])
+    refused(ValueError, "q_scale", qk_norm_rotary, q, k, torch.ones(7))
+    refused(ValueError, "k_scale", qk_norm_rotary, q, k, None, torch.ones(8).bfloat16())
+    refused(ValueError, "frequencies", qk_norm_rotary, q, k, frequencies=f.float())
+    refused(ValueError, "frequencies", qk_norm_rotary, q, k, frequencies=rotary_frequencies(10, device="cpu"))
+    refused(ValueError, "no gradient", qk_norm_rotary, q, k, frequencies=f.clone().requires_grad_())
+    refused(ValueError, "positions", qk_norm_rotary, q, k, positions=torch.zeros(2, 3, dtype=torch.int64))
+    refused(ValueError, "positions", qk_norm_rotary, q, k, positions=torch.zeros(3, dtype=torch.int32))
+
+
+def test_the_entry_points_refuse_without_launching():
+    lib = _lib.load()
+    st = (ctypes.c_int64 * 12)(*[0] * 12)
+    fwd = lib.ppo_linear_attention_fwd
+    sizes = (2, 4, 2, 2, 8, 8)   # batch, steps, heads, key heads, widths
+
+    def forward(dtype=0, q=1, strides=st, decay=1, final=1, work=None, nbytes=0, sizes=sizes):
+        return fwd(None, dtype, q, 1, 1, strides, decay, None, None, None, 1.0, 1, final, work, nbytes, *sizes)
+
+    assert forward(dtype=2) == -1
+    assert forward(q=None) == -1 and b"null buffer" in lib.ppo_last_error()
+    assert forward(strides=None) == -1 and forward(decay=None) == -1 and forward(final=None) == -1
+    assert forward(sizes=(2, 4, 3, 2, 8, 8)) == -1 and b"evenly" in lib.ppo_last_error()
+    assert forward(sizes=(2, 4, 3, 0, 8, 8)) == -1
+    assert forward(sizes=(2, 4, 2, 2, 129, 8)) == -1 and b"above 128" in lib.ppo_last_error()
+    assert forward(sizes=(-1, 4, 2, 2, 8, 8)) == -1
+    assert forward(sizes=(1 << 30, 4, 2, 2, 8, 8)) == -1
+    assert forward(sizes=(0, 4, 2, 2, 8, 8)) == 0
+    far = (ctypes.c_int64 * 12)(0, 1 << 24, 0, *[0] * 9)
+    assert forward(strides=far) == -1 and b"step stride" in lib.ppo_last_error()
+    long = (1, 1 << 16, 2, 2, 8, 8)
+    need = lib.ppo_linear_attention_workspace(0, *long[:3], 8, 8)
+    assert need > 0 and forward(sizes=long) == -3 and forward(sizes=long, work=1, nbytes=need - 1) == -3
+    assert lib.ppo_linear_attention_bwd_workspace(0, 2, 4, 4, 2, 8, 8) == 4 * 2 * 4 * 4 * 16
+    assert lib.ppo_linear_attention_bwd_workspace(0, 2, 4, 4, 4, 8, 8) == 0
+    bwd = lib.ppo_linear_attention_bwd
+    assert bwd(None, 0, 1, 1, 1, None, st, 1, None, None, None, 1.0, None, None, 1, 1, 1, None, None, 0, *sizes) == -1
+    assert bwd(None, 0, 1, 1, 1, 1, st, 1, None, None, None, 1.0, None, None, 1, 1, 1, None, None, 0, 2, 4, 4, 2, 8,
+               8) == -3
+    step = lib.ppo_linear_attention_step
+    assert step(None, 0, 1, 1, 1, st, 1, None, None, 1, 1, 1.0, 2, 2, 2, 8, 8) == -1
+    assert step(None, 0, 1, 1, 1, st, 1, None, 1, 1, 1, 1.0, 2, 3, 2, 8, 8) == -1
+    norm = lib.ppo_qk_norm_rotary_fwd
+    assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 2, 3, 4, 4, 8, 5) == -1   # 5 pairs of 8
+    assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 2, 3, 4, 4, 8, 4) == -1   # no frequencies
+    assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 2, 3, 4, 4, 257, 0) == -1
+    assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 1 << 16, 1 << 15, 4, 4, 8, 0) == -1
+    assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 0, 3, 4, 4, 8, 0) == 0
+    assert lib.ppo_qk_norm_rotary_bwd(None, 0, 1, 1, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 1, 1, None, 0, 2,
+                                      3, 4, 4, 8, 0) == -3
+    lib.ppo_clear_error()
