@@ -75,6 +75,7 @@ SIGNATURES = {
     "ppo_ssm_scan_fwd": (I, [P, I, P, P, P, P, P, P, I, I, I]),
     "ppo_ssm_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, I, I, I]),
     "ppo_linear_attention_max_width": (I, []),
+    "ppo_linear_attention_min_width": (I, [I]),
     "ppo_linear_attention_workspace": (SZ, [I, I, I, I, I, I]),
     "ppo_linear_attention_fwd": (I, [P, I, P, P, P, P, P, P, P, P, F, P, P, P, SZ, I, I, I, I, I, I]),
     "ppo_linear_attention_bwd_workspace": (SZ, [I, I, I, I, I, I, I]),

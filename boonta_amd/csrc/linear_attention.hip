@@ -61,15 +61,19 @@ struct AttnArgs {
 };
 
 // ---- per type: chunks of 128 bytes of steps; a lane's MFMA operand of 16
-// bytes (FR values).  One contraction block is 4 FR deep: a 16x16x32 bf16
-// MFMA, or four 16x16x4 fp32 MFMAs, whose lane group g supplies values
-// 4g .. 4g+3 of each 16 rows, which is how the accumulators hold them: a
-// state tile is an operand without a move.
+// bytes (FR values).  One contraction block is 4 FR deep, a 16x16x32 bf16 MFMA
+// or four 16x16x4 fp32 MFMAs: lane group g holds FR neighbouring values of it.
+// An accumulator tile holds rows 4 g .. 4 g + 3 in group g, so a state tile is
+// an operand over its rows without a move if slot 4 g + e of tile rt is row
+//   bf16: 32 (rt / 2) + 8 g + 4 (rt % 2) + e    fp32: 16 rt + 4 g + e.
 template <typename T> struct Type;
 
 template <> struct Type<uint16_t> {
   typedef bf16x8 Frag;
   static constexpr int FR = 8, C = 64, PIECES = 3;
+  static __device__ __forceinline__ constexpr int row(int rt, int slot) {
+    return 32 * (rt >> 1) + 4 * (rt & 1) + 8 * (slot >> 2) + (slot & 3);
+  }
   static __device__ __forceinline__ floatx4 mma(Frag a, Frag b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -77,6 +81,7 @@ template <> struct Type<uint16_t> {
 template <> struct Type<float> {
   typedef floatx4 Frag;
   static constexpr int FR = 4, C = 32, PIECES = 1;
+  static __device__ __forceinline__ constexpr int row(int rt, int slot) { return 16 * rt + slot; }
   static __device__ __forceinline__ floatx4 mma(Frag a, Frag b, floatx4 c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -93,15 +98,13 @@ __device__ __forceinline__ bf16x8 join(floatx4 lo, floatx4 hi) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// The state as an operand over its rows: contraction block kb of n-tile nt.
+// The state as an operand over its rows: contraction block kb.
 // bf16: the state itself stays float32; what enters the product is rounded
 // once, an error of the size of the output's own rounding.
-template <int RT> __device__ __forceinline__ bf16x8 state_frag(const floatx4 (&s)[RT][2], int kb, int nt, uint16_t) {
-  return join(s[2 * kb][nt], s[2 * kb + 1][nt]);
+template <int RT> __device__ __forceinline__ bf16x8 state_frag(const floatx4 (&s)[RT], int kb, uint16_t) {
+  return join(s[2 * kb], s[2 * kb + 1]);
 }
-template <int RT> __device__ __forceinline__ floatx4 state_frag(const floatx4 (&s)[RT][2], int kb, int nt, float) {
-  return s[kb][nt];
-}
+template <int RT> __device__ __forceinline__ floatx4 state_frag(const floatx4 (&s)[RT], int kb, float) { return s[kb]; }
 
 // z times its steps' weights, as operands whose sum is the product to float32:
 // one float32, or three bf16 pieces, each what the ones before leave (the
@@ -136,42 +139,35 @@ __device__ __forceinline__ int swizzle(int r) { return ((r >> 1) ^ (r >> 3)) & 7
 __device__ __forceinline__ int tile_byte(int lane_byte, int tile, int tb) {
   return (lane_byte ^ (((4 * tb) ^ (2 * (tile & 3))) << 4)) + tile * 2048;
 }
-
-struct Regs {
-  uint4 v[4];
-};
-
-// 16 bytes of a row, elements c0 .. c0 + FR - 1, as loaded and then (once they
-// are there: a use would wait for them) with what is past the row's `width`
-// zeros.  No branch on the lane: the last chunk of a width that FR does not
-// divide is read from its end and shifted.  Rows need no alignment beyond
-// their elements'.
-template <typename T>
-__device__ __forceinline__ uint4 load_chunk(const char* row, uint32_t byte, int c0, int width) {
-  constexpr int FR = Type<T>::FR;
-  uint4 v;
-  if (width >= FR) {
-    __builtin_memcpy(&v, row + byte, 16);
-  } else {
-    T e[FR];
-#pragma unroll
-    for (int j = 0; j < FR; ++j) {
-      T x;
-      __builtin_memcpy(&x, row + byte + min(j, width - 1) * sizeof(T), sizeof(T));
-      e[j] = c0 + j < width ? x : T(0);
-    }
-    __builtin_memcpy(&v, e, 16);
-  }
-  return v;
+// The same of the rows in slots l16 of state tile rt.
+__device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, uint16_t) {
+  return (lane_byte ^ (((4 * tb) ^ (2 * (rt & 1)) ^ (2 * (rt & 2))) << 4)) + (32 * (rt >> 1) + 4 * (rt & 1)) * 128;
 }
-// The column a chunk's load starts at.
-template <typename T> __device__ __forceinline__ int load_column(int c0, int width) {
-  return width >= Type<T>::FR ? min(c0, width - Type<T>::FR) : 0;
+__device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, float) { return tile_byte(lane_byte, rt, tb); }
+
+// 16 bytes at a lane's 32-bit offset from an address that is uniform in the
+// wave.  (Opaque, so that the sum stays in the load and each row of a lane
+// costs one register, not an address.)
+typedef __attribute__((address_space(1))) const char* GlobalBytes;
+
+__device__ __forceinline__ GlobalBytes uniform(const void* p) {
+  uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p);
+  uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)p >> 32));
+  asm("" : "+s"(lo), "+s"(hi));
+  return (GlobalBytes)((uintptr_t)hi << 32 | lo);
 }
+__device__ __forceinline__ uint4 load_chunk(GlobalBytes base, uint32_t byte) {
+  typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(2)));
+  const word4 v = *(__attribute__((address_space(1))) const word4*)(base + byte);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// A chunk of 16 bytes (elements c0 ..) with what is past the row's `width`
+// zeros: the last chunk of a width that FR does not divide was read from its
+// end, so that no load leaves the row, and is shifted.
 template <typename T>
 __device__ __forceinline__ uint4 trim_chunk(uint4 v, int c0, int width) {
   constexpr int FR = Type<T>::FR;
-  if (width < FR) return v;
   const int over = c0 + FR - width;   // elements past the row
   if (over <= 0) return v;
   const int s = min(over, FR) * (int)sizeof(T) * 8;
@@ -190,88 +186,63 @@ __device__ __forceinline__ bool odd_exponent(uint4 v, float) {
   return ((f(v.x) | f(v.y) | f(v.z) | f(v.w)) & 0x80000000u) != 0;
 }
 
-// Four rows' chunks of one step each as columns: element j of the chunk, over
-// the four steps.
-__device__ __forceinline__ void write_transposed(char* t, int dim0, int tg, const Regs& r, uint16_t) {
-  const uint32_t* a = reinterpret_cast<const uint32_t*>(&r.v[0]);
-  const uint32_t* b = reinterpret_cast<const uint32_t*>(&r.v[1]);
-  const uint32_t* c = reinterpret_cast<const uint32_t*>(&r.v[2]);
-  const uint32_t* d = reinterpret_cast<const uint32_t*>(&r.v[3]);
+// Four steps' chunks (columns FR dc .. of steps 4 tg ..) as columns: element j
+// of the chunk over the four steps, at a byte of the lane's with j's row and
+// what j adds to the swizzle.
+__device__ __forceinline__ int transposed_byte(int dc, int tg, uint16_t) {
+  return dc * 1024 + ((((tg >> 1) ^ (4 * (dc & 1)) ^ dc) & 7) << 4) + ((tg & 1) << 3);
+}
+__device__ __forceinline__ int transposed_byte(int dc, int tg, float) {
+  return dc * 512 + (((tg ^ (2 * dc) ^ (dc >> 1)) & 7) << 4);
+}
+__device__ __forceinline__ void write_transposed(char* t, int byte, const uint4 (&v)[4], uint16_t) {
+  const uint32_t q[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w},
+                            {v[1].x, v[1].y, v[1].z, v[1].w},
+                            {v[2].x, v[2].y, v[2].z, v[2].w},
+                            {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int row = dim0 + j, w = j >> 1;
-    uint2 x;
-    // bytes of two words by v_perm: the low or high half of each
-    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-    x.x = __builtin_amdgcn_perm(b[w], a[w], sel);
-    x.y = __builtin_amdgcn_perm(d[w], c[w], sel);
-    *reinterpret_cast<uint2*>(t + row * 128 + (((tg >> 1) ^ swizzle(row)) << 4) + ((tg & 1) << 3)) = x;
+    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;  // the high or low half of two words
+    *reinterpret_cast<uint2*>(t + (byte ^ ((j >> 1) << 4)) + j * 128) =
+        make_uint2(__builtin_amdgcn_perm(q[1][j >> 1], q[0][j >> 1], sel),
+                   __builtin_amdgcn_perm(q[3][j >> 1], q[2][j >> 1], sel));
   }
 }
-__device__ __forceinline__ void write_transposed(char* t, int dim0, int tg, const Regs& r, float) {
-  const uint32_t* a = reinterpret_cast<const uint32_t*>(&r.v[0]);
-  const uint32_t* b = reinterpret_cast<const uint32_t*>(&r.v[1]);
-  const uint32_t* c = reinterpret_cast<const uint32_t*>(&r.v[2]);
-  const uint32_t* d = reinterpret_cast<const uint32_t*>(&r.v[3]);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = dim0 + j;
-    *reinterpret_cast<uint4*>(t + row * 128 + ((tg ^ swizzle(row)) << 4)) = make_uint4(a[j], b[j], c[j], d[j]);
-  }
-}
-
-// Row-major rows; bf16 columns 16 h + 4 g + j of each 32 at 8 g + 4 h + j, so
-// that a lane's operand (see Type) is 16 contiguous bytes.
-__device__ __forceinline__ void write_rows(char* t, int pitch, int dc, int tg, const Regs& r, uint16_t) {
-  const int h = (dc & 3) >> 1, g = 2 * (dc & 1);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    char* p = t + (4 * tg + e) * pitch + 64 * (dc >> 2) + 16 * g + 8 * h;
-    *reinterpret_cast<uint2*>(p) = make_uint2(r.v[e].x, r.v[e].y);
-    *reinterpret_cast<uint2*>(p + 16) = make_uint2(r.v[e].z, r.v[e].w);
-  }
-}
-__device__ __forceinline__ void write_rows(char* t, int pitch, int dc, int tg, const Regs& r, float) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(t + (4 * tg + e) * pitch + 16 * dc) = r.v[e];
-}
-__device__ __forceinline__ float row_value(const char* t, int pitch, int i, int c, uint16_t) {
-  const int at = (c & ~31) + 8 * ((c >> 2) & 3) + 4 * ((c >> 4) & 1) + (c & 3);
-  return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(t + i * pitch)[at] << 16);
-}
-__device__ __forceinline__ float row_value(const char* t, int pitch, int i, int c, float) {
-  return reinterpret_cast<const float*>(t + i * pitch)[c];
-}
-__device__ __forceinline__ float column_value(const char* t, int row, int i, uint16_t) {
-  const char* p = t + row * 128 + (((i >> 3) ^ swizzle(row)) << 4);
-  return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i & 7] << 16);
-}
-__device__ __forceinline__ float column_value(const char* t, int row, int i, float) {
-  return reinterpret_cast<const float*>(t + row * 128 + (((i >> 2) ^ swizzle(row)) << 4))[i & 3];
+__device__ __forceinline__ void write_transposed(char* t, int byte, const uint4 (&v)[4], float) {
+  *reinterpret_cast<uint4*>(t + byte) = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x);
+  *reinterpret_cast<uint4*>(t + byte + 128) = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
+  *reinterpret_cast<uint4*>(t + (byte ^ 16) + 256) = make_uint4(v[0].z, v[1].z, v[2].z, v[3].z);
+  *reinterpret_cast<uint4*>(t + (byte ^ 16) + 384) = make_uint4(v[0].w, v[1].w, v[2].w, v[3].w);
 }
 
 // Four consecutive outputs of a row, `left` of them inside it.
-__device__ __forceinline__ void store4(uint16_t* p, floatx4 v, int left) {
-  uint2 w;
-  w.x = pack_bf16(v[0], v[1]);
-  w.y = pack_bf16(v[2], v[3]);
+typedef __attribute__((address_space(1))) char* GlobalOut;
+typedef uint32_t word2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float floatx4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ void store4(GlobalOut p, floatx4 v, int left, uint16_t) {
+  typedef __attribute__((address_space(1))) uint16_t* Out;
+  const uint32_t lo = pack_bf16(v[0], v[1]), hi = pack_bf16(v[2], v[3]);
   if (left >= 4) {
-    __builtin_memcpy(p, &w, 8);
+    *(__attribute__((address_space(1))) word2_a2*)p = word2_a2{lo, hi};
   } else {
-    if (left > 0) p[0] = (uint16_t)w.x;
-    if (left > 1) p[1] = (uint16_t)(w.x >> 16);
-    if (left > 2) p[2] = (uint16_t)w.y;
+    if (left > 0) ((Out)p)[0] = (uint16_t)lo;
+    if (left > 1) ((Out)p)[1] = (uint16_t)(lo >> 16);
+    if (left > 2) ((Out)p)[2] = (uint16_t)hi;
   }
 }
-__device__ __forceinline__ void store4(float* p, floatx4 v, int left) {
+__device__ __forceinline__ void store4(GlobalOut p, floatx4 v, int left, float) {
+  typedef __attribute__((address_space(1))) float* Out;
   if (left >= 4) {
-    __builtin_memcpy(p, &v, 16);
+    *(__attribute__((address_space(1))) floatx4_a4*)p = v;
   } else {
 #pragma unroll
     for (int e = 0; e < 3; ++e)
-      if (e < left) p[e] = v[e];
+      if (e < left) ((Out)p)[e] = v[e];
   }
 }
+__device__ __forceinline__ void store1(uint16_t* p, float v) { *p = (uint16_t)pack_bf16(v, v); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
 // The value, as if computed here: what depends on it is not moved out of the
 // loop, where it would hold registers for a part that is seldom run.
@@ -284,26 +255,31 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgcn_exp2f(g2 * (float)e); }
 
-// One workgroup per (role, head, segment, sequence): D / 32 waves, each with
-// 32 columns of the D x D state in its accumulators.  Widths below D are
+// One workgroup per (role, head, segment, sequence): D / 16 waves, each with
+// 16 columns of the D x D state in its accumulators.  Widths below D are
 // padded with zeros.  Each chunk of x, y, z is loaded once, a chunk ahead, into
 // registers, and laid out in LDS by rows (x, y: the pair products) and by
 // columns (y, z: contractions over steps).  STATE: only the state, from zeros,
 // for the segments before the last.
 template <typename T, int D, bool STATE>
-__global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
-  constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 32, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
+  constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
+  constexpr int PIECES = Type<T>::PIECES;
   constexpr int PITCH = D * (int)sizeof(T) + 16, ROWS = C * PITCH, COLS = D * 128;
-  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 128) + 2 * COLS + 16];
+  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 128) + 2 * COLS];
+  __shared__ __attribute__((aligned(16))) float weights[C];  // of the chunk's steps in the state after it
+  __shared__ float reaches[C];                               // factors of x St
+  __shared__ float powers[C];                                // intra lam^d
+  __shared__ volatile int odd[2];
   char* const yt = smem;
   char* const zt = smem + COLS;
-  char* const xr = STATE ? nullptr : smem + 2 * COLS;
-  char* const yr = STATE ? nullptr : smem + 2 * COLS + ROWS;
-  char* const pr = STATE ? nullptr : smem + 2 * COLS + 2 * ROWS;
-  volatile int* const odd = reinterpret_cast<volatile int*>(smem + sizeof(smem) - 16);
+  char* const xr = smem + 2 * COLS;
+  char* const yr = smem + 2 * COLS + ROWS;
+  char* const pr = smem + 2 * COLS + 2 * ROWS;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int at = ppo::xcd_tile().n;
   const int role = at % p.roles;
   at /= p.roles;
@@ -317,6 +293,7 @@ __global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
   const int R = c.x.width, N = c.z.width;
   const int64_t KV = (int64_t)R * N;
   const bool back = c.backward;
+  const int col = 16 * wave + l16;  // this lane's column of the state
 
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.steps) : p.steps;
   float g2 = p.log_decay[head] * 1.44269504088896341f;
@@ -324,169 +301,144 @@ __global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
   const uint8_t* done = p.done ? p.done + (int64_t)b * p.steps : nullptr;
   const int first = seg * p.seg_steps;                                        // steps in the order of processing
   const int last = min(len, first + p.seg_steps);
-
-  const T* xp = static_cast<const T*>(c.x.p) + b * c.x.sb + (head / c.x.group) * c.x.sh;
-  const T* yp = static_cast<const T*>(c.y.p) + b * c.y.sb + (head / c.y.group) * c.y.sh;
-  const T* zp = static_cast<const T*>(c.z.p) + b * c.z.sb + (head / c.z.group) * c.z.sh;
-  const int64_t pitch_o = (int64_t)p.heads * N, base_o = ((int64_t)b * p.steps * p.heads + head) * N;
+  const int pitch_o = p.heads * N;  // (at most 2^23)
+  const int64_t base_o = ((int64_t)b * p.steps * p.heads + head) * N;
 
   // rows past the sequence's end hold zeros
   if constexpr (!STATE) {
     const int end = min(p.steps, first + p.seg_steps);
     for (int t = max(len, first) + wave; t < end; t += W)
       for (int n = lane; n < N; n += 64) {
-        if (c.wide) static_cast<float*>(c.out)[base_o + t * pitch_o + n] = 0.f;
-        else static_cast<T*>(c.out)[base_o + t * pitch_o + n] = T(0);
+        if (c.wide) static_cast<float*>(c.out)[base_o + (int64_t)t * pitch_o + n] = 0.f;
+        else static_cast<T*>(c.out)[base_o + (int64_t)t * pitch_o + n] = T(0);
       }
   }
 
-  // the state entering the segment: rows 16 rt + 4 g4 + e, columns 32 wave + 16 nt + l16
-  floatx4 S[RT][2];
-  const float* entry = nullptr;
-  if constexpr (!STATE) entry = seg == 0 ? (c.carry ? c.carry + bh * KV : nullptr)
-                                         : c.states + (bh * (p.segments - 1) + seg - 1) * KV;
+  // a thread's share of a chunk: of y (the first half of the waves) or z four
+  // steps' chunks of columns, of x two steps'
+  const bool second = wave >= W / 2;
+  const Operand& oyz = second ? c.z : c.y;
+  const T* xp = static_cast<const T*>(c.x.p) + b * c.x.sb + (head / c.x.group) * c.x.sh;
+  const T* yzp = static_cast<const T*>(oyz.p) + b * oyz.sb + (head / oyz.group) * oyz.sh;
+  uint4 rx[2], ryz[4];
+  auto fetch = [&](auto& v, const Operand& o, const T* base, int r0, int chunk, int step) {
+    constexpr int ROWS_ = sizeof(v) / 16;
+    const int st = (int)o.st, at = min(chunk * FR, o.width - FR), count = min(C, last - r0);
+    const GlobalBytes low = uniform(base + (int64_t)(back ? len - r0 - count : r0) * st);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * rt + 4 * g4 + e, n = 32 * wave + 16 * nt + l16;
-        S[rt][nt][e] = 0.f;
-        if (entry && r < R && n < N) S[rt][nt][e] = entry[c.transposed ? (int64_t)n * R + r : (int64_t)r * N + n];
-      }
-
-  // this thread's share of a chunk: steps 4 tg .. 4 tg + 3, columns FR dc ..
-  const int dc = tid % (D / FR), tg = tid / (D / FR);
-  Regs rx, ry, rz;
-  auto fetch = [&](Regs& r, const Operand& o, const T* base, int r0) {
-    const int st = (int)o.st, col = load_column<T>(dc * FR, o.width);
-    if (r0 + C <= last) {  // a whole chunk: rows at one offset a lane from uniform addresses
-      const T* low = base + (int64_t)(back ? len - r0 - C : r0) * st;
-      const uint32_t byte = (uint32_t)((back ? C - 4 - 4 * tg : 4 * tg) * st + col) * (uint32_t)sizeof(T);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        r.v[e] = load_chunk<T>(reinterpret_cast<const char*>(low + (back ? 3 - e : e) * st), byte, dc * FR, o.width);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int s = min(4 * tg + e, last - 1 - r0);
-        const T* low = base + (int64_t)(back ? len - last : r0) * st;
-        const uint32_t byte = (uint32_t)((back ? last - 1 - r0 - s : s) * st + col) * (uint32_t)sizeof(T);
-        r.v[e] = load_chunk<T>(reinterpret_cast<const char*>(low), byte, dc * FR, o.width);
-      }
+    for (int e = 0; e < ROWS_; ++e) {
+      const int s = min(step + e, count - 1);
+      v[e] = load_chunk(low, (uint32_t)((back ? count - 1 - s : s) * st + at) * (uint32_t)sizeof(T));
     }
   };
-  auto finish = [&](Regs& r, int width, int n) {
+  auto finish = [&](auto& v, int width, int n, int chunk, int step) {
+    constexpr int ROWS_ = sizeof(v) / 16;
     if (width < D) {
-      const int c0 = here(dc * FR);
+      const int c0 = here(chunk * FR);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r.v[e] = trim_chunk<T>(r.v[e], c0, width);
+      for (int e = 0; e < ROWS_; ++e) v[e] = trim_chunk<T>(v[e], c0, width);
     }
     if (n < C) {
-      const int s = here(4 * tg);
+      const int s = here(step);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s + e >= n) r.v[e] = make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < ROWS_; ++e)
+        if (s + e >= n) v[e] = make_uint4(0, 0, 0, 0);
     }
   };
-  auto fetch_done = [&](int r0) -> int {  // whether the state entering step r0 + lane is dropped
+  auto fetch_done = [&](int r0, int lane) -> int {  // whether the state entering step r0 + lane is dropped
     const int s = r0 + lane;
     if (!done || lane >= C || s >= last) return 0;
     if (!back) return done[s];
     return s > 0 ? done[len - s] : 0;
   };
   int cut_next = 0;
-  if (first < last) {
-    if constexpr (!STATE) fetch(rx, c.x, xp, first);
-    fetch(ry, c.y, yp, first);
-    fetch(rz, c.z, zp, first);
-    cut_next = fetch_done(first);
+  auto fetch_all = [&](int r0, int tid) {
+    const int unit = tid & (2 * D - 1);
+    if constexpr (!STATE) fetch(rx, c.x, xp, r0, tid % (D / FR), 2 * (tid / (D / FR)));
+    fetch(ryz, oyz, yzp, r0, unit % (D / FR), 4 * (unit / (D / FR)));
+    cut_next = fetch_done(r0, tid & 63);
+  };
+  if (first < last) fetch_all(first, tid);
+
+  // the state entering the segment: rows 16 rt + 4 g4 + e of column col
+  floatx4 S[RT];
+  const float* entry = nullptr;
+  if constexpr (!STATE) entry = seg == 0 ? (c.carry ? c.carry + bh * KV : nullptr)
+                                         : c.states + (bh * (p.segments - 1) + seg - 1) * KV;
+  const int pitch_r = c.transposed ? 1 : N, pitch_n = c.transposed ? R : 1;  // of the state in memory
+  if (entry) {
+    const int at_n = min(col, N - 1) * pitch_n;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[rt][e] = entry[at_n + min(Type<T>::row(rt, 4 * g4 + e), R - 1) * pitch_r];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[rt][e] = Type<T>::row(rt, 4 * g4 + e) < R && col < N ? S[rt][e] : 0.f;
+  } else {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  if (tid < 4) odd[tid] = 0;
+  if (tid < 2) odd[tid] = 0;
+  if (tid < C) powers[tid] = c.intra * power(g2, tid);
   if constexpr (!STATE)
-    for (int i = tid; i < C * 8; i += 2 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < C * 8; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
   lds_barrier();
 
-  const int lane_byte = l16 * 128 + ((g4 ^ swizzle(l16)) << 4);
   float whole = 1.f;  // the segment's decay of its entry state, -1 once a reset dropped it
-  for (int r0 = first, it = 0; r0 < last; r0 += C, ++it) {
-    const int n = min(C, last - r0);
-    const uint64_t cut = __ballot(cut_next != 0);
-    if constexpr (!STATE) finish(rx, R, n);
-    finish(ry, R, n);
-    finish(rz, N, n);
-    bool is_odd = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) is_odd |= odd_exponent(ry.v[e], T()) | odd_exponent(rz.v[e], T());
-    if (__ballot(is_odd) && lane == 0) odd[it & 1] = 1;
-    if constexpr (!STATE) {
-      write_rows(xr, PITCH, dc, tg, rx, T());
-      write_rows(yr, PITCH, dc, tg, ry, T());
-    }
-    write_transposed(yt, dc * FR, tg, ry, T());
-    write_transposed(zt, dc * FR, tg, rz, T());
-    if (r0 + C < last) {
-      if constexpr (!STATE) fetch(rx, c.x, xp, r0 + C);
-      fetch(ry, c.y, yp, r0 + C);
-      fetch(rz, c.z, zp, r0 + C);
-      cut_next = fetch_done(r0 + C);
-    }
-    lds_barrier();
-    const bool careful = __builtin_amdgcn_readfirstlane(odd[it & 1]);
-    if (tid == 0) odd[(it + 1) & 1] = 0;
+  int span = C, single = 0;  // steps of a chunk; of a chunk taken step by step, how many are left
+  for (int r0 = first, it = 0, n; r0 < last; r0 += n, ++it) {
+    n = min(span, last - r0);
+    // (a lane's places, formed in every chunk: kept, they would spill)
+    const int tid = here(threadIdx.x), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int unit = tid & (2 * D - 1), dc = unit % (D / FR), tg = unit / (D / FR);
+    const int dx = tid % (D / FR), tx = tid / (D / FR);
     // a backward sequence's first step takes the state as it is
     const int skip = back && r0 == 0 ? 1 : 0;
-    const int last_cut = cut ? 63 - __clzll(cut) : -1;  // the last reset of the chunk
-    const float fade = power(g2, n - skip);
-
-    if (__builtin_expect(careful, 0)) {
-      // An infinity or NaN in y or z: the products above multiply it by the
-      // zeros of masked pairs, so the chunk is stepped through as defined.
-#pragma unroll 1
-      for (int i = 0; i < n; ++i) {
-        const int g4 = here(lane >> 4), l16 = here(lane & 15);
-        const float f = power(g2, i == 0 && skip ? 0 : 1);
-        const bool drop = cut >> i & 1;
-        float o[2] = {0.f, 0.f};
-        const int col0 = 32 * wave + l16;
-        const float z0 = column_value(zt, col0, i, T()) * c.update, z1 = column_value(zt, col0 + 16, i, T()) * c.update;
+    const uint64_t cut = __ballot(cut_next != 0 && lane < n);
+    if constexpr (!STATE) finish(rx, R, n, dx, 2 * tx);
+    finish(ryz, second ? N : R, n, dc, 4 * tg);
+    bool is_odd = false;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+    for (int e = 0; e < 4; ++e) is_odd |= odd_exponent(ryz[e], T());
+    if (__ballot(is_odd) && lane == 0) odd[it & 1] = 1;
+    if constexpr (!STATE) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 16 * rt + 4 * g4 + e;
-            const float y = column_value(yt, r, i, T());
-            const bool in = r < R;
-            S[rt][0][e] = in ? __fmaf_rn(y, z0, drop ? 0.f : f * S[rt][0][e]) : 0.f;
-            S[rt][1][e] = in ? __fmaf_rn(y, z1, drop ? 0.f : f * S[rt][1][e]) : 0.f;
-            if constexpr (!STATE) {
-              const float x = row_value(xr, PITCH, i, r, T());
-              if (in) {
-                o[0] = __fmaf_rn(x, S[rt][0][e], o[0]);
-                o[1] = __fmaf_rn(x, S[rt][1][e], o[1]);
-              }
-            }
-          }
-        if constexpr (!STATE) {
-          const int64_t row = base_o + (int64_t)(back ? len - 1 - (r0 + i) : r0 + i) * pitch_o;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const float v = ppo::add_xor32(ppo::add_xor16(o[nt])) * c.inter;
-            const int col = col0 + 16 * nt;
-            if (g4 == 0 && col < N) {
-              if (c.wide) static_cast<float*>(c.out)[row + col] = v;
-              else store4(static_cast<T*>(c.out) + row + col, floatx4{v, v, v, v}, 1);
-            }
-          }
-        }
-      }
-      lds_barrier();
-      if constexpr (!STATE) {
-        lds_barrier();
-      }
+      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(xr + (2 * tx + e) * PITCH + 16 * dx) = rx[e];
+    }
+    const int columns_byte = transposed_byte(dc, tg, T());
+    if (second) {
+      write_transposed(zt, columns_byte, ryz, T());
     } else {
-      floatx4 acc[2][QT];
+      if constexpr (!STATE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(yr + (4 * tg + e) * PITCH + 16 * dc) = ryz[e];
+      }
+      write_transposed(yt, columns_byte, ryz, T());
+    }
+    if (wave == 0 && lane < C) {
+      const int last_cut = cut ? 63 - __clzll(cut) : -1;
+      weights[lane] = lane < n && lane >= last_cut ? c.update * power(g2, n - 1 - lane) : 0.f;
+      reaches[lane] = (cut & (~0ull >> (63 - lane))) == 0 ? c.inter * power(g2, lane + 1 - skip) : 0.f;
+    }
+    if (r0 + n < last) fetch_all(r0 + n, tid);
+    lds_barrier();
+    const bool is_bad = __builtin_amdgcn_readfirstlane(odd[it & 1]);
+    if (tid == 0) odd[(it + 1) & 1] = 0;
+    if (__builtin_expect(is_bad && span > 1, 0)) {
+      // An infinity or NaN in y or z: the products below would multiply it by
+      // the zeros of masked pairs, so this chunk's steps are taken one by one.
+      span = 1;
+      single = n;
+      fetch_all(r0, tid);
+      lds_barrier();
+      n = 0;
+      continue;
+    }
+    const float fade = power(g2, n - skip);
+    const int lane_byte = l16 * 128 + ((g4 ^ swizzle(l16)) << 4);
+    {
       if constexpr (!STATE) {
         // pair products, keys as rows so that a lane holds four keys of one
         // query: tile (qt, kt) of the lower triangle, dealt to the waves
@@ -507,7 +459,7 @@ __global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int j = j0 + e;
-            a[e] = j <= i && j >= from ? a[e] * (c.intra * power(g2, i - j)) : 0.f;
+            a[e] = j <= i && j >= from ? a[e] * powers[max(i - j, 0)] : 0.f;
           }
           if constexpr (sizeof(T) == 2) {
             const int chunk = 2 * kt + (g4 >> 1);
@@ -518,91 +470,90 @@ __global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
           }
         }
         // x times the entry state (rows: its columns)
+        floatx4 acc[QT];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) acc[nt][qt] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int qt = 0; qt < QT; ++qt) acc[qt] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          const Frag s0 = state_frag(S, kb, 0, T()), s1 = state_frag(S, kb, 1, T());
+          const Frag s = state_frag(S, kb, T());
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            const Frag xb = *reinterpret_cast<const Frag*>(xr + (16 * qt + l16) * PITCH + 64 * kb + 16 * g4);
-            acc[0][qt] = Type<T>::mma(s0, xb, acc[0][qt]);
-            acc[1][qt] = Type<T>::mma(s1, xb, acc[1][qt]);
-          }
+          for (int qt = 0; qt < QT; ++qt)
+            acc[qt] = Type<T>::mma(
+                s, *reinterpret_cast<const Frag*>(xr + (16 * qt + l16) * PITCH + 64 * kb + 16 * g4), acc[qt]);
         }
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-          const int i = 16 * qt + l16;
-          const bool reach = (cut & (~0ull >> (63 - i))) == 0;
-          const float f = c.inter * power(g2, i + 1 - skip);
+          const float f = reaches[16 * qt + l16];
+          if (cut) {
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+            for (int e = 0; e < 4; ++e) acc[qt][e] = (cut & (~0ull >> (63 - (16 * qt + l16)))) == 0 ? acc[qt][e] : 0.f;
+          }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][qt][e] = reach ? acc[nt][qt][e] * f : 0.f;
+          for (int e = 0; e < 4; ++e) acc[qt][e] *= f;
         }
         lds_barrier();
-      }
-      if constexpr (!STATE) {
         // the pair products times z, and the outputs
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
-          Frag z[2];
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-            z[nt] = *reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, 2 * wave + nt, tb));
+          const Frag z = *reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb));
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
             if (16 * qt + 15 < 4 * FR * tb) continue;  // keys after the queries
-            const Frag pb = *reinterpret_cast<const Frag*>(pr + tile_byte(lane_byte, qt, tb));
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) acc[nt][qt] = Type<T>::mma(z[nt], pb, acc[nt][qt]);
+            acc[qt] = Type<T>::mma(z, *reinterpret_cast<const Frag*>(pr + tile_byte(lane_byte, qt, tb)), acc[qt]);
           }
         }
+        const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;
+        const GlobalOut low = (GlobalOut)uniform(static_cast<const char*>(c.out) +
+                                                 (base_o + (back ? len - r0 - n : r0) * (int64_t)pitch_o) * size);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           const int i = 16 * qt + l16;
           if (i < n) {
-            const int64_t row = base_o + (int64_t)(back ? len - 1 - (r0 + i) : r0 + i) * pitch_o;
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-              const int col = 32 * wave + 16 * nt + 4 * g4;
-              if (c.wide) store4(static_cast<float*>(c.out) + row + col, acc[nt][qt], N - col);
-              else store4(static_cast<T*>(c.out) + row + col, acc[nt][qt], N - col);
-            }
+            const uint32_t byte = (uint32_t)((back ? n - 1 - i : i) * pitch_o + n0) * size;
+            if (c.wide) store4(low + byte, acc[qt], N - n0, float());
+            else store4(low + byte, acc[qt], N - n0, T());
           }
         }
       }
       // state: its rows by y's columns, contracted over the steps
+      const int slot_row = Type<T>::row(0, l16), state_lane_byte = slot_row * 128 + ((g4 ^ swizzle(slot_row)) << 4);
+      if (cut) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[rt][e] *= fade;
+      }
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+        float weight[FR];
+#pragma unroll
+        for (int e = 0; e < FR; e += 4)
+          *reinterpret_cast<floatx4*>(weight + e) =
+              *reinterpret_cast<const floatx4*>(weights + 4 * FR * tb + FR * g4 + e);
+        Frag w[PIECES];
+        weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb)), weight, w);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          // (no more than four operands ahead: they would spill)
+          if (rt % 4 == 0) asm volatile("" ::: "memory");
+          const Frag ya = *reinterpret_cast<const Frag*>(yt + state_byte(state_lane_byte, rt, tb, T()));
+#pragma unroll
+          for (int q = PIECES - 1; q >= 0; --q) S[rt] = Type<T>::mma(ya, w[q], S[rt]);
+        }
+      }
+    }
+    lds_barrier();
+    if (single > 0) {
+      // (padding stays zero: a zero times an infinity is none)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[rt][nt][e] = cut ? 0.f : S[rt][nt][e] * fade;
-#pragma unroll
-      for (int tb = 0; tb < 2; ++tb) {
-        Frag w[2][Type<T>::PIECES];
-        float weight[FR];
-#pragma unroll
-        for (int e = 0; e < FR; ++e) {
-          const int j = 4 * FR * tb + FR * g4 + e;
-          weight[e] = j < n && j >= last_cut ? c.update * power(g2, n - 1 - j) : 0.f;
-        }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-          weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, 2 * wave + nt, tb)), weight, w[nt]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const Frag ya = *reinterpret_cast<const Frag*>(yt + tile_byte(lane_byte, rt, tb));
-#pragma unroll
-          for (int q = Type<T>::PIECES - 1; q >= 0; --q)
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) S[rt][nt] = Type<T>::mma(ya, w[nt][q], S[rt][nt]);
-        }
-      }
-      lds_barrier();
+        for (int e = 0; e < 4; ++e)
+          if (Type<T>::row(rt, 4 * g4 + e) >= R) S[rt][e] = 0.f;
+      if (--single == 0) span = C;
     }
     whole = cut || whole < 0.f ? -1.f : whole * fade;
   }
@@ -621,13 +572,10 @@ __global__ void __launch_bounds__(2 * D, 2) attention_kernel(AttnArgs p) {
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * rt + 4 * g4 + e, n = 32 * wave + 16 * nt + l16;
-        if (r < R && n < N)
-          exit[c.transposed ? (int64_t)n * R + r : (int64_t)r * N + n] = drop ? 0.f : S[rt][nt][e] * f;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int r = Type<T>::row(rt, 4 * g4 + e);
+      if (r < R && col < N) exit[r * pitch_r + col * pitch_n] = drop ? 0.f : S[rt][e] * f;
+    }
 }
 
 // The states entering each segment after the first, from what each segment
@@ -661,7 +609,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* x, T* out, 
   const float* p = x + i / width * width * group + i % width;
   float s = 0.f;
   for (int j = 0; j < group; ++j) s += p[(int64_t)j * width];
-  store4(out + i, floatx4{s, s, s, s}, 1);
+  store1(out + i, s);
 }
 
 // ---- one step
@@ -748,7 +696,7 @@ __global__ void __launch_bounds__(256) attention_step_kernel(StepArgs a) {
     const int n = slice * a.slice + tid;
     if (n < a.V) {
       const float s = ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])) * a.scale;
-      store4(static_cast<T*>(a.out) + bh * a.V + n, floatx4{s, s, s, s}, 1);
+      store1(static_cast<T*>(a.out) + bh * a.V + n, s);
     }
   }
 }
@@ -776,9 +724,9 @@ int segments_of(int dtype, int batch, int steps, int heads, int K, int V) {
 
 template <typename T, bool STATE>
 void launch_width(hipStream_t st, const AttnArgs& a, int D, unsigned grid) {
-  if (D == 32) hipLaunchKernelGGL((attention_kernel<T, 32, STATE>), dim3(grid), dim3(64), 0, st, a);
-  else if (D == 64) hipLaunchKernelGGL((attention_kernel<T, 64, STATE>), dim3(grid), dim3(128), 0, st, a);
-  else hipLaunchKernelGGL((attention_kernel<T, 128, STATE>), dim3(grid), dim3(256), 0, st, a);
+  if (D == 32) hipLaunchKernelGGL((attention_kernel<T, 32, STATE>), dim3(grid), dim3(128), 0, st, a);
+  else if (D == 64) hipLaunchKernelGGL((attention_kernel<T, 64, STATE>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attention_kernel<T, 128, STATE>), dim3(grid), dim3(512), 0, st, a);
 }
 
 // The pass from one direction's segments: their states from zeros, joined,
@@ -803,22 +751,25 @@ void outputs_pass(hipStream_t st, int dtype, const AttnArgs& a, int batch) {
   else launch_width<uint16_t, false>(st, a, D, grid);
 }
 
-int check_sizes(const char* what, int dtype, int batch, int steps, int heads, int kv_heads, int K, int V) {
+// `least`: rows of sequences are read 16 bytes at a time.
+int check_sizes(const char* what, int dtype, int batch, int steps, int heads, int kv_heads, int K, int V, int least) {
   if (dtype != ATTN_F32 && dtype != ATTN_BF16) return ppo::set_error(PPO_ERR_ARG, "%s: bad dtype %d", what, dtype);
-  if (batch < 0 || steps < 0 || heads < 0 || kv_heads < 0 || K < 0 || V < 0)
-    return ppo::set_error(PPO_ERR_ARG, "%s: negative size (batch %d steps %d heads %d kv_heads %d widths %d %d)", what,
-                          batch, steps, heads, kv_heads, K, V);
-  if (K > MAX_WIDTH || V > MAX_WIDTH)
-    return ppo::set_error(PPO_ERR_ARG, "%s: widths %d, %d above %d", what, K, V, MAX_WIDTH);
+  if (batch < 0 || steps < 0 || heads < 0 || kv_heads < 0)
+    return ppo::set_error(PPO_ERR_ARG, "%s: negative size (batch %d steps %d heads %d, %d)", what, batch, steps, heads,
+                          kv_heads);
+  if (K > MAX_WIDTH || V > MAX_WIDTH || K < least || V < least)
+    return ppo::set_error(PPO_ERR_ARG, "%s: widths %d, %d outside %d .. %d", what, K, V, least, MAX_WIDTH);
   if (heads > 0 && (kv_heads == 0 || heads % kv_heads))
     return ppo::set_error(PPO_ERR_ARG, "%s: %d heads do not share %d key heads evenly", what, heads, kv_heads);
+  if (heads > (1 << 23) / MAX_WIDTH)  // an output step's elements, as check_strides
+    return ppo::set_error(PPO_ERR_ARG, "%s: %d heads above %d", what, heads, (1 << 23) / MAX_WIDTH);
   // the grid: four workgroups a head at most (four slices of a step, three outputs of the backward pass)
   if ((int64_t)batch * heads > (1 << 29) - 1)
     return ppo::set_error(PPO_ERR_ARG, "%s: batch x heads above %d", what, (1 << 29) - 1);
   return PPO_OK;
 }
 
-bool empty(int batch, int heads, int K, int V) { return batch == 0 || heads == 0 || K == 0 || V == 0; }
+bool empty(int batch, int heads) { return batch == 0 || heads == 0; }
 
 // A lane's byte within a chunk is counted in 32 bits.
 int check_strides(const char* what, const int64_t* strides, int operands) {
@@ -853,18 +804,22 @@ AttnArgs common_args(int dtype, const float* log_decay, const uint8_t* done, con
 
 PPO_EXPORT int ppo_linear_attention_max_width(void) { return MAX_WIDTH; }
 
+PPO_EXPORT int ppo_linear_attention_min_width(int dtype) { return dtype == ATTN_BF16 ? 8 : 4; }
+
 PPO_EXPORT size_t ppo_linear_attention_workspace(int dtype, int batch, int steps, int heads, int key_width,
                                                  int value_width) {
-  if (check_sizes("ppo_linear_attention_workspace", dtype, batch, steps, heads, heads, key_width, value_width)) return 0;
-  if (empty(batch, heads, key_width, value_width)) return 0;
+  if (check_sizes("ppo_linear_attention_workspace", dtype, batch, steps, heads, heads, key_width, value_width, 1))
+    return 0;
+  if (empty(batch, heads)) return 0;
   return sizeof(float) * (size_t)state_floats(dtype, batch, steps, heads, key_width, value_width);
 }
 
 PPO_EXPORT size_t ppo_linear_attention_bwd_workspace(int dtype, int batch, int steps, int heads, int kv_heads,
                                                      int key_width, int value_width) {
-  if (check_sizes("ppo_linear_attention_bwd_workspace", dtype, batch, steps, heads, kv_heads, key_width, value_width))
+  if (check_sizes("ppo_linear_attention_bwd_workspace", dtype, batch, steps, heads, kv_heads, key_width, value_width,
+                  1))
     return 0;
-  if (empty(batch, heads, key_width, value_width)) return 0;
+  if (empty(batch, heads)) return 0;
   int64_t n = state_floats(dtype, batch, steps, heads, key_width, value_width);
   if (kv_heads < heads) n += (int64_t)batch * steps * heads * (key_width + value_width);
   return sizeof(float) * (size_t)n;
@@ -877,8 +832,8 @@ PPO_EXPORT int ppo_linear_attention_fwd(void* stream, int dtype, const void* q, 
                                         int heads, int kv_heads, int key_width, int value_width) {
   const char* what = "ppo_linear_attention_fwd";
   const int K = key_width, V = value_width;
-  if (int rc = check_sizes(what, dtype, batch, steps, heads, kv_heads, K, V)) return rc;
-  if (empty(batch, heads, K, V)) return PPO_OK;
+  if (int rc = check_sizes(what, dtype, batch, steps, heads, kv_heads, K, V, ppo_linear_attention_min_width(dtype))) return rc;
+  if (empty(batch, heads)) return PPO_OK;
   if (!log_decay || !final || !strides || (steps > 0 && (!q || !k || !v || !out)))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
   if (int rc = check_strides(what, strides, 3)) return rc;
@@ -914,8 +869,8 @@ PPO_EXPORT int ppo_linear_attention_bwd(void* stream, int dtype, const void* q, 
                                         int heads, int kv_heads, int key_width, int value_width) {
   const char* what = "ppo_linear_attention_bwd";
   const int K = key_width, V = value_width;
-  if (int rc = check_sizes(what, dtype, batch, steps, heads, kv_heads, K, V)) return rc;
-  if (empty(batch, heads, K, V)) return PPO_OK;
+  if (int rc = check_sizes(what, dtype, batch, steps, heads, kv_heads, K, V, ppo_linear_attention_min_width(dtype))) return rc;
+  if (empty(batch, heads)) return PPO_OK;
   if (!log_decay || !strides || (steps > 0 && (!q || !k || !v || !dout || !dq || !dk || !dv)))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
   if (int rc = check_strides(what, strides, 4)) return rc;
@@ -998,8 +953,8 @@ PPO_EXPORT int ppo_linear_attention_step(void* stream, int dtype, const void* q,
                                          int heads, int kv_heads, int key_width, int value_width) {
   const char* what = "ppo_linear_attention_step";
   const int K = key_width, V = value_width;
-  if (int rc = check_sizes(what, dtype, batch, 1, heads, kv_heads, K, V)) return rc;
-  if (empty(batch, heads, K, V)) return PPO_OK;
+  if (int rc = check_sizes(what, dtype, batch, 1, heads, kv_heads, K, V, 1)) return rc;
+  if (empty(batch, heads)) return PPO_OK;
   if (!q || !k || !v || !strides || !log_decay || !carry || !final || !out)
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
   StepArgs a{q, k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], log_decay, done, carry,

@@ -21,6 +21,7 @@ import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.nn.functional import pad
 
 from .. import _lib
 
@@ -91,8 +92,8 @@ def _check_attention(name, q, k, v, log_decay, carry, done, dims):
     if (kv_heads == 0) != (heads == 0) or (heads and heads % kv_heads):
         raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
     limit = _lib.load().ppo_linear_attention_max_width()
-    if q.shape[-1] > limit or v.shape[-1] > limit:
-        raise ValueError(f"{name} takes widths up to {limit}, not {q.shape[-1]} and {v.shape[-1]}")
+    if not (0 < q.shape[-1] <= limit and 0 < v.shape[-1] <= limit):
+        raise ValueError(f"{name} takes widths from 1 up to {limit}, not {q.shape[-1]} and {v.shape[-1]}")
     if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (heads,):
         raise ValueError(f"log_decay must be float32 [{heads}], got {log_decay.dtype} {tuple(log_decay.shape)}")
     if log_decay.requires_grad:
@@ -176,7 +177,15 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],)):
         raise ValueError(f"lengths must be int32 [{q.shape[0]}], got {lengths.dtype} {tuple(lengths.shape)}")
     _on_device("linear_attention", q, k, v, log_decay, carry, done, lengths)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    key, value = q.shape[-1], v.shape[-1]
+    scale = key ** -0.5 if scale is None else float(scale)
+    least = 16 // q.element_size()
+    if key < least or value < least:   # the kernels read rows 16 bytes at a time
+        more_k, more_v = max(least - key, 0), max(least - value, 0)
+        q, k, v = pad(q, (0, more_k)), pad(k, (0, more_k)), pad(v, (0, more_v))
+        carry = None if carry is None else pad(carry, (0, more_v, 0, more_k))
+        carry, out = linear_attention(q, k, v, log_decay, carry, done, lengths, scale)
+        return carry[..., :key, :value].contiguous(), out[..., :value].contiguous()
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     carry, done, lengths = (None if x is None else x.contiguous() for x in (carry, done, lengths))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad

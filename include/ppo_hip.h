@@ -376,7 +376,8 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  *   q, k, v (and dout in the backward); a step's stride is at most 2^23
  *   and none is negative.
  *   heads / kv_heads query heads in a row share a key head.  Widths are at most
- *   ppo_linear_attention_max_width().
+ *   ppo_linear_attention_max_width(), and of sequences at least
+ *   ppo_linear_attention_min_width(dtype) (16 bytes).
  *   log_decay float [heads] (<= 0; -inf: no memory), carry / final float
  *   [batch, heads, key_width, value_width] (carry may be NULL: zeros), done
  *   uint8 [batch, steps] (NULL: none), lengths int32 [batch] (NULL: steps),
@@ -384,6 +385,7 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  * The workspace (4-byte aligned) holds the states between pieces of long
  * sequences; the backward pass reads the forward's as fwd_workspace. */
 int ppo_linear_attention_max_width(void);
+int ppo_linear_attention_min_width(int dtype);
 size_t ppo_linear_attention_workspace(int dtype, int batch, int steps, int heads, int key_width, int value_width);
 int ppo_linear_attention_fwd(void* stream, int dtype, const void* q, const void* k, const void* v,
                              const int64_t* strides, const float* log_decay, const float* carry, const uint8_t* done,

@@ -29,6 +29,7 @@ def test_linear_attention_refuses_what_it_does_not_take():
     refused(ValueError, "evenly", linear_attention, q[:, :, :3], k, v, g[:3])
     refused(ValueError, "up to 128", linear_attention, *operands(K=129))
     refused(ValueError, "up to 128", linear_attention, *operands(V=129))
+    refused(ValueError, "up to 128", linear_attention, *operands(K=0))
     refused(ValueError, "log_decay", linear_attention, q, k, v, g[:2])
     refused(ValueError, "log_decay", linear_attention, q, k, v, g.double())
     refused(ValueError, "fixed schedule", linear_attention, q, k, v, g.clone().requires_grad_())
@@ -83,7 +84,11 @@ def test_the_entry_points_refuse_without_launching():
     assert forward(strides=None) == -1 and forward(decay=None) == -1 and forward(final=None) == -1
     assert forward(sizes=(2, 4, 3, 2, 8, 8)) == -1 and b"evenly" in lib.ppo_last_error()
     assert forward(sizes=(2, 4, 3, 0, 8, 8)) == -1
-    assert forward(sizes=(2, 4, 2, 2, 129, 8)) == -1 and b"above 128" in lib.ppo_last_error()
+    assert forward(sizes=(2, 4, 2, 2, 129, 8)) == -1 and b"outside 4 .. 128" in lib.ppo_last_error()
+    assert forward(sizes=(2, 4, 2, 2, 8, 3)) == -1 and forward(dtype=1, sizes=(2, 4, 2, 2, 7, 8)) == -1
+    assert forward(sizes=(2, 4, 1 << 17, 1 << 17, 8, 8)) == -1
+    near = (ctypes.c_int64 * 12)(0, -8, 0, *[0] * 9)
+    assert forward(strides=near) == -1 and b"step stride" in lib.ppo_last_error()
     assert forward(sizes=(-1, 4, 2, 2, 8, 8)) == -1
     assert forward(sizes=(1 << 30, 4, 2, 2, 8, 8)) == -1
     assert forward(sizes=(0, 4, 2, 2, 8, 8)) == 0
