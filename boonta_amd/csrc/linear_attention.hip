@@ -253,6 +253,14 @@ __device__ __forceinline__ int here(int x) {
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// x, or zero (a select: as a branch, each load before it would wait alone)
+__device__ __forceinline__ float keep_if(float x, bool keep) { return keep ? x : 0.f; }
+
+// A value every lane of the wave has, in a scalar register.
+__device__ __forceinline__ float same(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
 __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgcn_exp2f(g2 * (float)e); }
 
 // One workgroup per (role, head, segment, sequence): D / 16 waves, each with
@@ -271,7 +279,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
   __shared__ __attribute__((aligned(16))) float weights[C];  // of the chunk's steps in the state after it
   __shared__ float reaches[C];                               // factors of x St
   __shared__ float powers[C];                                // intra lam^d
-  __shared__ volatile int odd[2];
+  __shared__ int odd[2];
   char* const yt = smem;
   char* const zt = smem + COLS;
   char* const xr = smem + 2 * COLS;
@@ -297,7 +305,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
 
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.steps) : p.steps;
   float g2 = p.log_decay[head] * 1.44269504088896341f;
-  g2 = g2 < -1e30f ? -1e30f : g2;  // (a decay of zero: 0 times an infinite exponent is no number)
+  g2 = same(g2 < -1e30f ? -1e30f : g2);  // (a decay of zero: 0 times an infinite exponent is no number)
   const uint8_t* done = p.done ? p.done + (int64_t)b * p.steps : nullptr;
   const int first = seg * p.seg_steps;                                        // steps in the order of processing
   const int last = min(len, first + p.seg_steps);
@@ -387,16 +395,18 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
   lds_barrier();
 
   float whole = 1.f;  // the segment's decay of its entry state, -1 once a reset dropped it
-  int span = C, single = 0;  // steps of a chunk; of a chunk taken step by step, how many are left
-  for (int r0 = first, it = 0, n; r0 < last; r0 += n, ++it) {
-    n = min(span, last - r0);
-    // (a lane's places, formed in every chunk: kept, they would spill)
-    const int tid = here(threadIdx.x), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+  int r0 = first, it = 0;
+  uint64_t cut = 0;   // the chunk's steps that drop the state
+  // Lays out steps r0 .. r0 + n - 1, as loaded, and loads those after them.
+  // Whether y or z holds an infinity or NaN.  (Here and below a lane's places
+  // are formed in every chunk: kept, they would spill.)
+  auto stage = [&](int n) -> bool {
+    const int tid = here(threadIdx.x), lane = tid & 63;
     const int unit = tid & (2 * D - 1), dc = unit % (D / FR), tg = unit / (D / FR);
     const int dx = tid % (D / FR), tx = tid / (D / FR);
     // a backward sequence's first step takes the state as it is
     const int skip = back && r0 == 0 ? 1 : 0;
-    const uint64_t cut = __ballot(cut_next != 0 && lane < n);
+    cut = __ballot(cut_next != 0 && lane < n);
     if constexpr (!STATE) finish(rx, R, n, dx, 2 * tx);
     finish(ryz, second ? N : R, n, dc, 4 * tg);
     bool is_odd = false;
@@ -426,17 +436,13 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
     lds_barrier();
     const bool is_bad = __builtin_amdgcn_readfirstlane(odd[it & 1]);
     if (tid == 0) odd[(it + 1) & 1] = 0;
-    if (__builtin_expect(is_bad && span > 1, 0)) {
-      // An infinity or NaN in y or z: the products below would multiply it by
-      // the zeros of masked pairs, so this chunk's steps are taken one by one.
-      span = 1;
-      single = n;
-      fetch_all(r0, tid);
-      lds_barrier();
-      n = 0;
-      continue;
-    }
-    const float fade = power(g2, n - skip);
+    ++it;
+    return is_bad;
+  };
+  auto chunk = [&](int n) {
+    const int tid = here(threadIdx.x), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int skip = back && r0 == 0 ? 1 : 0;
+    const float fade = same(power(g2, n - skip));
     const int lane_byte = l16 * 128 + ((g4 ^ swizzle(l16)) << 4);
     {
       if constexpr (!STATE) {
@@ -456,11 +462,11 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
           const int i = 16 * qt + l16, j0 = 16 * kt + 4 * g4;
           const uint64_t upto = cut & (~0ull >> (63 - i));
           const int from = upto ? 63 - __clzll(upto) : 0;  // the last reset up to step i
+          float f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = j0 + e;
-            a[e] = j <= i && j >= from ? a[e] * powers[max(i - j, 0)] : 0.f;
-          }
+          for (int e = 0; e < 4; ++e) f[e] = powers[max(i - j0 - e, 0)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = keep_if(a[e] * f[e], j0 + e <= i && j0 + e >= from);
           if constexpr (sizeof(T) == 2) {
             const int chunk = 2 * kt + (g4 >> 1);
             *reinterpret_cast<uint2*>(pr + i * 128 + ((chunk ^ swizzle(i)) << 4) + ((g4 & 1) << 3)) =
@@ -520,12 +526,11 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
       if (cut) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
-      } else {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[rt][e] *= fade;
       }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[rt][e] *= fade;
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
         float weight[FR];
@@ -535,27 +540,53 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
               *reinterpret_cast<const floatx4*>(weights + 4 * FR * tb + FR * g4 + e);
         Frag w[PIECES];
         weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb)), weight, w);
+        // (in groups, so that products of one accumulator do not wait for each
+        // other and no more operands are ahead than fit)
+        constexpr int GROUP = RT < 4 ? RT : 4;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          // (no more than four operands ahead: they would spill)
-          if (rt % 4 == 0) asm volatile("" ::: "memory");
-          const Frag ya = *reinterpret_cast<const Frag*>(yt + state_byte(state_lane_byte, rt, tb, T()));
+        for (int r4 = 0; r4 < RT; r4 += GROUP) {
+          if (D == 128) __builtin_amdgcn_sched_barrier(0);
+          Frag ya[GROUP];
 #pragma unroll
-          for (int q = PIECES - 1; q >= 0; --q) S[rt] = Type<T>::mma(ya, w[q], S[rt]);
+          for (int i = 0; i < GROUP; ++i)
+            ya[i] = *reinterpret_cast<const Frag*>(yt + state_byte(state_lane_byte, r4 + i, tb, T()));
+#pragma unroll
+          for (int q = PIECES - 1; q >= 0; --q)
+#pragma unroll
+            for (int i = 0; i < GROUP; ++i) S[r4 + i] = Type<T>::mma(ya[i], w[q], S[r4 + i]);
         }
       }
     }
     lds_barrier();
-    if (single > 0) {
-      // (padding stays zero: a zero times an infinity is none)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (Type<T>::row(rt, 4 * g4 + e) >= R) S[rt][e] = 0.f;
-      if (--single == 0) span = C;
-    }
     whole = cut || whole < 0.f ? -1.f : whole * fade;
+    r0 += n;
+  };
+  while (r0 < last) {
+    bool is_bad = false;
+    while (r0 < last) {
+      const int n = min(C, last - r0);
+      is_bad = stage(n);
+      if (__builtin_expect(is_bad, 0)) break;
+      chunk(n);
+    }
+    if (__builtin_expect(is_bad, 0)) {
+      // The products multiply a masked pair by zero, which an infinity or NaN in
+      // y or z outlasts: such a chunk's steps are taken one by one.
+      const int end = min(last, r0 + C);
+#pragma unroll 1
+      while (r0 < end) {
+        lds_barrier();
+        fetch_all(r0, tid);
+        stage(1);
+        chunk(1);
+        // (padding stays zero: a zero times an infinity is none)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (Type<T>::row(rt, 4 * g4 + e) >= R) S[rt][e] = 0.f;
+      }
+    }
   }
 
   float* exit = STATE ? c.states + (bh * (p.segments - 1) + seg) * KV
