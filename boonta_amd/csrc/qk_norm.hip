@@ -11,11 +11,11 @@
 //
 // A workgroup takes a tile of steps with all heads of both: the angles' sines and cosines
 // are formed once a step and pair (p f in float64, since float32 is off by up
-// to p 2^-24 radians, and its turns brought below one before the float32
-// sine) and read from LDS by every head.  L lanes hold a row, each in units of
-// two chunks of VW columns that hold whole pairs, so the rotation needs no
-// lane exchange; the sums over a row are L-lane butterflies in float32.
-// Bound by HBM: x is read and out written once.
+// to p 2^-24 radians, and its turns brought within an eighth before the float32
+// series) and read from LDS by every head, while the first rows are on their
+// way.  L lanes hold a row, each in units of two chunks of VW columns that hold
+// whole pairs, so the rotation needs no lane exchange; the sums over a row are
+// L-lane butterflies in float32.  Bound by HBM: x is read and out written once.
 #include "split_f32.h"
 
 #include <algorithm>
@@ -26,7 +26,9 @@ enum NormDtype { NORM_F32 = 0, NORM_BF16 = 1 };
 
 constexpr int THREADS = 256;
 constexpr int MAX_DIM = 256, MAX_PAIRS = MAX_DIM / 2;
+constexpr int MAX_COLUMNS = MAX_DIM + 64;  // with those of a row's last lane past its end
 constexpr int MAX_TILE = 16;    // steps of a tile
+constexpr int UNROLL = 2;       // rows a lane group has in flight of each part
 constexpr int BWD_BLOCKS = 1024;  // most workgroups of the backward launch, each with its partial sums of dscale
 
 struct Rows {
@@ -37,6 +39,7 @@ struct Rows {
   int64_t sb, st, sh;   // element strides of x
   int64_t cb, ct, ch;   // and of cot
   int heads;
+  uint32_t inverse;     // 2^32 / heads, rounded up
 };
 
 struct NormArgs {
@@ -49,44 +52,54 @@ struct NormArgs {
   int D, P, interleaved, tile, lanes_log2;
 };
 
-__device__ __forceinline__ float widen(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
-__device__ __forceinline__ float widen(float x) { return x; }
-
-template <int VW> __device__ __forceinline__ void load_row(const uint16_t* p, int left, float (&v)[VW]) {
-  uint16_t e[VW];
+// A chunk of VW columns as loaded (words of 4 bytes, or one element of 2).
+template <typename T, int VW> struct Raw {
+  static constexpr int WORDS = VW * (int)sizeof(T) < 4 ? 1 : VW * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+};
+template <int VW> __device__ __forceinline__ void load_row(const uint16_t* p, int left, Raw<uint16_t, VW>& v) {
   if (left >= VW) {
-    __builtin_memcpy(e, p, 2 * VW);
+    if constexpr (VW == 1) v.w[0] = p[0];
+    else __builtin_memcpy(v.w, p, 2 * VW);
   } else {
 #pragma unroll
-    for (int j = 0; j < VW; ++j) e[j] = j < left ? p[j] : (uint16_t)0;
-  }
-#pragma unroll
-  for (int j = 0; j < VW; ++j) v[j] = widen(e[j]);
-}
-template <int VW> __device__ __forceinline__ void load_row(const float* p, int left, float (&v)[VW]) {
-  if (left >= VW) {
-    __builtin_memcpy(v, p, 4 * VW);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VW; ++j) v[j] = j < left ? p[j] : 0.f;
-  }
-}
-template <int VW> __device__ __forceinline__ void store_row(uint16_t* p, int left, const float (&v)[VW]) {
-  uint16_t e[VW];
-#pragma unroll
-  for (int j = 0; j < VW; ++j) e[j] = (uint16_t)ppo::pack_bf16(v[j], v[j]);
-  if constexpr (VW >= 2) {
-    if (left >= VW) {
-      uint32_t w[VW / 2];
-#pragma unroll
-      for (int j = 0; j < VW / 2; ++j) w[j] = ppo::pack_bf16(v[2 * j], v[2 * j + 1]);
-      __builtin_memcpy(p, w, 2 * VW);
-      return;
+    for (int i = 0; i < Raw<uint16_t, VW>::WORDS; ++i) {
+      const uint32_t lo = 2 * i < left ? p[2 * i] : 0, hi = 2 * i + 1 < left ? p[2 * i + 1] : 0;
+      v.w[i] = lo | hi << 16;
     }
   }
+}
+template <int VW> __device__ __forceinline__ void load_row(const float* p, int left, Raw<float, VW>& v) {
+  if (left >= VW) {
+    __builtin_memcpy(v.w, p, 4 * VW);
+  } else {
 #pragma unroll
-  for (int j = 0; j < VW; ++j)
-    if (j < left) p[j] = e[j];
+    for (int j = 0; j < VW; ++j) v.w[j] = j < left ? __float_as_uint(p[j]) : 0;
+  }
+}
+template <int VW> __device__ __forceinline__ void widen(const Raw<uint16_t, VW>& r, float (&v)[VW]) {
+#pragma unroll
+  for (int j = 0; j < VW; ++j) v[j] = __uint_as_float(j & 1 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+}
+template <int VW> __device__ __forceinline__ void widen(const Raw<float, VW>& r, float (&v)[VW]) {
+#pragma unroll
+  for (int j = 0; j < VW; ++j) v[j] = __uint_as_float(r.w[j]);
+}
+template <int VW> __device__ __forceinline__ void store_row(uint16_t* p, int left, const float (&v)[VW]) {
+  if constexpr (VW == 1) {
+    if (left > 0) p[0] = (uint16_t)ppo::pack_bf16(v[0], v[0]);
+  } else {
+    uint32_t w[VW / 2];
+#pragma unroll
+    for (int j = 0; j < VW / 2; ++j) w[j] = ppo::pack_bf16(v[2 * j], v[2 * j + 1]);
+    if (left >= VW) {
+      __builtin_memcpy(p, w, 2 * VW);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        if (j < left) p[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+    }
+  }
 }
 template <int VW> __device__ __forceinline__ void store_row(float* p, int left, const float (&v)[VW]) {
   if (left >= VW) {
@@ -96,6 +109,26 @@ template <int VW> __device__ __forceinline__ void store_row(float* p, int left, 
     for (int j = 0; j < VW; ++j)
       if (j < left) p[j] = v[j];
   }
+}
+
+// Cosine and sine of `turns` whole turns (|turns| <= 1/2): the Taylor series
+// about the nearest quarter turn, x within pi / 4; the terms left out are below
+// x^11 / 11! < 2e-9.
+__device__ __forceinline__ float2 cos_sin(float turns) {
+  const float q = rintf(4.f * turns);
+  const float x = __fmaf_rn(-0.25f, q, turns) * 6.283185307179586f, y = x * x;
+  float s = __fmaf_rn(y, 1.f / 362880.f, -1.f / 5040.f);
+  s = __fmaf_rn(y, s, 1.f / 120.f);
+  s = __fmaf_rn(y, s, -1.f / 6.f);
+  s = __fmaf_rn(x * y, s, x);
+  float c = __fmaf_rn(y, -1.f / 3628800.f, 1.f / 40320.f);
+  c = __fmaf_rn(y, c, -1.f / 720.f);
+  c = __fmaf_rn(y, c, 1.f / 24.f);
+  c = __fmaf_rn(y, c, -0.5f);
+  c = __fmaf_rn(y, c, 1.f);
+  const int k = (int)q & 3;   // the quarter
+  const float cn = k & 1 ? s : c, sn = k & 1 ? c : s;
+  return make_float2(k == 1 || k == 2 ? -cn : cn, k >= 2 ? -sn : sn);
 }
 
 // Sum over the row's lanes (2^log2 of them, neighbours).
@@ -133,6 +166,17 @@ template <int VW> __device__ __forceinline__ Unit unit_of(int u, int P, int inte
   return r;
 }
 
+template <int VW>
+__device__ __forceinline__ void load_scales(const float* scales, const Unit& u, float (&a)[VW], float (&b)[VW]) {
+  // (a lane past the row's end multiplies zeros)
+  const int at_a = min(u.a, MAX_COLUMNS - VW), at_b = min(u.b, MAX_COLUMNS - VW);
+#pragma unroll
+  for (int j = 0; j < VW; ++j) {
+    a[j] = scales[at_a + j];
+    b[j] = scales[at_b + j];
+  }
+}
+
 // (a, b) turned by the unit's angles, back for `sign` -1.
 template <int VW>
 __device__ __forceinline__ void turn(float (&a)[VW], float (&b)[VW], const Unit& u, const float2* cs, int P,
@@ -166,15 +210,28 @@ __device__ __forceinline__ void turn(float (&a)[VW], float (&b)[VW], const Unit&
   }
 }
 
+// The rows of one lane group in flight: UNROLL of them, by the group's place.
+template <typename T, int VW, int UPL, bool BWD> struct Batch {
+  Raw<T, VW> x[UNROLL][UPL][2];
+  Raw<T, VW> c[BWD ? UNROLL : 1][UPL][2];
+};
+
 template <typename T, int VW, int UPL, bool BWD>
 __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
   __shared__ float2 cs[MAX_TILE * MAX_PAIRS];
+  __shared__ __attribute__((aligned(16))) float scales[2][MAX_COLUMNS];
   __shared__ int64_t at[4][MAX_TILE];   // element offsets of a step's rows: x of both parts, cotangents of both
   __shared__ float red[BWD ? 2 * VW * UPL * THREADS : 1];
   const int tid = threadIdx.x, L = 1 << p.lanes_log2, l = tid & (L - 1), D = p.D, P = p.P;
+  const int group = tid >> p.lanes_log2, groups = THREADS >> p.lanes_log2;
+  const float over_d = 1.f / (float)D;
   Unit unit[UPL];
 #pragma unroll
   for (int k = 0; k < UPL; ++k) unit[k] = unit_of<VW>(l + k * L, P, p.interleaved);
+  for (int i = tid; i < 2 * MAX_COLUMNS; i += THREADS) {
+    const int w = i / MAX_COLUMNS, j = i % MAX_COLUMNS;
+    scales[w][j] = p.part[w].scale && j < D ? p.part[w].scale[j] : 1.f;
+  }
   float sum[2][UPL][2][VW];
   if constexpr (BWD) {
 #pragma unroll
@@ -184,16 +241,6 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const uint32_t t0 = tile * p.tile;
     const int n = (int)min((uint32_t)p.tile, p.tokens - t0);
-    for (int i = tid; i < n * P; i += THREADS) {
-      const int s = i / P, f = i - s * P;
-      const uint32_t token = t0 + s;
-      const double pos = p.positions ? (double)p.positions[token] : (double)(token % p.steps);
-      double turns = pos * p.frequencies[f] * 0.15915494309189533577;  // 1 / (2 pi)
-      turns -= rint(turns);
-      float sn, cn;
-      sincospif(2.f * (float)turns, &sn, &cn);
-      cs[s * P + f] = make_float2(cn, sn);
-    }
     if (tid < n) {
       const uint32_t token = t0 + tid, b = token / p.steps, t = token - b * p.steps;
 #pragma unroll
@@ -203,73 +250,95 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
+    // row r of part w: step r / heads, head r % heads (r heads < 2^32)
+    auto place = [&](int w, int r, int& s, int& h) {
+      s = p.part[w].heads == 1 ? r : (int)__umulhi((uint32_t)r, p.part[w].inverse);
+      h = r - s * p.part[w].heads;
+    };
+    auto load = [&](int w, int r0, Batch<T, VW, UPL, BWD>& v) {
       const Rows& q = p.part[w];
-      float wa[UPL][VW], wb[UPL][VW];
-#pragma unroll
-      for (int k = 0; k < UPL; ++k)
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          wa[k][j] = q.scale && unit[k].a + j < D ? q.scale[unit[k].a + j] : 1.f;
-          wb[k][j] = q.scale && unit[k].b + j < D ? q.scale[unit[k].b + j] : 1.f;
-        }
       const int rows = n * q.heads;
-      for (int r = tid >> p.lanes_log2; r < rows; r += THREADS >> p.lanes_log2) {
-        const int s = r / q.heads, h = r - s * q.heads;
-        const T* x = static_cast<const T*>(q.x) + at[w][s] + h * q.sh;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int r = r0 + u * groups;
+        if (r < rows) {
+          int s, h;
+          place(w, r, s, h);
+          const T* x = static_cast<const T*>(q.x) + at[w][s] + (int64_t)h * q.sh;
+#pragma unroll
+          for (int k = 0; k < UPL; ++k) {
+            load_row<VW>(x + unit[k].a, D - unit[k].a, v.x[u][k][0]);
+            load_row<VW>(x + unit[k].b, D - unit[k].b, v.x[u][k][1]);
+          }
+          if constexpr (BWD) {
+            const T* c = static_cast<const T*>(q.cot) + at[2 + w][s] + (int64_t)h * q.ch;
+#pragma unroll
+            for (int k = 0; k < UPL; ++k) {
+              load_row<VW>(c + unit[k].a, D - unit[k].a, v.c[u][k][0]);
+              load_row<VW>(c + unit[k].b, D - unit[k].b, v.c[u][k][1]);
+            }
+          }
+        }
+      }
+    };
+    auto finish = [&](int w, int r0, const Batch<T, VW, UPL, BWD>& v) {
+      const Rows& q = p.part[w];
+      const int rows = n * q.heads;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int r = r0 + u * groups;
+        if (r >= rows) continue;
+        int s, h;
+        place(w, r, s, h);
         T* out = static_cast<T*>(q.out) + ((int64_t)(t0 + s) * q.heads + h) * D;
+        const float2* angles = cs + s * P;
         float a[UPL][VW], b[UPL][VW];
         float ss = 0.f;
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          load_row<VW>(x + unit[k].a, D - unit[k].a, a[k]);
-          load_row<VW>(x + unit[k].b, D - unit[k].b, b[k]);
-        }
-        float ca[UPL][VW], cb[UPL][VW];
-        if constexpr (BWD) {
-          const T* c = static_cast<const T*>(q.cot) + at[2 + w][s] + h * q.ch;
-#pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            load_row<VW>(c + unit[k].a, D - unit[k].a, ca[k]);
-            load_row<VW>(c + unit[k].b, D - unit[k].b, cb[k]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < UPL; ++k)
+          widen(v.x[u][k][0], a[k]);
+          widen(v.x[u][k][1], b[k]);
 #pragma unroll
           for (int j = 0; j < VW; ++j) ss = __fmaf_rn(a[k][j], a[k][j], __fmaf_rn(b[k][j], b[k][j], ss));
+        }
         ss = lanes_sum(ss, p.lanes_log2);
-        const float rstd = 1.f / sqrtf(ss / (float)D + p.eps);
+        const float rstd = rsqrtf(__fmaf_rn(ss, over_d, p.eps));
         if constexpr (!BWD) {
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
+            float wa[VW], wb[VW];
+            load_scales(scales[w], unit[k], wa, wb);
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
-              a[k][j] = a[k][j] * rstd * wa[k][j];
-              b[k][j] = b[k][j] * rstd * wb[k][j];
+              a[k][j] = a[k][j] * rstd * wa[j];
+              b[k][j] = b[k][j] * rstd * wb[j];
             }
-            turn<VW>(a[k], b[k], unit[k], cs + s * P, P, p.interleaved, 1.f);
+            turn<VW>(a[k], b[k], unit[k], angles, P, p.interleaved, 1.f);
             store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
             store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
           }
         } else {
+          float ca[UPL][VW], cb[UPL][VW];
           float m = 0.f;
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
-            turn<VW>(ca[k], cb[k], unit[k], cs + s * P, P, p.interleaved, -1.f);
+            widen(v.c[u][k][0], ca[k]);
+            widen(v.c[u][k][1], cb[k]);
+            turn<VW>(ca[k], cb[k], unit[k], angles, P, p.interleaved, -1.f);
+            float wa[VW], wb[VW];
+            load_scales(scales[w], unit[k], wa, wb);
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
               a[k][j] *= rstd;
               b[k][j] *= rstd;
               sum[w][k][0][j] = __fmaf_rn(ca[k][j], a[k][j], sum[w][k][0][j]);
               sum[w][k][1][j] = __fmaf_rn(cb[k][j], b[k][j], sum[w][k][1][j]);
-              ca[k][j] *= wa[k][j];
-              cb[k][j] *= wb[k][j];
+              ca[k][j] *= wa[j];
+              cb[k][j] *= wb[j];
               m = __fmaf_rn(ca[k][j], a[k][j], __fmaf_rn(cb[k][j], b[k][j], m));
             }
           }
-          m = lanes_sum(m, p.lanes_log2) / (float)D;
+          m = lanes_sum(m, p.lanes_log2) * over_d;
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
 #pragma unroll
@@ -281,6 +350,26 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
             store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
           }
         }
+      }
+    };
+    Batch<T, VW, UPL, BWD> v[2];
+    load(0, group, v[0]);
+    load(1, group, v[1]);
+    for (int i = tid; i < n * P; i += THREADS) {
+      const int s = i / P, f = i - s * P;
+      const uint32_t token = t0 + s;
+      const double pos = p.positions ? (double)p.positions[token] : (double)(token % p.steps);
+      double turns = pos * p.frequencies[f] * 0.15915494309189533577;  // 1 / (2 pi)
+      turns -= rint(turns);
+      cs[s * P + f] = cos_sin((float)turns);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      finish(w, group, v[w]);
+      for (int r0 = group + UNROLL * groups; r0 < n * p.part[w].heads; r0 += UNROLL * groups) {
+        load(w, r0, v[w]);
+        finish(w, r0, v[w]);
       }
     }
     __syncthreads();
@@ -313,23 +402,23 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
   }
 }
 
-// dscale of both parts: the workgroups' sums, 16 columns by 16 groups of them
-// a workgroup, added in a fixed order.
+// dscale of both parts: the workgroups' sums, a column a wave, added in a fixed
+// order (lane by lane, then the lanes' butterfly).
 __global__ void __launch_bounds__(256) qk_norm_scale_kernel(const float* partials, int blocks, int D, float* dq_scale,
                                                             float* dk_scale) {
-  __shared__ float part[16][17];
-  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  const int lane = threadIdx.x & 63, col = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (col >= 2 * D) return;
   float s = 0.f;
-  if (col < 2 * D)
-    for (int b = g; b < blocks; b += 16) s += partials[(int64_t)b * 2 * D + col];
-  part[g][c] = s;
-  __syncthreads();
-  if (g == 0 && col < 2 * D) {
-    s = 0.f;
-    for (int i = 0; i < 16; ++i) s += part[i][c];
-    float* out = col < D ? dq_scale : dk_scale;
-    if (out) out[col < D ? col : col - D] = s;
+  for (int b0 = lane; b0 < blocks; b0 += 64 * 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = partials[(int64_t)min(b0 + 64 * u, blocks - 1) * 2 * D + col];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += b0 + 64 * u < blocks ? v[u] : 0.f;
   }
+  s = ppo::wave_sum_lanes(s);
+  float* out = col < D ? dq_scale : dk_scale;
+  if (out && lane == 0) out[col < D ? col : col - D] = s;
 }
 
 // ---- launches
@@ -342,6 +431,8 @@ int chunk_columns(int dtype, int P, int interleaved) {
   return v;
 }
 
+uint32_t inverse_of(int heads) { return heads > 1 ? (uint32_t)(((1ull << 32) + heads - 1) / heads) : 0; }
+
 int lanes_log2_of(int D, int v) {
   int log2 = 0;
   while (log2 < 6 && (2 * v << log2) < D) ++log2;
@@ -351,7 +442,7 @@ int lanes_log2_of(int D, int v) {
 // Steps of a tile: enough rows to keep the workgroup busy, but a tile for
 // every compute unit where there are few.
 int tile_of(int64_t tokens, int rows, int lanes_log2) {
-  const int64_t busy = std::max<int64_t>(1, 2048 / ((int64_t)rows << lanes_log2));
+  const int64_t busy = std::max<int64_t>(1, 2 * UNROLL * THREADS / ((int64_t)rows << lanes_log2));
   return (int)std::max<int64_t>(1, std::min<int64_t>({busy, MAX_TILE, ppo::ceil_div64(tokens, 512)}));
 }
 
@@ -365,7 +456,8 @@ int check(const char* what, int dtype, int batch, int steps, int heads, int kv_h
     return ppo::set_error(PPO_ERR_ARG, "%s: bad size (batch %d steps %d heads %d, %d width %d pairs %d)", what, batch,
                           steps, heads, kv_heads, dim, pairs);
   if (dim > MAX_DIM) return ppo::set_error(PPO_ERR_ARG, "%s: width %d above %d", what, dim, MAX_DIM);
-  if ((int64_t)heads + kv_heads > 65536) return ppo::set_error(PPO_ERR_ARG, "%s: more than 65536 heads", what);
+  if (heads > 8192 || kv_heads > 8192)
+    return ppo::set_error(PPO_ERR_ARG, "%s: %d, %d heads above 8192", what, heads, kv_heads);
   if ((int64_t)batch * steps > INT32_MAX) return ppo::set_error(PPO_ERR_ARG, "%s: batch x steps above 2^31 - 1", what);
   return PPO_OK;
 }
@@ -400,8 +492,8 @@ PPO_EXPORT int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, co
   if (!strides || (heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out)) || (pairs > 0 && !frequencies))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
   NormArgs a{};
-  a.part[0] = Rows{q, nullptr, q_scale, q_out, strides[0], strides[1], strides[2], 0, 0, 0, heads};
-  a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads};
+  a.part[0] = Rows{q, nullptr, q_scale, q_out, strides[0], strides[1], strides[2], 0, 0, 0, heads, inverse_of(heads)};
+  a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads, inverse_of(kv_heads)};
   a.frequencies = frequencies;
   a.positions = positions;
   a.eps = epsilon;
@@ -444,9 +536,9 @@ PPO_EXPORT int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, co
   if (!none) {
     NormArgs a{};
     a.part[0] = Rows{q, dq_out, q_scale, dq, strides[0], strides[1], strides[2], strides[6], strides[7], strides[8],
-                     heads};
+                     heads, inverse_of(heads)};
     a.part[1] = Rows{k, dk_out, k_scale, dk, strides[3], strides[4], strides[5], strides[9], strides[10], strides[11],
-                     kv_heads};
+                     kv_heads, inverse_of(kv_heads)};
     a.frequencies = frequencies;
     a.positions = positions;
     a.partials = static_cast<float*>(workspace);
@@ -464,7 +556,7 @@ PPO_EXPORT int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, co
     else launch_chunk<uint16_t, true>(ppo::as_stream(stream), a, v, (unsigned)blocks);
   }
   if (dq_scale || dk_scale)
-    hipLaunchKernelGGL(qk_norm_scale_kernel, dim3((unsigned)ppo::ceil_div(2 * width, 16)), dim3(256), 0,
+    hipLaunchKernelGGL(qk_norm_scale_kernel, dim3((unsigned)ppo::ceil_div(2 * width, 4)), dim3(256), 0,
                        ppo::as_stream(stream), static_cast<const float*>(workspace), blocks, width, dq_scale, dk_scale);
   return ppo::check_launch(what);
 }

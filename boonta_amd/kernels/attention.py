@@ -37,21 +37,16 @@ def _on_device(name, *tensors):
     return device
 
 
-class _Launch:
-    """A call's device and stream (the device made current where it is not)."""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (a build without devices has none)
 
-    def __init__(self, device):
-        self.device = device if device.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.device is not None:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *error):
-        if self.device is not None:
-            self.guard.__exit__(*error)
+def _launch(device, name, *args):
+    """Calls an entry point on the device's current stream (the device made current where it is not)."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, _raw_stream(device.index), *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, _raw_stream(device.index), *args)
 
 
 def _rows(x):
@@ -109,15 +104,14 @@ def _check_attention(name, q, k, v, log_decay, carry, done, dims):
 def _forward(q, k, v, log_decay, carry, done, lengths, scale):
     batch, steps, heads, key = q.shape
     kv_heads, value = v.shape[-2:]
-    with _Launch(q.device) as stream:
-        out = torch.empty(batch, steps, heads, value, dtype=q.dtype, device=q.device)
-        final = torch.empty(batch, heads, key, value, dtype=torch.float32, device=q.device)
-        dt = _DTYPES[q.dtype]
-        nbytes = _lib.load().ppo_linear_attention_workspace(dt, batch, steps, heads, key, value)
-        states = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-        _lib.call("ppo_linear_attention_fwd", stream, dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
-                  log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), scale, out.data_ptr(),
-                  final.data_ptr(), _ptr(states), nbytes, batch, steps, heads, kv_heads, key, value)
+    device, dt = q.device, _DTYPES[q.dtype]
+    out = torch.empty((batch, steps, heads, value), dtype=q.dtype, device=device)
+    final = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
+    nbytes = _lib.load().ppo_linear_attention_workspace(dt, batch, steps, heads, key, value)
+    states = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+    _launch(device, "ppo_linear_attention_fwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
+            log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), scale, out.data_ptr(), final.data_ptr(),
+            _ptr(states), nbytes, batch, steps, heads, kv_heads, key, value)
     return final, out, states
 
 
@@ -136,22 +130,19 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, log_decay, carry, done, lengths, states = ctx.saved_tensors
         batch, steps, heads, key = q.shape
         kv_heads, value = v.shape[-2:]
-        with _Launch(q.device) as stream:
-            if dout is None:   # (only the final carry was used)
-                dout = torch.zeros(value, dtype=q.dtype, device=q.device).expand(batch, steps, heads, value)
-            dout = _rows(dout)
-            dfinal = None if dfinal is None else dfinal.contiguous()
-            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            dcarry = None
-            if carry is not None and ctx.needs_input_grad[4]:
-                dcarry = torch.empty_like(carry)
-            dt = _DTYPES[q.dtype]
-            nbytes = _lib.load().ppo_linear_attention_bwd_workspace(dt, batch, steps, heads, kv_heads, key, value)
-            work = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-            _lib.call("ppo_linear_attention_bwd", stream, dt, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                      dout.data_ptr(), _strides(q, k, v, dout), log_decay.data_ptr(), _ptr(carry), _ptr(done),
-                      _ptr(lengths), ctx.scale, _ptr(dfinal), _ptr(states), dq.data_ptr(), dk.data_ptr(),
-                      dv.data_ptr(), _ptr(dcarry), _ptr(work), nbytes, batch, steps, heads, kv_heads, key, value)
+        device, dt = q.device, _DTYPES[q.dtype]
+        if dout is None:   # (only the final carry was used)
+            dout = torch.zeros(value, dtype=q.dtype, device=device).expand(batch, steps, heads, value)
+        dout = _rows(dout)
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+        dcarry = torch.empty_like(carry) if carry is not None and ctx.needs_input_grad[4] else None
+        nbytes = _lib.load().ppo_linear_attention_bwd_workspace(dt, batch, steps, heads, kv_heads, key, value)
+        work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+        _launch(device, "ppo_linear_attention_bwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+                _strides(q, k, v, dout), log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), ctx.scale,
+                _ptr(dfinal), _ptr(states), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dcarry), _ptr(work),
+                nbytes, batch, steps, heads, kv_heads, key, value)
         return dq, dk, dv, None, dcarry, None, None, None
 
 
@@ -213,13 +204,12 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     scale = key ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay, carry = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), carry.contiguous()
     done = None if done is None else done.contiguous()
-    with _Launch(device) as stream:
-        if out_carry is None:
-            out_carry = torch.empty(carry.shape, dtype=torch.float32, device=device)
-        out = torch.empty(batch, heads, value, dtype=q.dtype, device=device)
-        _lib.call("ppo_linear_attention_step", stream, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides(q, k, v), log_decay.data_ptr(), _ptr(done), carry.data_ptr(), out_carry.data_ptr(),
-                  out.data_ptr(), scale, batch, heads, kv_heads, key, value)
+    if out_carry is None:
+        out_carry = torch.empty(carry.shape, dtype=torch.float32, device=device)
+    out = torch.empty((batch, heads, value), dtype=q.dtype, device=device)
+    _launch(device, "ppo_linear_attention_step", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _strides(q, k, v), log_decay.data_ptr(), _ptr(done), carry.data_ptr(), out_carry.data_ptr(),
+            out.data_ptr(), scale, batch, heads, kv_heads, key, value)
     return out_carry, out
 
 
@@ -233,12 +223,13 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, device="cuda") -> tor
 
 def _norm_forward(q, k, q_scale, k_scale, frequencies, positions, epsilon, interleaved):
     batch, steps, heads, width = q.shape
-    with _Launch(q.device) as stream:
-        q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
-        _lib.call("ppo_qk_norm_rotary_fwd", stream, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), _strides(q, k),
-                  _ptr(q_scale), _ptr(k_scale), _ptr(frequencies), _ptr(positions), epsilon, interleaved,
-                  q_out.data_ptr(), k_out.data_ptr(), batch, steps, heads, k.shape[2], width,
-                  0 if frequencies is None else frequencies.numel())
+    device = q.device
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
+    _launch(device, "ppo_qk_norm_rotary_fwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), _strides(q, k),
+            _ptr(q_scale), _ptr(k_scale), _ptr(frequencies), _ptr(positions), epsilon, interleaved, q_out.data_ptr(),
+            k_out.data_ptr(), batch, steps, heads, k.shape[2], width,
+            0 if frequencies is None else frequencies.numel())
     return q_out, k_out
 
 
@@ -255,18 +246,19 @@ class _QKNormRotary(torch.autograd.Function):
         q, k, q_scale, k_scale, frequencies, positions = ctx.saved_tensors
         epsilon, interleaved = ctx.options
         batch, steps, heads, width = q.shape
-        with _Launch(q.device) as stream:
-            gq, gk = _rows(gq), _rows(gk)
-            dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
-            dq_scale = None if q_scale is None or not ctx.needs_input_grad[2] else torch.empty_like(q_scale)
-            dk_scale = None if k_scale is None or not ctx.needs_input_grad[3] else torch.empty_like(k_scale)
-            nbytes = _lib.load().ppo_qk_norm_rotary_bwd_workspace(width)
-            work = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-            _lib.call("ppo_qk_norm_rotary_bwd", stream, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), gq.data_ptr(),
-                      gk.data_ptr(), _strides(q, k, gq, gk), _ptr(q_scale), _ptr(k_scale), _ptr(frequencies),
-                      _ptr(positions), epsilon, interleaved, dq.data_ptr(), dk.data_ptr(), _ptr(dq_scale),
-                      _ptr(dk_scale), work.data_ptr(), nbytes, batch, steps, heads, k.shape[2], width,
-                      0 if frequencies is None else frequencies.numel())
+        device = q.device
+        gq, gk = _rows(gq), _rows(gk)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=device)
+        dq_scale = None if q_scale is None or not ctx.needs_input_grad[2] else torch.empty_like(q_scale)
+        dk_scale = None if k_scale is None or not ctx.needs_input_grad[3] else torch.empty_like(k_scale)
+        nbytes = _lib.load().ppo_qk_norm_rotary_bwd_workspace(width)
+        work = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+        _launch(device, "ppo_qk_norm_rotary_bwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), gq.data_ptr(),
+                gk.data_ptr(), _strides(q, k, gq, gk), _ptr(q_scale), _ptr(k_scale), _ptr(frequencies),
+                _ptr(positions), epsilon, interleaved, dq.data_ptr(), dk.data_ptr(), _ptr(dq_scale), _ptr(dk_scale),
+                work.data_ptr(), nbytes, batch, steps, heads, k.shape[2], width,
+                0 if frequencies is None else frequencies.numel())
         return dq, dk, dq_scale, dk_scale, None, None, None, None
 
 
