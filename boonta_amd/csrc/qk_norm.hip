@@ -9,13 +9,14 @@
 // Backward, from the cotangent c of out: e = c turned back, dscale += e x r,
 //   dx = r (e scale - x r^2 mean(e scale x)).
 //
-// A workgroup takes a tile of steps with all heads of both: the angles' sines and cosines
-// are formed once a step and pair (p f in float64, since float32 is off by up
-// to p 2^-24 radians, and its turns brought within an eighth before the float32
-// series) and read from LDS by every head, while the first rows are on their
-// way.  L lanes hold a row, each in units of two chunks of VW columns that hold
-// whole pairs, so the rotation needs no lane exchange; the sums over a row are
-// L-lane butterflies in float32.  Bound by HBM: x is read and out written once.
+// A wave takes a tile of steps with all heads of both: the angles' sines and
+// cosines are formed once a step and pair (p f in float64, since float32 is off
+// by up to p 2^-24 radians, and its turns brought within an eighth before the
+// float32 series) and read from LDS by every head, while the first rows are on
+// their way.  L lanes hold a row, each in units of two chunks of VW columns
+// that hold whole pairs, so the rotation needs no lane exchange; the sums over
+// a row are L-lane butterflies in float32.  Waves share nothing but the scales,
+// so none waits for another.  Bound by HBM: x is read and out written once.
 #include "split_f32.h"
 
 #include <algorithm>
@@ -24,12 +25,13 @@ namespace {
 
 enum NormDtype { NORM_F32 = 0, NORM_BF16 = 1 };
 
-constexpr int THREADS = 256;
-constexpr int MAX_DIM = 256, MAX_PAIRS = MAX_DIM / 2;
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int MAX_DIM = 256;
 constexpr int MAX_COLUMNS = MAX_DIM + 64;  // with those of a row's last lane past its end
-constexpr int MAX_TILE = 16;    // steps of a tile
-constexpr int UNROLL = 2;       // rows a lane group has in flight of each part
-constexpr int BWD_BLOCKS = 1024;  // most workgroups of the backward launch, each with its partial sums of dscale
+constexpr int TILE_ANGLES = 512;  // most angles of a wave's tile
+constexpr int UNROLL = 2;         // rows a lane group has in flight of each part
+constexpr int FWD_BLOCKS = 4096;  // most workgroups
+constexpr int BWD_BLOCKS = 1024;  // (each with its partial sums of dscale)
 
 struct Rows {
   const void* x;
@@ -48,8 +50,8 @@ struct NormArgs {
   const int32_t* positions;  // [batch, steps], or null (the step itself)
   float* partials;      // backward: [workgroups, 2, D]
   float eps;
-  uint32_t tokens, steps;
-  int D, P, interleaved, tile, lanes_log2;
+  uint32_t tokens, steps, inverse_steps, inverse_pairs;  // inverses: 2^32 / x, rounded up
+  int D, P, tile, lanes_log2;
 };
 
 // A chunk of VW columns as loaded (words of 4 bytes, or one element of 2).
@@ -142,26 +144,25 @@ __device__ __forceinline__ float lanes_sum(float v, int log2) {
   return v;
 }
 
-// The columns of a lane's unit u: chunks at a and b.  Columns of pairs come
-// first; in the layout of halves a chunk of first columns and that of their
-// partners, otherwise two neighbouring chunks.
+// The columns of unit u of a row's `units`: chunks at a and b and the first
+// pair of each (or -1: no rotation).  In the layout of halves the pairs'
+// units come first, a chunk of first columns and that of their partners;
+// otherwise chunks u and u + units, so that lanes read side by side.
 struct Unit {
-  int a, b, pair;  // pair: the first pair of the unit's first chunk, or -1 (no rotation)
+  int a, b, pair_a, pair_b;
 };
-template <int VW> __device__ __forceinline__ Unit unit_of(int u, int P, int interleaved) {
+template <int VW, bool INTER> __device__ __forceinline__ Unit unit_of(int u, int units, int P) {
   Unit r;
-  if (interleaved) {
-    r.a = 2 * VW * u;
-    r.b = r.a + VW;
-    r.pair = r.a < 2 * P ? VW * u : -1;
-  } else if (u * VW < P) {
+  const int rotated = INTER ? 0 : P / VW;
+  if (u < rotated) {
     r.a = u * VW;
     r.b = P + r.a;
-    r.pair = r.a;
+    r.pair_a = r.pair_b = r.a;
   } else {
-    r.a = 2 * VW * u;  // past the pairs' 2 VW (P / VW) columns
-    r.b = r.a + VW;
-    r.pair = -1;
+    r.a = (INTER ? 0 : 2 * P) + (u - rotated) * VW;
+    r.b = r.a + (units - rotated) * VW;
+    r.pair_a = INTER && r.a < 2 * P ? r.a / 2 : -1;
+    r.pair_b = INTER && r.b < 2 * P ? r.b / 2 : -1;
   }
   return r;
 }
@@ -178,31 +179,27 @@ __device__ __forceinline__ void load_scales(const float* scales, const Unit& u, 
 }
 
 // (a, b) turned by the unit's angles, back for `sign` -1.
-template <int VW>
+template <int VW, bool INTER>
 __device__ __forceinline__ void turn(float (&a)[VW], float (&b)[VW], const Unit& u, const float2* cs, int P,
-                                     int interleaved, float sign) {
-  if (u.pair < 0) return;
-  if (interleaved) {
-    if constexpr (VW >= 2) {
+                                     float sign) {
+  if constexpr (INTER) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float(&v)[VW] = c ? b : a;
+    for (int c = 0; c < 2; ++c) {
+      float(&v)[VW] = c ? b : a;
+      const int first = c ? u.pair_b : u.pair_a;
+      if (first < 0) continue;
 #pragma unroll
-        for (int j = 0; j < VW / 2; ++j) {
-          const int i = u.pair + c * (VW / 2) + j;
-          if (i < P) {
-            const float2 w = cs[i];
-            const float s = sign * w.y, x = v[2 * j], y = v[2 * j + 1];
-            v[2 * j] = x * w.x - y * s;
-            v[2 * j + 1] = y * w.x + x * s;
-          }
-        }
+      for (int j = 0; j < VW / 2; ++j) {
+        const float2 w = cs[min(first + j, P - 1)];
+        const float s = sign * w.y, x = v[2 * j], y = v[2 * j + 1];
+        v[2 * j] = first + j < P ? x * w.x - y * s : x;
+        v[2 * j + 1] = first + j < P ? y * w.x + x * s : y;
       }
     }
-  } else {
+  } else if (u.pair_a >= 0) {
 #pragma unroll
     for (int j = 0; j < VW; ++j) {
-      const float2 w = cs[u.pair + j];
+      const float2 w = cs[u.pair_a + j];
       const float s = sign * w.y, x = a[j], y = b[j];
       a[j] = x * w.x - y * s;
       b[j] = y * w.x + x * s;
@@ -210,24 +207,30 @@ __device__ __forceinline__ void turn(float (&a)[VW], float (&b)[VW], const Unit&
   }
 }
 
+// A wave's own LDS accesses in order.
+__device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // The rows of one lane group in flight: UNROLL of them, by the group's place.
 template <typename T, int VW, int UPL, bool BWD> struct Batch {
   Raw<T, VW> x[UNROLL][UPL][2];
   Raw<T, VW> c[BWD ? UNROLL : 1][UPL][2];
 };
 
-template <typename T, int VW, int UPL, bool BWD>
-__global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
-  __shared__ float2 cs[MAX_TILE * MAX_PAIRS];
+template <typename T, int VW, int UPL, bool INTER, bool BWD>
+__global__ void __launch_bounds__(THREADS, 2) qk_norm_kernel(NormArgs p) {
+  __shared__ union {
+    float2 angles[WAVES][TILE_ANGLES];
+    float sums[BWD ? 2 * VW * UPL * THREADS : 1];
+  } lds;
   __shared__ __attribute__((aligned(16))) float scales[2][MAX_COLUMNS];
-  __shared__ int64_t at[4][MAX_TILE];   // element offsets of a step's rows: x of both parts, cotangents of both
-  __shared__ float red[BWD ? 2 * VW * UPL * THREADS : 1];
-  const int tid = threadIdx.x, L = 1 << p.lanes_log2, l = tid & (L - 1), D = p.D, P = p.P;
-  const int group = tid >> p.lanes_log2, groups = THREADS >> p.lanes_log2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int L = 1 << p.lanes_log2, l = lane & (L - 1), D = p.D, P = p.P;
+  const int group = lane >> p.lanes_log2, groups = 64 >> p.lanes_log2;
+  float2* const cs = lds.angles[wave];
   const float over_d = 1.f / (float)D;
   Unit unit[UPL];
 #pragma unroll
-  for (int k = 0; k < UPL; ++k) unit[k] = unit_of<VW>(l + k * L, P, p.interleaved);
+  for (int k = 0; k < UPL; ++k) unit[k] = unit_of<VW, INTER>(l + k * L, UPL * L, P);
   for (int i = tid; i < 2 * MAX_COLUMNS; i += THREADS) {
     const int w = i / MAX_COLUMNS, j = i % MAX_COLUMNS;
     scales[w][j] = p.part[w].scale && j < D ? p.part[w].scale[j] : 1.f;
@@ -237,19 +240,21 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
 #pragma unroll
     for (int i = 0; i < 2 * UPL * 2 * VW; ++i) (&sum[0][0][0][0])[i] = 0.f;
   }
+  __syncthreads();
   const uint32_t tiles = (p.tokens + p.tile - 1) / p.tile;
-  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  for (uint32_t tile = blockIdx.x * WAVES + wave; tile < tiles; tile += gridDim.x * WAVES) {
     const uint32_t t0 = tile * p.tile;
     const int n = (int)min((uint32_t)p.tile, p.tokens - t0);
-    if (tid < n) {
-      const uint32_t token = t0 + tid, b = token / p.steps, t = token - b * p.steps;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        at[w][tid] = (int64_t)b * p.part[w].sb + (int64_t)t * p.part[w].st;
-        if constexpr (BWD) at[2 + w][tid] = (int64_t)b * p.part[w].cb + (int64_t)t * p.part[w].ct;
-      }
-    }
-    __syncthreads();
+    const uint32_t b0 = t0 / p.steps, s0 = t0 - b0 * p.steps;
+    // the tile's step s: sequence and step (a tile is at most 512 steps)
+    auto step_of = [&](int s, uint32_t& b, uint32_t& t) {
+      const uint32_t x = s0 + s;
+      const uint32_t wraps = p.steps > TILE_ANGLES ? (x >= p.steps ? 1 : 0)
+                             : p.steps > 1         ? __umulhi(x, p.inverse_steps)
+                                                   : x;
+      b = b0 + wraps;
+      t = x - wraps * p.steps;
+    };
     // row r of part w: step r / heads, head r % heads (r heads < 2^32)
     auto place = [&](int w, int r, int& s, int& h) {
       s = p.part[w].heads == 1 ? r : (int)__umulhi((uint32_t)r, p.part[w].inverse);
@@ -264,14 +269,16 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
         if (r < rows) {
           int s, h;
           place(w, r, s, h);
-          const T* x = static_cast<const T*>(q.x) + at[w][s] + (int64_t)h * q.sh;
+          uint32_t bb, tt;
+          step_of(s, bb, tt);
+          const T* x = static_cast<const T*>(q.x) + ((int64_t)bb * q.sb + (int64_t)tt * q.st + (int64_t)h * q.sh);
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
             load_row<VW>(x + unit[k].a, D - unit[k].a, v.x[u][k][0]);
             load_row<VW>(x + unit[k].b, D - unit[k].b, v.x[u][k][1]);
           }
           if constexpr (BWD) {
-            const T* c = static_cast<const T*>(q.cot) + at[2 + w][s] + (int64_t)h * q.ch;
+            const T* c = static_cast<const T*>(q.cot) + ((int64_t)bb * q.cb + (int64_t)tt * q.ct + (int64_t)h * q.ch);
 #pragma unroll
             for (int k = 0; k < UPL; ++k) {
               load_row<VW>(c + unit[k].a, D - unit[k].a, v.c[u][k][0]);
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
               a[k][j] = a[k][j] * rstd * wa[j];
               b[k][j] = b[k][j] * rstd * wb[j];
             }
-            turn<VW>(a[k], b[k], unit[k], angles, P, p.interleaved, 1.f);
+            turn<VW, INTER>(a[k], b[k], unit[k], angles, P, 1.f);
             store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
             store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
           }
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
           for (int k = 0; k < UPL; ++k) {
             widen(v.c[u][k][0], ca[k]);
             widen(v.c[u][k][1], cb[k]);
-            turn<VW>(ca[k], cb[k], unit[k], angles, P, p.interleaved, -1.f);
+            turn<VW, INTER>(ca[k], cb[k], unit[k], angles, P, -1.f);
             float wa[VW], wb[VW];
             load_scales(scales[w], unit[k], wa, wb);
 #pragma unroll
@@ -355,15 +362,16 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
     Batch<T, VW, UPL, BWD> v[2];
     load(0, group, v[0]);
     load(1, group, v[1]);
-    for (int i = tid; i < n * P; i += THREADS) {
-      const int s = i / P, f = i - s * P;
-      const uint32_t token = t0 + s;
-      const double pos = p.positions ? (double)p.positions[token] : (double)(token % p.steps);
+    for (int i = lane; i < n * P; i += 64) {
+      const int s = P == 1 ? i : (int)__umulhi((uint32_t)i, p.inverse_pairs), f = i - s * P;
+      uint32_t bb, tt;
+      step_of(s, bb, tt);
+      const double pos = p.positions ? (double)p.positions[t0 + s] : (double)tt;
       double turns = pos * p.frequencies[f] * 0.15915494309189533577;  // 1 / (2 pi)
       turns -= rint(turns);
-      cs[s * P + f] = cos_sin((float)turns);
+      cs[i] = cos_sin((float)turns);
     }
-    __syncthreads();
+    wave_lds();
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       finish(w, group, v[w]);
@@ -372,9 +380,10 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
         finish(w, r0, v[w]);
       }
     }
-    __syncthreads();
+    wave_lds();
   }
   if constexpr (BWD) {
+    __syncthreads();
     // this workgroup's sums of dscale: a row group's lanes side by side, added
     // in the groups' order
 #pragma unroll
@@ -384,16 +393,16 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(NormArgs p) {
       for (int k = 0; k < UPL; ++k)
 #pragma unroll
         for (int j = 0; j < VW; ++j) {
-          red[(k * 2 * VW + j) * THREADS + tid] = sum[w][k][0][j];
-          red[(k * 2 * VW + VW + j) * THREADS + tid] = sum[w][k][1][j];
+          lds.sums[(k * 2 * VW + j) * THREADS + tid] = sum[w][k][0][j];
+          lds.sums[(k * 2 * VW + VW + j) * THREADS + tid] = sum[w][k][1][j];
         }
       __syncthreads();
       for (int i = tid; i < PER * L; i += THREADS) {
         const int e = i >> p.lanes_log2, ll = i & (L - 1);
         float s = 0.f;
-        for (int g = ll; g < THREADS; g += L) s += red[e * THREADS + g];
+        for (int g = ll; g < THREADS; g += L) s += lds.sums[e * THREADS + g];
         const int k = e / (2 * VW), j = e % (2 * VW);
-        const Unit u = unit_of<VW>(ll + k * L, P, p.interleaved);
+        const Unit u = unit_of<VW, INTER>(ll + k * L, UPL * L, P);
         const int col = j < VW ? u.a + j : u.b + j - VW;
         if (col < D) p.partials[((int64_t)blockIdx.x * 2 + w) * D + col] = s;
       }
@@ -439,15 +448,36 @@ int lanes_log2_of(int D, int v) {
   return log2;
 }
 
-// Steps of a tile: enough rows to keep the workgroup busy, but a tile for
-// every compute unit where there are few.
-int tile_of(int64_t tokens, int rows, int lanes_log2) {
-  const int64_t busy = std::max<int64_t>(1, 2 * UNROLL * THREADS / ((int64_t)rows << lanes_log2));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({busy, MAX_TILE, ppo::ceil_div64(tokens, 512)}));
+// Steps of a wave's tile: rows of the part with fewer heads for every lane
+// group's loads, no more angles than there is room for, and a tile for every
+// wave where there are few steps.
+int tile_of(int64_t tokens, int heads, int pairs, int lanes_log2) {
+  const int64_t busy = std::max<int64_t>(1, 64 * UNROLL / ((int64_t)std::max(heads, 1) << lanes_log2));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({busy, TILE_ANGLES / std::max(pairs, 1), TILE_ANGLES,
+                                                      ppo::ceil_div64(tokens, 1024 * WAVES)}));
 }
 
-int blocks_of(int64_t tokens, int tile) {
-  return (int)std::min<int64_t>(BWD_BLOCKS, std::max<int64_t>(1, ppo::ceil_div64(tokens, tile)));
+int fewer(int a, int b) { return a && b ? std::min(a, b) : std::max(a, b); }
+
+unsigned blocks_of(int64_t tokens, int tile, int most) {
+  return (unsigned)std::min<int64_t>(most, ppo::ceil_div64(tokens, (int64_t)tile * WAVES));
+}
+
+NormArgs common_args(float epsilon, int64_t tokens, int steps, int width, int pairs, int interleaved, int dtype,
+                     int heads, const double* frequencies, const int32_t* positions) {
+  NormArgs a{};
+  a.frequencies = frequencies;
+  a.positions = positions;
+  a.eps = epsilon;
+  a.tokens = (uint32_t)tokens;
+  a.steps = (uint32_t)steps;
+  a.inverse_steps = inverse_of(steps);
+  a.inverse_pairs = inverse_of(pairs);
+  a.D = width;
+  a.P = pairs;
+  a.lanes_log2 = lanes_log2_of(width, chunk_columns(dtype, pairs, interleaved));
+  a.tile = tile_of(tokens, heads, pairs, a.lanes_log2);
+  return a;
 }
 
 int check(const char* what, int dtype, int batch, int steps, int heads, int kv_heads, int dim, int pairs) {
@@ -463,17 +493,14 @@ int check(const char* what, int dtype, int batch, int steps, int heads, int kv_h
 }
 
 template <typename T, bool BWD>
-void launch_chunk(hipStream_t st, const NormArgs& a, int v, unsigned grid) {
+void launch_chunk(hipStream_t st, const NormArgs& a, int v, bool interleaved, unsigned grid) {
+  constexpr int WIDE = 16 / (int)sizeof(T);
   const dim3 g(grid), t(THREADS);
-  if constexpr (sizeof(T) == 2) {
-    if (v == 8) {
-      hipLaunchKernelGGL((qk_norm_kernel<T, 8, 1, BWD>), g, t, 0, st, a);
-      return;
-    }
-  }
-  if (v == 4) hipLaunchKernelGGL((qk_norm_kernel<T, 4, 1, BWD>), g, t, 0, st, a);
-  else if (v == 2) hipLaunchKernelGGL((qk_norm_kernel<T, 2, 1, BWD>), g, t, 0, st, a);
-  else hipLaunchKernelGGL((qk_norm_kernel<T, 1, 2, BWD>), g, t, 0, st, a);
+  if (interleaved) hipLaunchKernelGGL((qk_norm_kernel<T, WIDE, 1, true, BWD>), g, t, 0, st, a);
+  else if (v == WIDE) hipLaunchKernelGGL((qk_norm_kernel<T, WIDE, 1, false, BWD>), g, t, 0, st, a);
+  else if (v == 4) hipLaunchKernelGGL((qk_norm_kernel<T, 4, 1, false, BWD>), g, t, 0, st, a);
+  else if (v == 2) hipLaunchKernelGGL((qk_norm_kernel<T, 2, 1, false, BWD>), g, t, 0, st, a);
+  else hipLaunchKernelGGL((qk_norm_kernel<T, 1, 2, false, BWD>), g, t, 0, st, a);
 }
 
 }  // namespace
@@ -491,23 +518,15 @@ PPO_EXPORT int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, co
   if (tokens == 0 || heads + kv_heads == 0 || width == 0) return PPO_OK;
   if (!strides || (heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out)) || (pairs > 0 && !frequencies))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
-  NormArgs a{};
+  NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, fewer(heads, kv_heads),
+                           frequencies, positions);
   a.part[0] = Rows{q, nullptr, q_scale, q_out, strides[0], strides[1], strides[2], 0, 0, 0, heads, inverse_of(heads)};
-  a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads, inverse_of(kv_heads)};
-  a.frequencies = frequencies;
-  a.positions = positions;
-  a.eps = epsilon;
-  a.tokens = (uint32_t)tokens;
-  a.steps = (uint32_t)steps;
-  a.D = width;
-  a.P = pairs;
-  a.interleaved = interleaved != 0;
-  const int v = chunk_columns(dtype, pairs, a.interleaved);
-  a.lanes_log2 = lanes_log2_of(width, v);
-  a.tile = tile_of(tokens, heads + kv_heads, a.lanes_log2);
-  const unsigned grid = (unsigned)ppo::ceil_div64(tokens, a.tile);
-  if (dtype == NORM_F32) launch_chunk<float, false>(ppo::as_stream(stream), a, v, grid);
-  else launch_chunk<uint16_t, false>(ppo::as_stream(stream), a, v, grid);
+  a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads,
+                   inverse_of(kv_heads)};
+  const int v = chunk_columns(dtype, pairs, interleaved);
+  const unsigned grid = blocks_of(tokens, a.tile, FWD_BLOCKS);
+  if (dtype == NORM_F32) launch_chunk<float, false>(ppo::as_stream(stream), a, v, interleaved != 0, grid);
+  else launch_chunk<uint16_t, false>(ppo::as_stream(stream), a, v, interleaved != 0, grid);
   return ppo::check_launch(what);
 }
 
@@ -534,26 +553,17 @@ PPO_EXPORT int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, co
     return ppo::set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   int blocks = 0;
   if (!none) {
-    NormArgs a{};
+    NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, fewer(heads, kv_heads),
+                             frequencies, positions);
     a.part[0] = Rows{q, dq_out, q_scale, dq, strides[0], strides[1], strides[2], strides[6], strides[7], strides[8],
                      heads, inverse_of(heads)};
     a.part[1] = Rows{k, dk_out, k_scale, dk, strides[3], strides[4], strides[5], strides[9], strides[10], strides[11],
                      kv_heads, inverse_of(kv_heads)};
-    a.frequencies = frequencies;
-    a.positions = positions;
     a.partials = static_cast<float*>(workspace);
-    a.eps = epsilon;
-    a.tokens = (uint32_t)tokens;
-    a.steps = (uint32_t)steps;
-    a.D = width;
-    a.P = pairs;
-    a.interleaved = interleaved != 0;
-    const int v = chunk_columns(dtype, pairs, a.interleaved);
-    a.lanes_log2 = lanes_log2_of(width, v);
-    a.tile = tile_of(tokens, heads + kv_heads, a.lanes_log2);
-    blocks = blocks_of(tokens, a.tile);
-    if (dtype == NORM_F32) launch_chunk<float, true>(ppo::as_stream(stream), a, v, (unsigned)blocks);
-    else launch_chunk<uint16_t, true>(ppo::as_stream(stream), a, v, (unsigned)blocks);
+    const int v = chunk_columns(dtype, pairs, interleaved);
+    blocks = (int)blocks_of(tokens, a.tile, BWD_BLOCKS);
+    if (dtype == NORM_F32) launch_chunk<float, true>(ppo::as_stream(stream), a, v, interleaved != 0, (unsigned)blocks);
+    else launch_chunk<uint16_t, true>(ppo::as_stream(stream), a, v, interleaved != 0, (unsigned)blocks);
   }
   if (dq_scale || dk_scale)
     hipLaunchKernelGGL(qk_norm_scale_kernel, dim3((unsigned)ppo::ceil_div(2 * width, 4)), dim3(256), 0,
