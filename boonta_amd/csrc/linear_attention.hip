@@ -145,6 +145,16 @@ __device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, uint16_
 }
 __device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, float) { return tile_byte(lane_byte, rt, tb); }
 
+// The same in a tile of rows of RB bytes: the XOR of row r's chunks, and the
+// byte of an operand (row 16 tile + l16, chunk 4 kb + g4).
+template <int RB> __device__ __forceinline__ int row_swizzle(int r) {
+  return RB >= 256 ? r & 15 : RB == 128 ? swizzle(r) : (r >> 2) & 3;
+}
+template <int RB> __device__ __forceinline__ int row_byte(int l16, int g4, int tile, int kb) {
+  const int lane_byte = l16 * RB + ((g4 ^ row_swizzle<RB>(l16)) << 4);
+  return RB == 128 ? tile_byte(lane_byte, tile, kb) : (lane_byte ^ (kb << 6)) + tile * 16 * RB;
+}
+
 // 16 bytes at a lane's 32-bit offset from an address that is uniform in the
 // wave.  (Opaque, so that the sum stays in the load and each row of a lane
 // costs one register, not an address.)
@@ -270,15 +280,17 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // columns (y, z: contractions over steps).  STATE: only the state, from zeros,
 // for the segments before the last.
 template <typename T, int D, bool STATE>
-__global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attention_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
   constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
   constexpr int PIECES = Type<T>::PIECES;
-  constexpr int PITCH = D * (int)sizeof(T) + 16, ROWS = C * PITCH, COLS = D * 128;
-  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 128) + 2 * COLS];
+  constexpr int RB = D * (int)sizeof(T), ROWS = C * RB, COLS = D * 128;
+  // y and z by columns, x and y by rows, and the pair products: all queries
+  // with the chunk's first half of keys, the later half with the other
+  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 96) + 2 * COLS];
   __shared__ __attribute__((aligned(16))) float weights[C];  // of the chunk's steps in the state after it
   __shared__ float reaches[C];                               // factors of x St
-  __shared__ float powers[C];                                // intra lam^d
+  __shared__ float powers[16 + C];                           // intra lam^d at 16 + d
   __shared__ int odd[2];
   char* const yt = smem;
   char* const zt = smem + COLS;
@@ -389,9 +401,9 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
     for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   if (tid < 2) odd[tid] = 0;
-  if (tid < C) powers[tid] = c.intra * power(g2, tid);
+  if (tid < 16 + C) powers[tid] = tid < 16 ? 0.f : c.intra * power(g2, tid - 16);
   if constexpr (!STATE)
-    for (int i = tid; i < C * 8; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < C * 6; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
   lds_barrier();
 
   float whole = 1.f;  // the segment's decay of its entry state, -1 once a reset dropped it
@@ -415,7 +427,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
     if (__ballot(is_odd) && lane == 0) odd[it & 1] = 1;
     if constexpr (!STATE) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(xr + (2 * tx + e) * PITCH + 16 * dx) = rx[e];
+      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(xr + (2 * tx + e) * RB + ((dx ^ row_swizzle<RB>(2 * tx + e)) << 4)) = rx[e];
     }
     const int columns_byte = transposed_byte(dc, tg, T());
     if (second) {
@@ -423,7 +435,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
     } else {
       if constexpr (!STATE) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(yr + (4 * tg + e) * PITCH + 16 * dc) = ryz[e];
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(yr + (4 * tg + e) * RB + ((dc ^ row_swizzle<RB>(4 * tg + e)) << 4)) = ryz[e];
       }
       write_transposed(yt, columns_byte, ryz, T());
     }
@@ -448,6 +460,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
       if constexpr (!STATE) {
         // pair products, keys as rows so that a lane holds four keys of one
         // query: tile (qt, kt) of the lower triangle, dealt to the waves
+        const int pair_byte = l16 * 64 + ((g4 ^ (l16 >> 2)) << 4);
 #pragma unroll 1
         for (int idx = wave; idx < QT * (QT + 1) / 2; idx += W) {
           const int qt = QT == 2 ? (idx > 0) : (idx > 0) + (idx > 2) + (idx > 5);
@@ -455,24 +468,29 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
           floatx4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
-            const Frag ya = *reinterpret_cast<const Frag*>(yr + (16 * kt + l16) * PITCH + 64 * kb + 16 * g4);
-            const Frag xb = *reinterpret_cast<const Frag*>(xr + (16 * qt + l16) * PITCH + 64 * kb + 16 * g4);
+            const Frag ya = *reinterpret_cast<const Frag*>(yr + row_byte<RB>(l16, g4, kt, kb));
+            const Frag xb = *reinterpret_cast<const Frag*>(xr + row_byte<RB>(l16, g4, qt, kb));
             a = Type<T>::mma(ya, xb, a);
           }
           const int i = 16 * qt + l16, j0 = 16 * kt + 4 * g4;
-          const uint64_t upto = cut & (~0ull >> (63 - i));
-          const int from = upto ? 63 - __clzll(upto) : 0;  // the last reset up to step i
-          float f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = powers[max(i - j0 - e, 0)];
+          for (int e = 0; e < 4; ++e) a[e] *= powers[16 + i - j0 - e];
+          if (cut) {
+            const uint64_t upto = cut & (~0ull >> (63 - i));
+            const int from = upto ? 63 - __clzll(upto) : 0;  // the last reset up to step i
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = keep_if(a[e] * f[e], j0 + e <= i && j0 + e >= from);
+            for (int e = 0; e < 4; ++e) a[e] = keep_if(a[e], j0 + e >= from);
+          }
+          if (kt == qt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = keep_if(a[e], j0 + e <= i);
+          }
           if constexpr (sizeof(T) == 2) {
-            const int chunk = 2 * kt + (g4 >> 1);
-            *reinterpret_cast<uint2*>(pr + i * 128 + ((chunk ^ swizzle(i)) << 4) + ((g4 & 1) << 3)) =
-                make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
+            const int chunk = 2 * (kt & 1) + (g4 >> 1);
+            *reinterpret_cast<uint2*>(pr + l16 * 64 + ((chunk ^ (l16 >> 2)) << 4) + ((g4 & 1) << 3) + qt * 1024 +
+                                      (kt >> 1) * C * 32) = make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
           } else {
-            *reinterpret_cast<floatx4*>(pr + i * 128 + (((4 * kt + g4) ^ swizzle(i)) << 4)) = a;
+            *reinterpret_cast<floatx4*>(pr + pair_byte + qt * 1024 + kt * C * 32) = a;
           }
         }
         // x times the entry state (rows: its columns)
@@ -485,7 +503,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
             acc[qt] = Type<T>::mma(
-                s, *reinterpret_cast<const Frag*>(xr + (16 * qt + l16) * PITCH + 64 * kb + 16 * g4), acc[qt]);
+                s, *reinterpret_cast<const Frag*>(xr + row_byte<RB>(l16, g4, qt, kb)), acc[qt]);
         }
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -505,7 +523,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 4 : D == 64 ? 3 : 2) attenti
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
             if (16 * qt + 15 < 4 * FR * tb) continue;  // keys after the queries
-            acc[qt] = Type<T>::mma(z, *reinterpret_cast<const Frag*>(pr + tile_byte(lane_byte, qt, tb)), acc[qt]);
+            acc[qt] = Type<T>::mma(z, *reinterpret_cast<const Frag*>(pr + pair_byte + qt * 1024 + tb * C * 32), acc[qt]);
           }
         }
         const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;
@@ -743,11 +761,11 @@ int padded(int K, int V) {
 int chunk(int dtype) { return dtype == ATTN_F32 ? 32 : 64; }
 
 // Pieces the step axis is cut into: enough workgroups to fill the chip, each
-// of at least eight chunks (a piece's state is written and read back).
+// of at least four chunks (a piece's state is written and read back).
 int segments_of(int dtype, int batch, int steps, int heads, int K, int V) {
   const int64_t pairs = std::max<int64_t>(1, (int64_t)batch * heads);
   const int c = chunk(dtype), D = padded(K, V);
-  const int64_t want = 1024 * 64 / D / pairs, most = ppo::ceil_div(steps, 8 * c);
+  const int64_t want = 1024 * 64 / D / pairs, most = ppo::ceil_div(steps, 4 * c);
   const int segs = (int)std::max<int64_t>(1, std::min(want, most));
   const int seg_steps = ppo::ceil_div(ppo::ceil_div(std::max(steps, 1), segs), c) * c;
   return std::max(1, ppo::ceil_div(steps, seg_steps));
