@@ -109,7 +109,7 @@ template <int RT> __device__ __forceinline__ floatx4 state_frag(const floatx4 (&
 // z times its steps' weights, as operands whose sum is the product to float32:
 // one float32, or three bf16 pieces, each what the ones before leave (the
 // states are float32 sums of exact products of these).
-__device__ __forceinline__ void weigh(bf16x8 z, const float (&w)[8], bf16x8 (&p)[3]) {
+__device__ __forceinline__ void weigh(bf16x8 z, const float (&w)[8], bf16x8 (&p)[3], bool exact) {
   const uint4 u = __builtin_bit_cast(uint4, z);
   const uint32_t q[4] = {u.x, u.y, u.z, u.w};
   floatx4 lo, hi;
@@ -121,9 +121,10 @@ __device__ __forceinline__ void weigh(bf16x8 z, const float (&w)[8], bf16x8 (&p)
     hi[2 * i + 1] = __uint_as_float(q[2 + i] & 0xffff0000u) * w[5 + 2 * i];
   }
 #pragma unroll
-  for (int i = 0; i < 3; ++i) p[i] = ppo::split_piece(lo, hi);
+  for (int i = 0; i < 2; ++i) p[i] = ppo::split_piece(lo, hi);
+  if (exact) p[2] = join(lo, hi);
 }
-__device__ __forceinline__ void weigh(floatx4 z, const float (&w)[4], floatx4 (&p)[1]) {
+__device__ __forceinline__ void weigh(floatx4 z, const float (&w)[4], floatx4 (&p)[1], bool) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) p[0][e] = z[e] * w[e];
 }
@@ -345,11 +346,21 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
     constexpr int ROWS_ = sizeof(v) / 16;
     const int st = (int)o.st, at = min(chunk * FR, o.width - FR), count = min(C, last - r0);
     const GlobalBytes low = uniform(base + (int64_t)(back ? len - r0 - count : r0) * st);
+    uint32_t byte[ROWS_];
+    if (count == C) {
+      const uint32_t next = (uint32_t)((back ? -st : st) * (int)sizeof(T));
+      byte[0] = (uint32_t)((back ? C - 1 - step : step) * st + at) * (uint32_t)sizeof(T);
 #pragma unroll
-    for (int e = 0; e < ROWS_; ++e) {
-      const int s = min(step + e, count - 1);
-      v[e] = load_chunk(low, (uint32_t)((back ? count - 1 - s : s) * st + at) * (uint32_t)sizeof(T));
+      for (int e = 1; e < ROWS_; ++e) byte[e] = byte[e - 1] + next;
+    } else {
+#pragma unroll
+      for (int e = 0; e < ROWS_; ++e) {
+        const int s = min(step + e, count - 1);
+        byte[e] = (uint32_t)((back ? count - 1 - s : s) * st + at) * (uint32_t)sizeof(T);
+      }
     }
+#pragma unroll
+    for (int e = 0; e < ROWS_; ++e) v[e] = load_chunk(low, byte[e]);
   };
   auto finish = [&](auto& v, int width, int n, int chunk, int step) {
     constexpr int ROWS_ = sizeof(v) / 16;
@@ -406,6 +417,9 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
     for (int i = tid; i < C * 6; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
   lds_barrier();
 
+  // Whether the state itself is an output: the third piece of its terms (2^-17
+  // of them) is below what a state keeps that only enters products.
+  const bool exact = STATE || (c.final && seg == p.segments - 1);
   float whole = 1.f;  // the segment's decay of its entry state, -1 once a reset dropped it
   int r0 = first, it = 0;
   uint64_t cut = 0;   // the chunk's steps that drop the state
@@ -463,8 +477,8 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
         const int pair_byte = l16 * 64 + ((g4 ^ (l16 >> 2)) << 4);
 #pragma unroll 1
         for (int idx = wave; idx < QT * (QT + 1) / 2; idx += W) {
-          const int qt = QT == 2 ? (idx > 0) : (idx > 0) + (idx > 2) + (idx > 5);
-          const int kt = idx - qt * (qt + 1) / 2;
+          // (0, 0), (1, 0), (1, 1), ..: two bits a tile
+          const int qt = 0xffa94u >> (2 * idx) & 3, kt = 0xe4910u >> (2 * idx) & 3;
           floatx4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
@@ -529,11 +543,11 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
         const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;
         const GlobalOut low = (GlobalOut)uniform(static_cast<const char*>(c.out) +
                                                  (base_o + (back ? len - r0 - n : r0) * (int64_t)pitch_o) * size);
+        uint32_t byte = (uint32_t)((back ? n - 1 - l16 : l16) * pitch_o + n0) * size;
+        const uint32_t next = (uint32_t)((back ? -16 : 16) * pitch_o * size);
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          const int i = 16 * qt + l16;
-          if (i < n) {
-            const uint32_t byte = (uint32_t)((back ? n - 1 - i : i) * pitch_o + n0) * size;
+        for (int qt = 0; qt < QT; ++qt, byte += next) {
+          if (16 * qt + l16 < n) {
             if (c.wide) store4(low + byte, acc[qt], N - n0, float());
             else store4(low + byte, acc[qt], N - n0, T());
           }
@@ -557,7 +571,7 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
           *reinterpret_cast<floatx4*>(weight + e) =
               *reinterpret_cast<const floatx4*>(weights + 4 * FR * tb + FR * g4 + e);
         Frag w[PIECES];
-        weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb)), weight, w);
+        weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb)), weight, w, exact);
         // (in groups, so that products of one accumulator do not wait for each
         // other and no more operands are ahead than fit)
         constexpr int GROUP = RT < 4 ? RT : 4;
@@ -569,9 +583,11 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
           for (int i = 0; i < GROUP; ++i)
             ya[i] = *reinterpret_cast<const Frag*>(yt + state_byte(state_lane_byte, r4 + i, tb, T()));
 #pragma unroll
-          for (int q = PIECES - 1; q >= 0; --q)
+          for (int q = PIECES - 1; q >= 0; --q) {
+            if (q == 2 && !exact) continue;
 #pragma unroll
             for (int i = 0; i < GROUP; ++i) S[r4 + i] = Type<T>::mma(ya[i], w[q], S[r4 + i]);
+          }
         }
       }
     }
