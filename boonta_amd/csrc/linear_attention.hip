@@ -156,6 +156,13 @@ template <int RB> __device__ __forceinline__ int row_byte(int l16, int g4, int t
   return RB == 128 ? tile_byte(lane_byte, tile, kb) : (lane_byte ^ (kb << 6)) + tile * 16 * RB;
 }
 
+// Byte of chunk c of row ROWS group + e there, e < ROWS: the group's own with
+// what e adds to the swizzle.
+template <int RB, int ROWS> __device__ __forceinline__ int rows_byte(int c, int group, int e) {
+  const int first = ROWS * group * RB + ((c ^ row_swizzle<RB>(ROWS * group)) << 4);
+  return (first ^ (row_swizzle<RB>(e) << 4)) + e * RB;
+}
+
 // 16 bytes at a lane's 32-bit offset from an address that is uniform in the
 // wave.  (Opaque, so that the sum stays in the load and each row of a lane
 // costs one register, not an address.)
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
     if (__ballot(is_odd) && lane == 0) odd[it & 1] = 1;
     if constexpr (!STATE) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(xr + (2 * tx + e) * RB + ((dx ^ row_swizzle<RB>(2 * tx + e)) << 4)) = rx[e];
+      for (int e = 0; e < 2; ++e) *reinterpret_cast<uint4*>(xr + rows_byte<RB, 2>(dx, tx, e)) = rx[e];
     }
     const int columns_byte = transposed_byte(dc, tg, T());
     if (second) {
@@ -449,7 +456,7 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
     } else {
       if constexpr (!STATE) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(yr + (4 * tg + e) * RB + ((dc ^ row_swizzle<RB>(4 * tg + e)) << 4)) = ryz[e];
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(yr + rows_byte<RB, 4>(dc, tg, e)) = ryz[e];
       }
       write_transposed(yt, columns_byte, ryz, T());
     }
@@ -645,23 +652,36 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
 
 // The states entering each segment after the first, from what each segment
 // before the last adds from zeros and how it fades what enters it; in place.
-__global__ void __launch_bounds__(256) join_segments_kernel(float* states, const float* factors, const float* carry,
-                                                            int64_t KV, int segs) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
-  if (i >= KV) return;
-  float s = carry ? carry[bh * KV + i] : 0.f;
+// Four neighbouring values a thread (a state's last ones apart).
+__global__ void __launch_bounds__(64) join_segments_kernel(float* states, const float* factors, const float* carry,
+                                                            int KV, int segs) {
+  const int i = (blockIdx.x * 64 + threadIdx.x) * 4, left = KV - i;
+  const int64_t bh = blockIdx.y;
+  if (left <= 0) return;
+  auto load = [&](const float* p) -> floatx4 {
+    if (left >= 4) return *reinterpret_cast<const floatx4_a4*>(p);
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < left; ++e) v[e] = p[e];
+    return v;
+  };
+  floatx4 s = carry ? load(carry + bh * KV + i) : floatx4{0.f, 0.f, 0.f, 0.f};
   float* p = states + bh * segs * KV + i;
   const float* f = factors + bh * segs;
-  for (int k0 = 0; k0 < segs; k0 += 8) {
-    float v[8];
+  constexpr int U = 4;
+  for (int k0 = 0; k0 < segs; k0 += U) {
+    floatx4 v[U];
+    float fade[U];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = p[min(k0 + k, segs - 1) * KV];
+    for (int k = 0; k < U; ++k) {
+      v[k] = load(p + (int64_t)min(k0 + k, segs - 1) * KV);
+      fade[k] = f[min(k0 + k, segs - 1)];
+    }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < U; ++k)
       if (k0 + k < segs) {
-        const float fade = f[k0 + k];
-        s = fade < 0.f ? v[k] : __fmaf_rn(fade, s, v[k]);
-        p[(k0 + k) * KV] = s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = fade[k] < 0.f ? v[k][e] : __fmaf_rn(fade[k], s[e], v[k][e]);
+        store4((GlobalOut)(p + (int64_t)(k0 + k) * KV), s, left, float());
       }
   }
 }
@@ -804,9 +824,9 @@ void states_pass(hipStream_t st, int dtype, AttnArgs a, const Contraction& c, in
   const unsigned grid = (unsigned)((int64_t)batch * a.heads * (a.segments - 1));
   if (dtype == ATTN_F32) launch_width<float, true>(st, a, D, grid);
   else launch_width<uint16_t, true>(st, a, D, grid);
-  const int64_t KV = (int64_t)c.x.width * c.z.width;
-  hipLaunchKernelGGL(join_segments_kernel, dim3((unsigned)ppo::ceil_div64(KV, 256), (unsigned)(batch * a.heads)),
-                     dim3(256), 0, st, c.states, a.factors, c.carry, KV, a.segments - 1);
+  const int KV = c.x.width * c.z.width;
+  hipLaunchKernelGGL(join_segments_kernel, dim3((unsigned)ppo::ceil_div(KV, 256), (unsigned)(batch * a.heads)),
+                     dim3(64), 0, st, c.states, a.factors, c.carry, KV, a.segments - 1);
 }
 
 void outputs_pass(hipStream_t st, int dtype, const AttnArgs& a, int batch) {
