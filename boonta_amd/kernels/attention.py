@@ -32,8 +32,10 @@ _MAX_STRIDE = 1 << 23   # of a step, in elements: the kernels count a chunk's by
 def _on_device(name, *tensors):
     device = tensors[0].device
     for x in tensors:
-        if x is not None and (not x.is_cuda or x.device != device):
+        if x is not None and x.device != device:
             raise TypeError(f"{name} runs on tensors of one device")
+    if device.type != "cuda":
+        raise TypeError(f"{name} runs on device tensors")
     return device
 
 
@@ -42,24 +44,28 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (a build 
 
 def _launch(device, name, *args):
     """Calls an entry point on the device's current stream (the device made current where it is not)."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, _raw_stream(device.index), *args)
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, _raw_stream(index), *args)
     else:
         with torch.cuda.device(device):
-            _lib.call(name, _raw_stream(device.index), *args)
+            _lib.call(name, _raw_stream(index), *args)
 
 
 def _rows(x):
-    """x, or a copy where its columns are not side by side or its rows too far apart."""
+    """x, or a copy where its columns are not side by side or its steps too far apart."""
     st = x.stride()
-    if (st[-1] != 1 and x.shape[-1] > 1) or (x.dim() == 4 and st[1] > _MAX_STRIDE):
+    if (st[-1] != 1 and x.shape[-1] > 1) or (len(st) == 4 and st[1] > _MAX_STRIDE):
         return x.contiguous()
     return x
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (6, 9, 12)}
+
+
 def _strides(*tensors):
     flat = [s for x in tensors for s in x.stride()[:-1]]
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
 
 
 def _ptr(x):
@@ -67,83 +73,90 @@ def _ptr(x):
 
 
 def _check_heads(name, q, k, v, dims):
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"{name} stores float32 or bfloat16, not {q.dtype}")
-    if k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+    dtype, qs, ks = q.dtype, q.shape, k.shape
+    if dtype not in _DTYPES:
+        raise TypeError(f"{name} stores float32 or bfloat16, not {dtype}")
+    if k.dtype != dtype or (v is not None and v.dtype != dtype):
         raise TypeError("q, k and v must share one dtype" if v is not None else "q and k must share one dtype")
     lead = dims - 2
-    ok = q.dim() == dims and k.dim() == dims and k.shape[:lead] == q.shape[:lead] and k.shape[-1] == q.shape[-1]
-    if v is not None:
-        ok = ok and v.dim() == dims and v.shape[:-1] == k.shape[:-1]
-    if not ok:
+    if (len(qs) != dims or len(ks) != dims or ks[:lead] != qs[:lead] or ks[-1] != qs[-1]
+            or (v is not None and (v.dim() != dims or v.shape[:-1] != ks[:-1]))):
         shapes = ", ".join(str(tuple(x.shape)) for x in (q, k, v) if x is not None)
         raise ValueError(f"need q [{'batch, steps' if dims == 4 else 'batch'}, heads, width], k (and v) of the same "
                          f"batch{' and steps' if dims == 4 else ''} with heads that divide q's; got {shapes}")
+    return qs, ks
+
+
+_max_width = 0
 
 
 def _check_attention(name, q, k, v, log_decay, carry, done, dims):
-    _check_heads(name, q, k, v, dims)
-    heads, kv_heads = q.shape[-2], k.shape[-2]
+    """The sizes (batch, steps or 1, heads, key heads, key and value width)."""
+    global _max_width
+    _max_width = _max_width or _lib.load().ppo_linear_attention_max_width()
+    qs, ks = _check_heads(name, q, k, v, dims)
+    batch, heads, kv_heads, key, value = qs[0], qs[-2], ks[-2], qs[-1], v.shape[-1]
     if (kv_heads == 0) != (heads == 0) or (heads and heads % kv_heads):
         raise ValueError(f"{heads} heads do not share {kv_heads} key heads evenly")
-    limit = _lib.load().ppo_linear_attention_max_width()
-    if not (0 < q.shape[-1] <= limit and 0 < v.shape[-1] <= limit):
-        raise ValueError(f"{name} takes widths from 1 up to {limit}, not {q.shape[-1]} and {v.shape[-1]}")
-    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (heads,):
+    if not (0 < key <= _max_width and 0 < value <= _max_width):
+        raise ValueError(f"{name} takes widths from 1 up to {_max_width}, not {key} and {value}")
+    if log_decay.dtype != torch.float32 or log_decay.shape != (heads,):
         raise ValueError(f"log_decay must be float32 [{heads}], got {log_decay.dtype} {tuple(log_decay.shape)}")
     if log_decay.requires_grad:
         raise ValueError("log_decay is a fixed schedule: it gets no gradient, pass it detached")
-    shape = (q.shape[0], heads, q.shape[-1], v.shape[-1])
-    if carry is not None and (carry.dtype != torch.float32 or tuple(carry.shape) != shape):
-        raise ValueError(f"carry must be float32 {shape}, got {carry.dtype} {tuple(carry.shape)}")
-    if done is not None and (done.dtype != torch.bool or done.shape != q.shape[:dims - 2]):
-        raise ValueError(f"done must be bool {tuple(q.shape[:dims - 2])}, got {done.dtype} {tuple(done.shape)}")
+    if carry is not None and (carry.dtype != torch.float32 or carry.shape != (batch, heads, key, value)):
+        raise ValueError(f"carry must be float32 {(batch, heads, key, value)}, got {carry.dtype} {tuple(carry.shape)}")
+    if done is not None and (done.dtype != torch.bool or done.shape != qs[:dims - 2]):
+        raise ValueError(f"done must be bool {tuple(qs[:dims - 2])}, got {done.dtype} {tuple(done.shape)}")
+    return batch, qs[1] if dims == 4 else 1, heads, kv_heads, key, value
 
 
 # --------------------------------------------------------------------- sequences
-def _forward(q, k, v, log_decay, carry, done, lengths, scale):
-    batch, steps, heads, key = q.shape
-    kv_heads, value = v.shape[-2:]
-    device, dt = q.device, _DTYPES[q.dtype]
-    out = torch.empty((batch, steps, heads, value), dtype=q.dtype, device=device)
+def _forward(q, k, v, log_decay, carry, done, lengths, scale, sizes):
+    batch, steps, heads, kv_heads, key, value = sizes
+    device, dtype = q.device, q.dtype
+    dt = _DTYPES[dtype]
+    out = torch.empty((batch, steps, heads, value), dtype=dtype, device=device)
     final = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
     nbytes = _lib.load().ppo_linear_attention_workspace(dt, batch, steps, heads, key, value)
     states = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
     _launch(device, "ppo_linear_attention_fwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
             log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), scale, out.data_ptr(), final.data_ptr(),
-            _ptr(states), nbytes, batch, steps, heads, kv_heads, key, value)
+            _ptr(states), nbytes, *sizes)
     return final, out, states
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, carry, done, lengths, scale):
-        final, out, states = _forward(q, k, v, log_decay, carry, done, lengths, scale)
+    def forward(ctx, q, k, v, log_decay, carry, done, lengths, scale, sizes):
+        final, out, states = _forward(q, k, v, log_decay, carry, done, lengths, scale, sizes)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, v, log_decay, carry, done, lengths, states)
-        ctx.scale = scale
+        ctx.scale, ctx.sizes = scale, sizes
         return final, out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dfinal, dout):
         q, k, v, log_decay, carry, done, lengths, states = ctx.saved_tensors
-        batch, steps, heads, key = q.shape
-        kv_heads, value = v.shape[-2:]
-        device, dt = q.device, _DTYPES[q.dtype]
+        batch, steps, heads, kv_heads, key, value = ctx.sizes
+        device, dtype = q.device, q.dtype
+        dt = _DTYPES[dtype]
         if dout is None:   # (only the final carry was used)
-            dout = torch.zeros(value, dtype=q.dtype, device=device).expand(batch, steps, heads, value)
+            dout = torch.zeros(value, dtype=dtype, device=device).expand(batch, steps, heads, value)
         dout = _rows(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+        dq = torch.empty((batch, steps, heads, key), dtype=dtype, device=device)
+        dk = torch.empty((batch, steps, kv_heads, key), dtype=dtype, device=device)
+        dv = torch.empty((batch, steps, kv_heads, value), dtype=dtype, device=device)
         dcarry = torch.empty_like(carry) if carry is not None and ctx.needs_input_grad[4] else None
         nbytes = _lib.load().ppo_linear_attention_bwd_workspace(dt, batch, steps, heads, kv_heads, key, value)
         work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
         _launch(device, "ppo_linear_attention_bwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
                 _strides(q, k, v, dout), log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), ctx.scale,
                 _ptr(dfinal), _ptr(states), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dcarry), _ptr(work),
-                nbytes, batch, steps, heads, kv_heads, key, value)
-        return dq, dk, dv, None, dcarry, None, None, None
+                nbytes, *ctx.sizes)
+        return dq, dk, dv, None, dcarry, None, None, None, None
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -164,11 +177,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     its outputs and gradients are zeros.  scale: key ** -0.5 by default.
     Widths up to 128.  A step's infinities and NaN reach the outputs that the
     recurrence gives them to, and no others."""
-    _check_attention("linear_attention", q, k, v, log_decay, carry, done, 4)
-    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],)):
-        raise ValueError(f"lengths must be int32 [{q.shape[0]}], got {lengths.dtype} {tuple(lengths.shape)}")
+    sizes = _check_attention("linear_attention", q, k, v, log_decay, carry, done, 4)
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != sizes[:1]):
+        raise ValueError(f"lengths must be int32 [{sizes[0]}], got {lengths.dtype} {tuple(lengths.shape)}")
     _on_device("linear_attention", q, k, v, log_decay, carry, done, lengths)
-    key, value = q.shape[-1], v.shape[-1]
+    key, value = sizes[4:]
     scale = key ** -0.5 if scale is None else float(scale)
     least = 16 // q.element_size()
     if key < least or value < least:   # the kernels read rows 16 bytes at a time
@@ -177,12 +190,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         carry = None if carry is None else pad(carry, (0, more_v, 0, more_k))
         carry, out = linear_attention(q, k, v, log_decay, carry, done, lengths, scale)
         return carry[..., :key, :value].contiguous(), out[..., :value].contiguous()
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-    carry, done, lengths = (None if x is None else x.contiguous() for x in (carry, done, lengths))
+    args = (_rows(q), _rows(k), _rows(v), log_decay.contiguous(), None if carry is None else carry.contiguous(),
+            None if done is None else done.contiguous(), None if lengths is None else lengths.contiguous(), scale, sizes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (carry is not None and carry.requires_grad)):
-        return _LinearAttention.apply(q, k, v, log_decay, carry, done, lengths, scale)
-    return _forward(q, k, v, log_decay, carry, done, lengths, scale)[:2]
+        return _LinearAttention.apply(*args)
+    return _forward(*args)[:2]
 
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -192,20 +205,19 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     q [batch, heads, key], k and v [batch, kv_heads, width], done [batch].  The new
     carry is written to ``out_carry`` where given (``carry`` itself: in place).
     Without gradients: a step that needs them is a sequence of one."""
-    _check_attention("linear_attention_step", q, k, v, log_decay, carry, done, 3)
+    batch, _, *sizes = _check_attention("linear_attention_step", q, k, v, log_decay, carry, done, 3)
+    heads, kv_heads, key, value = sizes
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or carry.requires_grad):
         raise ValueError("linear_attention_step has no gradients: use linear_attention on a sequence of one step")
     if out_carry is not None and (out_carry.dtype != torch.float32 or out_carry.shape != carry.shape
                                   or not out_carry.is_contiguous()):
         raise ValueError(f"out_carry must be contiguous float32 {tuple(carry.shape)}")
     device = _on_device("linear_attention_step", q, k, v, log_decay, carry, done, out_carry)
-    batch, heads, key = q.shape
-    kv_heads, value = v.shape[-2:]
     scale = key ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay, carry = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), carry.contiguous()
     done = None if done is None else done.contiguous()
     if out_carry is None:
-        out_carry = torch.empty(carry.shape, dtype=torch.float32, device=device)
+        out_carry = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
     out = torch.empty((batch, heads, value), dtype=q.dtype, device=device)
     _launch(device, "ppo_linear_attention_step", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
             _strides(q, k, v), log_decay.data_ptr(), _ptr(done), carry.data_ptr(), out_carry.data_ptr(),
@@ -262,6 +274,9 @@ class _QKNormRotary(torch.autograd.Function):
         return dq, dk, dq_scale, dk_scale, None, None, None, None
 
 
+_max_norm_width = 0
+
+
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_scale: torch.Tensor | None = None,
                    k_scale: torch.Tensor | None = None, frequencies: torch.Tensor | None = None,
                    positions: torch.Tensor | None = None, epsilon: float = 1e-6,
@@ -273,13 +288,14 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_scale: torch.Tensor | Non
     P), or interleaved (2 i, 2 i + 1), for the P frequencies (float64 [P],
     radians; None: no rotation).  positions: int32 [batch, steps]; None: the step.
     Widths up to 256.  Gradients reach q, k and the scales."""
-    _check_heads("qk_norm_rotary", q, k, None, 4)
-    width = q.shape[-1]
-    limit = _lib.load().ppo_qk_norm_rotary_max_width()
-    if width > limit:
-        raise ValueError(f"qk_norm_rotary takes widths up to {limit}, not {width}")
+    global _max_norm_width
+    _max_norm_width = _max_norm_width or _lib.load().ppo_qk_norm_rotary_max_width()
+    qs, _ = _check_heads("qk_norm_rotary", q, k, None, 4)
+    width = qs[3]
+    if width > _max_norm_width:
+        raise ValueError(f"qk_norm_rotary takes widths up to {_max_norm_width}, not {width}")
     for name, x in (("q_scale", q_scale), ("k_scale", k_scale)):
-        if x is not None and (x.dtype != torch.float32 or tuple(x.shape) != (width,)):
+        if x is not None and (x.dtype != torch.float32 or x.shape != (width,)):
             raise ValueError(f"{name} must be float32 [{width}], got {x.dtype} {tuple(x.shape)}")
     if frequencies is not None:
         if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or 2 * frequencies.numel() > width:
@@ -288,8 +304,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_scale: torch.Tensor | Non
         if frequencies.requires_grad:
             raise ValueError("frequencies get no gradient: pass them detached")
         frequencies = frequencies.contiguous() if frequencies.numel() else None
-    if positions is not None and (positions.dtype != torch.int32 or positions.shape != q.shape[:2]):
-        raise ValueError(f"positions must be int32 {tuple(q.shape[:2])}, got {positions.dtype} "
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != qs[:2]):
+        raise ValueError(f"positions must be int32 {tuple(qs[:2])}, got {positions.dtype} "
                          f"{tuple(positions.shape)}")
     _on_device("qk_norm_rotary", q, k, q_scale, k_scale, frequencies, positions)
     q, k = _rows(q), _rows(k)
