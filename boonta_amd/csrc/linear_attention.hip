@@ -146,14 +146,18 @@ __device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, uint16_
 }
 __device__ __forceinline__ int state_byte(int lane_byte, int rt, int tb, float) { return tile_byte(lane_byte, rt, tb); }
 
-// The same in a tile of rows of RB bytes: the XOR of row r's chunks, and the
-// byte of an operand (row 16 tile + l16, chunk 4 kb + g4).
+// The same in a tile of rows of RB bytes, which repeat their banks every 1, 2
+// or 4 rows: the XOR of row r's chunks, and the byte of an operand (row 16
+// tile + l16, chunk 4 kb + g4).
 template <int RB> __device__ __forceinline__ int row_swizzle(int r) {
-  return RB >= 256 ? r & 15 : RB == 128 ? swizzle(r) : (r >> 2) & 3;
+  return RB % 256 == 0 ? r & 15 : RB % 128 == 0 ? swizzle(r) : (r >> 2) & 3;
 }
 template <int RB> __device__ __forceinline__ int row_byte(int l16, int g4, int tile, int kb) {
   const int lane_byte = l16 * RB + ((g4 ^ row_swizzle<RB>(l16)) << 4);
-  return RB == 128 ? tile_byte(lane_byte, tile, kb) : (lane_byte ^ (kb << 6)) + tile * 16 * RB;
+  const int at = tile * 16 * RB;
+  if (RB % 256 == 0) return (lane_byte ^ ((kb & 3) << 6)) + (kb >> 2) * 256 + at;
+  if (RB % 128 == 0) return (lane_byte ^ (((4 * (kb & 1)) ^ (2 * (tile & 3))) << 4)) + (kb >> 1) * 128 + at;
+  return lane_byte + kb * 64 + at;
 }
 
 // Byte of chunk c of row ROWS group + e there, e < ROWS: the group's own with
@@ -288,7 +292,7 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // columns (y, z: contractions over steps).  STATE: only the state, from zeros,
 // for the segments before the last.
 template <typename T, int D, bool STATE>
-__global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
   constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
   constexpr int PIECES = Type<T>::PIECES;
@@ -391,9 +395,9 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
   };
   int cut_next = 0;
   auto fetch_all = [&](int r0, int tid) {
-    const int unit = tid & (2 * D - 1);
-    if constexpr (!STATE) fetch(rx, c.x, xp, r0, tid % (D / FR), 2 * (tid / (D / FR)));
-    fetch(ryz, oyz, yzp, r0, unit % (D / FR), 4 * (unit / (D / FR)));
+    const uint32_t unit = second ? tid - 2 * D : tid, chunks = D / FR;
+    if constexpr (!STATE) fetch(rx, c.x, xp, r0, (uint32_t)tid % chunks, 2 * ((uint32_t)tid / chunks));
+    fetch(ryz, oyz, yzp, r0, unit % chunks, 4 * (unit / chunks));
     cut_next = fetch_done(r0, tid & 63);
   };
   if (first < last) fetch_all(first, tid);
@@ -435,8 +439,8 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
   // are formed in every chunk: kept, they would spill.)
   auto stage = [&](int n) -> bool {
     const int tid = here(threadIdx.x), lane = tid & 63;
-    const int unit = tid & (2 * D - 1), dc = unit % (D / FR), tg = unit / (D / FR);
-    const int dx = tid % (D / FR), tx = tid / (D / FR);
+    const uint32_t unit = second ? tid - 2 * D : tid, chunks = D / FR;
+    const int dc = unit % chunks, tg = unit / chunks, dx = (uint32_t)tid % chunks, tx = (uint32_t)tid / chunks;
     // a backward sequence's first step takes the state as it is
     const int skip = back && r0 == 0 ? 1 : 0;
     cut = __ballot(cut_next != 0 && lane < n);
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(4 * D, D == 32 ? 3 : 4) attention_kernel(AttnA
         weigh(*reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb)), weight, w, exact);
         // (in groups, so that products of one accumulator do not wait for each
         // other and no more operands are ahead than fit)
-        constexpr int GROUP = RT < 4 ? RT : 4;
+        constexpr int GROUP = RT % 4 == 0 ? 4 : RT % 3 == 0 ? 3 : 2;
 #pragma unroll
         for (int r4 = 0; r4 < RT; r4 += GROUP) {
           if (D == 128) __builtin_amdgcn_sched_barrier(0);
@@ -689,12 +693,12 @@ __global__ void __launch_bounds__(64) join_segments_kernel(float* states, const 
 // Gradients of heads that `group` query heads share: their sum.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* x, T* out, int64_t n, int width, int group) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const float* p = x + i / width * width * group + i % width;
-  float s = 0.f;
-  for (int j = 0; j < group; ++j) s += p[(int64_t)j * width];
-  store1(out + i, s);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const float* p = x + i / width * width * group + i % width;
+    float s = 0.f;
+    for (int j = 0; j < group; ++j) s += p[(int64_t)j * width];
+    store1(out + i, s);
+  }
 }
 
 // ---- one step
@@ -791,7 +795,7 @@ constexpr int MAX_WIDTH = 128;
 
 int padded(int K, int V) {
   const int w = std::max(K, V);
-  return w <= 32 ? 32 : w <= 64 ? 64 : 128;
+  return w <= 32 ? 32 : w <= 64 ? 64 : w <= 96 ? 96 : 128;
 }
 
 int chunk(int dtype) { return dtype == ATTN_F32 ? 32 : 64; }
@@ -811,6 +815,7 @@ template <typename T, bool STATE>
 void launch_width(hipStream_t st, const AttnArgs& a, int D, unsigned grid) {
   if (D == 32) hipLaunchKernelGGL((attention_kernel<T, 32, STATE>), dim3(grid), dim3(128), 0, st, a);
   else if (D == 64) hipLaunchKernelGGL((attention_kernel<T, 64, STATE>), dim3(grid), dim3(256), 0, st, a);
+  else if (D == 96) hipLaunchKernelGGL((attention_kernel<T, 96, STATE>), dim3(grid), dim3(384), 0, st, a);
   else hipLaunchKernelGGL((attention_kernel<T, 128, STATE>), dim3(grid), dim3(512), 0, st, a);
 }
 
@@ -848,9 +853,12 @@ int check_sizes(const char* what, int dtype, int batch, int steps, int heads, in
     return ppo::set_error(PPO_ERR_ARG, "%s: %d heads do not share %d key heads evenly", what, heads, kv_heads);
   if (heads > (1 << 23) / MAX_WIDTH)  // an output step's elements, as check_strides
     return ppo::set_error(PPO_ERR_ARG, "%s: %d heads above %d", what, heads, (1 << 23) / MAX_WIDTH);
-  // the grid: four workgroups a head at most (four slices of a step, three outputs of the backward pass)
-  if ((int64_t)batch * heads > (1 << 29) - 1)
-    return ppo::set_error(PPO_ERR_ARG, "%s: batch x heads above %d", what, (1 << 29) - 1);
+  // a launch's threads (three outputs of the backward pass, 512 each; two slices of a step, 256 each) are
+  // counted in 32 bits
+  const int64_t most = least > 1 ? 1 << 21 : (1 << 23) - 1;
+  if ((int64_t)batch * heads > most)
+    return ppo::set_error(PPO_ERR_ARG, "%s: batch x heads above %lld", what, (long long)most);
+  if (steps > 1 << 30) return ppo::set_error(PPO_ERR_ARG, "%s: %d steps above 2^30", what, steps);
   return PPO_OK;
 }
 
@@ -1020,7 +1028,7 @@ PPO_EXPORT int ppo_linear_attention_bwd(void* stream, int dtype, const void* q, 
       const int64_t n = rows * width;
       const float* src = i ? wide_v : wide_k;
       void* dst = i ? dv : dk;
-      const dim3 grid((unsigned)ppo::ceil_div64(n, 256));
+      const dim3 grid((unsigned)std::min<int64_t>(1 << 16, ppo::ceil_div64(n, 256)));
       if (dtype == ATTN_F32)
         hipLaunchKernelGGL((sum_heads_kernel<float>), grid, dim3(256), 0, ppo::as_stream(stream), src,
                            static_cast<float*>(dst), n, width, group);

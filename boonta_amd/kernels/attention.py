@@ -210,14 +210,16 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or carry.requires_grad):
         raise ValueError("linear_attention_step has no gradients: use linear_attention on a sequence of one step")
     if out_carry is not None and (out_carry.dtype != torch.float32 or out_carry.shape != carry.shape
-                                  or not out_carry.is_contiguous()):
-        raise ValueError(f"out_carry must be contiguous float32 {tuple(carry.shape)}")
+                                  or not out_carry.is_contiguous() or out_carry.requires_grad):
+        raise ValueError(f"out_carry must be contiguous float32 {tuple(carry.shape)} that needs no gradient")
     device = _on_device("linear_attention_step", q, k, v, log_decay, carry, done, out_carry)
     scale = key ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay, carry = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), carry.contiguous()
     done = None if done is None else done.contiguous()
     if out_carry is None:
         out_carry = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
+    else:
+        torch.autograd.graph.increment_version(out_carry)   # (written in place)
     out = torch.empty((batch, heads, value), dtype=q.dtype, device=device)
     _launch(device, "ppo_linear_attention_step", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
             _strides(q, k, v), log_decay.data_ptr(), _ptr(done), carry.data_ptr(), out_carry.data_ptr(),

@@ -50,6 +50,7 @@ def test_linear_attention_step_refuses_what_it_does_not_take():
     refused(ValueError, "done", linear_attention_step, q, k, v, g, carry, torch.zeros(2, 1).bool())
     refused(ValueError, "no gradients", linear_attention_step, q, k, v, g, carry.clone().requires_grad_())
     refused(ValueError, "out_carry", linear_attention_step, q, k, v, g, carry, out_carry=carry.transpose(2, 3))
+    refused(ValueError, "no gradient", linear_attention_step, q, k, v, g, carry, out_carry=carry.clone().requires_grad_())
 
 
 def test_qk_norm_rotary_refuses_what_it_does_not_take():
@@ -92,6 +93,8 @@ def test_the_entry_points_refuse_without_launching():
     assert forward(sizes=(-1, 4, 2, 2, 8, 8)) == -1
     assert forward(sizes=(1 << 30, 4, 2, 2, 8, 8)) == -1
     assert forward(sizes=(0, 4, 2, 2, 8, 8)) == 0
+    assert forward(sizes=(1 << 21, 4, 2, 2, 8, 8)) == -1 and b"batch x heads" in lib.ppo_last_error()
+    assert forward(sizes=(1, (1 << 30) + 1, 2, 2, 8, 8)) == -1 and b"steps" in lib.ppo_last_error()
     far = (ctypes.c_int64 * 12)(0, 1 << 24, 0, *[0] * 9)
     assert forward(strides=far) == -1 and b"step stride" in lib.ppo_last_error()
     long = (1, 1 << 16, 2, 2, 8, 8)
@@ -106,6 +109,7 @@ def test_the_entry_points_refuse_without_launching():
     step = lib.ppo_linear_attention_step
     assert step(None, 0, 1, 1, 1, st, 1, None, None, 1, 1, 1.0, 2, 2, 2, 8, 8) == -1
     assert step(None, 0, 1, 1, 1, st, 1, None, 1, 1, 1, 1.0, 2, 3, 2, 8, 8) == -1
+    assert step(None, 0, 1, 1, 1, st, 1, None, 1, 1, 1, 1.0, 1 << 23, 1, 1, 8, 8) == -1
     norm = lib.ppo_qk_norm_rotary_fwd
     assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 2, 3, 4, 4, 8, 5) == -1   # 5 pairs of 8
     assert norm(None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, 2, 3, 4, 4, 8, 4) == -1   # no frequencies

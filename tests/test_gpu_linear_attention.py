@@ -102,7 +102,7 @@ def check(q, k, v, g, carry, done, lengths, seed=0, scale=None):
 SHAPES = [  # batch, steps, heads, key heads, widths
     (1, 1, 1, 1, 1, 1), (2, 3, 2, 1, 5, 7), (1, 15, 3, 3, 16, 16), (2, 31, 2, 2, 32, 32), (1, 33, 2, 2, 33, 20),
     (2, 64, 4, 4, 64, 64), (1, 65, 4, 2, 64, 48), (3, 127, 2, 2, 8, 64), (1, 130, 2, 1, 128, 128), (2, 70, 1, 1, 100, 77),
-    (2, 200, 6, 2, 24, 40),
+    (2, 200, 6, 2, 24, 40), (2, 150, 2, 1, 96, 96), (1, 90, 3, 3, 80, 65),
 ]
 
 
@@ -124,7 +124,8 @@ def test_resets_lengths_and_strides(shape, done, ragged, carry, packed, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("shape,done,ragged", [((1, 1100, 1, 1, 24, 40), 0.0, False), ((2, 1300, 2, 1, 64, 64), 0.002, True),
-                                               ((1, 1500, 1, 1, 128, 128), 0.001, False)])
+                                               ((1, 1500, 1, 1, 128, 128), 0.001, False),
+                                               ((2, 1100, 2, 2, 96, 72), 0.002, True)])
 def test_long_sequences_are_cut_into_segments(shape, done, ragged, dtype):
     ops = problem(sum(shape), *shape, dtype, done=done, ragged=ragged, slow=True)
     check(*ops, seed=1)
