@@ -400,7 +400,9 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
     fetch(ryz, oyz, yzp, r0, unit % chunks, 4 * (unit / chunks));
     cut_next = fetch_done(r0, tid & 63);
   };
-  if (first < last) fetch_all(first, tid);
+  // (STATE goes from the segment's last chunk to its first)
+  int r0 = STATE && first < last ? first + (last - first - 1) / C * C : first, it = 0;
+  if (first < last) fetch_all(r0, tid);
 
   // the state entering the segment: rows 16 rt + 4 g4 + e of column col
   floatx4 S[RT];
@@ -431,13 +433,11 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
   // Whether the state itself is an output: the third piece of its terms (2^-17
   // of them) is below what a state keeps that only enters products.
   const bool exact = STATE || (c.final && seg == p.segments - 1);
-  float whole = 1.f;  // the segment's decay of its entry state, -1 once a reset dropped it
-  int r0 = first, it = 0;
   uint64_t cut = 0;   // the chunk's steps that drop the state
-  // Lays out steps r0 .. r0 + n - 1, as loaded, and loads those after them.
+  // Lays out steps r0 .. r0 + n - 1, as loaded, and loads the chunk from `next` (>= 0) on.
   // Whether y or z holds an infinity or NaN.  (Here and below a lane's places
   // are formed in every chunk: kept, they would spill.)
-  auto stage = [&](int n) -> bool {
+  auto stage = [&](int n, int next) -> bool {
     const int tid = here(threadIdx.x), lane = tid & 63;
     const uint32_t unit = second ? tid - 2 * D : tid, chunks = D / FR;
     const int dc = unit % chunks, tg = unit / chunks, dx = (uint32_t)tid % chunks, tx = (uint32_t)tid / chunks;
@@ -466,10 +466,11 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
     }
     if (wave == 0 && lane < C) {
       const int last_cut = cut ? 63 - __clzll(cut) : -1;
-      weights[lane] = lane < n && lane >= last_cut ? c.update * power(g2, n - 1 - lane) : 0.f;
-      reaches[lane] = (cut & (~0ull >> (63 - lane))) == 0 ? c.inter * power(g2, lane + 1 - skip) : 0.f;
+      const int left = (STATE ? last - r0 : n) - 1 - lane;
+      weights[lane] = lane < n && lane >= last_cut ? c.update * power(g2, left) : 0.f;
+      if (!STATE) reaches[lane] = (cut & (~0ull >> (63 - lane))) == 0 ? c.inter * power(g2, lane + 1 - skip) : 0.f;
     }
-    if (r0 + n < last) fetch_all(r0 + n, tid);
+    if (next >= 0) fetch_all(next, tid);
     lds_barrier();
     const bool is_bad = __builtin_amdgcn_readfirstlane(odd[it & 1]);
     if (tid == 0) odd[(it + 1) & 1] = 0;
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
   auto chunk = [&](int n) {
     const int tid = here(threadIdx.x), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
     const int skip = back && r0 == 0 ? 1 : 0;
-    const float fade = same(power(g2, n - skip));
+    const float fade = STATE ? 1.f : same(power(g2, n - skip));
     const int lane_byte = l16 * 128 + ((g4 ^ swizzle(l16)) << 4);
     {
       if constexpr (!STATE) {
@@ -564,16 +565,19 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
           }
         }
       }
-      // state: its rows by y's columns, contracted over the steps
+      // state: its rows by y's columns, contracted over the steps (from zeros
+      // every step's weight is that at the segment's end)
       const int slot_row = Type<T>::row(0, l16), state_lane_byte = slot_row * 128 + ((g4 ^ swizzle(slot_row)) << 4);
-      if (cut) {
+      if constexpr (!STATE) {
+        if (cut) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
+          for (int rt = 0; rt < RT; ++rt) S[rt] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[rt][e] *= fade;
       }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[rt][e] *= fade;
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb) {
         float weight[FR];
@@ -603,41 +607,81 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
       }
     }
     lds_barrier();
-    whole = cut || whole < 0.f ? -1.f : whole * fade;
-    r0 += n;
   };
-  while (r0 < last) {
-    bool is_bad = false;
+  // The products multiply a masked pair by zero, which an infinity or NaN in y or
+  // z outlasts: the steps of such a chunk are taken one by one.  (Padding stays
+  // zero: a zero times an infinity is none.)
+  auto clear_padding = [&]() {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (Type<T>::row(rt, 4 * g4 + e) >= R) S[rt][e] = 0.f;
+  };
+  if constexpr (!STATE) {
     while (r0 < last) {
-      const int n = min(C, last - r0);
-      is_bad = stage(n);
-      if (__builtin_expect(is_bad, 0)) break;
-      chunk(n);
-    }
-    if (__builtin_expect(is_bad, 0)) {
-      // The products multiply a masked pair by zero, which an infinity or NaN in
-      // y or z outlasts: such a chunk's steps are taken one by one.
-      const int end = min(last, r0 + C);
+      bool is_bad = false;
+      while (r0 < last) {
+        const int n = min(C, last - r0);
+        is_bad = stage(n, r0 + n < last ? r0 + n : -1);
+        if (__builtin_expect(is_bad, 0)) break;
+        chunk(n);
+        r0 += n;
+      }
+      if (__builtin_expect(is_bad, 0)) {
+        const int end = min(last, r0 + C);
 #pragma unroll 1
-      while (r0 < end) {
-        lds_barrier();
-        fetch_all(r0, tid);
-        stage(1);
-        chunk(1);
-        // (padding stays zero: a zero times an infinity is none)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (Type<T>::row(rt, 4 * g4 + e) >= R) S[rt][e] = 0.f;
+        while (r0 < end) {
+          lds_barrier();
+          fetch_all(r0, tid);
+          stage(1, r0 + 1 < last ? r0 + 1 : -1);
+          chunk(1);
+          r0 += 1;
+          clear_padding();
+        }
       }
     }
+  } else {
+    // From the segment's last chunk to its first, or to the last reset: what is
+    // before it reaches no state after the segment.  (And what the outputs'
+    // launch reads first is what this one read last.)
+    bool reset = false;
+    while (r0 >= first && first < last && !reset) {
+      bool is_bad = false;
+      while (r0 >= first && !reset) {
+        const int n = min(C, last - r0);
+        is_bad = stage(n, r0 > first ? r0 - C : -1);
+        if (__builtin_expect(is_bad, 0)) break;
+        chunk(n);
+        reset = cut != 0;
+        r0 -= C;
+      }
+      if (__builtin_expect(is_bad, 0)) {
+        const int low = r0;
+        r0 = min(low + C, last);
+#pragma unroll 1
+        while (r0 > low && !reset) {
+          lds_barrier();
+          r0 -= 1;
+          fetch_all(r0, tid);
+          stage(1, -1);
+          chunk(1);
+          reset = cut != 0;
+          clear_padding();
+        }
+        r0 = low - C;
+        lds_barrier();
+        if (r0 >= first) fetch_all(r0, tid);
+      }
+    }
+    if (tid == 0)
+      p.factors[bh * (p.segments - 1) + seg] =
+          reset ? -1.f : power(g2, max(last - first, 0) - (back && first == 0 && last > 0 ? 1 : 0));
   }
 
   float* exit = STATE ? c.states + (bh * (p.segments - 1) + seg) * KV
                       : (c.final && seg == p.segments - 1 ? c.final + bh * KV : nullptr);
   if (!exit) return;
-  if (STATE && tid == 0) p.factors[bh * (p.segments - 1) + seg] = whole;
   // the cotangent of the state before the first step
   float f = 1.f;
   bool drop = false;

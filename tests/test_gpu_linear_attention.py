@@ -198,6 +198,31 @@ def test_a_bad_step_reaches_its_own_future_only(where, bad, dtype):
     assert fine.any()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("reset", [None, 360, 700])
+@pytest.mark.parametrize("bad", [0, 330, 355, 1299])
+def test_a_bad_step_of_a_long_sequence(bad, reset, dtype):
+    """In a segment whose state is formed from its end: finite where the recurrence is, forward and backward."""
+    q, k, v, g, carry, _, _ = problem(17, 1, 1300, 1, 1, 33, 48, dtype, slow=True)
+    done = torch.zeros(1, 1300, dtype=torch.bool, device="cuda")
+    if reset is not None:
+        done[0, reset] = True
+    v[0, bad, 0, 7] = float("nan")
+    got = check_raw(q, k, v, g, carry, done, None)
+    n = [np64(x) for x in (q, k, v, g, carry)]
+    gen = torch.Generator().manual_seed(77)
+    dout = torch.randn(1, 1300, 1, 48, generator=gen).to(dtype).double().numpy()
+    dfinal = torch.randn(1, 1, 33, 48, generator=gen).double().numpy()
+    with np.errstate(invalid="ignore"):
+        want = (*oat.linear_attention(*n, flags(done), None, 33 ** -0.5),
+                *oat.linear_attention_vjp(*n, flags(done), None, 33 ** -0.5, dfinal, dout))
+    for name, a, b in zip(("final", "out", "dq", "dk", "dv", "dcarry"), got, want):
+        fine = np.isfinite(b)
+        assert (np.isfinite(np64(a)) == fine).all(), name
+        a = np64(a)[fine]
+        assert np.linalg.norm(a - b[fine]) <= (1e-5 if dtype == F32 else 2 ** -7) * np.linalg.norm(b[fine]), name
+
+
 def test_a_decay_of_zero_keeps_the_step_alone():
     q, k, v, _, carry, _, _ = problem(9, 1, 50, 2, 2, 16, 16, F32)
     g = torch.tensor([float("-inf"), -200.0], device="cuda")
