@@ -292,7 +292,7 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // columns (y, z: contractions over steps).  STATE: only the state, from zeros,
 // for the segments before the last.
 template <typename T, int D, bool STATE>
-__global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
   constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
   constexpr int PIECES = Type<T>::PIECES;
@@ -431,7 +431,9 @@ __global__ void __launch_bounds__(4 * D, D % 64 == 0 ? 4 : 3) attention_kernel(A
   lds_barrier();
 
   // Whether the state itself is an output: the third piece of its terms (2^-17
-  // of them) is below what a state keeps that only enters products.
+  // of them) is below what a state keeps that only enters products, rounded to
+  // bf16 (2^-8).  With it, 16 heads of 128: 65536 steps 388 -> 406 us, both
+  // passes of 8 x 4096 steps 640 -> 675 us.
   const bool exact = STATE || (c.final && seg == p.segments - 1);
   uint64_t cut = 0;   // the chunk's steps that drop the state
   // Lays out steps r0 .. r0 + n - 1, as loaded, and loads the chunk from `next` (>= 0) on.
@@ -837,6 +839,10 @@ __global__ void __launch_bounds__(256) attention_step_kernel(StepArgs a) {
 // ---- launches
 constexpr int MAX_WIDTH = 128;
 
+// The width of a launch.  96 of its own, batch 8, 4096 steps, 16 heads against
+// padded to 128: bf16 179 us (183) forward and 596 (582) with the backward,
+// batch 2, 512 steps, 4 heads of 80 22.8 us (25.5); float32, 2048 steps, 238 us
+// (304).
 int padded(int K, int V) {
   const int w = std::max(K, V);
   return w <= 32 ? 32 : w <= 64 ? 64 : w <= 96 ? 96 : 128;
@@ -844,17 +850,17 @@ int padded(int K, int V) {
 
 int chunk(int dtype) { return dtype == ATTN_F32 ? 32 : 64; }
 
-// Segments the step axis is cut into: 1024 workgroups of four waves (or their
-// waves' worth) fill the chip, and a segment keeps two chunks or more, since
-// its state is written, joined and read back.  Measured, bf16: against half and
-// twice as many, batch 1, 65536 steps, 16 heads of 128 took 397 us (437, 421)
-// and the both passes of batch 8, 4096 steps, 16 heads of 128 took 620 us
-// (628, 659); against segments of four chunks, batch 4, 2048 steps, 8 heads of
-// 64 went from 31.7 to 28.9 us (47 us with eight).
+// Segments the step axis is cut into: as many workgroups as the chip's 256 CUs
+// hold at a time (16 waves each), while a segment keeps two chunks or more,
+// since its state is written, joined and read back.  Measured, bf16: against
+// half and twice as many, batch 1, 65536 steps, 16 heads of 128 takes 397 us
+// (437, 421) and both passes of batch 8, 4096 steps, 16 heads of 128 take 620
+// us (628, 659); against segments of four chunks, batch 4, 2048 steps, 8 heads
+// of 64 takes 28.9 us (31.7; 47 with eight).
 int segments_of(int dtype, int batch, int steps, int heads, int K, int V) {
   const int64_t pairs = std::max<int64_t>(1, (int64_t)batch * heads);
   const int c = chunk(dtype), D = padded(K, V);
-  const int64_t want = 1024 * 64 / D / pairs, most = ppo::ceil_div(steps, 2 * c);
+  const int64_t want = 256 * (256 / D) / pairs, most = ppo::ceil_div(steps, 2 * c);
   const int segs = (int)std::max<int64_t>(1, std::min(want, most));
   const int seg_steps = ppo::ceil_div(ppo::ceil_div(std::max(steps, 1), segs), c) * c;
   return std::max(1, ppo::ceil_div(steps, seg_steps));
@@ -1102,7 +1108,8 @@ PPO_EXPORT int ppo_linear_attention_step(void* stream, int dtype, const void* q,
   StepArgs a{q, k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], log_decay, done, carry,
              final, out, scale, heads, heads / kv_heads, K, V, 0, 0};
   // a workgroup a head, or slices of at least 32 columns where those are too
-  // few to fill the chip
+  // few to fill the chip (float32 heads of 128 whole / in slices of 32: 32 of
+  // them 6.6 / 4.2 us, 128 of them 7.5 / 5.5, 2048 of them 46.4 / 49.1)
   const int64_t pairs = (int64_t)batch * heads;
   const bool vec = V % 4 == 0;
   int width = V > 64 && vec ? 128 : V > 32 ? 64 : 32;
