@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(THREADS, 2) qk_norm_kernel(NormArgs p) {
       b = b0 + wraps;
       t = x - wraps * p.steps;
     };
-    // row r of part w: step r / heads, head r % heads (r heads < 2^32)
+    // row r of part w: step r / heads, head r % heads (exact: r heads < 2^32)
     auto place = [&](int w, int r, int& s, int& h) {
       s = p.part[w].heads == 1 ? r : (int)__umulhi((uint32_t)r, p.part[w].inverse);
       h = r - s * p.part[w].heads;
@@ -449,22 +449,22 @@ int lanes_log2_of(int D, int v) {
 }
 
 // Steps of a wave's tile: rows of the part with fewer heads for every lane
-// group's loads, no more angles than there is room for, and a tile for every
-// wave where there are few steps.
-int tile_of(int64_t tokens, int heads, int pairs, int lanes_log2) {
-  const int64_t busy = std::max<int64_t>(1, 64 * UNROLL / ((int64_t)std::max(heads, 1) << lanes_log2));
+// group's loads, no more angles than there is room for, a tile for every wave
+// where there are few steps, and rows whose heads a 32-bit product tells.
+int tile_of(int64_t tokens, int heads, int kv_heads, int pairs, int lanes_log2) {
+  const int64_t most = std::max(heads, kv_heads), fewer = heads && kv_heads ? std::min(heads, kv_heads) : most;
+  const int64_t busy = std::max<int64_t>(1, 64 * UNROLL / (fewer << lanes_log2));
   return (int)std::max<int64_t>(1, std::min<int64_t>({busy, TILE_ANGLES / std::max(pairs, 1), TILE_ANGLES,
-                                                      ppo::ceil_div64(tokens, 1024 * WAVES)}));
+                                                      ppo::ceil_div64(tokens, 1024 * WAVES),
+                                                      (1ll << 32) / (most * most) - 1}));
 }
-
-int fewer(int a, int b) { return a && b ? std::min(a, b) : std::max(a, b); }
 
 unsigned blocks_of(int64_t tokens, int tile, int most) {
   return (unsigned)std::min<int64_t>(most, ppo::ceil_div64(tokens, (int64_t)tile * WAVES));
 }
 
 NormArgs common_args(float epsilon, int64_t tokens, int steps, int width, int pairs, int interleaved, int dtype,
-                     int heads, const double* frequencies, const int32_t* positions) {
+                     int heads, int kv_heads, const double* frequencies, const int32_t* positions) {
   NormArgs a{};
   a.frequencies = frequencies;
   a.positions = positions;
@@ -476,7 +476,7 @@ NormArgs common_args(float epsilon, int64_t tokens, int steps, int width, int pa
   a.D = width;
   a.P = pairs;
   a.lanes_log2 = lanes_log2_of(width, chunk_columns(dtype, pairs, interleaved));
-  a.tile = tile_of(tokens, heads, pairs, a.lanes_log2);
+  a.tile = tile_of(tokens, heads, kv_heads, pairs, a.lanes_log2);
   return a;
 }
 
@@ -518,7 +518,7 @@ PPO_EXPORT int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, co
   if (tokens == 0 || heads + kv_heads == 0 || width == 0) return PPO_OK;
   if (!strides || (heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out)) || (pairs > 0 && !frequencies))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
-  NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, fewer(heads, kv_heads),
+  NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, heads, kv_heads,
                            frequencies, positions);
   a.part[0] = Rows{q, nullptr, q_scale, q_out, strides[0], strides[1], strides[2], 0, 0, 0, heads, inverse_of(heads)};
   a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads,
@@ -553,7 +553,7 @@ PPO_EXPORT int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, co
     return ppo::set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   int blocks = 0;
   if (!none) {
-    NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, fewer(heads, kv_heads),
+    NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, heads, kv_heads,
                              frequencies, positions);
     a.part[0] = Rows{q, dq_out, q_scale, dq, strides[0], strides[1], strides[2], strides[6], strides[7], strides[8],
                      heads, inverse_of(heads)};

@@ -126,6 +126,20 @@ def test_many_rows_and_the_same_twice():
         assert np.linalg.norm(np64(runs[0][4 + i]) - dscale) <= 2e-6 * np.linalg.norm(dscale)
 
 
+def test_thousands_of_heads_shared_by_many_steps():
+    """8191 key heads beside one query head, the keys' step stride zero: every
+    step's row of each head is that head's, whatever the rows of a tile."""
+    T, G = 66 * 4096, 8191
+    gen = torch.Generator().manual_seed(8)
+    q = torch.randn(1, T, 1, 1, generator=gen).to(BF16).cuda()
+    k = torch.randn(1, 1, G, 1, generator=gen).to(BF16).cuda()
+    want = (k.float() / (k.float().square() + 1e-6).sqrt())[0, 0]
+    q_out, k_out = qk_norm_rotary(q, k.expand(1, T, G, 1))
+    assert (k_out[0] == k_out[0, :1]).all()
+    assert ((k_out[0, 0].float() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20).all()
+    assert ((q_out[..., 0] > 0) == (q[..., 0] > 0)).all()
+
+
 def test_a_captured_pass_replays():
     sets = [problem(7 + i, 2, 50, 2, 1, 32, F32, False, False) for i in range(3)]
     f = rotary_frequencies(32)
