@@ -919,11 +919,11 @@ int check_sizes(const char* what, int dtype, int batch, int steps, int heads, in
 
 bool empty(int batch, int heads) { return batch == 0 || heads == 0; }
 
-// A lane's byte within a chunk is counted in 32 bits.
-int check_strides(const char* what, const int64_t* strides, int operands) {
+// A lane's byte within a chunk is counted in 32 bits.  (One step has no stride.)
+int check_strides(const char* what, const int64_t* strides, int operands, int steps) {
   for (int i = 0; i < operands; ++i) {
     const int64_t st = strides[3 * i + 1];
-    if (st < 0 || st > 1 << 23)
+    if (steps > 1 && (st < 0 || st > 1 << 23))
       return ppo::set_error(PPO_ERR_ARG, "%s: step stride %lld outside 0 .. %d", what, (long long)st, 1 << 23);
   }
   return PPO_OK;
@@ -984,7 +984,7 @@ PPO_EXPORT int ppo_linear_attention_fwd(void* stream, int dtype, const void* q, 
   if (empty(batch, heads)) return PPO_OK;
   if (!log_decay || !final || !strides || (steps > 0 && (!q || !k || !v || !out)))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
-  if (int rc = check_strides(what, strides, 3)) return rc;
+  if (int rc = check_strides(what, strides, 3, steps)) return rc;
   const int64_t floats = state_floats(dtype, batch, steps, heads, K, V);
   if (floats > 0 && (!workspace || workspace_bytes < sizeof(float) * (size_t)floats))
     return ppo::set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes,
@@ -1021,7 +1021,7 @@ PPO_EXPORT int ppo_linear_attention_bwd(void* stream, int dtype, const void* q, 
   if (empty(batch, heads)) return PPO_OK;
   if (!log_decay || !strides || (steps > 0 && (!q || !k || !v || !dout || !dq || !dk || !dv)))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
-  if (int rc = check_strides(what, strides, 4)) return rc;
+  if (int rc = check_strides(what, strides, 4, steps)) return rc;
   const int64_t floats = state_floats(dtype, batch, steps, heads, K, V);
   const size_t need = ppo_linear_attention_bwd_workspace(dtype, batch, steps, heads, kv_heads, K, V);
   if (need > 0 && (!workspace || workspace_bytes < need))

@@ -55,7 +55,7 @@ def _launch(device, name, *args):
 def _rows(x):
     """x, or a copy where its columns are not side by side or its steps too far apart."""
     st = x.stride()
-    if (st[-1] != 1 and x.shape[-1] > 1) or (len(st) == 4 and st[1] > _MAX_STRIDE):
+    if (st[-1] != 1 and x.shape[-1] > 1) or (len(st) == 4 and st[1] > _MAX_STRIDE and x.shape[1] > 1):
         return x.contiguous()
     return x
 
@@ -203,7 +203,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                           out_carry: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(carry, output [batch, heads, value]) of one step of ``linear_attention``:
     q [batch, heads, key], k and v [batch, kv_heads, width], done [batch].  The new
-    carry is written to ``out_carry`` where given (``carry`` itself: in place).
+    carry is written to ``out_carry`` where given (``carry`` itself: in place; else apart from it).
     Without gradients: a step that needs them is a sequence of one."""
     batch, _, *sizes = _check_attention("linear_attention_step", q, k, v, log_decay, carry, done, 3)
     heads, kv_heads, key, value = sizes
@@ -212,6 +212,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if out_carry is not None and (out_carry.dtype != torch.float32 or out_carry.shape != carry.shape
                                   or not out_carry.is_contiguous() or out_carry.requires_grad):
         raise ValueError(f"out_carry must be contiguous float32 {tuple(carry.shape)} that needs no gradient")
+    if out_carry is not None and 0 < abs(out_carry.data_ptr() - carry.data_ptr()) < 4 * carry.numel():
+        raise ValueError("out_carry must be carry itself or memory apart from it")
     device = _on_device("linear_attention_step", q, k, v, log_decay, carry, done, out_carry)
     scale = key ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay, carry = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), carry.contiguous()

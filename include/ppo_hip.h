@@ -373,8 +373,8 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  *   q [batch, steps, heads, key_width], k [batch, steps, kv_heads, key_width],
  *   v [batch, steps, kv_heads, value_width]: columns side by side, element
  *   strides of (batch, step, head) in the host array `strides`, 3 for each of
- *   q, k, v (and dout in the backward); a step's stride is at most 2^23
- *   and none is negative.
+ *   q, k, v (and dout in the backward); a step's stride (of more than
+ *   one step) is at most 2^23 and none is negative.
  *   heads / kv_heads query heads in a row share a key head.  Widths are at most
  *   ppo_linear_attention_max_width(), and of sequences at least
  *   ppo_linear_attention_min_width(dtype) (16 bytes).

@@ -51,6 +51,9 @@ def test_linear_attention_step_refuses_what_it_does_not_take():
     refused(ValueError, "no gradients", linear_attention_step, q, k, v, g, carry.clone().requires_grad_())
     refused(ValueError, "out_carry", linear_attention_step, q, k, v, g, carry, out_carry=carry.transpose(2, 3))
     refused(ValueError, "no gradient", linear_attention_step, q, k, v, g, carry, out_carry=carry.clone().requires_grad_())
+    whole = torch.zeros(3, 4, 8, 6)
+    refused(ValueError, "apart", linear_attention_step, q, k, v, g, whole[:2], out_carry=whole[1:])
+    refused(TypeError, "device", linear_attention_step, q, k, v, g, whole[:2], out_carry=whole[:2])
 
 
 def test_qk_norm_rotary_refuses_what_it_does_not_take():
@@ -97,6 +100,7 @@ def test_the_entry_points_refuse_without_launching():
     assert forward(sizes=(1, (1 << 30) + 1, 2, 2, 8, 8)) == -1 and b"steps" in lib.ppo_last_error()
     far = (ctypes.c_int64 * 12)(0, 1 << 24, 0, *[0] * 9)
     assert forward(strides=far) == -1 and b"step stride" in lib.ppo_last_error()
+    assert forward(strides=far, sizes=(0, 1, 2, 2, 8, 8)) == 0
     long = (1, 1 << 16, 2, 2, 8, 8)
     need = lib.ppo_linear_attention_workspace(0, *long[:3], 8, 8)
     assert need > 0 and forward(sizes=long) == -3 and forward(sizes=long, work=1, nbytes=need - 1) == -3

@@ -332,6 +332,29 @@ def test_orders_of_axes_and_the_same_twice():
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_one_step_of_a_wide_time_major_batch():
+    """Of one step the step's stride says nothing: here it is that of a whole
+    batch, past what the kernels count in."""
+    B, H, K = 66000, 16, 8
+    gen = torch.Generator().manual_seed(17)
+    ops = [torch.randn(1, B, H, K, generator=gen).to(BF16).cuda().transpose(0, 1).requires_grad_() for _ in range(3)]
+    assert ops[0].stride(1) > 1 << 23
+    g = torch.full((H,), -0.1).cuda()
+    final, out = linear_attention(*ops, g)
+    grads = torch.autograd.grad(out, ops, out.detach())
+    q, k, v = (x.detach()[:, 0].float() for x in ops)
+    w = (q * k).sum(-1, keepdim=True) * K ** -0.5
+    # one product of at most K + 2 float32 roundings of 2^-24, the pair products rounded to bf16, and the outputs
+    close = lambda a, b, terms: ((a[:, 0].float() - b).abs() <= 2.0 ** -8 * b.abs() + 2.0 ** -7 * terms + 1e-30).all()
+    assert close(out, w * v, (q * k).abs().sum(-1, keepdim=True) * K ** -0.5 * v.abs())
+    assert torch.equal(final, k[..., None] * v[..., None, :])
+    do = out.detach()[:, 0].float()
+    assert close(grads[2], w * do, (q * k).abs().sum(-1, keepdim=True) * K ** -0.5 * do.abs())
+    d = (do * v).sum(-1, keepdim=True) * K ** -0.5
+    terms = (do * v).abs().sum(-1, keepdim=True) * K ** -0.5
+    assert close(grads[0], d * k, terms * k.abs()) and close(grads[1], d * q, terms * q.abs())
+
+
 def test_a_second_derivative_is_refused():
     q, k, v, g, _, _, _ = problem(16, 1, 5, 1, 1, 8, 8, F32)
     q.requires_grad_()
