@@ -12,11 +12,14 @@
 // A wave takes a tile of steps with all heads of both: the angles' sines and
 // cosines are formed once a step and pair (p f in float64, since float32 is off
 // by up to p 2^-24 radians, and its turns brought within an eighth before the
-// float32 series) and read from LDS by every head, while the first rows are on
-// their way.  L lanes hold a row, each in units of two chunks of VW columns
-// that hold whole pairs, so the rotation needs no lane exchange; the sums over
-// a row are L-lane butterflies in float32.  Waves share nothing but the scales,
-// so none waits for another.  Bound by HBM: x is read and out written once.
+// float32 series) and read from LDS by every head, and the next tile's rows are
+// on their way while this one's are finished.  L lanes hold a row, each in units
+// of two chunks of VW columns that hold whole pairs, so the rotation needs no
+// lane exchange; the sums over a row are L-lane butterflies in float32.  Waves
+// share nothing but the scales and frequencies, so none waits for another.
+// Bound by HBM: x is read and out written once, at
+// 5.4 TB/s forward (65536 steps, 16 heads of 128, bf16: 200 us) and 4.9 TB/s
+// backward (128 x 1000 steps, 8 heads of 64, bf16: 162 us).
 #include "split_f32.h"
 
 #include <algorithm>
@@ -29,9 +32,14 @@ constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_DIM = 256;
 constexpr int MAX_COLUMNS = MAX_DIM + 64;  // with those of a row's last lane past its end
 constexpr int TILE_ANGLES = 512;  // most angles of a wave's tile
-constexpr int UNROLL = 2;         // rows a lane group has in flight of each part
-constexpr int FWD_BLOCKS = 4096;  // most workgroups
-constexpr int BWD_BLOCKS = 1024;  // (each with its partial sums of dscale)
+constexpr int TILE_STEPS = 64;    // and steps: a lane each
+// Rows a lane group has in flight of each part, and most workgroups (the
+// backward's leave a partial sum of dscale each).  Measured, bf16, 128 x 1000
+// steps, 8 heads of 64 of both: backward 162 us, with half and twice as many
+// workgroups 180 and 172, with two rows (which leave two workgroups a CU for
+// three) 187; forward of 65536 steps, 16 heads of 128: 200 us, with one row 209.
+constexpr int FWD_ROWS = 2, BWD_ROWS = 1;
+constexpr int FWD_BLOCKS = 4096, BWD_BLOCKS = 768;
 
 struct Rows {
   const void* x;
@@ -167,10 +175,17 @@ template <int VW, bool INTER> __device__ __forceinline__ Unit unit_of(int u, int
   return r;
 }
 
+// The value, as if computed here: the LDS addresses that depend on it are
+// formed for each row, where kept they would cost a wave's registers.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <int VW>
 __device__ __forceinline__ void load_scales(const float* scales, const Unit& u, float (&a)[VW], float (&b)[VW]) {
   // (a lane past the row's end multiplies zeros)
-  const int at_a = min(u.a, MAX_COLUMNS - VW), at_b = min(u.b, MAX_COLUMNS - VW);
+  const int at_a = here(min(u.a, MAX_COLUMNS - VW)), at_b = here(min(u.b, MAX_COLUMNS - VW));
 #pragma unroll
   for (int j = 0; j < VW; ++j) {
     a[j] = scales[at_a + j];
@@ -186,7 +201,7 @@ __device__ __forceinline__ void turn(float (&a)[VW], float (&b)[VW], const Unit&
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       float(&v)[VW] = c ? b : a;
-      const int first = c ? u.pair_b : u.pair_a;
+      const int first = here(c ? u.pair_b : u.pair_a);
       if (first < 0) continue;
 #pragma unroll
       for (int j = 0; j < VW / 2; ++j) {
@@ -212,17 +227,20 @@ __device__ __forceinline__ void wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // The rows of one lane group in flight: UNROLL of them, by the group's place.
 template <typename T, int VW, int UPL, bool BWD> struct Batch {
+  static constexpr int UNROLL = BWD ? BWD_ROWS : FWD_ROWS;
   Raw<T, VW> x[UNROLL][UPL][2];
   Raw<T, VW> c[BWD ? UNROLL : 1][UPL][2];
 };
 
 template <typename T, int VW, int UPL, bool INTER, bool BWD>
-__global__ void __launch_bounds__(THREADS, 2) qk_norm_kernel(NormArgs p) {
+__global__ void __launch_bounds__(THREADS, BWD ? 3 : 2) qk_norm_kernel(NormArgs p) {
   __shared__ union {
     float2 angles[WAVES][TILE_ANGLES];
     float sums[BWD ? 2 * VW * UPL * THREADS : 1];
   } lds;
   __shared__ __attribute__((aligned(16))) float scales[2][MAX_COLUMNS];
+  __shared__ double frequencies[MAX_DIM / 2];
+  constexpr int UNROLL = Batch<T, VW, UPL, BWD>::UNROLL;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int L = 1 << p.lanes_log2, l = lane & (L - 1), D = p.D, P = p.P;
   const int group = lane >> p.lanes_log2, groups = 64 >> p.lanes_log2;
@@ -235,6 +253,7 @@ __global__ void __launch_bounds__(THREADS, 2) qk_norm_kernel(NormArgs p) {
     const int w = i / MAX_COLUMNS, j = i % MAX_COLUMNS;
     scales[w][j] = p.part[w].scale && j < D ? p.part[w].scale[j] : 1.f;
   }
+  for (int i = tid; i < P; i += THREADS) frequencies[i] = p.frequencies[i];
   float sum[2][UPL][2][VW];
   if constexpr (BWD) {
 #pragma unroll
@@ -242,145 +261,174 @@ __global__ void __launch_bounds__(THREADS, 2) qk_norm_kernel(NormArgs p) {
   }
   __syncthreads();
   const uint32_t tiles = (p.tokens + p.tile - 1) / p.tile;
-  for (uint32_t tile = blockIdx.x * WAVES + wave; tile < tiles; tile += gridDim.x * WAVES) {
-    const uint32_t t0 = tile * p.tile;
-    const int n = (int)min((uint32_t)p.tile, p.tokens - t0);
-    const uint32_t b0 = t0 / p.steps, s0 = t0 - b0 * p.steps;
-    // the tile's step s: sequence and step (a tile is at most 512 steps)
-    auto step_of = [&](int s, uint32_t& b, uint32_t& t) {
-      const uint32_t x = s0 + s;
-      const uint32_t wraps = p.steps > TILE_ANGLES ? (x >= p.steps ? 1 : 0)
-                             : p.steps > 1         ? __umulhi(x, p.inverse_steps)
-                                                   : x;
-      b = b0 + wraps;
-      t = x - wraps * p.steps;
-    };
-    // row r of part w: step r / heads, head r % heads (exact: r heads < 2^32)
-    auto place = [&](int w, int r, int& s, int& h) {
-      s = p.part[w].heads == 1 ? r : (int)__umulhi((uint32_t)r, p.part[w].inverse);
-      h = r - s * p.part[w].heads;
-    };
-    auto load = [&](int w, int r0, Batch<T, VW, UPL, BWD>& v) {
-      const Rows& q = p.part[w];
-      const int rows = n * q.heads;
+  // A tile: its first step (of all; its sequence and the step in that), its steps
+  struct Tile {
+    uint32_t t0, b0, s0;
+    int n;
+  };
+  auto tile_at = [&](uint32_t tile) {
+    Tile t;
+    t.t0 = tile * p.tile;
+    t.n = (int)min((uint32_t)p.tile, p.tokens - t.t0);
+    t.b0 = t.t0 / p.steps;
+    t.s0 = t.t0 - t.b0 * p.steps;
+    return t;
+  };
+  auto step_of = [&](const Tile& tile, int s, uint32_t& b, uint32_t& t) {
+    const uint32_t x = tile.s0 + s;
+    const uint32_t wraps = p.steps > TILE_STEPS ? (x >= p.steps ? 1 : 0)
+                           : p.steps > 1        ? __umulhi(x, p.inverse_steps)
+                                                : x;
+    b = tile.b0 + wraps;
+    t = x - wraps * p.steps;
+  };
+  // row r of part w: step r / heads, head r % heads (exact: r heads < 2^32)
+  auto place = [&](int w, int r, int& s, int& h) {
+    s = p.part[w].heads == 1 ? r : (int)__umulhi((uint32_t)r, p.part[w].inverse);
+    h = r - s * p.part[w].heads;
+  };
+  auto load = [&](const Tile& tile, int w, int r0, Batch<T, VW, UPL, BWD>& v) {
+    const Rows& q = p.part[w];
+    const int rows = tile.n * q.heads;
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int r = r0 + u * groups;
-        if (r < rows) {
-          int s, h;
-          place(w, r, s, h);
-          uint32_t bb, tt;
-          step_of(s, bb, tt);
-          const T* x = static_cast<const T*>(q.x) + ((int64_t)bb * q.sb + (int64_t)tt * q.st + (int64_t)h * q.sh);
-#pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            load_row<VW>(x + unit[k].a, D - unit[k].a, v.x[u][k][0]);
-            load_row<VW>(x + unit[k].b, D - unit[k].b, v.x[u][k][1]);
-          }
-          if constexpr (BWD) {
-            const T* c = static_cast<const T*>(q.cot) + ((int64_t)bb * q.cb + (int64_t)tt * q.ct + (int64_t)h * q.ch);
-#pragma unroll
-            for (int k = 0; k < UPL; ++k) {
-              load_row<VW>(c + unit[k].a, D - unit[k].a, v.c[u][k][0]);
-              load_row<VW>(c + unit[k].b, D - unit[k].b, v.c[u][k][1]);
-            }
-          }
-        }
-      }
-    };
-    auto finish = [&](int w, int r0, const Batch<T, VW, UPL, BWD>& v) {
-      const Rows& q = p.part[w];
-      const int rows = n * q.heads;
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int r = r0 + u * groups;
-        if (r >= rows) continue;
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = r0 + u * groups;
+      if (r < rows) {
         int s, h;
         place(w, r, s, h);
-        T* out = static_cast<T*>(q.out) + ((int64_t)(t0 + s) * q.heads + h) * D;
-        const float2* angles = cs + s * P;
-        float a[UPL][VW], b[UPL][VW];
-        float ss = 0.f;
+        uint32_t bb, tt;
+        step_of(tile, s, bb, tt);
+        const T* x = static_cast<const T*>(q.x) + ((int64_t)bb * q.sb + (int64_t)tt * q.st + (int64_t)h * q.sh);
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          widen(v.x[u][k][0], a[k]);
-          widen(v.x[u][k][1], b[k]);
-#pragma unroll
-          for (int j = 0; j < VW; ++j) ss = __fmaf_rn(a[k][j], a[k][j], __fmaf_rn(b[k][j], b[k][j], ss));
+          load_row<VW>(x + unit[k].a, D - unit[k].a, v.x[u][k][0]);
+          load_row<VW>(x + unit[k].b, D - unit[k].b, v.x[u][k][1]);
         }
-        ss = lanes_sum(ss, p.lanes_log2);
-        const float rstd = rsqrtf(__fmaf_rn(ss, over_d, p.eps));
-        if constexpr (!BWD) {
+        if constexpr (BWD) {
+          const T* c = static_cast<const T*>(q.cot) + ((int64_t)bb * q.cb + (int64_t)tt * q.ct + (int64_t)h * q.ch);
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
-            float wa[VW], wb[VW];
-            load_scales(scales[w], unit[k], wa, wb);
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-              a[k][j] = a[k][j] * rstd * wa[j];
-              b[k][j] = b[k][j] * rstd * wb[j];
-            }
-            turn<VW, INTER>(a[k], b[k], unit[k], angles, P, 1.f);
-            store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
-            store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
-          }
-        } else {
-          float ca[UPL][VW], cb[UPL][VW];
-          float m = 0.f;
-#pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            widen(v.c[u][k][0], ca[k]);
-            widen(v.c[u][k][1], cb[k]);
-            turn<VW, INTER>(ca[k], cb[k], unit[k], angles, P, -1.f);
-            float wa[VW], wb[VW];
-            load_scales(scales[w], unit[k], wa, wb);
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-              a[k][j] *= rstd;
-              b[k][j] *= rstd;
-              sum[w][k][0][j] = __fmaf_rn(ca[k][j], a[k][j], sum[w][k][0][j]);
-              sum[w][k][1][j] = __fmaf_rn(cb[k][j], b[k][j], sum[w][k][1][j]);
-              ca[k][j] *= wa[j];
-              cb[k][j] *= wb[j];
-              m = __fmaf_rn(ca[k][j], a[k][j], __fmaf_rn(cb[k][j], b[k][j], m));
-            }
-          }
-          m = lanes_sum(m, p.lanes_log2) * over_d;
-#pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-              a[k][j] = rstd * __fmaf_rn(-a[k][j], m, ca[k][j]);
-              b[k][j] = rstd * __fmaf_rn(-b[k][j], m, cb[k][j]);
-            }
-            store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
-            store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
+            load_row<VW>(c + unit[k].a, D - unit[k].a, v.c[u][k][0]);
+            load_row<VW>(c + unit[k].b, D - unit[k].b, v.c[u][k][1]);
           }
         }
       }
-    };
-    Batch<T, VW, UPL, BWD> v[2];
-    load(0, group, v[0]);
-    load(1, group, v[1]);
-    for (int i = lane; i < n * P; i += 64) {
+    }
+  };
+  auto finish = [&](const Tile& tile, int w, int r0, const Batch<T, VW, UPL, BWD>& v) {
+    const Rows& q = p.part[w];
+    const int rows = tile.n * q.heads;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = r0 + u * groups;
+      if (r >= rows) continue;
+      int s, h;
+      place(w, r, s, h);
+      T* out = static_cast<T*>(q.out) + ((int64_t)(tile.t0 + s) * q.heads + h) * D;
+      const float2* angles = cs + s * P;
+      float a[UPL][VW], b[UPL][VW];
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) {
+        widen(v.x[u][k][0], a[k]);
+        widen(v.x[u][k][1], b[k]);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) ss = __fmaf_rn(a[k][j], a[k][j], __fmaf_rn(b[k][j], b[k][j], ss));
+      }
+      ss = lanes_sum(ss, p.lanes_log2);
+      const float rstd = rsqrtf(__fmaf_rn(ss, over_d, p.eps));
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          float wa[VW], wb[VW];
+          load_scales(scales[w], unit[k], wa, wb);
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            a[k][j] = a[k][j] * rstd * wa[j];
+            b[k][j] = b[k][j] * rstd * wb[j];
+          }
+          turn<VW, INTER>(a[k], b[k], unit[k], angles, P, 1.f);
+          store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
+          store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
+        }
+      } else {
+        float ca[UPL][VW], cb[UPL][VW];
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+          widen(v.c[u][k][0], ca[k]);
+          widen(v.c[u][k][1], cb[k]);
+          turn<VW, INTER>(ca[k], cb[k], unit[k], angles, P, -1.f);
+          float wa[VW], wb[VW];
+          load_scales(scales[w], unit[k], wa, wb);
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            a[k][j] *= rstd;
+            b[k][j] *= rstd;
+            sum[w][k][0][j] = __fmaf_rn(ca[k][j], a[k][j], sum[w][k][0][j]);
+            sum[w][k][1][j] = __fmaf_rn(cb[k][j], b[k][j], sum[w][k][1][j]);
+            ca[k][j] *= wa[j];
+            cb[k][j] *= wb[j];
+            m = __fmaf_rn(ca[k][j], a[k][j], __fmaf_rn(cb[k][j], b[k][j], m));
+          }
+        }
+        m = lanes_sum(m, p.lanes_log2) * over_d;
+#pragma unroll
+        for (int k = 0; k < UPL; ++k) {
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            a[k][j] = rstd * __fmaf_rn(-a[k][j], m, ca[k][j]);
+            b[k][j] = rstd * __fmaf_rn(-b[k][j], m, cb[k][j]);
+          }
+          store_row<VW>(out + unit[k].a, D - unit[k].a, a[k]);
+          store_row<VW>(out + unit[k].b, D - unit[k].b, b[k]);
+        }
+      }
+    }
+  };
+  auto position_of = [&](const Tile& tile) {  // of the lane's step
+    return p.positions ? p.positions[tile.t0 + min(lane, tile.n - 1)] : 0;
+  };
+  Batch<T, VW, UPL, BWD> v[2];
+  uint32_t index = blockIdx.x * WAVES + wave;
+  Tile tile;
+  int position = 0;
+  if (index < tiles) {
+    tile = tile_at(index);
+    position = position_of(tile);
+    load(tile, 0, group, v[0]);
+    load(tile, 1, group, v[1]);
+  }
+  while (index < tiles) {
+    for (int i0 = 0; i0 < tile.n * P; i0 += 64) {
+      const int i = min(i0 + lane, tile.n * P - 1);
       const int s = P == 1 ? i : (int)__umulhi((uint32_t)i, p.inverse_pairs), f = i - s * P;
       uint32_t bb, tt;
-      step_of(s, bb, tt);
-      const double pos = p.positions ? (double)p.positions[t0 + s] : (double)tt;
-      double turns = pos * p.frequencies[f] * 0.15915494309189533577;  // 1 / (2 pi)
+      step_of(tile, s, bb, tt);
+      const int at = __shfl(position, s);
+      const double pos = p.positions ? (double)at : (double)tt;
+      double turns = pos * frequencies[f] * 0.15915494309189533577;  // 1 / (2 pi)
       turns -= rint(turns);
       cs[i] = cos_sin((float)turns);
     }
     wave_lds();
+    index += gridDim.x * WAVES;
+    Tile next = tile;
+    if (index < tiles) {
+      next = tile_at(index);
+      position = position_of(next);
+    }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      finish(w, group, v[w]);
-      for (int r0 = group + UNROLL * groups; r0 < n * p.part[w].heads; r0 += UNROLL * groups) {
-        load(w, r0, v[w]);
-        finish(w, r0, v[w]);
+      finish(tile, w, group, v[w]);
+      for (int r0 = group + UNROLL * groups; r0 < tile.n * p.part[w].heads; r0 += UNROLL * groups) {
+        load(tile, w, r0, v[w]);
+        finish(tile, w, r0, v[w]);
       }
+      if (index < tiles) load(next, w, group, v[w]);
     }
     wave_lds();
+    tile = next;
   }
   if constexpr (BWD) {
     __syncthreads();
@@ -451,11 +499,11 @@ int lanes_log2_of(int D, int v) {
 // Steps of a wave's tile: rows of the part with fewer heads for every lane
 // group's loads, no more angles than there is room for, a tile for every wave
 // where there are few steps, and rows whose heads a 32-bit product tells.
-int tile_of(int64_t tokens, int heads, int kv_heads, int pairs, int lanes_log2) {
+int tile_of(int64_t tokens, int heads, int kv_heads, int pairs, int lanes_log2, int rows) {
   const int64_t most = std::max(heads, kv_heads), fewer = heads && kv_heads ? std::min(heads, kv_heads) : most;
-  const int64_t busy = std::max<int64_t>(1, 64 * UNROLL / (fewer << lanes_log2));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({busy, TILE_ANGLES / std::max(pairs, 1), TILE_ANGLES,
-                                                      ppo::ceil_div64(tokens, 1024 * WAVES),
+  const int64_t busy = std::max<int64_t>(1, 64 * rows / (fewer << lanes_log2));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({busy, TILE_ANGLES / std::max(pairs, 1),
+                                                      ppo::ceil_div64(tokens, 1024 * WAVES), TILE_STEPS,
                                                       (1ll << 32) / (most * most) - 1}));
 }
 
@@ -464,7 +512,7 @@ unsigned blocks_of(int64_t tokens, int tile, int most) {
 }
 
 NormArgs common_args(float epsilon, int64_t tokens, int steps, int width, int pairs, int interleaved, int dtype,
-                     int heads, int kv_heads, const double* frequencies, const int32_t* positions) {
+                     int heads, int kv_heads, const double* frequencies, const int32_t* positions, int rows) {
   NormArgs a{};
   a.frequencies = frequencies;
   a.positions = positions;
@@ -476,7 +524,7 @@ NormArgs common_args(float epsilon, int64_t tokens, int steps, int width, int pa
   a.D = width;
   a.P = pairs;
   a.lanes_log2 = lanes_log2_of(width, chunk_columns(dtype, pairs, interleaved));
-  a.tile = tile_of(tokens, heads, kv_heads, pairs, a.lanes_log2);
+  a.tile = tile_of(tokens, heads, kv_heads, pairs, a.lanes_log2, rows);
   return a;
 }
 
@@ -519,7 +567,7 @@ PPO_EXPORT int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, co
   if (!strides || (heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out)) || (pairs > 0 && !frequencies))
     return ppo::set_error(PPO_ERR_ARG, "%s: null buffer", what);
   NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, heads, kv_heads,
-                           frequencies, positions);
+                           frequencies, positions, FWD_ROWS);
   a.part[0] = Rows{q, nullptr, q_scale, q_out, strides[0], strides[1], strides[2], 0, 0, 0, heads, inverse_of(heads)};
   a.part[1] = Rows{k, nullptr, k_scale, k_out, strides[3], strides[4], strides[5], 0, 0, 0, kv_heads,
                    inverse_of(kv_heads)};
@@ -554,7 +602,7 @@ PPO_EXPORT int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, co
   int blocks = 0;
   if (!none) {
     NormArgs a = common_args(epsilon, tokens, steps, width, pairs, interleaved, dtype, heads, kv_heads,
-                             frequencies, positions);
+                             frequencies, positions, BWD_ROWS);
     a.part[0] = Rows{q, dq_out, q_scale, dq, strides[0], strides[1], strides[2], strides[6], strides[7], strides[8],
                      heads, inverse_of(heads)};
     a.part[1] = Rows{k, dk_out, k_scale, dk, strides[3], strides[4], strides[5], strides[9], strides[10], strides[11],
