@@ -430,11 +430,11 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
     for (int i = tid; i < C * 6; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
   lds_barrier();
 
-  // Whether the state itself is an output: the third piece of its terms (2^-17
-  // of them) is below what a state keeps that only enters products, rounded to
-  // bf16 (2^-8).  With it, 16 heads of 128: 65536 steps 388 -> 406 us, both
-  // passes of 8 x 4096 steps 640 -> 675 us.
-  const bool exact = STATE || (c.final && seg == p.segments - 1);
+  // Whether the state itself is an output (or, STATE, leads to one): the third
+  // piece of its terms (2^-17 of them) is below what a state keeps that only
+  // enters products, rounded to bf16 (2^-8).  With it, 16 heads of 128: 65536
+  // steps 388 -> 406 us, both passes of 8 x 4096 steps 640 -> 675 us.
+  const bool exact = c.final && (STATE || seg == p.segments - 1);
   uint64_t cut = 0;   // the chunk's steps that drop the state
   // Lays out steps r0 .. r0 + n - 1, as loaded, and loads the chunk from `next` (>= 0) on.
   // Whether y or z holds an infinity or NaN.  (Here and below a lane's places
