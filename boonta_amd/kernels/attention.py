@@ -13,7 +13,12 @@ reference, whose attention block is boonta/networks/blocks/self_attention.py.
   usual frequencies.
 
 float32 or bfloat16 storage; states, sums and norms are float32.  There is no CPU path:
-the kernels run on the device the tensors live on, on its current stream.
+the kernels run on the device the tensors live on, on its current stream, and can
+be captured into a graph.  Before a backward pass is captured, drop every eager
+autograd graph of the same leaves: such a graph keeps the leaves' gradient nodes
+on the stream it was made on, which a capture on another stream must not join.
+At most 2^21 sequences of linear_attention (batch * heads), 2^23 - 1 of its
+step; larger ones are refused.
 """
 from __future__ import annotations
 

@@ -131,6 +131,13 @@ def test_long_sequences_are_cut_into_segments(shape, done, ragged, dtype):
     check(*ops, seed=1)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(1, 1100, 2, 1, 64, 64), (2, 1200, 1, 1, 128, 128)])
+def test_long_sequences_without_a_carry(shape, dtype):
+    """Nothing asks for the backward's own states: their terms are kept shorter."""
+    check(*problem(sum(shape), *shape, dtype, done=0.001, carry=False, slow=True), seed=2)
+
+
 def test_lengths_of_zero_leave_the_carry():
     q, k, v, g, carry, _, _ = problem(5, 2, 40, 2, 2, 16, 16, F32)
     lengths = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
@@ -411,3 +418,40 @@ def test_work_on_another_stream():
         got = check_raw(*s)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_two_graphs_and_two_streams_at_once():
+    """Two captured passes, replayed at the same time, and two eager calls: each
+    has its own workspace."""
+    sets = [problem(40 + i, 2, 900, 2, 1, 64, 64, BF16, done=0.01, slow=True) for i in range(2)]
+    gen = torch.Generator().manual_seed(5)
+    dout = torch.randn(2, 900, 2, 64, generator=gen).to(BF16).cuda()
+    dfinal = torch.randn(2, 2, 64, 64, generator=gen).cuda()
+
+    def both_passes(q, k, v, g, carry, done, _):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, carry)]
+        final, out = linear_attention(*leaves[:3], g, carry=leaves[3], done=done)
+        return (final.detach(), out.detach(), *torch.autograd.grad([out, final], leaves, [dout, dfinal]))
+
+    want = [both_passes(*s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(both_passes(*s))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        eager = []
+        for stream, graph in zip(streams, graphs):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                eager.append(both_passes(*s))
+        torch.cuda.synchronize()
+        for results in (got, eager):
+            for a, b in zip(results, want):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
