@@ -35,25 +35,25 @@ _MAX_STRIDE = 1 << 23   # of a step, in elements: the kernels count a chunk's by
 
 
 def _on_device(name, *tensors):
-    device = tensors[0].device
+    """The index of the device that all of them (None aside) are on."""
+    index = tensors[0].get_device()   # (-1: the host)
     for x in tensors:
-        if x is not None and x.device != device:
+        if x is not None and x.get_device() != index:
             raise TypeError(f"{name} runs on tensors of one device")
-    if device.type != "cuda":
+    if index < 0:
         raise TypeError(f"{name} runs on device tensors")
-    return device
+    return index
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (a build without devices has none)
 
 
-def _launch(device, name, *args):
+def _launch(index, name, *args):
     """Calls an entry point on the device's current stream (the device made current where it is not)."""
-    index = device.index
     if index == torch.cuda.current_device():
         _lib.call(name, _raw_stream(index), *args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             _lib.call(name, _raw_stream(index), *args)
 
 
@@ -119,13 +119,12 @@ def _check_attention(name, q, k, v, log_decay, carry, done, dims):
 # --------------------------------------------------------------------- sequences
 def _forward(q, k, v, log_decay, carry, done, lengths, scale, sizes):
     batch, steps, heads, kv_heads, key, value = sizes
-    device, dtype = q.device, q.dtype
-    dt = _DTYPES[dtype]
-    out = torch.empty((batch, steps, heads, value), dtype=dtype, device=device)
-    final = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
+    dt = _DTYPES[q.dtype]
+    out = q.new_empty((batch, steps, heads, value))
+    final = log_decay.new_empty((batch, heads, key, value))   # (float32)
     nbytes = _lib.load().ppo_linear_attention_workspace(dt, batch, steps, heads, key, value)
-    states = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
-    _launch(device, "ppo_linear_attention_fwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
+    states = log_decay.new_empty(nbytes // 4) if nbytes else None
+    _launch(q.get_device(), "ppo_linear_attention_fwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v),
             log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), scale, out.data_ptr(), final.data_ptr(),
             _ptr(states), nbytes, *sizes)
     return final, out, states
@@ -145,19 +144,18 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, dfinal, dout):
         q, k, v, log_decay, carry, done, lengths, states = ctx.saved_tensors
         batch, steps, heads, kv_heads, key, value = ctx.sizes
-        device, dtype = q.device, q.dtype
-        dt = _DTYPES[dtype]
+        dt = _DTYPES[q.dtype]
         if dout is None:   # (only the final carry was used)
-            dout = torch.zeros(value, dtype=dtype, device=device).expand(batch, steps, heads, value)
+            dout = q.new_zeros(value).expand(batch, steps, heads, value)
         dout = _rows(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
-        dq = torch.empty((batch, steps, heads, key), dtype=dtype, device=device)
-        dk = torch.empty((batch, steps, kv_heads, key), dtype=dtype, device=device)
-        dv = torch.empty((batch, steps, kv_heads, value), dtype=dtype, device=device)
+        dq = q.new_empty((batch, steps, heads, key))
+        dk = q.new_empty((batch, steps, kv_heads, key))
+        dv = q.new_empty((batch, steps, kv_heads, value))
         dcarry = torch.empty_like(carry) if carry is not None and ctx.needs_input_grad[4] else None
         nbytes = _lib.load().ppo_linear_attention_bwd_workspace(dt, batch, steps, heads, kv_heads, key, value)
-        work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
-        _launch(device, "ppo_linear_attention_bwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
+        work = log_decay.new_empty(nbytes // 4) if nbytes else None
+        _launch(q.get_device(), "ppo_linear_attention_bwd", dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(),
                 _strides(q, k, v, dout), log_decay.data_ptr(), _ptr(carry), _ptr(done), _ptr(lengths), ctx.scale,
                 _ptr(dfinal), _ptr(states), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dcarry), _ptr(work),
                 nbytes, *ctx.sizes)
@@ -219,16 +217,16 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         raise ValueError(f"out_carry must be contiguous float32 {tuple(carry.shape)} that needs no gradient")
     if out_carry is not None and 0 < abs(out_carry.data_ptr() - carry.data_ptr()) < 4 * carry.numel():
         raise ValueError("out_carry must be carry itself or memory apart from it")
-    device = _on_device("linear_attention_step", q, k, v, log_decay, carry, done, out_carry)
+    index = _on_device("linear_attention_step", q, k, v, log_decay, carry, done, out_carry)
     scale = key ** -0.5 if scale is None else float(scale)
     q, k, v, log_decay, carry = _rows(q), _rows(k), _rows(v), log_decay.contiguous(), carry.contiguous()
     done = None if done is None else done.contiguous()
     if out_carry is None:
-        out_carry = torch.empty((batch, heads, key, value), dtype=torch.float32, device=device)
+        out_carry = carry.new_empty((batch, heads, key, value))
     else:
         torch.autograd.graph.increment_version(out_carry)   # (written in place)
-    out = torch.empty((batch, heads, value), dtype=q.dtype, device=device)
-    _launch(device, "ppo_linear_attention_step", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    out = q.new_empty((batch, heads, value))
+    _launch(index, "ppo_linear_attention_step", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
             _strides(q, k, v), log_decay.data_ptr(), _ptr(done), carry.data_ptr(), out_carry.data_ptr(),
             out.data_ptr(), scale, batch, heads, kv_heads, key, value)
     return out_carry, out
@@ -244,10 +242,8 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, device="cuda") -> tor
 
 def _norm_forward(q, k, q_scale, k_scale, frequencies, positions, epsilon, interleaved):
     batch, steps, heads, width = q.shape
-    device = q.device
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
-    _launch(device, "ppo_qk_norm_rotary_fwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), _strides(q, k),
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    _launch(q.get_device(), "ppo_qk_norm_rotary_fwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), _strides(q, k),
             _ptr(q_scale), _ptr(k_scale), _ptr(frequencies), _ptr(positions), epsilon, interleaved, q_out.data_ptr(),
             k_out.data_ptr(), batch, steps, heads, k.shape[2], width,
             0 if frequencies is None else frequencies.numel())
@@ -267,15 +263,13 @@ class _QKNormRotary(torch.autograd.Function):
         q, k, q_scale, k_scale, frequencies, positions = ctx.saved_tensors
         epsilon, interleaved = ctx.options
         batch, steps, heads, width = q.shape
-        device = q.device
         gq, gk = _rows(gq), _rows(gk)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dq_scale = None if q_scale is None or not ctx.needs_input_grad[2] else torch.empty_like(q_scale)
         dk_scale = None if k_scale is None or not ctx.needs_input_grad[3] else torch.empty_like(k_scale)
         nbytes = _lib.load().ppo_qk_norm_rotary_bwd_workspace(width)
-        work = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
-        _launch(device, "ppo_qk_norm_rotary_bwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), gq.data_ptr(),
+        work = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+        _launch(q.get_device(), "ppo_qk_norm_rotary_bwd", _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), gq.data_ptr(),
                 gk.data_ptr(), _strides(q, k, gq, gk), _ptr(q_scale), _ptr(k_scale), _ptr(frequencies),
                 _ptr(positions), epsilon, interleaved, dq.data_ptr(), dk.data_ptr(), _ptr(dq_scale), _ptr(dk_scale),
                 work.data_ptr(), nbytes, batch, steps, heads, k.shape[2], width,
