@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
 // before the last adds from zeros and how it fades what enters it; in place.
 // Four neighbouring values a thread (a state's last ones apart), four segments'
 // loads in flight; bound by HBM, or by its launch: 128 pairs of 3 states of
-// 128 x 128 take 9 to 11 us (50 MB, 5 TB/s), 192 of 3 of 64 x 64 6 us.
+// 128 x 128 take 9 to 11 us (50 MB, 5 TB/s), 192 of 4 of 64 x 64 6 us.
 __global__ void __launch_bounds__(64) join_segments_kernel(float* states, const float* factors, const float* carry,
                                                             int KV, int segs) {
   const int i = (blockIdx.x * 64 + threadIdx.x) * 4, left = KV - i;
