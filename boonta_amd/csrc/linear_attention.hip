@@ -58,6 +58,7 @@ struct AttnArgs {
   const int32_t* lengths;   // [batch], or null
   float* factors;           // [batch * heads, segments - 1]: a segment's decay of its entry state (-1: reset)
   int steps, heads, segments, seg_steps, roles;
+  int streamed;             // the outputs are stored in whole rows past the caches
 };
 
 // ---- per type: chunks of 128 bytes of steps; a lane's MFMA operand of 16
@@ -237,16 +238,16 @@ __device__ __forceinline__ void write_transposed(char* t, int byte, const uint4 
   *reinterpret_cast<uint4*>(t + (byte ^ 16) + 384) = make_uint4(v[0].w, v[1].w, v[2].w, v[3].w);
 }
 
-// Four consecutive outputs of a row, `left` of them inside it.
 typedef __attribute__((address_space(1))) char* GlobalOut;
-typedef uint32_t word2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float floatx4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// Four consecutive outputs of a row, `left` of them inside it.
 __device__ __forceinline__ void store4(GlobalOut p, floatx4 v, int left, uint16_t) {
   typedef __attribute__((address_space(1))) uint16_t* Out;
+  typedef uint32_t word2 __attribute__((ext_vector_type(2), aligned(2)));
   const uint32_t lo = pack_bf16(v[0], v[1]), hi = pack_bf16(v[2], v[3]);
   if (left >= 4) {
-    *(__attribute__((address_space(1))) word2_a2*)p = word2_a2{lo, hi};
+    *(__attribute__((address_space(1))) word2*)p = word2{lo, hi};
   } else {
     if (left > 0) ((Out)p)[0] = (uint16_t)lo;
     if (left > 1) ((Out)p)[1] = (uint16_t)(lo >> 16);
@@ -263,6 +264,23 @@ __device__ __forceinline__ void store4(GlobalOut p, floatx4 v, int left, float) 
       if (e < left) ((Out)p)[e] = v[e];
   }
 }
+// A chunk of 16 bytes of a row of T, `left` elements inside it, past the caches.
+template <typename T> __device__ __forceinline__ void stream_chunk(GlobalOut p, uint4 v, int left) {
+  typedef __attribute__((address_space(1))) uint16_t* Halves;
+  typedef __attribute__((address_space(1))) uint32_t* Words;
+  typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(2)));
+  const word4 w = {v.x, v.y, v.z, v.w};
+  if (left >= Type<T>::FR) {
+    __builtin_nontemporal_store(w, (__attribute__((address_space(1))) word4*)p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < Type<T>::FR - 1; ++e)
+      if (e < left) {
+        if constexpr (sizeof(T) == 2) ((Halves)p)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+        else ((Words)p)[e] = w[e];
+      }
+  }
+}
 __device__ __forceinline__ void store1(uint16_t* p, float v) { *p = (uint16_t)pack_bf16(v, v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
@@ -272,6 +290,10 @@ __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+
+// Waits for this wave's loads.  Before the stores that follow a chunk, and on
+// every way to the next chunk: what is waited for later counts the stores too.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // (no other counter)
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -308,6 +330,9 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
   constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
   constexpr int PIECES = Type<T>::PIECES;
   constexpr int RB = D * (int)sizeof(T), ROWS = C * RB, COLS = D * 128;
+  // Streamed outputs go through LDS to be stored in whole rows.  (96-wide, rows
+  // of one and a half lines and few waves: 175 -> 181 us, so not there.)
+  constexpr bool ROWS_OUT = !STATE && D != 96;
   // y and z by columns, x and y by rows, and the pair products: all queries
   // with the chunk's first half of keys, the later half with the other
   __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 96) + 2 * COLS];
@@ -335,6 +360,7 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
   const int64_t bh = (int64_t)b * p.heads + head;
   const int R = c.x.width, N = c.z.width;
   const int64_t KV = (int64_t)R * N;
+  const bool streamed = ROWS_OUT && p.streamed && !c.wide;
   const bool back = c.backward;
   const int col = 16 * wave + l16;  // this lane's column of the state
 
@@ -568,22 +594,34 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
             acc[qt] = Type<T>::mma(z, *reinterpret_cast<const Frag*>(pr + pair_byte + qt * 1024 + tb * C * 32), acc[qt]);
           }
         }
-        const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;
-        const GlobalOut low = (GlobalOut)uniform(static_cast<const char*>(c.out) +
-                                                 (base_o + (back ? len - r0 - n : r0) * (int64_t)pitch_o) * size);
-        uint32_t byte = (uint32_t)((back ? n - 1 - l16 : l16) * pitch_o + n0) * size;
-        const uint32_t next = (uint32_t)((back ? -16 : 16) * pitch_o * size);
-        // (whole tiles without their tests: 128 x 1000 steps, 8 heads of 64, both passes 466 -> 453 us; 65536
-        // steps of 16 heads of 128 387 -> 396 us, so not there)
-        if (D < 128 && n == C && 16 * wave + 16 <= N && !c.wide) {
+        if (!streamed) {
+          const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;
+          const GlobalOut low = (GlobalOut)uniform(static_cast<const char*>(c.out) +
+                                                   (base_o + (back ? len - r0 - n : r0) * (int64_t)pitch_o) * size);
+          uint32_t byte = (uint32_t)((back ? n - 1 - l16 : l16) * pitch_o + n0) * size;
+          const uint32_t next = (uint32_t)((back ? -16 : 16) * pitch_o * size);
+          if (n == C && 16 * wave + 16 <= N && !c.wide) {  // (without the tests: 96-wide 180 -> 175 us)
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt, byte += next) store4(low + byte, acc[qt], 4, T());
+            for (int qt = 0; qt < QT; ++qt, byte += next) store4(low + byte, acc[qt], 4, T());
+          } else {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt, byte += next) {
+              if (16 * qt + l16 < n) {
+                if (c.wide) store4(low + byte, acc[qt], N - n0, float());
+                else store4(low + byte, acc[qt], N - n0, T());
+              }
+            }
+          }
         } else {
+          // for whole rows: in place of x, which no wave reads any more
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt, byte += next) {
-            if (16 * qt + l16 < n) {
-              if (c.wide) store4(low + byte, acc[qt], N - n0, float());
-              else store4(low + byte, acc[qt], N - n0, T());
+          for (int qt = 0; qt < QT; ++qt) {
+            if constexpr (sizeof(T) == 2) {
+              *reinterpret_cast<uint2*>(xr + row_byte<RB>(l16, 2 * (wave & 1) + (g4 >> 1), qt, wave >> 1) +
+                                        ((g4 & 1) << 3)) =
+                  make_uint2(pack_bf16(acc[qt][0], acc[qt][1]), pack_bf16(acc[qt][2], acc[qt][3]));
+            } else {
+              *reinterpret_cast<floatx4*>(xr + row_byte<RB>(l16, g4, qt, wave)) = acc[qt];
             }
           }
         }
@@ -631,6 +669,20 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
     }
     __builtin_amdgcn_s_setprio(0);
     lds_barrier();
+    if (!streamed) return;
+    // whole rows of outputs, from where this thread lays out x next
+    const int dx = (uint32_t)tid % (D / FR), tx = (uint32_t)tid / (D / FR), left = N - dx * FR;
+    const GlobalOut low = (GlobalOut)uniform(static_cast<const T*>(c.out) + base_o +
+                                             (back ? len - r0 - n : r0) * (int64_t)pitch_o);
+    uint4 v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = *reinterpret_cast<const uint4*>(xr + rows_byte<RB, 2>(dx, tx, e));
+    loads_done();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 2 * tx + e, at = (back ? n - 1 - row : row) * pitch_o + dx * FR;
+      if (row < n) stream_chunk<T>(low + (uint32_t)at * (uint32_t)sizeof(T), v[e], left);
+    }
   };
   // The products multiply a masked pair by zero, which an infinity or NaN in y or
   // z outlasts: the steps of such a chunk are taken one by one.  (Padding stays
@@ -645,10 +697,14 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
   if constexpr (!STATE) {
     while (r0 < last) {
       bool is_bad = false;
+      loads_done();
       while (r0 < last) {
         const int n = min(C, last - r0);
         is_bad = stage(n, r0 + n < last ? r0 + n : -1);
-        if (__builtin_expect(is_bad, 0)) break;
+        if (__builtin_expect(is_bad, 0)) {
+          loads_done();
+          break;
+        }
         chunk(n);
         r0 += n;
       }
@@ -914,8 +970,19 @@ void states_pass(hipStream_t st, int dtype, AttnArgs a, const Contraction& c, in
                      dim3(64), 0, st, c.states, a.factors, c.carry, KV, a.segments - 1);
 }
 
-void outputs_pass(hipStream_t st, int dtype, const AttnArgs& a, int batch) {
+// Outputs too large for the caches to hold for what reads them next are
+// streamed: in whole rows past the caches, which keep the operands that other
+// workgroups read again.  Measured, bf16, alone and with a product that reads
+// them next: 134 MB (64 x 2048 steps, 8 heads of 64) 170 -> 152 and 224 -> 215
+// us, 67 MB 94 -> 80 and 118 -> 115, 33 MB 56 -> 55 but 69 -> 70; both passes of
+// 128 x 1000 steps, 8 heads of 64, 453 -> 430 us, 65536 steps of 16 heads of 128
+// 388 -> 373.  (Whole rows through the caches gained half of that, and lost 2 %
+// where outputs are small; 32 bytes of a row past the caches lost a quarter.)
+void outputs_pass(hipStream_t st, int dtype, AttnArgs a, int batch) {
   const int D = padded(a.role[0].x.width, a.role[0].z.width);
+  int64_t columns = 0;
+  for (int i = 0; i < a.roles; ++i) columns += a.role[i].z.width;
+  a.streamed = (int64_t)batch * a.steps * a.heads * columns * (dtype == ATTN_F32 ? 4 : 2) >= 64 << 20;
   const unsigned grid = (unsigned)((int64_t)batch * a.heads * a.segments * a.roles);
   if (dtype == ATTN_F32) launch_width<float, false>(st, a, D, grid);
   else launch_width<uint16_t, false>(st, a, D, grid);

@@ -420,6 +420,38 @@ def test_work_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(8192, 70, 2, 2, 20, 33), (12000, 69, 2, 2, 24, 32), (8192, 65, 2, 2, 64, 64),
+                                   (4096, 70, 2, 2, 128, 120), (8192, 66, 2, 1, 40, 64)])
+def test_large_batches_are_their_parts(shape, dtype):
+    """Outputs large enough to be streamed, an infinity and a NaN among them: to
+    the bit those of eighths of the batch, which are not."""
+    _, T, H, G, K, V = shape
+    B = shape[0] * 2 // dtype.itemsize
+    assert B * T * H * V * dtype.itemsize >= 64 << 20
+    assert B // 8 * T * H * (2 * K + V) * dtype.itemsize < 64 << 20
+    gen = torch.Generator("cuda").manual_seed(sum(shape))
+    q, k, v, dout = (torch.randn(B, T, h, d, generator=gen, device="cuda").to(dtype)
+                     for h, d in ((H, K), (G, K), (G, V), (H, V)))
+    q[5, 30, 0, 3], k[B // 2, 11, 0, 1], v[B - 1, T - 2, 0, 0] = float("inf"), float("nan"), float("-inf")
+    carry = torch.randn(B, H, K, V, generator=gen, device="cuda")
+    done = torch.rand(B, T, generator=gen, device="cuda") < 0.01
+    lengths = torch.randint(0, T + 1, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    lengths[[5, B // 2, B - 1]] = T
+    g = torch.tensor([-0.01, -0.2], device="cuda")
+
+    def both_passes(rows):
+        leaves = [x[rows].requires_grad_() for x in (q, k, v, carry)]
+        final, out = linear_attention(*leaves[:3], g, carry=leaves[3], done=done[rows], lengths=lengths[rows])
+        return final.detach(), out.detach(), *torch.autograd.grad(out, leaves, dout[rows])
+
+    whole = both_passes(slice(0, B))
+    for i in range(8):
+        rows = slice(i * B // 8, (i + 1) * B // 8)
+        for a, b in zip(whole, both_passes(rows)):
+            torch.testing.assert_close(a[rows], b, rtol=0, atol=0, equal_nan=True)
+
+
 def test_two_graphs_and_two_streams_at_once():
     """Two captured passes, replayed at the same time, and two eager calls: each
     has its own workspace."""
