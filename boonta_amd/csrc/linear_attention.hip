@@ -291,8 +291,10 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
-// Waits for this wave's loads.  Before the stores that follow a chunk, and on
-// every way to the next chunk: what is waited for later counts the stores too.
+// Waits for this wave's loads: before the streamed stores, and where a chunk
+// begins without them, since what is waited for later counts the stores too.
+// (Without: both passes of 128 x 1000 steps, 8 heads of 64, 431 -> 435 us,
+// float32 ones of 4 x 4000 steps, 4 heads of 128, 317 -> 321.)
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // (no other counter)
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -317,11 +319,11 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // products' operands in 128 registers, four waves a SIMD: 64-wide bf16 takes
 // 40 KB of LDS, four workgroups a CU, 128-wide 73 KB, two.  Bound by HBM with a
 // chunk's LDS and vector work close behind.  Measured, bf16: 128 x 1000 steps,
-// 8 heads of 64 with resets, forward 140 us (558 MB, 4.0 TB/s), backward 305
-// (1.37 GB, 4.5 TB/s); 65536 steps, 16 heads of 128, states 125 us (553 MB, 4.4
-// TB/s) and outputs 245 (1.11 GB, 4.5 TB/s); 8 x 4096 steps, 16 heads of 128,
+// 8 heads of 64 with resets, forward 130 us (558 MB, 4.3 TB/s), backward 298
+// (1.32 GB, 4.4 TB/s); 65536 steps, 16 heads of 128, states 124 us (553 MB, 4.5
+// TB/s) and outputs 236 (1.11 GB, 4.7 TB/s); 8 x 4096 steps, 16 heads of 128,
 // states 60 to 70 us (227 MB: one and a half workgroups a CU, bound by
-// instructions), outputs 140, backward 390 (1.49 GB, 3.8 TB/s, vector
+// instructions), outputs 140, backward 385 (1.44 GB, 3.8 TB/s, vector
 // instructions issuing 47 % of the time).  float32, 256 x 64 steps, 4 heads of
 // 64: 30 us, a third of it matrix products (16x16x4), backward 72.
 template <typename T, int D, bool STATE>
