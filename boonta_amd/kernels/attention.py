@@ -17,6 +17,7 @@ the kernels run on the device the tensors live on, on its current stream, and ca
 be captured into a graph.  Before a backward pass is captured, drop every eager
 autograd graph of the same leaves: such a graph keeps the leaves' gradient nodes
 on the stream it was made on, which a capture on another stream must not join.
+Forward-mode tangents are refused.
 At most 2^21 sequences of linear_attention (batch * heads), 2^23 - 1 of its
 step; larger ones are refused.
 """
@@ -25,6 +26,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.nn.functional import pad
 
@@ -34,8 +36,16 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _MAX_STRIDE = 1 << 23   # of a step, in elements: the kernels count a chunk's bytes in 32 bits
 
 
+def _no_tangents(name, *tensors):
+    """Refuses forward-mode tangents, which a launch would drop: their tensors need not require gradients."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # (inside a dual level: elsewhere no tensor has one)
+        if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+            raise NotImplementedError(f"{name} has no forward-mode derivatives")
+
+
 def _on_device(name, *tensors):
     """The index of the device that all of them (None aside) are on."""
+    _no_tangents(name, *tensors)
     index = tensors[0].get_device()   # (-1: the host)
     for x in tensors:
         if x is not None and x.get_device() != index:
@@ -142,6 +152,7 @@ class _LinearAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dfinal, dout):
+        _no_tangents("linear_attention", dfinal, dout)
         q, k, v, log_decay, carry, done, lengths, states = ctx.saved_tensors
         batch, steps, heads, kv_heads, key, value = ctx.sizes
         dt = _DTYPES[q.dtype]
@@ -260,6 +271,7 @@ class _QKNormRotary(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
+        _no_tangents("qk_norm_rotary", gq, gk)
         q, k, q_scale, k_scale, frequencies, positions = ctx.saved_tensors
         epsilon, interleaved = ctx.options
         batch, steps, heads, width = q.shape

@@ -74,6 +74,45 @@ def test_qk_norm_rotary_refuses_what_it_does_not_take():
     refused(ValueError, "positions", qk_norm_rotary, q, k, positions=torch.zeros(3, dtype=torch.int32))
 
 
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor does not require gradients, so a plain launch would drop its tangent."""
+    from torch.autograd import forward_ad
+    q, k, v, g = operands()
+    carry = torch.zeros(2, 4, 8, 6)
+    first = [q[:, 0], k[:, 0], v[:, 0], g, carry]
+    norms = [q, k, torch.ones(8), torch.ones(8), rotary_frequencies(8, device="cpu")]
+    with forward_ad.dual_level():
+        for f, args in ((linear_attention, [q, k, v, g, carry]), (linear_attention_step, first), (qk_norm_rotary, norms)):
+            for i, x in enumerate(args):
+                dual = [*args[:i], forward_ad.make_dual(x, torch.ones_like(x)), *args[i + 1:]]
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad):
+                        refused(NotImplementedError, "forward-mode", f, *dual)
+            refused(TypeError, "device", f, *args)
+        narrow = operands(K=3, V=2)
+        refused(NotImplementedError, "forward-mode", linear_attention,
+                forward_ad.make_dual(narrow[0], torch.ones_like(narrow[0])), *narrow[1:])
+        refused(NotImplementedError, "forward-mode", linear_attention_step, *first,
+                out_carry=forward_ad.make_dual(torch.zeros(2, 4, 8, 6), torch.ones(2, 4, 8, 6)))
+
+
+def test_forward_mode_tangents_of_cotangents_are_refused(monkeypatch):
+    """Their launches stubbed out: what is refused is refused before them."""
+    from torch.autograd import forward_ad
+    from boonta_amd.kernels import attention
+    monkeypatch.setattr(attention, "_on_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda *a: None)
+    q, k, v, g = operands()
+    calls = ((lambda: linear_attention(q.requires_grad_(), k, v, g), "linear_attention has no forward-mode"),
+             (lambda: qk_norm_rotary(q.requires_grad_(), k), "qk_norm_rotary has no forward-mode"))
+    for call, match in calls:
+        for i in (0, 1):
+            with forward_ad.dual_level():
+                out = call()[i]
+                dual = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+                refused(NotImplementedError, match, torch.autograd.grad, out, q, dual)
+
+
 def test_the_entry_points_refuse_without_launching():
     lib = _lib.load()
     st = (ctypes.c_int64 * 12)(*[0] * 12)
