@@ -71,7 +71,7 @@ template <typename T> struct Type;
 
 template <> struct Type<uint16_t> {
   typedef bf16x8 Frag;
-  static constexpr int FR = 8, C = 64, PIECES = 3;
+  static constexpr int FR = 8, C = 64, PIECES = 3, PARTS = 2;
   static __device__ __forceinline__ constexpr int row(int rt, int slot) {
     return 32 * (rt >> 1) + 4 * (rt & 1) + 8 * (slot >> 2) + (slot & 3);
   }
@@ -81,7 +81,7 @@ template <> struct Type<uint16_t> {
 };
 template <> struct Type<float> {
   typedef floatx4 Frag;
-  static constexpr int FR = 4, C = 32, PIECES = 1;
+  static constexpr int FR = 4, C = 32, PIECES = 1, PARTS = 1;
   static __device__ __forceinline__ constexpr int row(int rt, int slot) { return 16 * rt + slot; }
   static __device__ __forceinline__ floatx4 mma(Frag a, Frag b, floatx4 c) {
 #pragma unroll
@@ -99,13 +99,22 @@ __device__ __forceinline__ bf16x8 join(floatx4 lo, floatx4 hi) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// The state as an operand over its rows: contraction block kb.
-// bf16: the state itself stays float32; what enters the product is rounded
-// once, an error of the size of the output's own rounding.
-template <int RT> __device__ __forceinline__ bf16x8 state_frag(const floatx4 (&s)[RT], int kb, uint16_t) {
-  return join(s[2 * kb], s[2 * kb + 1]);
+// The state as operands over its rows: contraction block kb, whose products
+// are summed.  bf16: the state itself stays float32, and two pieces of it enter
+// the product, as of the pair products: what they leave is at most 2^-17 of a
+// term, where one bf16 would leave as much as the output's own rounding (outputs
+// 2.4e-3 off in the norm in place of 1.7e-3).  (A second piece, against one:
+// both passes of 128 x 1000 steps, 8 heads of 64, 432 -> 470 us, of 8 x 4096
+// steps, 16 heads of 128, 611 -> 680; a third would gain nothing that an output
+// in bf16 shows.)
+template <int RT> __device__ __forceinline__ void state_frags(const floatx4 (&s)[RT], int kb, bf16x8 (&p)[2]) {
+  floatx4 lo = s[2 * kb], hi = s[2 * kb + 1];
+  p[0] = ppo::split_piece(lo, hi);
+  p[1] = join(lo, hi);
 }
-template <int RT> __device__ __forceinline__ floatx4 state_frag(const floatx4 (&s)[RT], int kb, float) { return s[kb]; }
+template <int RT> __device__ __forceinline__ void state_frags(const floatx4 (&s)[RT], int kb, floatx4 (&p)[1]) {
+  p[0] = s[kb];
+}
 
 // z times its steps' weights, as operands whose sum is the product to float32:
 // one float32, or three bf16 pieces, each what the ones before leave (the
@@ -327,17 +336,23 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // instructions issuing 47 % of the time).  float32, 256 x 64 steps, 4 heads of
 // 64: 30 us, a third of it matrix products (16x16x4), backward 72.
 template <typename T, int D, bool STATE>
-__global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(4 * D, D == 96 ? 2 : D == 32 ? 3 : 4) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
   constexpr int FR = Type<T>::FR, C = Type<T>::C, W = D / 16, KB = D / (4 * FR), RT = D / 16, QT = C / 16;
-  constexpr int PIECES = Type<T>::PIECES;
-  constexpr int RB = D * (int)sizeof(T), ROWS = C * RB, COLS = D * 128;
+  constexpr int PIECES = Type<T>::PIECES, PARTS = Type<T>::PARTS, TILES = QT * (QT + 1) / 2;
+  constexpr int RB = D * (int)sizeof(T), ROWS = C * RB, COLS = D * 128, PAIRS = C * 96;
+  // The pair products' second pieces: after the first ones, or, where that would
+  // leave a workgroup less a CU (64-wide: 46 KB; forward 134 -> 162 us, backward
+  // 336 -> 367), in place of y's rows (and what those lack) once the pair
+  // products are formed.
+  constexpr bool OVER_Y = PARTS == 2 && D <= 64;
+  constexpr int MORE = !OVER_Y ? (PARTS - 1) * PAIRS : ROWS < PAIRS ? PAIRS - ROWS : 0;
   // Streamed outputs go through LDS to be stored in whole rows.  (96-wide, rows
   // of one and a half lines and few waves: 175 -> 181 us, so not there.)
   constexpr bool ROWS_OUT = !STATE && D != 96;
   // y and z by columns, x and y by rows, and the pair products: all queries
   // with the chunk's first half of keys, the later half with the other
-  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + C * 96) + 2 * COLS];
+  __shared__ __attribute__((aligned(16))) char smem[(STATE ? 0 : 2 * ROWS + MORE + PAIRS) + 2 * COLS];
   __shared__ __attribute__((aligned(16))) float weights[C];  // of the chunk's steps in the state after it
   __shared__ float reaches[C];                               // factors of x St
   __shared__ float powers[16 + C];                           // intra lam^d at 16 + d
@@ -346,7 +361,8 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
   char* const zt = smem + COLS;
   char* const xr = smem + 2 * COLS;
   char* const yr = smem + 2 * COLS + ROWS;
-  char* const pr = smem + 2 * COLS + 2 * ROWS;
+  char* const pr = smem + 2 * COLS + 2 * ROWS + (OVER_Y ? MORE : 0);
+  char* const pr_low = OVER_Y ? yr : pr + PAIRS;
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -466,13 +482,14 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
   if (tid < 2) odd[tid] = 0;
   if (tid < 16 + C) powers[tid] = tid < 16 ? 0.f : c.intra * power(g2, tid - 16);
   if constexpr (!STATE)
-    for (int i = tid; i < C * 6; i += 4 * D) reinterpret_cast<uint4*>(pr)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < (MORE + PAIRS) / 16; i += 4 * D)
+      reinterpret_cast<uint4*>(smem + 2 * COLS + 2 * ROWS)[i] = make_uint4(0, 0, 0, 0);
   lds_barrier();
 
   // Whether the state itself is an output (or, STATE, leads to one): the third
-  // piece of its terms (2^-17 of them) is below what a state keeps that only
-  // enters products, rounded to bf16 (2^-8).  With it, 16 heads of 128: 65536
-  // steps 388 -> 406 us, both passes of 8 x 4096 steps 640 -> 675 us.
+  // piece of its terms (2^-17 of them) is no more than what a state loses that
+  // only enters products, in two pieces.  With it, 16 heads of 128: 65536 steps
+  // 415 -> 430 us, both passes of 8 x 4096 steps 682 -> 720 us.
   const bool exact = c.final && (STATE || seg == p.segments - 1);
   uint64_t cut = 0;   // the chunk's steps that drop the state
   // Lays out steps r0 .. r0 + n - 1, as loaded, and loads the chunk from `next` (>= 0) on.
@@ -531,10 +548,15 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
         // pair products, keys as rows so that a lane holds four keys of one
         // query: tile (qt, kt) of the lower triangle, dealt to the waves
         const int pair_byte = l16 * 64 + ((g4 ^ (l16 >> 2)) << 4);
-#pragma unroll 1
-        for (int idx = wave; idx < QT * (QT + 1) / 2; idx += W) {
-          // (0, 0), (1, 0), (1, 1), ..: two bits a tile
-          const int qt = 0xffa94u >> (2 * idx) & 3, kt = 0xe4910u >> (2 * idx) & 3;
+        // (0, 0), (1, 0), (1, 1), ..: two bits a tile
+        auto query_tile = [](int idx) { return (int)(0xffa94u >> (2 * idx) & 3); };
+        auto key_tile = [](int idx) { return (int)(0xe4910u >> (2 * idx) & 3); };
+        auto half_byte = [&](int qt, int kt) {  // bf16: of this lane's four keys
+          const int chunk = 2 * (kt & 1) + (g4 >> 1);
+          return l16 * 64 + ((chunk ^ (l16 >> 2)) << 4) + ((g4 & 1) << 3) + qt * 1024 + (kt >> 1) * C * 32;
+        };
+        auto pair = [&](int idx, uint2& low) {  // low: the second pieces, where they are written later
+          const int qt = query_tile(idx), kt = key_tile(idx);
           floatx4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
@@ -555,13 +577,39 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
 #pragma unroll
             for (int e = 0; e < 4; ++e) a[e] = keep_if(a[e], j0 + e <= i);
           }
-          if constexpr (sizeof(T) == 2) {
-            const int chunk = 2 * (kt & 1) + (g4 >> 1);
-            *reinterpret_cast<uint2*>(pr + l16 * 64 + ((chunk ^ (l16 >> 2)) << 4) + ((g4 & 1) << 3) + qt * 1024 +
-                                      (kt >> 1) * C * 32) = make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
+          if constexpr (PARTS == 2) {
+            const int at = half_byte(qt, kt);
+            const uint32_t u = pack_bf16(a[0], a[1]), w = pack_bf16(a[2], a[3]);
+            *reinterpret_cast<uint2*>(pr + at) = make_uint2(u, w);
+            a[0] -= __uint_as_float(u << 16);
+            a[1] -= __uint_as_float(u & 0xffff0000u);
+            a[2] -= __uint_as_float(w << 16);
+            a[3] -= __uint_as_float(w & 0xffff0000u);
+            low = make_uint2(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]));
+            if constexpr (!OVER_Y) *reinterpret_cast<uint2*>(pr_low + at) = low;
           } else {
             *reinterpret_cast<floatx4*>(pr + pair_byte + qt * 1024 + kt * C * 32) = a;
           }
+        };
+        if constexpr (OVER_Y) {
+          constexpr int DEALT = (TILES + W - 1) / W;
+          uint2 low[DEALT];
+#pragma unroll
+          for (int i = 0; i < DEALT; ++i)
+            if (wave + i * W < TILES) pair(wave + i * W, low[i]);
+          lds_barrier();
+#pragma unroll
+          for (int i = 0; i < DEALT; ++i)
+            if (wave + i * W < TILES) {
+              const int qt = query_tile(wave + i * W), kt = key_tile(wave + i * W);
+              *reinterpret_cast<uint2*>(pr_low + half_byte(qt, kt)) = low[i];
+              // the masked tile that the products take with an even diagonal one (of the first pieces it stays zero)
+              if (kt == qt && !(kt & 1)) *reinterpret_cast<uint2*>(pr_low + half_byte(qt, kt + 1)) = make_uint2(0, 0);
+            }
+        } else {
+          uint2 low;
+#pragma unroll 1
+          for (int idx = wave; idx < TILES; idx += W) pair(idx, low);
         }
         // x times the entry state (rows: its columns)
         floatx4 acc[QT];
@@ -569,11 +617,14 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
         for (int qt = 0; qt < QT; ++qt) acc[qt] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          const Frag s = state_frag(S, kb, T());
+          Frag s[PARTS], x[QT];
+          state_frags(S, kb, s);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            acc[qt] = Type<T>::mma(
-                s, *reinterpret_cast<const Frag*>(xr + row_byte<RB>(l16, g4, qt, kb)), acc[qt]);
+          for (int qt = 0; qt < QT; ++qt) x[qt] = *reinterpret_cast<const Frag*>(xr + row_byte<RB>(l16, g4, qt, kb));
+#pragma unroll
+          for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) acc[qt] = Type<T>::mma(s[q], x[qt], acc[qt]);
         }
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -587,14 +638,19 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : 4) attention_kernel(AttnA
         }
         lds_barrier();
         // the pair products times z, and the outputs
+        Frag z[2];
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-          const Frag z = *reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb));
+        for (int tb = 0; tb < 2; ++tb) z[tb] = *reinterpret_cast<const Frag*>(zt + tile_byte(lane_byte, wave, tb));
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            if (16 * qt + 15 < 4 * FR * tb) continue;  // keys after the queries
-            acc[qt] = Type<T>::mma(z, *reinterpret_cast<const Frag*>(pr + pair_byte + qt * 1024 + tb * C * 32), acc[qt]);
-          }
+        for (int q = PARTS - 1; q >= 0; --q) {
+          const char* const a = (q ? pr_low : pr) + pair_byte;
+#pragma unroll
+          for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              if (16 * qt + 15 < 4 * FR * tb) continue;  // keys after the queries
+              acc[qt] = Type<T>::mma(z[tb], *reinterpret_cast<const Frag*>(a + qt * 1024 + tb * C * 32), acc[qt]);
+            }
         }
         if (!streamed) {
           const int size = c.wide ? 4 : (int)sizeof(T), n0 = 16 * wave + 4 * g4;

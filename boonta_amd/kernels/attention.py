@@ -12,7 +12,13 @@ reference, whose attention block is boonta/networks/blocks/self_attention.py.
   differentiable in q, k and the scales; ``rotary_frequencies`` makes its
   usual frequencies.
 
-float32 or bfloat16 storage; states, sums and norms are float32.  There is no CPU path:
+float32 or bfloat16 storage; states, sums and norms are float32, and outputs are
+rounded to their type once.  Inside a bfloat16 sequence the pair products and
+the states enter matrix products as two bfloat16 pieces (16 bits or more of
+their 24), and a state that is neither an output nor leads to one is formed from
+terms of two pieces: what these leave, at most 2^-17 of a term each, is small
+beside the outputs' rounding of 2^-8.  The step and the final carry keep all 24.
+There is no CPU path:
 the kernels run on the device the tensors live on, on its current stream, and can
 be captured into a graph.  Before a backward pass is captured, drop every eager
 autograd graph of the same leaves: such a graph keeps the leaves' gradient nodes

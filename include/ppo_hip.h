@@ -369,7 +369,8 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  *   o_t = scale q_t S_t
  * for t < lengths[b]; later rows of q, k, v are not read and those of the
  * outputs and gradients are zeros.  dtype 0 = float32, 1 = bf16 storage of q,
- * k, v, out and their gradients; the states are float32.
+ * k, v, out and their gradients; the states are float32, and bf16 sequences'
+ * pair products and states enter products as two bf16 pieces.
  *   q [batch, steps, heads, key_width], k [batch, steps, kv_heads, key_width],
  *   v [batch, steps, kv_heads, value_width]: columns side by side, element
  *   strides of (batch, step, head) in the host array `strides`, 3 for each of

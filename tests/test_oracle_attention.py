@@ -66,3 +66,41 @@ def test_norm_gradients_match_differences(interleaved):
         dx, _difference(lambda y: (oat.norm_rotary(y, scale, f, pos, 1e-6, interleaved) * cot).sum(), x), atol=1e-8)
     np.testing.assert_allclose(
         dscale, _difference(lambda y: (oat.norm_rotary(x, y, f, pos, 1e-6, interleaved) * cot).sum(), scale), atol=1e-8)
+
+
+def _bf16(x):
+    bits = np.asarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    return ((bits + 0x7fff + (bits >> 16 & 1)) >> 16 << 16).astype(np.uint32).view(np.float32).astype(np.float64)
+
+
+def _pieces(x, count):
+    """The sum of the bf16 values nearest to x and to what the ones before leave."""
+    x, total = np.asarray(x, np.float32).astype(np.float64), 0.0
+    for _ in range(count):
+        p = _bf16(x)
+        x, total = x - p, total + p
+    return total
+
+
+@pytest.mark.parametrize("width", [32, 128])
+def test_the_norms_bounds_tell_one_piece_from_two_and_two_from_three(width):
+    """What the bounds of test_gpu_attention_precision.py see: a state whose
+    decayed terms keep two bf16 pieces is outside the float32 bound, with three
+    inside; outputs whose pair products keep one piece before bf16's own
+    rounding are outside the bf16 bounds, with two inside."""
+    rng = np.random.default_rng(2)
+    T, g = 300, -0.003
+    q, k, v = (_bf16(rng.normal(size=(T, width))) for _ in range(3))
+    i = np.arange(T)
+    w = np.exp(g * (T - 1 - i)).astype(np.float32).astype(np.float64)
+    state = k.T @ (v * w[:, None])
+    off = [np.linalg.norm(k.T @ _pieces(v * w[:, None], n) - state) / np.linalg.norm(state) for n in (2, 3)]
+    assert off[1] < 1e-7 and 1e-6 < off[0] < 1e-5
+    weights = np.where(i[:, None] >= i, np.exp(g * (i[:, None] - i)), 0) * width ** -0.5
+    pairs, terms = (q @ k.T) * weights, (np.abs(q) @ np.abs(k.T) * weights) @ np.abs(v)
+    out = pairs @ v
+    for n, inside in ((1, False), (2, True)):
+        off = np.abs(_bf16(_pieces(pairs, n) @ v) - out)
+        tol = 2.0 ** -16 * terms
+        assert (off <= tol + 2.0 ** -8 * (np.abs(out) + tol)).all() == inside
+        assert (np.linalg.norm(off) <= 2.0 ** -8 / 3 ** 0.5 * np.linalg.norm(out)) == inside
