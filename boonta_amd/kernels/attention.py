@@ -109,6 +109,14 @@ def _check_heads(name, q, k, v, dims):
 
 
 _max_width = 0
+_min_widths = {}   # by dtype
+
+
+def _min_width(dt):
+    width = _min_widths.get(dt)
+    if width is None:
+        width = _min_widths[dt] = _lib.load().ppo_linear_attention_min_width(dt)
+    return width
 
 
 def _check_attention(name, q, k, v, log_decay, carry, done, dims):
@@ -203,10 +211,13 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     _on_device("linear_attention", q, k, v, log_decay, carry, done, lengths)
     key, value = sizes[4:]
     scale = key ** -0.5 if scale is None else float(scale)
-    least = 16 // q.element_size()
+    least = _min_width(_DTYPES[q.dtype])
     if key < least or value < least:   # the kernels read rows 16 bytes at a time
         more_k, more_v = max(least - key, 0), max(least - value, 0)
-        q, k, v = pad(q, (0, more_k)), pad(k, (0, more_k)), pad(v, (0, more_v))
+        if more_k:   # (padding by nothing copies)
+            q, k = pad(q, (0, more_k)), pad(k, (0, more_k))
+        if more_v:
+            v = pad(v, (0, more_v))
         carry = None if carry is None else pad(carry, (0, more_v, 0, more_k))
         carry, out = linear_attention(q, k, v, log_decay, carry, done, lengths, scale)
         return carry[..., :key, :value].contiguous(), out[..., :value].contiguous()

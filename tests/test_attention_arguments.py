@@ -113,6 +113,23 @@ def test_forward_mode_tangents_of_cotangents_are_refused(monkeypatch):
                 refused(NotImplementedError, match, torch.autograd.grad, out, q, dual)
 
 
+@pytest.mark.parametrize("dtype,least", [(torch.float32, 4), (torch.bfloat16, 8)])
+def test_only_operands_of_narrow_heads_are_padded(dtype, least, monkeypatch):
+    """The launch gets the other operands as they are."""
+    from boonta_amd.kernels import attention
+    calls = []
+    monkeypatch.setattr(attention, "_on_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda index, name, *a: calls.append(a))
+    for K, V in ((least, least), (least, least - 1), (least - 1, least), (1, 1)):
+        q, k, v, g = operands(K=K, V=V, dtype=dtype)
+        carry, out = linear_attention(q, k, v, g)
+        assert carry.shape == (2, 4, K, V) and out.shape == (2, 3, 4, V)
+        passed, widths = calls[-1][1:4], calls[-1][-2:]
+        assert widths == (max(K, least), max(V, least))
+        for x, at, width in ((q, passed[0], K), (k, passed[1], K), (v, passed[2], V)):
+            assert (x.data_ptr() == at) == (width >= least)
+
+
 def test_the_entry_points_refuse_without_launching():
     lib = _lib.load()
     st = (ctypes.c_int64 * 12)(*[0] * 12)
