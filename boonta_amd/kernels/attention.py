@@ -74,11 +74,13 @@ def _launch(index, name, *args):
 
 
 def _rows(x):
+    """x, or a copy where its columns are not side by side."""
+    return x.contiguous() if x.stride(-1) != 1 and x.shape[-1] > 1 else x
+
+
+def _near_rows(x):
     """x, or a copy where its columns are not side by side or its steps too far apart."""
-    st = x.stride()
-    if (st[-1] != 1 and x.shape[-1] > 1) or (len(st) == 4 and st[1] > _MAX_STRIDE and x.shape[1] > 1):
-        return x.contiguous()
-    return x
+    return x.contiguous() if x.stride(1) > _MAX_STRIDE and x.shape[1] > 1 else _rows(x)
 
 
 _STRIDES = {n: ctypes.c_int64 * n for n in (6, 9, 12)}
@@ -172,7 +174,7 @@ class _LinearAttention(torch.autograd.Function):
         dt = _DTYPES[q.dtype]
         if dout is None:   # (only the final carry was used)
             dout = q.new_zeros(value).expand(batch, steps, heads, value)
-        dout = _rows(dout)
+        dout = _near_rows(dout)
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq = q.new_empty((batch, steps, heads, key))
         dk = q.new_empty((batch, steps, kv_heads, key))
@@ -221,7 +223,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         carry = None if carry is None else pad(carry, (0, more_v, 0, more_k))
         carry, out = linear_attention(q, k, v, log_decay, carry, done, lengths, scale)
         return carry[..., :key, :value].contiguous(), out[..., :value].contiguous()
-    args = (_rows(q), _rows(k), _rows(v), log_decay.contiguous(), None if carry is None else carry.contiguous(),
+    args = (_near_rows(q), _near_rows(k), _near_rows(v), log_decay.contiguous(), None if carry is None else carry.contiguous(),
             None if done is None else done.contiguous(), None if lengths is None else lengths.contiguous(), scale, sizes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (carry is not None and carry.requires_grad)):

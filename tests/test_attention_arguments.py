@@ -113,6 +113,19 @@ def test_forward_mode_tangents_of_cotangents_are_refused(monkeypatch):
                 refused(NotImplementedError, match, torch.autograd.grad, out, q, dual)
 
 
+def test_steps_far_apart_are_copied_where_the_kernel_needs_it(monkeypatch):
+    """The norms count in 64 bits: theirs stay where they are."""
+    from boonta_amd.kernels import attention
+    calls = []
+    monkeypatch.setattr(attention, "_on_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda index, name, *a: calls.append(a))
+    far = torch.zeros((1 << 23) + 64, dtype=torch.bfloat16).as_strided((1, 2, 1, 8), (0, (1 << 23) + 8, 8, 1))
+    qk_norm_rotary(far, far)
+    assert calls[-1][1:3] == (far.data_ptr(), far.data_ptr())
+    linear_attention(far, far, far, torch.zeros(1))
+    assert far.data_ptr() not in calls[-1][1:4] and all(s <= 1 << 23 for s in calls[-1][4])
+
+
 @pytest.mark.parametrize("dtype,least", [(torch.float32, 4), (torch.bfloat16, 8)])
 def test_only_operands_of_narrow_heads_are_padded(dtype, least, monkeypatch):
     """The launch gets the other operands as they are."""

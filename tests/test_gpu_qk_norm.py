@@ -169,3 +169,16 @@ def test_a_captured_pass_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+
+def test_steps_far_apart():
+    """A time-major batch wider than 2^23 elements a step, read where it is, forward and backward."""
+    wide = torch.randn((2 << 23) + 512, generator=torch.Generator().manual_seed(9)).to(BF16).cuda()
+    q = wide.as_strided((1, 3, 2, 64), (0, (1 << 23) + 64, 64, 1)).requires_grad_()
+    near = q.detach().clone().contiguous().requires_grad_()
+    assert q.stride(1) > 1 << 23 and near.is_contiguous()
+    cot = wide.as_strided((1, 3, 2, 64), (0, (1 << 23) + 128, 64, 1))
+    f = rotary_frequencies(64)
+    a, b = (qk_norm_rotary(x, x.detach(), frequencies=f) for x in (q, near))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(*(torch.autograd.grad(x, y, cot)[0] for x, y in ((a[0], q), (b[0], near))))
