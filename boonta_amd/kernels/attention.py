@@ -24,8 +24,10 @@ be captured into a graph.  Before a backward pass is captured, drop every eager
 autograd graph of the same leaves: such a graph keeps the leaves' gradient nodes
 on the stream it was made on, which a capture on another stream must not join.
 Forward-mode tangents are refused.
-At most 2^21 sequences of linear_attention (batch * heads), 2^23 - 1 of its
-step; larger ones are refused.
+
+Limits, past which a call is refused: linear_attention 2^21 sequences (batch *
+heads), its step 2^23 - 1, both 65536 heads and 2^30 steps; qk_norm_rotary 8192
+heads of either operand and 2^31 - 1 rows of steps (batch * steps).
 """
 from __future__ import annotations
 
@@ -206,7 +208,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     [batch], steps of each sequence: what follows in q, k, v is not read, and
     its outputs and gradients are zeros.  scale: key ** -0.5 by default.
     Widths up to 128.  A step's infinities and NaN reach the outputs that the
-    recurrence gives them to, and no others."""
+    recurrence gives them to, and no others; what the recurrence gives an
+    infinity may come out as NaN."""
     sizes = _check_attention("linear_attention", q, k, v, log_decay, carry, done, 4)
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != sizes[:1]):
         raise ValueError(f"lengths must be int32 [{sizes[0]}], got {lengths.dtype} {tuple(lengths.shape)}")

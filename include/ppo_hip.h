@@ -378,7 +378,8 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  *   one step) is at most 2^23 and none is negative.
  *   heads / kv_heads query heads in a row share a key head.  Widths are at most
  *   ppo_linear_attention_max_width(), and of sequences at least
- *   ppo_linear_attention_min_width(dtype) (16 bytes).
+ *   ppo_linear_attention_min_width(dtype) (16 bytes).  At most 65536 heads,
+ *   2^30 steps, and 2^21 sequences (batch x heads; of one step 2^23 - 1).
  *   log_decay float [heads] (<= 0; -inf: no memory), carry / final float
  *   [batch, heads, key_width, value_width] (carry may be NULL: zeros), done
  *   uint8 [batch, steps] (NULL: none), lengths int32 [batch] (NULL: steps),
@@ -420,7 +421,8 @@ int ppo_linear_attention_step(void* stream, int dtype, const void* q, const void
  * outputs and gradients contiguous.  scales float [width] (NULL: ones),
  * frequencies double [pairs] in radians, positions int32 [batch, steps] (NULL:
  * the step).  dtype 0 = float32, 1 = bf16 storage.  width at most
- * ppo_qk_norm_rotary_max_width(). */
+ * ppo_qk_norm_rotary_max_width(), heads and kv_heads at most 8192, batch x steps
+ * at most 2^31 - 1. */
 int ppo_qk_norm_rotary_max_width(void);
 int ppo_qk_norm_rotary_fwd(void* stream, int dtype, const void* q, const void* k, const int64_t* strides,
                            const float* q_scale, const float* k_scale, const double* frequencies,

@@ -74,6 +74,34 @@ def test_qk_norm_rotary_refuses_what_it_does_not_take():
     refused(ValueError, "positions", qk_norm_rotary, q, k, positions=torch.zeros(3, dtype=torch.int32))
 
 
+def test_the_limits_are_those_stated():
+    """One past each of the header's limits is refused, and says which."""
+    lib = _lib.load()
+    st = (ctypes.c_int64 * 12)(*[0] * 12)
+
+    def refusal(f, *args):
+        assert f(*args) == -1
+        return lib.ppo_last_error().decode()
+
+    def sequences(batch, steps, heads):
+        return refusal(lib.ppo_linear_attention_fwd, None, 0, 1, 1, 1, st, 1, None, None, None, 1.0, 1, 1, None, 0, batch,
+                       steps, heads, heads, 8, 8)
+
+    def step(batch, heads):
+        return refusal(lib.ppo_linear_attention_step, None, 0, 1, 1, 1, st, 1, None, 1, 1, 1, 1.0, batch, heads, heads, 8, 8)
+
+    def norms(batch, steps, heads, kv_heads):
+        return refusal(lib.ppo_qk_norm_rotary_fwd, None, 0, 1, 1, st, None, None, None, None, 1e-6, 0, 1, 1, batch, steps,
+                       heads, kv_heads, 8, 0)
+
+    assert "heads above 65536" in sequences(1, 4, 65537) and "steps above 2^30" in sequences(1, (1 << 30) + 1, 1)
+    assert f"batch x heads above {1 << 21}" in sequences((1 << 21) + 1, 4, 1)
+    assert f"batch x heads above {(1 << 23) - 1}" in step(1 << 23, 1) and "heads above 65536" in step(1, 65537)
+    assert "heads above 8192" in norms(1, 1, 8193, 1) and "heads above 8192" in norms(1, 1, 1, 8193)
+    assert "batch x steps above" in norms(1 << 16, 1 << 15, 1, 1)
+    lib.ppo_clear_error()
+
+
 def test_forward_mode_tangents_are_refused():
     """A dual tensor does not require gradients, so a plain launch would drop its tangent."""
     from torch.autograd import forward_ad
