@@ -104,8 +104,8 @@ __device__ __forceinline__ bf16x8 join(floatx4 lo, floatx4 hi) {
 // the product, as of the pair products: what they leave is at most 2^-17 of a
 // term, where one bf16 would leave as much as the output's own rounding (outputs
 // 2.4e-3 off in the norm in place of 1.7e-3).  (A second piece, against one:
-// both passes of 128 x 1000 steps, 8 heads of 64, 432 -> 470 us, of 8 x 4096
-// steps, 16 heads of 128, 611 -> 680; a third would gain nothing that an output
+// both passes of 128 x 1000 steps, 8 heads of 64, 432 -> 469 us, of 8 x 4096
+// steps, 16 heads of 128, 611 -> 672; a third would gain nothing that an output
 // in bf16 shows.)
 template <int RT> __device__ __forceinline__ void state_frags(const floatx4 (&s)[RT], int kb, bf16x8 (&p)[2]) {
   floatx4 lo = s[2 * kb], hi = s[2 * kb + 1];
@@ -302,8 +302,8 @@ __device__ __forceinline__ int here(int x) {
 
 // Waits for this wave's loads: before the streamed stores, and where a chunk
 // begins without them, since what is waited for later counts the stores too.
-// (Without: both passes of 128 x 1000 steps, 8 heads of 64, 431 -> 435 us,
-// float32 ones of 4 x 4000 steps, 4 heads of 128, 317 -> 321.)
+// (Without, products of one piece: both passes of 128 x 1000 steps, 8 heads of
+// 64, 431 -> 435 us, float32 ones of 4 x 4000 steps, 4 heads of 128, 317 -> 321.)
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // (no other counter)
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -326,15 +326,16 @@ __device__ __forceinline__ float power(float g2, int e) { return __builtin_amdgc
 // for the segments before the last.
 // Sixteen columns a wave keep a 128 x 128 state, the chunk ahead and the
 // products' operands in 128 registers, four waves a SIMD: 64-wide bf16 takes
-// 40 KB of LDS, four workgroups a CU, 128-wide 73 KB, two.  Bound by HBM with a
-// chunk's LDS and vector work close behind.  Measured, bf16: 128 x 1000 steps,
-// 8 heads of 64 with resets, forward 130 us (558 MB, 4.3 TB/s), backward 298
-// (1.32 GB, 4.4 TB/s); 65536 steps, 16 heads of 128, states 124 us (553 MB, 4.5
-// TB/s) and outputs 236 (1.11 GB, 4.7 TB/s); 8 x 4096 steps, 16 heads of 128,
-// states 60 to 70 us (227 MB: one and a half workgroups a CU, bound by
-// instructions), outputs 140, backward 385 (1.44 GB, 3.8 TB/s, vector
-// instructions issuing 47 % of the time).  float32, 256 x 64 steps, 4 heads of
-// 64: 30 us, a third of it matrix products (16x16x4), backward 72.
+// 40 KB of LDS, four workgroups a CU, 128-wide 79 KB, two.  Bound by HBM and a
+// chunk's vector and LDS work together.  Measured (traces of calls one after
+// the other, operands of three sets in turn), bf16: 128 x 1000 steps, 8 heads of
+// 64 with resets, forward 136 us (558 MB, 4.1 TB/s), backward 340 (1.32 GB, 3.9
+// TB/s); 65536 steps, 16 heads of 128, states 121 us (553 MB, 4.6 TB/s) and
+// outputs 287 (1.12 GB, 3.9 TB/s); 8 x 4096 steps, 16 heads of 128, states 57 us
+// (227 MB: one and a half workgroups a CU, bound by instructions), outputs 144,
+// backward 392 (1.46 GB, 3.7 TB/s, vector instructions issuing 60 % of the time,
+// matrix units busy 31 %).  float32, 256 x 64 steps, 4 heads of 64: 30 us, a
+// third of it matrix products (16x16x4), backward 68.
 template <typename T, int D, bool STATE>
 __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : D == 32 ? 3 : 4) attention_kernel(AttnArgs p) {
   typedef typename Type<T>::Frag Frag;
@@ -342,13 +343,14 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : D == 32 ? 3 : 4) attentio
   constexpr int PIECES = Type<T>::PIECES, PARTS = Type<T>::PARTS, TILES = QT * (QT + 1) / 2;
   constexpr int RB = D * (int)sizeof(T), ROWS = C * RB, COLS = D * 128, PAIRS = C * 96;
   // The pair products' second pieces: after the first ones, or, where that would
-  // leave a workgroup less a CU (64-wide: 46 KB; forward 134 -> 162 us, backward
-  // 336 -> 367), in place of y's rows (and what those lack) once the pair
-  // products are formed.
+  // leave a workgroup less a CU (64-wide: 46 KB; 128 x 1000 steps, 8 heads,
+  // forward 137 -> 156 us, backward 333 -> 350), in place of y's rows (and what
+  // those lack) once the pair products are formed.
   constexpr bool OVER_Y = PARTS == 2 && D <= 64;
   constexpr int MORE = !OVER_Y ? (PARTS - 1) * PAIRS : ROWS < PAIRS ? PAIRS - ROWS : 0;
   // Streamed outputs go through LDS to be stored in whole rows.  (96-wide, rows
-  // of one and a half lines and few waves: 175 -> 181 us, so not there.)
+  // of one and a half lines and few waves, products of one piece: 175 -> 181 us, so
+  // not there.)
   constexpr bool ROWS_OUT = !STATE && D != 96;
   // y and z by columns, x and y by rows, and the pair products: all queries
   // with the chunk's first half of keys, the later half with the other
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : D == 32 ? 3 : 4) attentio
   // Whether the state itself is an output (or, STATE, leads to one): the third
   // piece of its terms (2^-17 of them) is no more than what a state loses that
   // only enters products, in two pieces.  With it, 16 heads of 128: 65536 steps
-  // 415 -> 430 us, both passes of 8 x 4096 steps 682 -> 720 us.
+  // 407 -> 421 us, both passes of 8 x 4096 steps 672 -> 702 us.
   const bool exact = c.final && (STATE || seg == p.segments - 1);
   uint64_t cut = 0;   // the chunk's steps that drop the state
   // Lays out steps r0 .. r0 + n - 1, as loaded, and loads the chunk from `next` (>= 0) on.
@@ -536,8 +538,8 @@ __global__ void __launch_bounds__(4 * D, D == 96 ? 2 : D == 32 ? 3 : 4) attentio
     return is_bad;
   };
   auto chunk = [&](int n) {
-    // (the products before another workgroup's laying out: 16 heads of 128, both passes of 8 x 4096 steps 640 ->
-    // 620 us, 65536 steps 400 -> 392 us)
+    // (the products before another workgroup's laying out: 16 heads of 128, both passes of 8 x 4096 steps 681 ->
+    // 672 us, 65536 steps 422 -> 407 us)
     __builtin_amdgcn_s_setprio(1);
     const int tid = here(threadIdx.x), lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
     const int skip = back && r0 == 0 ? 1 : 0;
@@ -979,9 +981,9 @@ __global__ void __launch_bounds__(256) attention_step_kernel(StepArgs a) {
 constexpr int MAX_WIDTH = 128;
 
 // The width of a launch.  96 of its own, batch 8, 4096 steps, 16 heads against
-// padded to 128: bf16 179 us (183) forward and 596 (582) with the backward,
-// batch 2, 512 steps, 4 heads of 80 22.8 us (25.5); float32, 2048 steps, 238 us
-// (304).
+// padded to 128: bf16 188 us (199) forward and 627 (632) with the backward,
+// batch 2, 512 steps, 4 heads of 80 23.7 us (27.0); float32, 2048 steps, 229 us
+// (300).
 int padded(int K, int V) {
   const int w = std::max(K, V);
   return w <= 32 ? 32 : w <= 64 ? 64 : w <= 96 ? 96 : 128;
@@ -992,10 +994,10 @@ int chunk(int dtype) { return dtype == ATTN_F32 ? 32 : 64; }
 // Segments the step axis is cut into: as many workgroups as the chip's 256 CUs
 // hold at a time (16 waves each), while a segment keeps two chunks or more,
 // since its state is written, joined and read back.  Measured, bf16: against
-// half and twice as many, batch 1, 65536 steps, 16 heads of 128 takes 397 us
-// (437, 421) and both passes of batch 8, 4096 steps, 16 heads of 128 take 620
-// us (628, 659); against segments of four chunks, batch 4, 2048 steps, 8 heads
-// of 64 takes 28.9 us (31.7; 47 with eight).
+// half and twice as many, batch 1, 65536 steps, 16 heads of 128 takes 407 us
+// (468, 434) and both passes of batch 8, 4096 steps, 16 heads of 128 take 672
+// us (712, 740); against segments of four chunks, batch 4, 2048 steps, 8 heads
+// of 64 takes 31.4 us (34.1).
 int segments_of(int dtype, int batch, int steps, int heads, int K, int V) {
   const int64_t pairs = std::max<int64_t>(1, (int64_t)batch * heads);
   const int c = chunk(dtype), D = padded(K, V);
@@ -1030,11 +1032,12 @@ void states_pass(hipStream_t st, int dtype, AttnArgs a, const Contraction& c, in
 
 // Outputs too large for the caches to hold for what reads them next are
 // streamed: in whole rows past the caches, which keep the operands that other
-// workgroups read again.  Measured, bf16, alone and with a product that reads
-// them next: 134 MB (64 x 2048 steps, 8 heads of 64) 170 -> 152 and 224 -> 215
-// us, 67 MB 94 -> 80 and 118 -> 115, 33 MB 56 -> 55 but 69 -> 70; both passes of
-// 128 x 1000 steps, 8 heads of 64, 453 -> 430 us, 65536 steps of 16 heads of 128
-// 388 -> 373.  (Whole rows through the caches gained half of that, and lost 2 %
+// workgroups read again.  Measured, bf16: 134 MB (64 x 2048 steps, 8 heads of
+// 64) 176 -> 164 us, 67 MB 109 -> 98; both passes of 128 x 1000 steps, 8 heads of
+// 64, 493 -> 469 us, of 8 x 4096 steps, 16 heads of 128, 685 -> 672, 65536 steps of
+// those 414 -> 407.  (With products of one piece and a product that reads the
+// outputs next: 134 MB 224 -> 215 us, 67 MB 118 -> 115, 33 MB 69 -> 70, and 56 ->
+// 55 alone.  Whole rows through the caches gained half of that, and lost 2 %
 // where outputs are small; 32 bytes of a row past the caches lost a quarter.)
 void outputs_pass(hipStream_t st, int dtype, AttnArgs a, int batch) {
   const int D = padded(a.role[0].x.width, a.role[0].z.width);
