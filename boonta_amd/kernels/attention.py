@@ -226,8 +226,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         carry = None if carry is None else pad(carry, (0, more_v, 0, more_k))
         carry, out = linear_attention(q, k, v, log_decay, carry, done, lengths, scale)
         return carry[..., :key, :value].contiguous(), out[..., :value].contiguous()
-    args = (_near_rows(q), _near_rows(k), _near_rows(v), log_decay.contiguous(), None if carry is None else carry.contiguous(),
-            None if done is None else done.contiguous(), None if lengths is None else lengths.contiguous(), scale, sizes)
+    args = (_near_rows(q), _near_rows(k), _near_rows(v), log_decay.contiguous(),
+            None if carry is None else carry.contiguous(), None if done is None else done.contiguous(),
+            None if lengths is None else lengths.contiguous(), scale, sizes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (carry is not None and carry.requires_grad)):
         return _LinearAttention.apply(*args)
