@@ -1,0 +1,440 @@
+// The norms after and before a block, with the block's gate, the residual
+// scale and the sum into the residual stream in the same pass, and its
+// vector-Jacobian product.
+//
+// Per row of D columns (one step of one sequence), u the block's output, x the
+// residual stream:
+//   n = u / sqrt(mean(u^2) + eps) * post     (or n = u: no norm of the block's output)
+//   y = x + scale * gate * n                 (gate: 1, g, or sigmoid(g))
+//   z = y / sqrt(mean(y^2) + eps) * pre
+// y is the new stream, z what the next block reads, both from the unrounded y.
+// Backward, from the cotangents dy and dz, with u' = u ru and y' = y ry (ru, ry
+// the two rows' 1 / rms, kept by the forward), q = scale gate:
+//   e = dz pre, m = mean(e y'), dx = dy + ry (e - y' m),
+//   dgate = dx scale n, f = dx q post, du = ru (f - u' mean(f u')),
+//   dpre = sum dz y', dscale = sum dx gate n, dpost = sum dx q u'.
+// mean(f u') is linear in m, so that one exchange of three sums serves both:
+//   mean(f u') = mean((dy + ry e) q post u') - m mean(ry y' q post u').
+//
+// A thread holds 8 columns of a row and their scales for all its rows; a row is
+// L lanes of a wave (up to 512 columns) or one workgroup.  Sums are float32, the
+// lanes' by butterflies, the waves' in order.
+#include "row_io.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace ppo;
+
+enum NormDtype { NORM_F32 = 0, NORM_BF16 = 1 };
+
+constexpr int THREADS = 256;               // of a workgroup of narrow rows
+constexpr int MAX_THREADS = 1024;
+constexpr int NARROW = 64 * UNIT;          // widest row of one wave's lanes
+constexpr int MAX_WIDTH = MAX_THREADS * UNIT;
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;  // most workgroups
+
+struct ResidualArgs {
+  const void* block;
+  const void* gate;       // or null
+  const void* residual;
+  const float* post;      // scales [D], or null (ones)
+  const float* scale;
+  const float* pre;
+  void* stream;           // forward
+  void* normed;
+  float* stats;           // [rows, 2]: ru, ry (forward: or null)
+  const void* dstream;    // backward, each or null (zeros)
+  const void* dnormed;
+  void* dblock;
+  void* dgate;            // or null
+  void* dresidual;
+  float* partials;        // [workgroups, 3, D]: dpost, dscale, dpre
+  RowStride block_s, gate_s, residual_s, dstream_s, dnormed_s;
+  Divisor steps;
+  uint32_t rows;
+  int D, lanes_log2;
+  float eps;
+  bool post_norm, sigmoid_gate;
+};
+
+__device__ __forceinline__ void load_scales(const float* p, int col, int D, float (&v)[UNIT]) {
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) v[j] = p && col + j < D ? p[col + j] : 1.f;
+}
+
+// Sums over a row: its lanes (narrow), or the workgroup, whose waves' sums
+// meet in LDS.  `slot`: another at each call until every wave has passed a
+// later one.
+template <bool WIDE, int N> struct RowSum {
+  float (*waves)[MAX_THREADS / 64][N];
+  int log2;
+  __device__ __forceinline__ void operator()(float (&v)[N], int slot) const {
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i], log2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = wave_sum_lanes(v[i]);
+      const int wave = threadIdx.x >> 6, count = blockDim.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) waves[slot][wave][i] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.f;
+      for (int w = 0; w < count; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += waves[slot][w][i];
+    }
+  }
+};
+
+// Which rows and columns a thread takes.
+struct Place {
+  uint32_t row, step;  // its first row, and from one to its next
+  int col, left;       // first column; columns from there to the row's end
+};
+template <bool WIDE> __device__ __forceinline__ Place place_of(const ResidualArgs& p) {
+  Place r;
+  if constexpr (WIDE) {
+    r.row = blockIdx.x;
+    r.step = gridDim.x;
+    r.col = threadIdx.x * UNIT;
+  } else {
+    const int L = 1 << p.lanes_log2;
+    r.row = (blockIdx.x * THREADS + threadIdx.x) >> p.lanes_log2;
+    r.step = (gridDim.x * THREADS) >> p.lanes_log2;
+    r.col = (threadIdx.x & (L - 1)) * UNIT;
+  }
+  r.left = p.D - r.col;
+  return r;
+}
+
+template <typename T, typename R> struct Loaded {
+  Unit8<T> u, g, dz;
+  Unit8<R> x, dy;
+};
+
+template <typename T, typename R, bool BWD>
+__device__ __forceinline__ void load(const ResidualArgs& p, uint32_t row, const Place& at, Loaded<T, R>& v) {
+  load_unit(static_cast<const T*>(p.block) + row_offset(row, p.steps, p.block_s) + at.col, at.left, v.u);
+  load_unit(static_cast<const R*>(p.residual) + row_offset(row, p.steps, p.residual_s) + at.col, at.left, v.x);
+  if (p.gate) load_unit(static_cast<const T*>(p.gate) + row_offset(row, p.steps, p.gate_s) + at.col, at.left, v.g);
+  if constexpr (BWD) {
+    if (p.dnormed)
+      load_unit(static_cast<const T*>(p.dnormed) + row_offset(row, p.steps, p.dnormed_s) + at.col, at.left, v.dz);
+    if (p.dstream)
+      load_unit(static_cast<const R*>(p.dstream) + row_offset(row, p.steps, p.dstream_s) + at.col, at.left, v.dy);
+  }
+}
+
+__device__ __forceinline__ float gate_of(const ResidualArgs& p, float g) {
+  return !p.gate ? 1.f : p.sigmoid_gate ? sigmoid(g) : g;
+}
+
+template <typename T, typename R, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_fwd_kernel(ResidualArgs p) {
+  __shared__ float waves[2][MAX_THREADS / 64][1];
+  const RowSum<WIDE, 1> row_sum{waves, p.lanes_log2};
+  const Place at = place_of<WIDE>(p);
+  float post[UNIT], scale[UNIT], pre[UNIT];
+  load_scales(p.post, at.col, p.D, post);
+  load_scales(p.scale, at.col, p.D, scale);
+  load_scales(p.pre, at.col, p.D, pre);
+  const float over_d = 1.f / (float)p.D;
+  int slot = 0;
+  for (uint32_t row0 = at.row; __any(row0 < p.rows); row0 += at.step) {
+    const bool live = row0 < p.rows;
+    const uint32_t row = live ? row0 : p.rows - 1;   // (a wave's rows end together)
+    Loaded<T, R> v;
+    load<T, R, false>(p, row, at, v);
+    float u[UNIT], y[UNIT], ru = 1.f, sum[1];
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) u[j] = value(v.u, j);
+    if (p.post_norm) {
+      sum[0] = 0.f;
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) sum[0] = __fmaf_rn(u[j], u[j], sum[0]);
+      row_sum(sum, slot);
+      slot ^= 1;
+      ru = rsqrtf(__fmaf_rn(sum[0], over_d, p.eps));
+    }
+    sum[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) {
+      const float q = p.gate ? scale[j] * gate_of(p, value(v.g, j)) : scale[j];
+      y[j] = __fmaf_rn(q, u[j] * ru * post[j], value(v.x, j));   // (past the row's end 0)
+      sum[0] = __fmaf_rn(y[j], y[j], sum[0]);
+    }
+    row_sum(sum, slot);
+    slot ^= 1;
+    const float ry = rsqrtf(__fmaf_rn(sum[0], over_d, p.eps));
+    if (!live) continue;
+    const int64_t out = (int64_t)row * p.D + at.col;
+    store_unit(static_cast<R*>(p.stream) + out, at.left, y);
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) y[j] = y[j] * ry * pre[j];
+    store_unit(static_cast<T*>(p.normed) + out, at.left, y);
+    if (p.stats && at.col == 0) {
+      p.stats[2 * (int64_t)row] = ru;
+      p.stats[2 * (int64_t)row + 1] = ry;
+    }
+  }
+}
+
+template <typename T, typename R, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_bwd_kernel(ResidualArgs p) {
+  __shared__ float waves[2][MAX_THREADS / 64][3];
+  const RowSum<WIDE, 3> row_sum{waves, p.lanes_log2};
+  const Place at = place_of<WIDE>(p);
+  float post[UNIT], scale[UNIT], pre[UNIT], dpost[UNIT], dscale[UNIT], dpre[UNIT];
+  load_scales(p.post, at.col, p.D, post);
+  load_scales(p.scale, at.col, p.D, scale);
+  load_scales(p.pre, at.col, p.D, pre);
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) dpost[j] = dscale[j] = dpre[j] = 0.f;
+  const float over_d = 1.f / (float)p.D;
+  int slot = 0;
+  for (uint32_t row0 = at.row; __any(row0 < p.rows); row0 += at.step) {
+    const bool live = row0 < p.rows;
+    const uint32_t row = live ? row0 : p.rows - 1;
+    Loaded<T, R> v;
+    load<T, R, true>(p, row, at, v);
+    const float ru = p.stats[2 * (int64_t)row], ry = p.stats[2 * (int64_t)row + 1];
+    // (columns past the row's end have u = x = dz = dy = 0)
+    float un[UNIT], q[UNIT], yn[UNIT], e[UNIT], dx[UNIT], sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) {
+      q[j] = p.gate ? scale[j] * gate_of(p, value(v.g, j)) : scale[j];
+      un[j] = value(v.u, j) * ru;
+      yn[j] = __fmaf_rn(q[j], un[j] * post[j], value(v.x, j)) * ry;
+      const float dz = p.dnormed ? value(v.dz, j) : 0.f;
+      if (live) dpre[j] = __fmaf_rn(dz, yn[j], dpre[j]);
+      e[j] = dz * pre[j];
+      dx[j] = __fmaf_rn(ry, e[j], p.dstream ? value(v.dy, j) : 0.f);
+      sum[0] = __fmaf_rn(e[j], yn[j], sum[0]);
+      const float k = q[j] * post[j] * un[j];
+      sum[1] = __fmaf_rn(dx[j], k, sum[1]);
+      sum[2] = __fmaf_rn(yn[j], k, sum[2]);
+    }
+    row_sum(sum, slot);
+    slot ^= 1;
+    const float m = sum[0] * over_d * ry;
+    const float mu = p.post_norm ? __fmaf_rn(-m, sum[2], sum[1]) * over_d : 0.f;
+    float du[UNIT], dg[UNIT];
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) {
+      dx[j] = __fmaf_rn(-yn[j], m, dx[j]);
+      const float gate = gate_of(p, p.gate ? value(v.g, j) : 1.f);
+      const float n = un[j] * post[j], dn = dx[j] * q[j];
+      if (live) {
+        dscale[j] = __fmaf_rn(dx[j], gate * n, dscale[j]);
+        dpost[j] = __fmaf_rn(dn, un[j], dpost[j]);
+      }
+      dg[j] = dx[j] * scale[j] * n * (p.sigmoid_gate ? gate * (1.f - gate) : 1.f);
+      du[j] = ru * __fmaf_rn(-un[j], mu, dn * post[j]);
+    }
+    if (!live) continue;
+    const int64_t out = (int64_t)row * p.D + at.col;
+    store_unit(static_cast<R*>(p.dresidual) + out, at.left, dx);
+    store_unit(static_cast<T*>(p.dblock) + out, at.left, du);
+    if (p.dgate) store_unit(static_cast<T*>(p.dgate) + out, at.left, dg);
+  }
+  if (!p.partials) return;
+  float* mine = p.partials + (int64_t)blockIdx.x * 3 * p.D;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) {
+      if (j >= at.left) break;
+      mine[at.col + j] = dpost[j];
+      mine[p.D + at.col + j] = dscale[j];
+      mine[2 * p.D + at.col + j] = dpre[j];
+    }
+  } else {
+    // the rows of the workgroup side by side, added in their order
+    __shared__ float sums[THREADS * UNIT];
+    const int L = 1 << p.lanes_log2;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) sums[j * THREADS + threadIdx.x] = w == 0 ? dpost[j] : w == 1 ? dscale[j] : dpre[j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.D; c += THREADS) {
+        float s = 0.f;
+        for (int g = c / UNIT; g < THREADS; g += L) s += sums[(c % UNIT) * THREADS + g];
+        mine[w * p.D + c] = s;
+      }
+    }
+  }
+}
+
+// The scales' gradients from the workgroups' sums: 64 columns a workgroup, each
+// wave its share of the sums in their order, then the waves'.
+__global__ void __launch_bounds__(1024) residual_norm_scale_kernel(const float* partials, int blocks, int D,
+                                                                   float* dpost, float* dscale, float* dpre) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+  const int share = (blocks + 15) / 16, b1 = min(blocks, (wave + 1) * share);
+  float s = 0.f;
+  if (i < 3 * D) {
+    for (int b0 = wave * share; b0 < b1; b0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = partials[(int64_t)min(b0 + k, b1 - 1) * 3 * D + i];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += b0 + k < b1 ? v[k] : 0.f;
+    }
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0 || i >= 3 * D) return;
+  s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += sums[w][lane];
+  const int which = i / D, col = i - which * D;
+  float* out = which == 0 ? dpost : which == 1 ? dscale : dpre;
+  if (out) out[col] = s;
+}
+
+// ---- launches
+int lanes_log2_of(int D) {
+  int log2 = 0;
+  while ((UNIT << log2) < D) ++log2;
+  return log2;
+}
+
+// Threads and most useful workgroups of a launch.
+struct Shape {
+  bool wide;
+  unsigned threads, blocks;
+};
+Shape shape_of(int64_t rows, int D, int most) {
+  Shape s;
+  s.wide = D > NARROW;
+  s.threads = s.wide ? (unsigned)(64 * ceil_div(D, NARROW)) : THREADS;
+  const int64_t at_once = s.wide ? 1 : THREADS >> lanes_log2_of(D);
+  s.blocks = (unsigned)std::min<int64_t>(most, ceil_div64(rows, at_once));
+  return s;
+}
+
+int check(const char* what, int dtype, int stream_dtype, int batch, int steps, int width) {
+  if ((dtype != NORM_F32 && dtype != NORM_BF16) || (stream_dtype != NORM_F32 && stream_dtype != dtype))
+    return set_error(PPO_ERR_ARG, "%s: bad dtype %d, stream %d", what, dtype, stream_dtype);
+  if (batch < 0 || steps < 0 || width < 0)
+    return set_error(PPO_ERR_ARG, "%s: bad size (batch %d steps %d width %d)", what, batch, steps, width);
+  if (width > MAX_WIDTH) return set_error(PPO_ERR_ARG, "%s: width %d above %d", what, width, MAX_WIDTH);
+  if ((int64_t)batch * steps > INT32_MAX - (1 << 20))
+    return set_error(PPO_ERR_ARG, "%s: batch x steps above 2^31 - 2^20 - 1", what);
+  return PPO_OK;
+}
+
+ResidualArgs common_args(const void* block, const void* gate, const void* residual, const int64_t* strides,
+                         const float* post, const float* scale, const float* pre, int post_norm, int gate_sigmoid,
+                         float epsilon, int batch, int steps, int width) {
+  ResidualArgs a{};
+  a.block = block;
+  a.gate = gate;
+  a.residual = residual;
+  a.post = post;
+  a.scale = scale;
+  a.pre = pre;
+  a.block_s = RowStride{strides[0], strides[1]};
+  a.residual_s = RowStride{strides[2], strides[3]};
+  a.gate_s = RowStride{strides[4], strides[5]};
+  a.steps = divisor((uint32_t)steps);
+  a.rows = (uint32_t)((int64_t)batch * steps);
+  a.D = width;
+  a.lanes_log2 = width <= NARROW ? lanes_log2_of(width) : 0;
+  a.eps = epsilon;
+  a.post_norm = post_norm != 0;
+  a.sigmoid_gate = gate && gate_sigmoid;
+  return a;
+}
+
+template <typename T, typename R, bool BWD> void launch(hipStream_t st, const ResidualArgs& a, const Shape& s) {
+  const dim3 g(s.blocks), t(s.threads);
+  if constexpr (BWD) {
+    if (s.wide) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, R, true>), g, t, 0, st, a);
+    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, R, false>), g, t, 0, st, a);
+  } else {
+    if (s.wide) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, R, true>), g, t, 0, st, a);
+    else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, R, false>), g, t, 0, st, a);
+  }
+}
+template <bool BWD>
+void launch_typed(hipStream_t st, const ResidualArgs& a, const Shape& s, int dtype, int stream_dtype) {
+  if (dtype == NORM_F32) launch<float, float, BWD>(st, a, s);
+  else if (stream_dtype == NORM_F32) launch<uint16_t, float, BWD>(st, a, s);
+  else launch<uint16_t, uint16_t, BWD>(st, a, s);
+}
+
+}  // namespace
+
+PPO_EXPORT int ppo_residual_norm_max_width(void) { return MAX_WIDTH; }
+
+PPO_EXPORT int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, const void* block,
+                                     const void* residual, const void* gate, const int64_t* strides,
+                                     const float* post_scale, const float* residual_scale, const float* pre_scale,
+                                     int post_norm, int gate_sigmoid, float epsilon, void* stream_out, void* normed,
+                                     float* stats, int batch, int steps, int width) {
+  const char* what = "ppo_residual_norm_fwd";
+  if (int rc = check(what, dtype, stream_dtype, batch, steps, width)) return rc;
+  if ((int64_t)batch * steps == 0 || width == 0) return PPO_OK;
+  if (!block || !residual || !strides || !stream_out || !normed) return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  ResidualArgs a = common_args(block, gate, residual, strides, post_scale, residual_scale, pre_scale, post_norm,
+                               gate_sigmoid, epsilon, batch, steps, width);
+  a.stream = stream_out;
+  a.normed = normed;
+  a.stats = stats;
+  launch_typed<false>(as_stream(stream), a, shape_of(a.rows, width, FWD_BLOCKS), dtype, stream_dtype);
+  return check_launch(what);
+}
+
+PPO_EXPORT size_t ppo_residual_norm_bwd_workspace(int batch, int steps, int width) {
+  if (batch <= 0 || steps <= 0 || width <= 0 || width > MAX_WIDTH) return 0;
+  return sizeof(float) * 3 * (size_t)width * shape_of((int64_t)batch * steps, width, BWD_BLOCKS).blocks;
+}
+
+PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block,
+                                     const void* residual, const void* gate, const void* dstream,
+                                     const void* dnormed, const int64_t* strides, const float* post_scale,
+                                     const float* residual_scale, const float* pre_scale, int post_norm,
+                                     int gate_sigmoid, const float* stats, void* dblock, void* dresidual, void* dgate,
+                                     float* dpost_scale, float* dresidual_scale, float* dpre_scale, void* workspace,
+                                     size_t workspace_bytes, int batch, int steps, int width) {
+  const char* what = "ppo_residual_norm_bwd";
+  if (int rc = check(what, dtype, stream_dtype, batch, steps, width)) return rc;
+  if (width == 0) return PPO_OK;
+  const bool none = (int64_t)batch * steps == 0, scales = dpost_scale || dresidual_scale || dpre_scale;
+  if (!none && (!block || !residual || !strides || !stats || !dblock || !dresidual))
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  const size_t need = scales ? ppo_residual_norm_bwd_workspace(batch, steps, width) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  unsigned blocks = 0;
+  if (!none) {
+    ResidualArgs a = common_args(block, gate, residual, strides, post_scale, residual_scale, pre_scale, post_norm,
+                                 gate_sigmoid, 0.f, batch, steps, width);
+    a.stats = const_cast<float*>(stats);
+    a.dstream = dstream;
+    a.dnormed = dnormed;
+    a.dstream_s = RowStride{strides[6], strides[7]};
+    a.dnormed_s = RowStride{strides[8], strides[9]};
+    a.dblock = dblock;
+    a.dgate = gate ? dgate : nullptr;
+    a.dresidual = dresidual;
+    a.partials = scales ? static_cast<float*>(workspace) : nullptr;
+    const Shape s = shape_of(a.rows, width, BWD_BLOCKS);
+    blocks = s.blocks;
+    launch_typed<true>(as_stream(stream), a, s, dtype, stream_dtype);
+  }
+  if (scales)
+    hipLaunchKernelGGL(residual_norm_scale_kernel, dim3((unsigned)ceil_div(3 * width, 64)), dim3(1024), 0,
+                       as_stream(stream), static_cast<const float*>(workspace), (int)blocks, width, dpost_scale,
+                       dresidual_scale, dpre_scale);
+  return check_launch(what);
+}

@@ -1,6 +1,7 @@
 """Stand-alone kernels behind boonta's network blocks (boonta/networks/kernels)."""
 from .attention import linear_attention, linear_attention_step, qk_norm_rotary, rotary_frequencies
+from .residual import residual_norm
 from .scan import get_scan_implementation, hip, scan, ssm, ssm_scan
 
 __all__ = ["get_scan_implementation", "hip", "linear_attention", "linear_attention_step", "qk_norm_rotary",
-           "rotary_frequencies", "scan", "ssm", "ssm_scan"]
+           "residual_norm", "rotary_frequencies", "scan", "ssm", "ssm_scan"]

@@ -437,6 +437,36 @@ int ppo_qk_norm_rotary_bwd(void* stream, int dtype, const void* q, const void* k
                            size_t workspace_bytes, int batch, int steps, int heads, int kv_heads, int width,
                            int pairs);
 
+/* The norms after and before a block with its gate, the residual scale and the
+ * sum into the residual stream (no counterpart in the reference).  Per row of
+ * `width` columns: n = block / sqrt(mean(block^2) + epsilon) * post_scale
+ * (post_norm 0: n = block), stream_out = residual + residual_scale * gate * n
+ * (gate NULL: 1; gate_sigmoid: sigmoid(gate)), normed = stream_out /
+ * sqrt(mean(stream_out^2) + epsilon) * pre_scale, from the sum before it is
+ * rounded.  block, gate and normed are of `dtype` (0 = float32, 1 = bf16),
+ * residual and stream_out of `stream_dtype` (float32, or dtype); columns side by
+ * side, element strides of (batch, step) in the host array `strides`, 2 for each
+ * of block, residual, gate (any pair where that is NULL); outputs contiguous.
+ * scales float [width] (NULL: ones); stats float [batch x steps, 2] for the
+ * backward (NULL: none).  width at most ppo_residual_norm_max_width(), batch x
+ * steps at most 2^31 - 2^20 - 1. */
+int ppo_residual_norm_max_width(void);
+int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, const void* block, const void* residual,
+                          const void* gate, const int64_t* strides, const float* post_scale,
+                          const float* residual_scale, const float* pre_scale, int post_norm, int gate_sigmoid,
+                          float epsilon, void* stream_out, void* normed, float* stats, int batch, int steps,
+                          int width);
+/* From the cotangents of stream_out and normed (either NULL: zeros; strides: 2
+ * more for each): dblock, dresidual and dgate (may be NULL) contiguous, typed as
+ * their values; the scales' gradients float [width] (may be NULL). */
+size_t ppo_residual_norm_bwd_workspace(int batch, int steps, int width);
+int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block, const void* residual,
+                          const void* gate, const void* dstream, const void* dnormed, const int64_t* strides,
+                          const float* post_scale, const float* residual_scale, const float* pre_scale, int post_norm,
+                          int gate_sigmoid, const float* stats, void* dblock, void* dresidual, void* dgate,
+                          float* dpost_scale, float* dresidual_scale, float* dpre_scale, void* workspace,
+                          size_t workspace_bytes, int batch, int steps, int width);
+
 /* ------------------------------------------------------------------ GEMM
  * Dense layers of the torso and heads (flax.linen.Dense as composed in
  * hangar/recipes/*.py; forward at boonta/networks/network.py:38-49, backward
