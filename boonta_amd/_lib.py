@@ -89,6 +89,11 @@ SIGNATURES = {
     "ppo_residual_norm_fwd": (I, [P, I, I, P, P, P, P, P, P, P, I, I, F, P, P, P, I, I, I]),
     "ppo_residual_norm_bwd_workspace": (SZ, [I, I, I]),
     "ppo_residual_norm_bwd": (I, [P, I, I, P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, P, P, P, SZ, I, I, I]),
+    "ppo_token_log_probs_max_top": (I, []),
+    "ppo_token_log_probs_max_vocab": (I, []),
+    "ppo_token_log_probs_workspace": (SZ, [I, I, I, I]),
+    "ppo_token_log_probs_fwd": (I, [P, I, P, P, I, P, P, F, I, P, P, P, P, P, P, SZ, I, I, I]),
+    "ppo_token_log_probs_bwd": (I, [P, I, P, P, I, P, P, F, P, P, P, P, P, P, I, I, I]),
     "ppo_gemm_f32": (I, [P, I, I, P, I64, P, P, I64, P, I64, I, I, I, I, I64, I, P, I, P, P, I64, P, I]),
     "ppo_gemm_f32_towers": (I, [P, I, I, I, P, I64, P, P, I64, P, I64, I, I, I, I, I64, I, P, I, P, P, I64, P, I,
                                 I64, I64, I64, I64, I64, I64, I64]),

@@ -1,0 +1,509 @@
+// Log probabilities of given tokens, entropies and top alternatives of rows of
+// logits, and their vector-Jacobian product.
+//
+// Per row x of V logits, x_j = -inf where the mask does not allow j, temperature T:
+//   w_j = (x_j - max x) / T, S = sum e^w, log p_j = w_j - ln S
+//   log_prob = log p_token, entropy = ln S - sum e^w w / S
+// (both sums of one sign, so neither cancels).  One pass: a thread keeps the
+// maximum so far with S and sum e^w w relative to it, and rescales them when it
+// grows.  A row that allows nothing has p = 0 and entropy 0.
+// Backward: dx_j = (g (1_{j = token} - p_j) - h p_j (log p_j + entropy)) / T.
+//
+// The `top` largest x, equal ones by index.  A thread also keeps its best unit
+// of 8 columns, by its largest value, then the lowest index.  The units of the
+// `top` best threads hold the `top` best values: every one of those threads
+// has a value that is better than all of any other thread.  So only their units
+// are read again, those worse than the last of them left out, and ranked.
+#include "row_io.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace ppo;
+
+enum TokenDtype { TOKEN_F32 = 0, TOKEN_BF16 = 1 };
+
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int NARROW = 64 * UNIT;       // widest row of one wave's lanes
+constexpr int MAX_TOP = 32;
+constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of a row
+constexpr int MAX_SEGMENTS = 256;
+constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
+constexpr int BLOCKS = 4096;            // most workgroups of a launch over narrow rows
+constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
+constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
+constexpr float LN2 = 0.6931471805599453f;
+
+struct TokenArgs {
+  const void* logits;
+  const uint8_t* mask;      // or null
+  const void* tokens;       // int32 or int64 [rows]
+  float* log_prob;          // forward, [rows]
+  float* entropy;
+  float* stats;             // [rows, 2]: max, log2 S (forward: or null)
+  float* top_log_probs;     // [rows, top]
+  void* top_tokens;
+  float* partials;          // rows in segments
+  const float* dlog_prob;   // backward, each or null (zeros)
+  const float* dentropy;
+  void* dlogits;
+  RowStride logits_s, mask_s, dlog_prob_s, dentropy_s;
+  Divisor steps, units;     // units: of a row
+  uint32_t rows;
+  int V, top, lanes_log2, segments, segment_units, row_block;
+  float c, inverse_t;       // log2(e) / T, 1 / T
+  bool wide_tokens;
+};
+
+__device__ __forceinline__ int64_t token_of(const TokenArgs& p, uint32_t row) {
+  return p.wide_tokens ? static_cast<const int64_t*>(p.tokens)[row] : static_cast<const int32_t*>(p.tokens)[row];
+}
+
+// The 8 values of a unit, -inf where masked or past the row's end.
+template <typename T>
+__device__ __forceinline__ void read_unit(const T* x, const uint8_t* mask, int col, int V, float (&v)[UNIT]) {
+  Unit8<T> raw;
+  const int left = V - col;
+  load_unit(x + col, left, raw);
+  uint64_t allowed = ~0ull;
+  if (mask) {
+    if (left >= UNIT) {
+      __builtin_memcpy(&allowed, mask + col, 8);
+    } else {
+      allowed = 0;
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j)
+        if (j < left) allowed |= (uint64_t)mask[col + j] << (8 * j);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) v[j] = j < left && ((allowed >> (8 * j)) & 0xff) ? value(raw, j) : -INF;
+}
+__device__ __forceinline__ float max8(const float (&v)[UNIT]) {
+  return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+}
+
+// Maximum, sum of 2^w and sum of 2^w w, w = (x - maximum) c.
+struct Sums {
+  float m, s, t;
+};
+__device__ __forceinline__ Sums no_sums() { return Sums{LOWEST, 0.f, 0.f}; }
+__device__ __forceinline__ float exponent(float x, float m, float c) { return (x - m) * c; }
+// (an infinite x or a NaN makes s NaN, and so the row's results)
+__device__ __forceinline__ Sums rescaled(const Sums& a, float m, float c) {
+  const float d = exponent(a.m, m, c), f = __builtin_amdgcn_exp2f(d);
+  return Sums{m, a.s * f, f * __fmaf_rn(fmaxf(d, FAR), a.s, a.t)};
+}
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const Sums x = rescaled(a, m, c), y = rescaled(b, m, c);
+  return Sums{m, x.s + y.s, x.t + y.t};
+}
+__device__ __forceinline__ void add_unit(Sums& a, const float (&v)[UNIT], float most, float c) {
+  a = rescaled(a, fmaxf(a.m, most), c);
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) {
+    const float w = exponent(v[j], a.m, c), e = __builtin_amdgcn_exp2f(w);
+    a.s += e;
+    a.t = __fmaf_rn(e, fmaxf(w, FAR), a.t);
+  }
+}
+// Over 2^log2 neighbouring lanes (all active).
+__device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
+  for (int i = 0; i < log2; ++i) {
+    const int o = 1 << i;
+    const Sums b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
+    a = joined(a, b, c);
+  }
+  return a;
+}
+
+// A row's results from its sums, by one thread.
+template <typename T>
+__device__ __forceinline__ void finish_row(const TokenArgs& p, uint32_t row, const Sums& a, const T* x,
+                                           const uint8_t* mask) {
+  const bool none = a.s == 0.f;
+  const float l = none ? INF : __builtin_amdgcn_logf(a.s);   // log2
+  p.entropy[row] = none ? 0.f : LN2 * (l - a.t / a.s);
+  const int64_t token = token_of(p, row);
+  float lp = 0.f;
+  if (token >= 0 && token < p.V) {
+    float v;
+    if constexpr (sizeof(T) == 2) v = __uint_as_float((uint32_t)x[token] << 16);
+    else v = x[token];
+    lp = v == -INF || (mask && !mask[token]) ? -INF : LN2 * (exponent(v, a.m, p.c) - l);
+  }
+  p.log_prob[row] = lp;
+  if (p.stats) {
+    p.stats[2 * (int64_t)row] = none ? 0.f : a.m;
+    p.stats[2 * (int64_t)row + 1] = l;
+  }
+}
+
+// ---- top alternatives
+// A key orders values, equal ones by the lower index; 0: no value (masked, or NaN).
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
+  const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
+  const uint32_t ordered = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return x > -INF ? (uint64_t)ordered << 32 | (uint32_t)~index : 0;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
+
+__device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int place, uint64_t key, float m, float l) {
+  const int64_t at = (int64_t)row * p.top + place;
+  p.top_log_probs[at] = key ? LN2 * (exponent(value_of(key), m, p.c) - l) : -INF;
+  const int32_t token = key ? (int32_t)index_of(key) : -1;
+  if (p.wide_tokens) static_cast<int64_t*>(p.top_tokens)[at] = token;
+  else static_cast<int32_t*>(p.top_tokens)[at] = token;
+}
+
+// ---- rows of up to 512 columns: lanes of a wave
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
+  const int L = 1 << p.lanes_log2, lane = threadIdx.x & (L - 1), col = lane * UNIT;
+  const uint32_t step = (gridDim.x * THREADS) >> p.lanes_log2;
+  for (uint32_t row0 = (blockIdx.x * THREADS + threadIdx.x) >> p.lanes_log2; __any(row0 < p.rows); row0 += step) {
+    const bool live = row0 < p.rows;
+    const uint32_t row = live ? row0 : p.rows - 1;
+    const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+    const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+    float v[UNIT];
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) v[j] = -INF;
+    if (col < p.V) read_unit(x, mask, col, p.V, v);
+    Sums a = no_sums();
+    add_unit(a, v, max8(v), p.c);
+    a = lanes_joined(a, p.lanes_log2, p.c);
+    if (live && lane == 0) finish_row(p, row, a, x, mask);
+    if constexpr (TOP) {
+      const float l = __builtin_amdgcn_logf(a.s);
+      uint64_t last = ~0ull;
+      for (int k = 0; k < p.top; ++k) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j) {
+          const uint64_t key = key_of(v[j], (uint32_t)(col + j));
+          best = key < last && key > best ? key : best;
+        }
+        for (int o = 1; o < L; o <<= 1) {
+          const uint64_t other = __shfl_xor((unsigned long long)best, o);
+          best = other > best ? other : best;
+        }
+        last = best;
+        if (live && lane == (k & (L - 1))) write_top(p, row, k, best, a.m, l);
+      }
+    }
+  }
+}
+
+// ---- wider rows: a workgroup for each row, or each segment of it
+// What a segment leaves: its sums, then its best keys.
+__device__ __forceinline__ int64_t partial_floats(int top) { return 4 + 2 * top; }
+
+struct TopSpace {
+  uint64_t keys[THREADS];
+  uint64_t candidates[MAX_TOP * (SEGMENT / (UNIT * THREADS))];
+  uint32_t winners[THREADS];
+  uint64_t best[MAX_TOP];
+  int count;
+};
+
+// keys' rank: how many of n are better.
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
+  int r = 0;
+  for (int i = 0; i < n; ++i) r += keys[i] > key;
+  return r;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
+  __shared__ Sums sums[WAVES];
+  __shared__ typename std::conditional<TOP, TopSpace, int>::type space;
+  const int tid = threadIdx.x;
+  const uint32_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+  const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+  const int units = (p.V + UNIT - 1) / UNIT, first = blockIdx.y * p.segment_units;
+  const int end = min(units, first + p.segment_units);
+  Sums a = no_sums();
+  float best = -INF;
+  int best_unit = 0;
+  for (int u = first + tid; u < end; u += THREADS) {
+    float v[UNIT];
+    read_unit(x, mask, u * UNIT, p.V, v);
+    const float most = max8(v);
+    add_unit(a, v, most, p.c);
+    if constexpr (TOP) {
+      best_unit = most > best ? u : best_unit;
+      best = most > best ? most : best;
+    }
+  }
+  a = lanes_joined(a, 6, p.c);
+  if ((tid & 63) == 0) sums[tid >> 6] = a;
+  if constexpr (TOP) {
+    space.keys[tid] = key_of(best, (uint32_t)best_unit);
+    if (tid == 0) space.count = 0;
+    if (tid < MAX_TOP) space.best[tid] = 0;
+  }
+  __syncthreads();
+  a = sums[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) a = joined(a, sums[w], p.c);
+  float* partial = p.partials + ((int64_t)row * p.segments + blockIdx.y) * partial_floats(p.top);
+  if (tid == 0) {
+    if (p.segments == 1) {
+      finish_row(p, row, a, x, mask);
+    } else {
+      partial[0] = a.m;
+      partial[1] = a.s;
+      partial[2] = a.t;
+    }
+  }
+  if constexpr (TOP) {
+    const uint64_t mine = space.keys[tid];
+    const int rank = rank_of(mine, space.keys, THREADS);
+    if (mine && rank < p.top) {
+      space.winners[rank] = (uint32_t)tid;
+      atomicMax(&space.count, rank + 1);
+    }
+    __syncthreads();
+    // the winners' units that are no worse than the last winner's best
+    const int winners = space.count;
+    const uint64_t least = winners < p.top ? 1 : space.keys[space.winners[winners - 1]];
+    const int each = (end - first + THREADS - 1) / THREADS;
+    __syncthreads();
+    if (tid == 0) space.count = 0;
+    __syncthreads();
+    for (int i = tid; i < winners * each; i += THREADS) {
+      const int w = i / each, u = first + (int)space.winners[w] + (i - w * each) * THREADS;
+      if (u >= end) continue;
+      float v[UNIT];
+      read_unit(x, mask, u * UNIT, p.V, v);
+      const uint64_t key = key_of(max8(v), (uint32_t)u);
+      if (key >= least) space.candidates[atomicAdd(&space.count, 1)] = key;
+    }
+    __syncthreads();
+    // the best units among them, and their values
+    const int candidates = space.count;
+    for (int i = tid; i < candidates; i += THREADS) {
+      const uint64_t key = space.candidates[i];
+      const int r = rank_of(key, space.candidates, candidates);
+      if (r < p.top) space.winners[r] = index_of(key);
+    }
+    __syncthreads();
+    const int best_units = min(candidates, p.top);
+    uint64_t value = 0;
+    if (tid < best_units * UNIT) {
+      float v[UNIT];
+      const int col = (int)space.winners[tid / UNIT] * UNIT;
+      read_unit(x, mask, col, p.V, v);
+      float one = -INF;
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) one = tid % UNIT == j ? v[j] : one;
+      value = key_of(one, (uint32_t)(col + tid % UNIT));
+    }
+    space.keys[tid] = value;
+    __syncthreads();
+    if (value) {
+      const int r = rank_of(value, space.keys, best_units * UNIT);
+      if (r < p.top) space.best[r] = value;
+    }
+    __syncthreads();
+    if (tid < p.top) {
+      if (p.segments == 1) write_top(p, row, tid, space.best[tid], a.m, __builtin_amdgcn_logf(a.s));
+      else __builtin_memcpy(partial + 4 + 2 * tid, &space.best[tid], 8);
+    }
+  }
+}
+
+// A row's segments joined, by one wave: the sums in the segments' order, the
+// best of their keys one after the other.
+template <typename T> __global__ void __launch_bounds__(64) token_join_kernel(TokenArgs p) {
+  const uint32_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float* partial = p.partials + (int64_t)row * p.segments * partial_floats(p.top);
+  Sums a = no_sums();
+  for (int s = lane; s < p.segments; s += 64) {
+    const float* q = partial + s * partial_floats(p.top);
+    a = joined(a, Sums{q[0], q[1], q[2]}, p.c);
+  }
+  a = lanes_joined(a, 6, p.c);
+  const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+  const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+  if (lane == 0) finish_row(p, row, a, x, mask);
+  const float l = __builtin_amdgcn_logf(a.s);
+  uint64_t last = ~0ull;
+  for (int k = 0; k < p.top; ++k) {
+    uint64_t best = 0;
+    for (int i = lane; i < p.segments * p.top; i += 64) {
+      uint64_t key;
+      __builtin_memcpy(&key, partial + (i / p.top) * partial_floats(p.top) + 4 + 2 * (i % p.top), 8);
+      best = key < last && key > best ? key : best;
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)best, o);
+      best = other > best ? other : best;
+    }
+    last = best;
+    if (lane == 0) write_top(p, row, k, best, a.m, l);
+  }
+}
+
+// ---- backward: a workgroup takes `row_block` rows' units, or a segment of one row's
+template <typename T> __global__ void __launch_bounds__(THREADS) token_bwd_kernel(TokenArgs p) {
+  const uint32_t units = p.units.d;
+  const int first = blockIdx.y * p.segment_units, end = min((int)units, first + p.segment_units);
+  for (uint32_t row0 = blockIdx.x * p.row_block; row0 < p.rows; row0 += gridDim.x * p.row_block) {
+    const uint32_t rows = min((uint32_t)p.row_block, p.rows - row0);
+    const uint32_t count = p.row_block > 1 ? rows * units : (uint32_t)(end - first);
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+      const uint32_t r = p.row_block > 1 ? quotient(i, p.units) : 0, row = row0 + r;
+      const int col = (p.row_block > 1 ? (int)(i - r * units) : first + (int)i) * UNIT, left = p.V - col;
+      const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+      const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+      const float m = p.stats[2 * (int64_t)row], l = p.stats[2 * (int64_t)row + 1];
+      const int64_t token = token_of(p, row);
+      // a token that is none, or not allowed, passes nothing
+      float g = 0.f;
+      if (p.dlog_prob && token >= 0 && token < p.V && p.log_prob[row] > -INF)
+        g = p.dlog_prob[row_offset(row, p.steps, p.dlog_prob_s)];
+      const float h = p.dentropy ? p.dentropy[row_offset(row, p.steps, p.dentropy_s)] : 0.f, H = p.entropy[row];
+      float v[UNIT];
+      read_unit(x, mask, col, p.V, v);
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) {
+        const float w = exponent(v[j], m, p.c) - l, e = __builtin_amdgcn_exp2f(w);
+        const float d = -e * __fmaf_rn(h, __fmaf_rn(LN2, fmaxf(w, -1e4f), H), g);
+        v[j] = v[j] == -INF ? 0.f : (col + j == token ? d + g : d) * p.inverse_t;
+      }
+      store_unit(static_cast<T*>(p.dlogits) + (int64_t)row * p.V + col, left, v);
+    }
+  }
+}
+
+// ---- launches
+int check(const char* what, int dtype, int batch, int steps, int vocab, float temperature) {
+  if (dtype != TOKEN_F32 && dtype != TOKEN_BF16) return set_error(PPO_ERR_ARG, "%s: bad dtype %d", what, dtype);
+  if (batch < 0 || steps < 0 || vocab < 1 || vocab > MAX_VOCAB)
+    return set_error(PPO_ERR_ARG, "%s: bad size (batch %d steps %d vocabulary %d of 1 .. %d)", what, batch, steps, vocab,
+                     MAX_VOCAB);
+  if ((int64_t)batch * steps > (1 << 24) - 1)
+    return set_error(PPO_ERR_ARG, "%s: batch x steps above 2^24 - 1", what);
+  if (!(temperature >= 1e-30f && temperature <= 1e30f))   // (its inverse is a float32 number)
+    return set_error(PPO_ERR_ARG, "%s: temperature %g is not from 1e-30 to 1e30", what, (double)temperature);
+  return PPO_OK;
+}
+
+// Parts of a wide row: as many as keep every CU busy where rows are few, of at
+// least 4096 columns.
+int segments_of(int64_t rows, int vocab) {
+  if (vocab <= NARROW) return 1;
+  const int64_t fill = std::min(ceil_div64(1024, std::max<int64_t>(rows, 1)), ceil_div64(vocab, 4096));
+  return (int)std::min<int64_t>(MAX_SEGMENTS, std::max(fill, ceil_div64(vocab, SEGMENT)));
+}
+
+TokenArgs common_args(const void* logits, const void* tokens, int wide_tokens, const uint8_t* mask,
+                      const int64_t* strides, float temperature, int batch, int steps, int vocab) {
+  TokenArgs a{};
+  a.logits = logits;
+  a.mask = mask;
+  a.tokens = tokens;
+  a.logits_s = RowStride{strides[0], strides[1]};
+  a.mask_s = RowStride{strides[2], strides[3]};
+  a.steps = divisor((uint32_t)steps);
+  a.units = divisor((uint32_t)ceil_div(vocab, UNIT));
+  a.rows = (uint32_t)((int64_t)batch * steps);
+  a.V = vocab;
+  a.c = (float)(1.4426950408889634 / (double)temperature);
+  a.inverse_t = (float)(1.0 / (double)temperature);
+  a.wide_tokens = wide_tokens != 0;
+  return a;
+}
+
+template <typename T> void launch_fwd(hipStream_t st, TokenArgs& a) {
+  if (a.V <= NARROW) {
+    while ((UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
+    const unsigned blocks = (unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS));
+    if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true>), dim3(blocks), dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((token_narrow_kernel<T, false>), dim3(blocks), dim3(THREADS), 0, st, a);
+    return;
+  }
+  const dim3 grid(a.rows, a.segments);
+  if (a.top) hipLaunchKernelGGL((token_wide_kernel<T, true>), grid, dim3(THREADS), 0, st, a);
+  else hipLaunchKernelGGL((token_wide_kernel<T, false>), grid, dim3(THREADS), 0, st, a);
+  if (a.segments > 1) hipLaunchKernelGGL((token_join_kernel<T>), dim3(a.rows), dim3(64), 0, st, a);
+}
+
+}  // namespace
+
+PPO_EXPORT int ppo_token_log_probs_max_top(void) { return MAX_TOP; }
+PPO_EXPORT int ppo_token_log_probs_max_vocab(void) { return MAX_VOCAB; }
+
+PPO_EXPORT size_t ppo_token_log_probs_workspace(int batch, int steps, int vocab, int top) {
+  if (batch <= 0 || steps <= 0 || vocab <= NARROW || vocab > MAX_VOCAB || top < 0 || top > MAX_TOP) return 0;
+  const int64_t rows = (int64_t)batch * steps;
+  const int s = segments_of(rows, vocab);
+  return s > 1 ? sizeof(float) * (size_t)(4 + 2 * top) * (size_t)rows * s : 0;
+}
+
+PPO_EXPORT int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logits, const void* tokens,
+                                       int wide_tokens, const uint8_t* mask, const int64_t* strides,
+                                       float temperature, int top, float* log_prob, float* entropy, float* stats,
+                                       float* top_log_probs, void* top_tokens, void* workspace,
+                                       size_t workspace_bytes, int batch, int steps, int vocab) {
+  const char* what = "ppo_token_log_probs_fwd";
+  if (int rc = check(what, dtype, batch, steps, vocab, temperature)) return rc;
+  if (top < 0 || top > MAX_TOP) return set_error(PPO_ERR_ARG, "%s: %d alternatives of 0 .. %d", what, top, MAX_TOP);
+  if ((int64_t)batch * steps == 0) return PPO_OK;
+  if (!logits || !tokens || !strides || !log_prob || !entropy || (top > 0 && (!top_log_probs || !top_tokens)))
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  const size_t need = ppo_token_log_probs_workspace(batch, steps, vocab, top);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  TokenArgs a = common_args(logits, tokens, wide_tokens, mask, strides, temperature, batch, steps, vocab);
+  a.log_prob = log_prob;
+  a.entropy = entropy;
+  a.stats = stats;
+  a.top = top;
+  a.top_log_probs = top_log_probs;
+  a.top_tokens = top_tokens;
+  a.partials = static_cast<float*>(workspace);
+  a.segments = segments_of(a.rows, vocab);
+  a.segment_units = ceil_div(ceil_div(vocab, UNIT), a.segments);
+  if (dtype == TOKEN_F32) launch_fwd<float>(as_stream(stream), a);
+  else launch_fwd<uint16_t>(as_stream(stream), a);
+  return check_launch(what);
+}
+
+PPO_EXPORT int ppo_token_log_probs_bwd(void* stream, int dtype, const void* logits, const void* tokens,
+                                       int wide_tokens, const uint8_t* mask, const int64_t* strides,
+                                       float temperature, const float* log_prob, const float* entropy,
+                                       const float* stats, const float* dlog_prob, const float* dentropy,
+                                       void* dlogits, int batch, int steps, int vocab) {
+  const char* what = "ppo_token_log_probs_bwd";
+  if (int rc = check(what, dtype, batch, steps, vocab, temperature)) return rc;
+  if ((int64_t)batch * steps == 0) return PPO_OK;
+  if (!logits || !tokens || !strides || !log_prob || !entropy || !stats || !dlogits)
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  TokenArgs a = common_args(logits, tokens, wide_tokens, mask, strides, temperature, batch, steps, vocab);
+  a.log_prob = const_cast<float*>(log_prob);
+  a.entropy = const_cast<float*>(entropy);
+  a.stats = const_cast<float*>(stats);
+  a.dlog_prob = dlog_prob;
+  a.dentropy = dentropy;
+  a.dlog_prob_s = RowStride{strides[4], strides[5]};
+  a.dentropy_s = RowStride{strides[6], strides[7]};
+  a.dlogits = dlogits;
+  const int units = (int)a.units.d;
+  a.row_block = std::max(1, 2 * THREADS / units);
+  a.segment_units = a.row_block > 1 ? units : std::min(units, 8 * THREADS);
+  const dim3 grid((unsigned)ceil_div64(a.rows, a.row_block), (unsigned)ceil_div(units, a.segment_units));
+  if (dtype == TOKEN_F32) hipLaunchKernelGGL((token_bwd_kernel<float>), grid, dim3(THREADS), 0, as_stream(stream), a);
+  else hipLaunchKernelGGL((token_bwd_kernel<uint16_t>), grid, dim3(THREADS), 0, as_stream(stream), a);
+  return check_launch(what);
+}

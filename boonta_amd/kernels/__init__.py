@@ -2,6 +2,7 @@
 from .attention import linear_attention, linear_attention_step, qk_norm_rotary, rotary_frequencies
 from .residual import residual_norm
 from .scan import get_scan_implementation, hip, scan, ssm, ssm_scan
+from .tokens import TokenLogProbs, token_log_probs
 
-__all__ = ["get_scan_implementation", "hip", "linear_attention", "linear_attention_step", "qk_norm_rotary",
-           "residual_norm", "rotary_frequencies", "scan", "ssm", "ssm_scan"]
+__all__ = ["TokenLogProbs", "get_scan_implementation", "hip", "linear_attention", "linear_attention_step",
+           "qk_norm_rotary", "residual_norm", "rotary_frequencies", "scan", "ssm", "ssm_scan", "token_log_probs"]

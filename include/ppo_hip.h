@@ -467,6 +467,35 @@ int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void*
                           float* dpost_scale, float* dresidual_scale, float* dpre_scale, void* workspace,
                           size_t workspace_bytes, int batch, int steps, int width);
 
+/* Log probabilities of given tokens, entropies and the `top` best alternatives
+ * of rows of logits (boonta/networks/distributions.py:8-38 for any vocabulary,
+ * with a mask).  Per row of `vocab` logits over `temperature`, -inf where the
+ * mask does not allow: log_prob float [batch x steps] of the row's token (-inf
+ * where it is not allowed; a token outside 0 .. vocab - 1 is none: 0), entropy
+ * float [batch x steps] (0 where nothing is allowed), top_log_probs float and
+ * top_tokens [batch x steps, top] in falling order, equal ones by index (-inf
+ * and -1 past the allowed ones; a NaN is none).  dtype 0 = float32, 1 = bf16
+ * logits; tokens and top_tokens int64 where wide_tokens, else int32; mask uint8
+ * or NULL.  Columns side by side, element strides of (batch, step) in the host
+ * array `strides`, 2 for each of logits and mask (any where NULL).  stats float
+ * [batch x steps, 2] for the backward (NULL: none).  top at most
+ * ppo_token_log_probs_max_top(), vocab ppo_token_log_probs_max_vocab(), batch x
+ * steps 2^24 - 1; workspace 8-byte aligned. */
+int ppo_token_log_probs_max_top(void);
+int ppo_token_log_probs_max_vocab(void);
+size_t ppo_token_log_probs_workspace(int batch, int steps, int vocab, int top);
+int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logits, const void* tokens, int wide_tokens,
+                            const uint8_t* mask, const int64_t* strides, float temperature, int top, float* log_prob,
+                            float* entropy, float* stats, float* top_log_probs, void* top_tokens, void* workspace,
+                            size_t workspace_bytes, int batch, int steps, int vocab);
+/* dlogits contiguous, of the logits' type, from the cotangents of log_prob and
+ * entropy (either NULL: zeros; strides: 2 more for each).  A token that is none
+ * or not allowed passes none, and logits that are not allowed get 0. */
+int ppo_token_log_probs_bwd(void* stream, int dtype, const void* logits, const void* tokens, int wide_tokens,
+                            const uint8_t* mask, const int64_t* strides, float temperature, const float* log_prob,
+                            const float* entropy, const float* stats, const float* dlog_prob, const float* dentropy,
+                            void* dlogits, int batch, int steps, int vocab);
+
 /* ------------------------------------------------------------------ GEMM
  * Dense layers of the torso and heads (flax.linen.Dense as composed in
  * hangar/recipes/*.py; forward at boonta/networks/network.py:38-49, backward
