@@ -74,6 +74,12 @@ SIGNATURES = {
     "ppo_linear_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, I, I, I]),
     "ppo_ssm_scan_fwd": (I, [P, I, P, P, P, P, P, P, I, I, I]),
     "ppo_ssm_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, I, I, I]),
+    "ppo_gated_scan_workspace": (SZ, [I, I, I, I]),
+    "ppo_gated_scan_states": (SZ, [I, I, I, I]),
+    "ppo_gated_scan_fwd": (I, [P, I, P, P, P, P, P, P, P, P, P, P, P, P, SZ, I, I, I]),
+    "ppo_gated_scan_bwd_workspace": (SZ, [I, I, I, I]),
+    "ppo_gated_scan_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, SZ, I, I, I]),
+    "ppo_gated_scan_step": (I, [P, I, P, P, P, P, P, P, P, P, P, I, I]),
     "ppo_linear_attention_max_width": (I, []),
     "ppo_linear_attention_min_width": (I, [I]),
     "ppo_linear_attention_workspace": (SZ, [I, I, I, I, I, I]),

@@ -1,0 +1,899 @@
+// A linear recurrence whose decay and input weight are gated step by step, the
+// gates formed in the same pass, and its vector-Jacobian product.
+//
+// Per feature, with r = sigmoid(decay_gate), i = sigmoid(input_gate):
+//   a = exp(-rate r), w = sqrt(1 - a^2), h_t = a_t (done_t ? 0 : h_{t-1}) + w_t i_t x_t
+// Backward, from the cotangents g of h and that of the final state:
+//   E_t = a'_t (g_t + E_{t+1}) (a' = a, 0 where done; E after the last step: the
+//   final state's cotangent; E_0: the carry's), D_t = g_t + E_{t+1},
+//   dx = D w i, dinput_gate = D w x i (1 - i), and with
+//   dL = D (a h_{t-1} - a^2 i x / w) (h_{t-1} = 0 where done; L = -rate r)
+//   ddecay_gate = dL L (1 - r), drate = sum of -dL r.
+// 1 - a^2 = -expm1(-2 rate r) is a series where it is small: a^2 rounds away
+// there.  A rate of 0 keeps the state: w = 0, and the term through 1 / w is taken as 0.
+//
+// Both directions compose affine maps.  A lane holds a chunk of steps of VW
+// features in registers, LF lanes stand side by side over the features and the
+// rest of the workgroup over the time: a chunk's map, composed with those of the
+// chunks before it (lanes by shuffles, waves through LDS), gives the state that
+// enters it, and its outputs come from the same registers, so that every operand
+// is read once.  Tile follows tile with the state in registers and the next
+// tile's operands on their way.  Where sequences and features do not fill the
+// chip, the time is cut into segments as well: a launch before forms the map of
+// each, and each composes those before it.  The backward forms the states of a
+// tile again from the one entering it, which the forward leaves in float32, and
+// so needs no output.
+//
+// A map's decay is -0 where a step of it starts an episode: then nothing of what
+// enters, an infinity or NaN neither, passes.
+#include "row_io.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace ppo;
+
+enum GateDtype { GATE_F32 = 0, GATE_BF16 = 1 };
+
+constexpr int MAX_WAVES = 8;
+constexpr int FWD_STEPS = 8, BWD_STEPS = 4;   // of a lane's chunk
+constexpr float LOG2E = 1.4426950408889634f, LN2_2 = 1.3862943611198906f;
+constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
+constexpr int MAX_SEGMENTS = 64;
+
+struct GatedArgs {
+  const void *x, *input_gate, *decay_gate;
+  const float* rate;
+  const float* carry;       // [batch, F], or null (zeros)
+  const uint8_t* done;      // [batch, steps], or null
+  const int32_t* lengths;   // [batch], or null (steps)
+  void* out;                // forward
+  float* final;
+  float* states;            // [batch, saved, F], entering every `save`-th step
+  float* maps;              // [batch, segments, 2, F]: decay, sum
+  const void* dout;         // backward
+  const float* dfinal;      // or null (zeros)
+  void *dx, *dinput_gate, *ddecay_gate;
+  float* dcarry;            // or null
+  float* partials;          // [batch, segments, F]: drate, or null
+  RowStride x_s, input_s, decay_s, dout_s;
+  int steps, F, blocks;     // blocks: workgroups over the features
+  int segment, segments;    // steps of one; how many
+  int save_log2, saved;
+};
+
+__device__ __forceinline__ bool is_reset(float a) { return __float_as_uint(a) == 0x80000000u; }
+// The map (a, b) of h; b alone past a reset.
+__device__ __forceinline__ float apply(float a, float b, float h) { return is_reset(a) ? b : __fmaf_rn(a, h, b); }
+// The decay of two maps one after the other.
+__device__ __forceinline__ float decay_of(float later, float earlier) { return is_reset(later) ? later : later * earlier; }
+
+struct Gates {
+  float i, r, a, w, over_w;   // over_w: 1 / w, or 0
+  float not_i, not_r;         // 1 - i, 1 - r
+};
+// rl = rate log2(e)
+__device__ __forceinline__ Gates gates_of(float input, float decay, float rl) {
+  Gates g;
+  g.i = sigmoid(input, g.not_i);
+  g.r = sigmoid(decay, g.not_r);
+  const float q = rl * g.r;
+  g.a = __builtin_amdgcn_exp2f(-q);
+  // 1 - a^2 = 1 - e^-z = z - z^2 / 2 + ...: below z = 1/4 the terms left out are under 5e-8 of it
+  const float z = LN2_2 * q;
+  float s = __fmaf_rn(z, -1.f / 720.f, 1.f / 120.f);
+  s = __fmaf_rn(z, s, -1.f / 24.f);
+  s = __fmaf_rn(z, s, 1.f / 6.f);
+  s = __fmaf_rn(z, s, -0.5f);
+  s = __fmaf_rn(z, s, 1.f);
+  const float w2 = z < 0.25f ? z * s : __fmaf_rn(-g.a, g.a, 1.f);
+  g.over_w = w2 > 0.f ? __builtin_amdgcn_rsqf(w2) : w2 * 0.f;   // (NaN of NaN)
+  g.w = w2 * g.over_w;
+  return g;
+}
+
+// VW values as stored.
+template <typename S, int VW> struct Raw {
+  S v[VW];
+};
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+template <typename S, int VW> __device__ __forceinline__ Raw<S, VW> load_raw(const char* base, int64_t offset) {
+  Raw<S, VW> r;
+  __builtin_memcpy(r.v, base + offset, sizeof(r.v));
+  return r;
+}
+// (a base of the whole wave and a lane's 32-bit offset)
+template <typename S, int VW> __device__ __forceinline__ Raw<S, VW> load_near(const char* base, uint32_t offset) {
+  Raw<S, VW> r;
+  __builtin_memcpy(r.v, base + offset, sizeof(r.v));
+  return r;
+}
+template <int VW> __device__ __forceinline__ void store_near(float* base, uint32_t offset, const float (&v)[VW]) {
+  __builtin_memcpy(reinterpret_cast<char*>(base) + offset, v, 4 * VW);
+}
+template <int VW> __device__ __forceinline__ void store_near(uint16_t* base, uint32_t offset, const float (&v)[VW]) {
+  char* p = reinterpret_cast<char*>(base) + offset;
+  if constexpr (VW == 1) {
+    const uint16_t u = (uint16_t)pack_bf16(v[0], v[0]);
+    __builtin_memcpy(p, &u, 2);
+  } else {
+    uint32_t u[VW / 2];
+#pragma unroll
+    for (int k = 0; k < VW / 2; ++k) u[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
+    __builtin_memcpy(p, u, 2 * VW);
+  }
+}
+
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Flags of up to 8 steps from t on (those below `steps`), a byte each.
+template <int N> __device__ __forceinline__ uint64_t load_flags(const uint8_t* done, int t, int steps) {
+  uint64_t f = 0;
+  if (t + N <= steps) {
+    __builtin_memcpy(&f, done + t, N);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (t + i < steps) f |= (uint64_t)done[t + i] << (8 * i);
+  }
+  return f;
+}
+__device__ __forceinline__ bool flag(uint64_t f, int i) { return (f >> (8 * i)) & 0xff; }
+
+// Where a lane stands: LF lanes over the features, SLOTS of a wave over the
+// time, each with a chunk of N steps.
+template <int VW, int LF, int N> struct Lane {
+  static constexpr int SLOTS = 64 / LF;
+  int lane, wave, waves, slot, b, f0, tile;
+  __device__ __forceinline__ explicit Lane(const GatedArgs& p) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    waves = blockDim.x >> 6;
+    slot = lane / LF;
+    b = blockIdx.x / p.blocks;
+    const int fb = blockIdx.x - b * p.blocks;
+    // lanes past the row's end repeat its last features: they read and write the same values
+    f0 = min((fb * LF + lane % LF) * VW, p.F - VW);
+    tile = waves * SLOTS * N;
+  }
+  // first step of the wave's, and the lane's, chunks in the tile from t0 on
+  __device__ __forceinline__ int wave_step(int t0) const { return t0 + wave * SLOTS * N; }
+  __device__ __forceinline__ int chunk_step(int t0) const { return wave_step(t0) + slot * N; }
+};
+
+// A tensor's N steps of a lane's chunk: row offsets within 32 bits of the
+// wave's first where the tile is whole, clamped rows of it otherwise.
+template <typename S, int VW, int N, typename L>
+__device__ __forceinline__ void fetch_steps(const void* x, const RowStride& s, const L& at, int t0, int end, bool whole,
+                                            Raw<S, VW> (&v)[N]) {
+  const char* base = static_cast<const char*>(x) + (int64_t)at.b * s.batch * (int64_t)sizeof(S);
+  if (whole) {
+    const uint32_t near = (uint32_t)(at.slot * N * (int)s.step + at.f0) * (uint32_t)sizeof(S);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = load_near<S, VW>(base + (at.wave_step(t0) + i) * s.step * (int64_t)sizeof(S), near);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = load_raw<S, VW>(base, (min(at.chunk_step(t0) + i, end - 1) * s.step + at.f0) * (int64_t)sizeof(S));
+  }
+}
+// and of an output [batch, steps, F]: steps below `end`.
+template <typename S, int VW, int N, typename L>
+__device__ __forceinline__ void store_step(void* out, const GatedArgs& p, const L& at, int t0, int i, int end, bool whole,
+                                           const float (&v)[VW]) {
+  if (!whole && at.chunk_step(t0) + i >= end) return;
+  S* base = static_cast<S*>(out) + ((int64_t)at.b * p.steps + at.wave_step(t0) + i) * p.F;
+  store_near<VW>(base, (uint32_t)(at.slot * N * p.F + at.f0) * (uint32_t)sizeof(S), v);
+}
+template <typename S, int VW, int LF, int N>
+__device__ __forceinline__ void clear_steps(void* out, const GatedArgs& p, const Lane<VW, LF, N>& at, int from, int end) {
+  float zero[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) zero[k] = 0.f;
+  for (int t = from + at.wave * at.SLOTS + at.slot; t < end; t += at.waves * at.SLOTS)
+    store_near<VW>(static_cast<S*>(out) + ((int64_t)at.b * p.steps + t) * p.F, (uint32_t)at.f0 * (uint32_t)sizeof(S), zero);
+}
+
+// The state of VW features at b's row of a [batch, F] array, or zeros.
+template <int VW> __device__ __forceinline__ void load_state(const float* p, int64_t at, float (&h)[VW]) {
+#pragma unroll
+  for (int k = 0; k < VW; ++k) h[k] = p ? p[at + k] : 0.f;
+}
+
+// The maps (A, B) of a wave's slots composed: on return those of the slots
+// before (REVERSE: after) the lane's, and in LDS the wave's own.
+template <int VW, int LF, bool REVERSE>
+__device__ __forceinline__ void compose_slots(float (&A)[VW], float (&B)[VW], int lane, float* wave_a, float* wave_b) {
+  constexpr int SLOTS = 64 / LF;
+  const int slot = REVERSE ? SLOTS - 1 - lane / LF : lane / LF;   // (in the order of the maps)
+#pragma unroll
+  for (int d = 1; d < SLOTS; d <<= 1) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      const int from = REVERSE ? lane + d * LF : lane - d * LF;
+      const float a = __shfl(A[k], from), b = __shfl(B[k], from);
+      if (slot >= d) {
+        B[k] = apply(A[k], B[k], b);
+        A[k] = decay_of(A[k], a);
+      }
+    }
+  }
+  if (slot == SLOTS - 1) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      wave_a[(lane % LF) * VW + k] = A[k];
+      wave_b[(lane % LF) * VW + k] = B[k];
+    }
+  }
+  if constexpr (SLOTS > 1) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      const int from = REVERSE ? lane + LF : lane - LF;
+      const float a = __shfl(A[k], from), b = __shfl(B[k], from);
+      A[k] = slot > 0 ? a : 1.f;
+      B[k] = slot > 0 ? b : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      A[k] = 1.f;
+      B[k] = 0.f;
+    }
+  }
+}
+// The state h entering the tile carried through the waves' maps: on return h
+// leaves the tile, and `mine` enters the lane's chunk, whose slots' map before it is (A, B).
+template <int VW, int LF, bool REVERSE>
+__device__ __forceinline__ void through_waves(float (&h)[VW], float (&mine)[VW], const float (&A)[VW],
+                                              const float (&B)[VW], const float* wave_a, const float* wave_b, int lane,
+                                              int wave, int waves) {
+  for (int i = 0; i < waves; ++i) {
+    const int w = REVERSE ? waves - 1 - i : i;
+    if (w == wave) {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) mine[k] = h[k];
+    }
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      const int at = (w * LF + lane % LF) * VW + k;
+      h[k] = apply(wave_a[at], wave_b[at], h[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VW; ++k) mine[k] = apply(A[k], B[k], mine[k]);
+}
+
+// The state entering the segment from those before (REVERSE: after) it.
+template <int VW, bool REVERSE>
+__device__ __forceinline__ void through_segments(const GatedArgs& p, int64_t b, int f0, int segment, float (&h)[VW]) {
+  const int n = REVERSE ? p.segments - 1 - segment : segment;
+  for (int i = 0; i < n; ++i) {
+    const int64_t at = ((b * p.segments + (REVERSE ? p.segments - 1 - i : i)) * 2) * p.F + f0;
+#pragma unroll
+    for (int k = 0; k < VW; ++k) h[k] = apply(p.maps[at + k], p.maps[at + p.F + k], h[k]);
+  }
+}
+
+template <typename S, int VW, int LF, bool MAPS>
+__global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) {
+  constexpr int N = FWD_STEPS;
+  __shared__ float wave_a[2][MAX_WAVES * LF * VW], wave_b[2][MAX_WAVES * LF * VW];
+  const Lane<VW, LF, N> at(p);
+  const int segment = blockIdx.y, begin = segment * p.segment, end = min(p.steps, begin + p.segment);
+  const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
+  const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
+  float h[VW], decay[VW], rl[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) rl[k] = p.rate[at.f0 + k] * LOG2E;
+  if constexpr (MAPS) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      h[k] = 0.f;
+      decay[k] = 1.f;
+    }
+  } else {
+    load_state<VW>(p.carry, (int64_t)at.b * p.F + at.f0, h);
+    through_segments<VW, false>(p, at.b, at.f0, segment, h);
+  }
+  Raw<S, VW> x[2][N], ig[2][N], dg[2][N];
+  uint64_t flags[2] = {0, 0};
+  auto fetch = [&](int set, int t0) {
+    const bool whole = t0 + at.tile <= live_end;
+    fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x[set]);
+    fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig[set]);
+    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg[set]);
+    if (done) flags[set] = load_flags<N>(done, at.chunk_step(t0), p.steps);
+  };
+  auto step_tile = [&](int set, int t0) {
+    const bool whole = t0 + at.tile <= live_end;
+    const int t = at.chunk_step(t0);
+    const bool resets = __any(flags[set] != 0);
+    float a[N][VW], b[N][VW], A[VW], B[VW], mine[VW];
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      A[k] = 1.f;
+      B[k] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates g = gates_of(widen(ig[set][i].v[k]), widen(dg[set][i].v[k]), rl[k]);
+        a[i][k] = g.a;
+        b[i][k] = g.w * g.i * widen(x[set][i].v[k]);
+      }
+    if (resets || !whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool live = t + i < live_end, cut = flag(flags[set], i);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          a[i][k] = live ? (cut ? -0.f : a[i][k]) : 1.f;
+          b[i][k] = live ? b[i][k] : 0.f;
+          B[k] = apply(a[i][k], b[i][k], B[k]);
+          A[k] = decay_of(a[i][k], A[k]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          B[k] = __fmaf_rn(a[i][k], B[k], b[i][k]);
+          A[k] *= a[i][k];
+        }
+    }
+    const int next = t0 + at.tile;
+    if (next < live_end) fetch(set ^ 1, next);
+    float *pa = wave_a[set], *pb = wave_b[set];
+    compose_slots<VW, LF, false>(A, B, at.lane, pa + at.wave * LF * VW, pb + at.wave * LF * VW);
+    lds_barrier();
+    if constexpr (MAPS) {
+      for (int w = 0; w < at.waves; ++w)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const int j = (w * LF + at.lane % LF) * VW + k;
+          h[k] = apply(pa[j], pb[j], h[k]);
+          decay[k] = decay_of(pa[j], decay[k]);
+        }
+    } else {
+      through_waves<VW, LF, false>(h, mine, A, B, pa, pb, at.lane, at.wave, at.waves);
+      if (p.states && t < live_end && (t & ((1 << p.save_log2) - 1)) == 0) {
+        float* s = p.states + ((int64_t)at.b * p.saved + (t >> p.save_log2)) * p.F + at.f0;
+#pragma unroll
+        for (int k = 0; k < VW; ++k) s[k] = mine[k];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float o[VW];
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          mine[k] = resets ? apply(a[i][k], b[i][k], mine[k]) : __fmaf_rn(a[i][k], mine[k], b[i][k]);
+          o[k] = whole || t + i < live_end ? mine[k] : 0.f;
+        }
+        store_step<S, VW, N>(p.out, p, at, t0, i, end, whole, o);
+      }
+    }
+  };
+  // (the register sets alternate by unrolling, so that each is indexed by a constant)
+  if (begin < live_end) fetch(0, begin);
+  int t0 = begin;
+  while (t0 < live_end) {
+    step_tile(0, t0);
+    t0 += at.tile;
+    if (t0 >= live_end) break;
+    step_tile(1, t0);
+    t0 += at.tile;
+  }
+  if constexpr (MAPS) {
+    if (at.wave == 0 && at.slot == 0) {
+      float* m = p.maps + (((int64_t)at.b * p.segments + segment) * 2) * p.F + at.f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        m[k] = decay[k];
+        m[p.F + k] = h[k];
+      }
+    }
+  } else {
+    clear_steps<S>(p.out, p, at, t0, end);
+    if (segment == p.segments - 1 && at.wave == 0 && at.slot == 0) {
+      float* f = p.final + (int64_t)at.b * p.F + at.f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) f[k] = h[k];
+    }
+  }
+}
+
+template <typename S, int VW, int LF, bool MAPS>
+__global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) {
+  constexpr int N = BWD_STEPS;
+  __shared__ float fwd_a[2][MAX_WAVES * LF * VW], fwd_b[2][MAX_WAVES * LF * VW];
+  __shared__ float rev_a[2][MAX_WAVES * LF * VW], rev_b[2][MAX_WAVES * LF * VW];
+  const Lane<VW, LF, N> at(p);
+  const int segment = blockIdx.y + (MAPS ? 1 : 0), begin = segment * p.segment;   // (of the first no map is needed)
+  const int end = min(p.steps, begin + p.segment);
+  const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
+  const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
+  const int64_t state = (int64_t)at.b * p.F + at.f0;
+  float E[VW], decay[VW], rl[VW], drate[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    rl[k] = p.rate[at.f0 + k] * LOG2E;
+    drate[k] = 0.f;
+    decay[k] = 1.f;
+    E[k] = 0.f;
+  }
+  if constexpr (!MAPS) {
+    load_state<VW>(p.dfinal, state, E);
+    through_segments<VW, true>(p, at.b, at.f0, segment, E);
+  }
+  Raw<S, VW> x[2][N], ig[2][N], dg[2][N], go[2][N];
+  float entering[2][VW];
+  uint64_t flags[2] = {0, 0};
+  auto fetch = [&](int set, int t0) {
+    const bool whole = t0 + at.tile <= live_end;
+    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg[set]);
+    fetch_steps<S, VW, N>(p.dout, p.dout_s, at, t0, live_end, whole, go[set]);
+    if constexpr (!MAPS) {
+      fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x[set]);
+      fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig[set]);
+      load_state<VW>(p.states, ((int64_t)at.b * p.saved + (t0 >> p.save_log2)) * p.F + at.f0, entering[set]);
+    }
+    if (done) flags[set] = load_flags<N>(done, at.chunk_step(t0), p.steps);
+  };
+  auto step_tile = [&](int set, int t0) {
+    const bool whole = t0 + at.tile <= live_end;
+    const int t = at.chunk_step(t0);
+    const bool resets = __any(flags[set] != 0);
+    Gates g[N][VW];
+    float a[N][VW], go_[N][VW], b[N][VW];   // a: with resets, and 1 past the end
+    float A[VW], B[VW], RA[VW], RB[VW];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        g[i][k] = gates_of(MAPS ? 0.f : widen(ig[set][i].v[k]), widen(dg[set][i].v[k]), rl[k]);
+        a[i][k] = g[i][k].a;
+        go_[i][k] = widen(go[set][i].v[k]);
+        b[i][k] = MAPS ? 0.f : g[i][k].w * g[i][k].i * widen(x[set][i].v[k]);
+      }
+    if (resets || !whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool live = t + i < live_end, cut = flag(flags[set], i);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          a[i][k] = live ? (cut ? -0.f : a[i][k]) : 1.f;
+          b[i][k] = live ? b[i][k] : 0.f;
+          go_[i][k] = live ? go_[i][k] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      A[k] = 1.f;
+      B[k] = RB[k] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        B[k] = apply(a[i][k], b[i][k], B[k]);
+        A[k] = decay_of(a[i][k], A[k]);
+        // E through step N - 1 - i: a (g + E)
+        const float aa = a[N - 1 - i][k], sum = go_[N - 1 - i][k] + RB[k];
+        RB[k] = is_reset(aa) ? 0.f : aa * sum;
+      }
+#pragma unroll
+    for (int k = 0; k < VW; ++k) RA[k] = A[k];
+    const int next = t0 - at.tile;
+    if (next >= begin) fetch(set ^ 1, next);
+    const int mine_at = at.wave * LF * VW;
+    if constexpr (!MAPS) compose_slots<VW, LF, false>(A, B, at.lane, fwd_a[set] + mine_at, fwd_b[set] + mine_at);
+    compose_slots<VW, LF, true>(RA, RB, at.lane, rev_a[set] + mine_at, rev_b[set] + mine_at);
+    lds_barrier();
+    if constexpr (MAPS) {
+      for (int w = at.waves - 1; w >= 0; --w)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const int j = (w * LF + at.lane % LF) * VW + k;
+          E[k] = apply(rev_a[set][j], rev_b[set][j], E[k]);
+          decay[k] = decay_of(rev_a[set][j], decay[k]);
+        }
+      return;
+    }
+    float h[VW], mine[VW], after[VW], before[N][VW];
+#pragma unroll
+    for (int k = 0; k < VW; ++k) h[k] = entering[set][k];
+    through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
+    through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        before[i][k] = is_reset(a[i][k]) ? 0.f : mine[k];
+        mine[k] = apply(a[i][k], b[i][k], mine[k]);
+      }
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) {
+      const bool live = whole || t + i < live_end;
+      float ox[VW], oi[VW], od[VW];
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates& q = g[i][k];
+        const float D = go_[i][k] + after[k], xv = widen(x[set][i].v[k]);
+        after[k] = is_reset(a[i][k]) ? 0.f : a[i][k] * D;
+        const float dw = D * q.w * q.i;
+        ox[k] = live ? dw : 0.f;
+        oi[k] = live ? dw * xv * q.not_i : 0.f;
+        const float dr = D * (q.a * __fmaf_rn(-q.a * q.over_w, q.i * xv, before[i][k])) * q.r;   // dL r
+        od[k] = live ? -dr * rl[k] * (1.f / LOG2E) * q.not_r : 0.f;
+        drate[k] -= live ? dr : 0.f;
+      }
+      store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
+      store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
+      store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
+    }
+  };
+  const int tiles = live_end > begin ? (live_end - begin + at.tile - 1) / at.tile : 0;
+  int t0 = begin + (tiles - 1) * at.tile;
+  if (tiles > 0) fetch(0, t0);
+  while (t0 >= begin) {
+    step_tile(0, t0);
+    t0 -= at.tile;
+    if (t0 < begin) break;
+    step_tile(1, t0);
+    t0 -= at.tile;
+  }
+  if constexpr (MAPS) {
+    if (at.wave == 0 && at.slot == 0) {
+      float* m = p.maps + (((int64_t)at.b * p.segments + segment) * 2) * p.F + at.f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        m[k] = decay[k];
+        m[p.F + k] = E[k];
+      }
+    }
+  } else {
+    const int cleared = begin + tiles * at.tile;
+    clear_steps<S>(p.dx, p, at, cleared, end);
+    clear_steps<S>(p.dinput_gate, p, at, cleared, end);
+    clear_steps<S>(p.ddecay_gate, p, at, cleared, end);
+    if (p.dcarry && segment == 0 && at.wave == 0 && at.slot == 0) {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) p.dcarry[state + k] = E[k];
+    }
+    if (p.partials) {
+      // the slots' sums, added in their order
+      float* sums = &fwd_a[0][0];
+      static_assert(sizeof(fwd_a) >= sizeof(float) * MAX_WAVES * LF * VW, "a wave's sums each");
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        for (int o = LF; o < 64; o <<= 1) drate[k] += __shfl_xor(drate[k], o);
+      }
+      __syncthreads();
+      if (at.slot == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) sums[(at.wave * LF + at.lane) * VW + k] = drate[k];
+      }
+      __syncthreads();
+      if (at.wave == 0 && at.slot == 0) {
+        float* out = p.partials + ((int64_t)at.b * p.segments + segment) * p.F + at.f0;
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          float s = 0.f;
+          for (int w = 0; w < at.waves; ++w) s += sums[(w * LF + at.lane) * VW + k];
+          out[k] = s;
+        }
+      }
+    }
+  }
+}
+
+// Sums over rows [from, from + each) of parts [rows, F]: 64 columns a workgroup,
+// each wave its share of the rows in their order, then the waves'.
+__global__ void __launch_bounds__(1024) gated_rate_kernel(const float* parts, int64_t rows, int each, int F, float* out) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, f = blockIdx.x * 64 + lane;
+  const int64_t from = (int64_t)blockIdx.y * each, to = min(rows, from + each);
+  const int share = (each + 15) / 16;
+  const int64_t b1 = min(to, from + (int64_t)(wave + 1) * share);
+  float s = 0.f;
+  if (f < F) {
+    for (int64_t b0 = from + (int64_t)wave * share; b0 < b1; b0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = parts[min(b0 + k, b1 - 1) * F + f];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += b0 + k < b1 ? v[k] : 0.f;
+    }
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0 || f >= F) return;
+  s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) s += sums[w][lane];
+  out[(int64_t)blockIdx.y * F + f] = s;
+}
+
+// One step: a thread for VW features of a sequence, fewer at the row's end (the
+// new state may be the old one's memory, so that each is read by its writer alone).
+template <typename S, int VW>
+__global__ void __launch_bounds__(256) gated_step_kernel(GatedArgs p, int64_t threads, int per_row) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= threads) return;
+  const int64_t b = i / per_row;
+  const int f0 = (int)(i - b * per_row) * VW, left = p.F - f0;
+  const S* x = static_cast<const S*>(p.x) + b * p.x_s.batch + f0;
+  const S* ig = static_cast<const S*>(p.input_gate) + b * p.input_s.batch + f0;
+  const S* dg = static_cast<const S*>(p.decay_gate) + b * p.decay_s.batch + f0;
+  const float* carry = p.carry + b * p.F + f0;
+  float* final = p.final + b * p.F + f0;
+  S* out = static_cast<S*>(p.out) + b * p.F + f0;
+  const bool cut = p.done && p.done[b];
+  auto step = [&](float xv, float i_, float d, float rate, float h) {
+    const Gates g = gates_of(i_, d, rate * LOG2E);
+    return apply(cut ? -0.f : g.a, g.w * g.i * xv, h);
+  };
+  if (left >= VW) {
+    Raw<S, VW> rx, ri, rd;
+    float h[VW], rate[VW];
+    __builtin_memcpy(rx.v, x, sizeof(rx.v));
+    __builtin_memcpy(ri.v, ig, sizeof(ri.v));
+    __builtin_memcpy(rd.v, dg, sizeof(rd.v));
+    __builtin_memcpy(h, carry, sizeof(h));
+    __builtin_memcpy(rate, p.rate + f0, sizeof(rate));
+#pragma unroll
+    for (int k = 0; k < VW; ++k) h[k] = step(widen(rx.v[k]), widen(ri.v[k]), widen(rd.v[k]), rate[k], h[k]);
+    store_near<VW>(final, 0, h);
+    store_near<VW>(out, 0, h);
+  } else {
+    for (int k = 0; k < left; ++k) {
+      const float h[1] = {step(widen(x[k]), widen(ig[k]), widen(dg[k]), p.rate[f0 + k], carry[k])};
+      store_near<1>(final + k, 0, h);
+      store_near<1>(out + k, 0, h);
+    }
+  }
+}
+
+// ---- launches
+// How a direction lays its lanes: features of a lane and lanes over the
+// features, waves, workgroups over the features, segments.
+struct Plan {
+  int vw, lf, waves, blocks, tile, segment, segments;
+};
+constexpr int TARGET = 512;   // workgroups that fill the chip
+
+Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
+  Plan s;
+  const int N = backward ? BWD_STEPS : FWD_STEPS;
+  s.vw = backward ? 2 : 4;
+  if (F < s.vw) s.vw = 1;
+  s.lf = s.vw == 1 ? 8 : 64;
+  while (s.lf > 8 && (s.lf / 2 * s.vw >= F || (int64_t)batch * ceil_div(F, s.lf * s.vw) < TARGET) &&
+         128 / s.lf * N < 2 * (int64_t)steps)
+    s.lf /= 2;
+  const int slots = 64 / s.lf;
+  s.waves = std::min(MAX_WAVES, ceil_div(steps, slots * N));
+  s.blocks = ceil_div(F, s.lf * s.vw);
+  s.tile = s.waves * slots * N;
+  // segments of at least two tiles, as many as fill the chip
+  const int64_t groups = (int64_t)batch * s.blocks;
+  const int64_t most = std::min<int64_t>(MAX_SEGMENTS, std::max(1, steps / (2 * s.tile)));
+  s.segments = (int)std::max<int64_t>(1, std::min<int64_t>(most, TARGET / std::max<int64_t>(groups, 1)));
+  const int tiles = ceil_div(steps, s.tile);
+  const int each = ceil_div(tiles, s.segments);
+  s.segment = each * s.tile;
+  s.segments = ceil_div(tiles, each);
+  return s;
+}
+
+// The steps between states that the forward leaves: the backward's tile, as a
+// power of two.
+int save_log2_of(const Plan& bwd) {
+  int log2 = 0;
+  while ((1 << log2) < bwd.tile) ++log2;
+  return log2;
+}
+
+int check(const char* what, int dtype, int batch, int steps, int features) {
+  if (dtype != GATE_F32 && dtype != GATE_BF16) return set_error(PPO_ERR_ARG, "%s: bad dtype %d", what, dtype);
+  if (batch < 0 || steps < 0 || features < 0)
+    return set_error(PPO_ERR_ARG, "%s: bad size (batch %d steps %d features %d)", what, batch, steps, features);
+  if (batch > 1 << 21 || steps > 1 << 30 || features > 1 << 20 || (int64_t)batch * features > 1 << 29)
+    return set_error(PPO_ERR_ARG, "%s: batch %d above 2^21, steps %d above 2^30, features %d above 2^20 or batch x "
+                     "features above 2^29", what, batch, steps, features);
+  return PPO_OK;
+}
+int check_strides(const char* what, const int64_t* strides, int tensors, int steps) {
+  for (int i = 0; i < tensors; ++i)
+    if (strides[2 * i + 1] < 0 || (steps > 1 && strides[2 * i + 1] > MAX_STRIDE))
+      return set_error(PPO_ERR_ARG, "%s: a step stride of %lld is not from 0 to 2^23", what, (long long)strides[2 * i + 1]);
+  return PPO_OK;
+}
+
+template <typename S, int VW, int LF, bool BWD>
+void launch_shape(hipStream_t st, const GatedArgs& a, const Plan& s, int batch) {
+  const unsigned groups = (unsigned)batch * (unsigned)s.blocks;
+  const dim3 t(64 * s.waves);
+  if constexpr (BWD) {
+    if (s.segments > 1)
+      hipLaunchKernelGGL((gated_bwd_kernel<S, VW, LF, true>), dim3(groups, s.segments - 1), t, 0, st, a);
+    hipLaunchKernelGGL((gated_bwd_kernel<S, VW, LF, false>), dim3(groups, s.segments), t, 0, st, a);
+  } else {
+    if (s.segments > 1)
+      hipLaunchKernelGGL((gated_fwd_kernel<S, VW, LF, true>), dim3(groups, s.segments - 1), t, 0, st, a);
+    hipLaunchKernelGGL((gated_fwd_kernel<S, VW, LF, false>), dim3(groups, s.segments), t, 0, st, a);
+  }
+}
+template <typename S, bool BWD> void launch(hipStream_t st, GatedArgs a, const Plan& s, int batch) {
+  constexpr int VW = BWD ? 2 : 4;
+  a.blocks = s.blocks;
+  a.segment = s.segment;
+  a.segments = s.segments;
+  if (s.vw == 1) launch_shape<S, 1, 8, BWD>(st, a, s, batch);
+  else if (s.lf == 64) launch_shape<S, VW, 64, BWD>(st, a, s, batch);
+  else if (s.lf == 32) launch_shape<S, VW, 32, BWD>(st, a, s, batch);
+  else if (s.lf == 16) launch_shape<S, VW, 16, BWD>(st, a, s, batch);
+  else launch_shape<S, VW, 8, BWD>(st, a, s, batch);
+}
+
+constexpr int RATE_ROWS = 512;   // of partial sums that a workgroup adds
+
+size_t maps_floats(const Plan& s, int batch, int F) { return s.segments > 1 ? 2 * (size_t)batch * s.segments * F : 0; }
+
+}  // namespace
+
+PPO_EXPORT size_t ppo_gated_scan_workspace(int dtype, int batch, int steps, int features) {
+  if (batch <= 0 || steps <= 0 || features <= 0) return 0;
+  return sizeof(float) * maps_floats(plan_of(dtype, false, batch, steps, features), batch, features);
+}
+
+PPO_EXPORT size_t ppo_gated_scan_states(int dtype, int batch, int steps, int features) {
+  if (batch <= 0 || steps <= 0 || features <= 0) return 0;
+  const int log2 = save_log2_of(plan_of(dtype, true, batch, steps, features));
+  return sizeof(float) * (size_t)batch * ceil_div64(steps, 1ll << log2) * features;
+}
+
+PPO_EXPORT int ppo_gated_scan_fwd(void* stream, int dtype, const void* x, const void* input_gate,
+                                  const void* decay_gate, const int64_t* strides, const float* rate,
+                                  const float* carry, const uint8_t* done, const int32_t* lengths, void* out,
+                                  float* final, float* states, void* workspace, size_t workspace_bytes, int batch,
+                                  int steps, int features) {
+  const char* what = "ppo_gated_scan_fwd";
+  if (int rc = check(what, dtype, batch, steps, features)) return rc;
+  if (batch == 0 || steps == 0 || features == 0) return PPO_OK;
+  if (!x || !input_gate || !decay_gate || !strides || !rate || !out || !final)
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  if (int rc = check_strides(what, strides, 3, steps)) return rc;
+  const size_t need = ppo_gated_scan_workspace(dtype, batch, steps, features);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  GatedArgs a{};
+  a.x = x;
+  a.input_gate = input_gate;
+  a.decay_gate = decay_gate;
+  a.rate = rate;
+  a.carry = carry;
+  a.done = done;
+  a.lengths = lengths;
+  a.out = out;
+  a.final = final;
+  a.states = states;
+  a.maps = static_cast<float*>(workspace);
+  a.x_s = RowStride{strides[0], strides[1]};
+  a.input_s = RowStride{strides[2], strides[3]};
+  a.decay_s = RowStride{strides[4], strides[5]};
+  a.steps = steps;
+  a.F = features;
+  a.save_log2 = save_log2_of(plan_of(dtype, true, batch, steps, features));
+  a.saved = (int)ceil_div64(steps, 1ll << a.save_log2);
+  const Plan s = plan_of(dtype, false, batch, steps, features);
+  if (dtype == GATE_F32) launch<float, false>(as_stream(stream), a, s, batch);
+  else launch<uint16_t, false>(as_stream(stream), a, s, batch);
+  return check_launch(what);
+}
+
+PPO_EXPORT size_t ppo_gated_scan_bwd_workspace(int dtype, int batch, int steps, int features) {
+  if (batch <= 0 || steps <= 0 || features <= 0) return 0;
+  const Plan s = plan_of(dtype, true, batch, steps, features);
+  const int64_t rows = (int64_t)batch * s.segments;
+  const int64_t sums = rows + (rows > RATE_ROWS ? ceil_div64(rows, RATE_ROWS) : 0);
+  return sizeof(float) * (maps_floats(s, batch, features) + (size_t)sums * features);
+}
+
+PPO_EXPORT int ppo_gated_scan_bwd(void* stream, int dtype, const void* x, const void* input_gate,
+                                  const void* decay_gate, const void* dout, const int64_t* strides, const float* rate,
+                                  const uint8_t* done, const int32_t* lengths, const float* states,
+                                  const float* dfinal, void* dx, void* dinput_gate, void* ddecay_gate, float* drate,
+                                  float* dcarry, void* workspace, size_t workspace_bytes, int batch, int steps,
+                                  int features) {
+  const char* what = "ppo_gated_scan_bwd";
+  if (int rc = check(what, dtype, batch, steps, features)) return rc;
+  if (batch == 0 || steps == 0 || features == 0) return PPO_OK;
+  if (!x || !input_gate || !decay_gate || !dout || !strides || !rate || !states || !dx || !dinput_gate || !ddecay_gate)
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  if (int rc = check_strides(what, strides, 4, steps)) return rc;
+  const size_t need = ppo_gated_scan_bwd_workspace(dtype, batch, steps, features);
+  if (!workspace || workspace_bytes < need)
+    return set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  const Plan s = plan_of(dtype, true, batch, steps, features);
+  GatedArgs a{};
+  a.x = x;
+  a.input_gate = input_gate;
+  a.decay_gate = decay_gate;
+  a.dout = dout;
+  a.rate = rate;
+  a.done = done;
+  a.lengths = lengths;
+  a.states = const_cast<float*>(states);
+  a.dfinal = dfinal;
+  a.dx = dx;
+  a.dinput_gate = dinput_gate;
+  a.ddecay_gate = ddecay_gate;
+  a.dcarry = dcarry;
+  a.maps = static_cast<float*>(workspace);
+  float* partials = a.maps + maps_floats(s, batch, features);
+  a.partials = drate ? partials : nullptr;
+  a.x_s = RowStride{strides[0], strides[1]};
+  a.input_s = RowStride{strides[2], strides[3]};
+  a.decay_s = RowStride{strides[4], strides[5]};
+  a.dout_s = RowStride{strides[6], strides[7]};
+  a.steps = steps;
+  a.F = features;
+  a.save_log2 = save_log2_of(s);
+  a.saved = (int)ceil_div64(steps, 1ll << a.save_log2);
+  if (dtype == GATE_F32) launch<float, true>(as_stream(stream), a, s, batch);
+  else launch<uint16_t, true>(as_stream(stream), a, s, batch);
+  if (drate) {
+    const int64_t rows = (int64_t)batch * s.segments;
+    const unsigned columns = (unsigned)ceil_div(features, 64);
+    if (rows > RATE_ROWS) {
+      const int64_t some = ceil_div64(rows, RATE_ROWS);
+      float* sums = partials + rows * features;
+      hipLaunchKernelGGL(gated_rate_kernel, dim3(columns, (unsigned)some), dim3(1024), 0, as_stream(stream), partials, rows,
+                         RATE_ROWS, features, sums);
+      hipLaunchKernelGGL(gated_rate_kernel, dim3(columns), dim3(1024), 0, as_stream(stream), sums, some, (int)some, features,
+                         drate);
+    } else {
+      hipLaunchKernelGGL(gated_rate_kernel, dim3(columns), dim3(1024), 0, as_stream(stream), partials, rows, (int)rows,
+                         features, drate);
+    }
+  }
+  return check_launch(what);
+}
+
+PPO_EXPORT int ppo_gated_scan_step(void* stream, int dtype, const void* x, const void* input_gate,
+                                   const void* decay_gate, const int64_t* strides, const float* rate,
+                                   const float* carry, const uint8_t* done, void* out, float* final, int batch,
+                                   int features) {
+  const char* what = "ppo_gated_scan_step";
+  if (int rc = check(what, dtype, batch, 1, features)) return rc;
+  if (batch == 0 || features == 0) return PPO_OK;
+  if (!x || !input_gate || !decay_gate || !strides || !rate || !carry || !out || !final)
+    return set_error(PPO_ERR_ARG, "%s: null buffer", what);
+  GatedArgs a{};
+  a.x = x;
+  a.input_gate = input_gate;
+  a.decay_gate = decay_gate;
+  a.rate = rate;
+  a.carry = carry;
+  a.done = done;
+  a.out = out;
+  a.final = final;
+  a.x_s = RowStride{strides[0], 0};
+  a.input_s = RowStride{strides[1], 0};
+  a.decay_s = RowStride{strides[2], 0};
+  a.steps = 1;
+  a.F = features;
+  const int per_row = ceil_div(features, 4);
+  const int64_t threads = (int64_t)batch * per_row;
+  const dim3 grid((unsigned)ceil_div64(threads, 256)), block(256);
+  if (dtype == GATE_F32) hipLaunchKernelGGL((gated_step_kernel<float, 4>), grid, block, 0, as_stream(stream), a, threads, per_row);
+  else hipLaunchKernelGGL((gated_step_kernel<uint16_t, 4>), grid, block, 0, as_stream(stream), a, threads, per_row);
+  return check_launch(what);
+}

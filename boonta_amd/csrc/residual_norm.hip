@@ -228,13 +228,14 @@ __global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_bw
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) {
       dx[j] = __fmaf_rn(-yn[j], m, dx[j]);
-      const float gate = gate_of(p, p.gate ? value(v.g, j) : 1.f);
+      float rest = 1.f;
+      const float gate = !p.gate ? 1.f : p.sigmoid_gate ? sigmoid(value(v.g, j), rest) : value(v.g, j);
       const float n = un[j] * post[j], dn = dx[j] * q[j];
       if (live) {
         dscale[j] = __fmaf_rn(dx[j], gate * n, dscale[j]);
         dpost[j] = __fmaf_rn(dn, un[j], dpost[j]);
       }
-      dg[j] = dx[j] * scale[j] * n * (p.sigmoid_gate ? gate * (1.f - gate) : 1.f);
+      dg[j] = dx[j] * scale[j] * n * (p.sigmoid_gate ? gate * rest : 1.f);
       du[j] = ru * __fmaf_rn(-un[j], mu, dn * post[j]);
     }
     if (!live) continue;

@@ -97,9 +97,16 @@ __device__ __forceinline__ float lanes_sum(float v, int log2) {
 }
 
 // A sigmoid from the hardware's exponential and reciprocal (1 ulp each): 0 and
-// 1 at the infinities, NaN of NaN.
+// 1 at the infinities, NaN of NaN.  And 1 - sigmoid, e / (1 + e) where the
+// difference would cancel (elsewhere e may be infinite).
+__device__ __forceinline__ float sigmoid(float x, float& rest) {
+  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * x), s = __builtin_amdgcn_rcpf(1.f + e);
+  rest = s > 0.5f ? e * s : 1.f - s;
+  return s;
+}
 __device__ __forceinline__ float sigmoid(float x) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+  float rest;
+  return sigmoid(x, rest);
 }
 
 }  // namespace ppo

@@ -362,6 +362,43 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
                      const void* carry, const void* cot, void* da, void* db, void* dcarry, int batch, int steps,
                      int features);
 
+/* A linear recurrence gated step by step, the gates formed in the same pass (no
+ * counterpart in the reference, whose MinGRU and SSM cells form them apart).
+ * Per feature f, with r = sigmoid(decay_gate), i = sigmoid(input_gate),
+ * a = exp(-rate[f] r), w = sqrt(1 - a^2):
+ *   h_t = a_t (done_t ? 0 : h_{t-1}) + w_t i_t x_t,  h_{-1} = carry
+ * for t < lengths[b]; later rows are not read, and theirs of the outputs and
+ * gradients are zeros.  dtype 0 = float32, 1 = bf16 storage of x, the gates, out
+ * and their gradients; states are float32.
+ *   x, input_gate, decay_gate [batch, steps, features]: columns side by side,
+ *   element strides of (batch, step) in the host array `strides`, 2 for each
+ *   (and dout in the backward); a step's stride (of more than one step) is at
+ *   most 2^23 and none is negative.  rate float [features] (>= 0), carry / final
+ *   float [batch, features] (carry may be NULL: zeros), done uint8 [batch, steps]
+ *   (NULL: none), lengths int32 [batch] (NULL: steps), out contiguous.
+ *   At most 2^21 sequences, 2^30 steps, 2^20 features, 2^29 batch x features.
+ * states: ppo_gated_scan_states() bytes for the backward (NULL: none). */
+size_t ppo_gated_scan_workspace(int dtype, int batch, int steps, int features);
+size_t ppo_gated_scan_states(int dtype, int batch, int steps, int features);
+int ppo_gated_scan_fwd(void* stream, int dtype, const void* x, const void* input_gate, const void* decay_gate,
+                       const int64_t* strides, const float* rate, const float* carry, const uint8_t* done,
+                       const int32_t* lengths, void* out, float* final, float* states, void* workspace,
+                       size_t workspace_bytes, int batch, int steps, int features);
+/* From the cotangents of out (dout) and final (dfinal, NULL: zeros): dx,
+ * dinput_gate, ddecay_gate contiguous; drate float [features], dcarry float
+ * [batch, features] (either may be NULL). */
+size_t ppo_gated_scan_bwd_workspace(int dtype, int batch, int steps, int features);
+int ppo_gated_scan_bwd(void* stream, int dtype, const void* x, const void* input_gate, const void* decay_gate,
+                       const void* dout, const int64_t* strides, const float* rate, const uint8_t* done,
+                       const int32_t* lengths, const float* states, const float* dfinal, void* dx, void* dinput_gate,
+                       void* ddecay_gate, float* drate, float* dcarry, void* workspace, size_t workspace_bytes,
+                       int batch, int steps, int features);
+/* One step: x and the gates [batch, features] with an element stride of the
+ * batch each; done uint8 [batch] or NULL; final may be carry. */
+int ppo_gated_scan_step(void* stream, int dtype, const void* x, const void* input_gate, const void* decay_gate,
+                        const int64_t* strides, const float* rate, const float* carry, const uint8_t* done, void* out,
+                        float* final, int batch, int features);
+
 /* ------------------------------------------------------ linear attention
  * The scan's recurrence with a matrix for a state (no counterpart in the
  * reference): per sequence b and head h, lam = exp(log_decay[h]),
