@@ -38,6 +38,7 @@ enum GateDtype { GATE_F32 = 0, GATE_BF16 = 1 };
 
 constexpr int MAX_WAVES = 8;
 constexpr int FWD_STEPS = 8, BWD_STEPS = 4;   // of a lane's chunk
+constexpr int LANE = 2;                       // features of a lane
 constexpr float LOG2E = 1.4426950408889634f, LN2_2 = 1.3862943611198906f;
 constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
 constexpr int MAX_SEGMENTS = 64;
@@ -287,48 +288,48 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
   const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
   float h[VW], decay[VW], rl[VW];
 #pragma unroll
-  for (int k = 0; k < VW; ++k) rl[k] = p.rate[at.f0 + k] * LOG2E;
-  if constexpr (MAPS) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k) {
-      h[k] = 0.f;
-      decay[k] = 1.f;
-    }
-  } else {
+  for (int k = 0; k < VW; ++k) {
+    rl[k] = p.rate[at.f0 + k] * LOG2E;
+    h[k] = 0.f;
+    decay[k] = 1.f;
+  }
+  Raw<S, VW> x[N], ig[N], dg[N];   // of the next tile
+  uint64_t flags = 0;
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+    const bool whole = t0 + at.tile <= live_end;
+    fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x);
+    fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig);
+    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg);
+    if (done) flags = load_flags<N>(done, at.chunk_step(t0), p.steps);
+  };
+  if (begin < live_end) fetch(begin);
+  if constexpr (!MAPS) {
     load_state<VW>(p.carry, (int64_t)at.b * p.F + at.f0, h);
     through_segments<VW, false>(p, at.b, at.f0, segment, h);
   }
-  Raw<S, VW> x[2][N], ig[2][N], dg[2][N];
-  uint64_t flags[2] = {0, 0};
-  auto fetch = [&](int set, int t0) {
-    const bool whole = t0 + at.tile <= live_end;
-    fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x[set]);
-    fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig[set]);
-    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg[set]);
-    if (done) flags[set] = load_flags<N>(done, at.chunk_step(t0), p.steps);
-  };
-  auto step_tile = [&](int set, int t0) {
+  int set = 0, t0 = begin;
+  for (; t0 < live_end; t0 += at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
     const int t = at.chunk_step(t0);
-    const bool resets = __any(flags[set] != 0);
+    const bool resets = __any(flags != 0);
     float a[N][VW], b[N][VW], A[VW], B[VW], mine[VW];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates g = gates_of(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        a[i][k] = g.a;
+        b[i][k] = g.w * g.i * widen(x[i].v[k]);
+      }
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
       A[k] = 1.f;
       B[k] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const Gates g = gates_of(widen(ig[set][i].v[k]), widen(dg[set][i].v[k]), rl[k]);
-        a[i][k] = g.a;
-        b[i][k] = g.w * g.i * widen(x[set][i].v[k]);
-      }
     if (resets || !whole) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bool live = t + i < live_end, cut = flag(flags[set], i);
+        const bool live = t + i < live_end, cut = flag(flags, i);
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
           a[i][k] = live ? (cut ? -0.f : a[i][k]) : 1.f;
@@ -346,8 +347,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
           A[k] *= a[i][k];
         }
     }
-    const int next = t0 + at.tile;
-    if (next < live_end) fetch(set ^ 1, next);
+    if (t0 + at.tile < live_end) fetch(t0 + at.tile);
     float *pa = wave_a[set], *pb = wave_b[set];
     compose_slots<VW, LF, false>(A, B, at.lane, pa + at.wave * LF * VW, pb + at.wave * LF * VW);
     lds_barrier();
@@ -366,27 +366,26 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
 #pragma unroll
         for (int k = 0; k < VW; ++k) s[k] = mine[k];
       }
+      if (resets || !whole) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float o[VW];
+        for (int i = 0; i < N; ++i) {
+          float o[VW];
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          mine[k] = resets ? apply(a[i][k], b[i][k], mine[k]) : __fmaf_rn(a[i][k], mine[k], b[i][k]);
-          o[k] = whole || t + i < live_end ? mine[k] : 0.f;
+          for (int k = 0; k < VW; ++k) {
+            mine[k] = apply(a[i][k], b[i][k], mine[k]);
+            o[k] = t + i < live_end ? mine[k] : 0.f;
+          }
+          store_step<S, VW, N>(p.out, p, at, t0, i, end, whole, o);
         }
-        store_step<S, VW, N>(p.out, p, at, t0, i, end, whole, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+          for (int k = 0; k < VW; ++k) mine[k] = __fmaf_rn(a[i][k], mine[k], b[i][k]);
+          store_step<S, VW, N>(p.out, p, at, t0, i, end, true, mine);
+        }
       }
     }
-  };
-  // (the register sets alternate by unrolling, so that each is indexed by a constant)
-  if (begin < live_end) fetch(0, begin);
-  int t0 = begin;
-  while (t0 < live_end) {
-    step_tile(0, t0);
-    t0 += at.tile;
-    if (t0 >= live_end) break;
-    step_tile(1, t0);
-    t0 += at.tile;
   }
   if constexpr (MAPS) {
     if (at.wave == 0 && at.slot == 0) {
@@ -407,6 +406,13 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
   }
 }
 
+// What the backward keeps of an element while the maps are composed.
+struct Kept {
+  float a, b, g;        // decay (-0 at a reset, 1 past the end), input, cotangent
+  float wi, rest, c;    // w i; 1 - i; a^2 i x / w
+  float r, not_r;       // 1 - r
+};
+
 template <typename S, int VW, int LF, bool MAPS>
 __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) {
   constexpr int N = BWD_STEPS;
@@ -426,71 +432,86 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
     decay[k] = 1.f;
     E[k] = 0.f;
   }
+  Raw<S, VW> x[N], ig[N], dg[N], go[N];   // of the tile before
+  float entering[VW];
+  uint64_t flags = 0;
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+    const bool whole = t0 + at.tile <= live_end;
+    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg);
+    fetch_steps<S, VW, N>(p.dout, p.dout_s, at, t0, live_end, whole, go);
+    if constexpr (!MAPS) {
+      fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x);
+      fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig);
+      load_state<VW>(p.states, ((int64_t)at.b * p.saved + (t0 >> p.save_log2)) * p.F + at.f0, entering);
+    }
+    if (done) flags = load_flags<N>(done, at.chunk_step(t0), p.steps);
+  };
+  const int tiles = live_end > begin ? (live_end - begin + at.tile - 1) / at.tile : 0;
+  int set = 0, t0 = begin + (tiles - 1) * at.tile;
+  if (tiles > 0) fetch(t0);
   if constexpr (!MAPS) {
     load_state<VW>(p.dfinal, state, E);
     through_segments<VW, true>(p, at.b, at.f0, segment, E);
   }
-  Raw<S, VW> x[2][N], ig[2][N], dg[2][N], go[2][N];
-  float entering[2][VW];
-  uint64_t flags[2] = {0, 0};
-  auto fetch = [&](int set, int t0) {
-    const bool whole = t0 + at.tile <= live_end;
-    fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg[set]);
-    fetch_steps<S, VW, N>(p.dout, p.dout_s, at, t0, live_end, whole, go[set]);
-    if constexpr (!MAPS) {
-      fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x[set]);
-      fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig[set]);
-      load_state<VW>(p.states, ((int64_t)at.b * p.saved + (t0 >> p.save_log2)) * p.F + at.f0, entering[set]);
-    }
-    if (done) flags[set] = load_flags<N>(done, at.chunk_step(t0), p.steps);
-  };
-  auto step_tile = [&](int set, int t0) {
+  for (; t0 >= begin; t0 -= at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
     const int t = at.chunk_step(t0);
-    const bool resets = __any(flags[set] != 0);
-    Gates g[N][VW];
-    float a[N][VW], go_[N][VW], b[N][VW];   // a: with resets, and 1 past the end
-    float A[VW], B[VW], RA[VW], RB[VW];
+    const bool resets = __any(flags != 0);
+    Kept q[N][VW];
+    float h[VW], A[VW], B[VW], RA[VW], RB[VW];
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
-        g[i][k] = gates_of(MAPS ? 0.f : widen(ig[set][i].v[k]), widen(dg[set][i].v[k]), rl[k]);
-        a[i][k] = g[i][k].a;
-        go_[i][k] = widen(go[set][i].v[k]);
-        b[i][k] = MAPS ? 0.f : g[i][k].w * g[i][k].i * widen(x[set][i].v[k]);
+        Kept& e = q[i][k];
+        const Gates g = gates_of(MAPS ? 0.f : widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const float xv = MAPS ? 0.f : widen(x[i].v[k]);
+        e.a = g.a;
+        e.g = widen(go[i].v[k]);
+        e.wi = g.w * g.i;
+        e.b = e.wi * xv;
+        e.rest = g.not_i;
+        e.c = g.a * g.over_w * g.a * (g.i * xv);
+        e.r = g.r;
+        e.not_r = g.not_r;
       }
-    if (resets || !whole) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool live = t + i < live_end, cut = flag(flags[set], i);
-#pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          a[i][k] = live ? (cut ? -0.f : a[i][k]) : 1.f;
-          b[i][k] = live ? b[i][k] : 0.f;
-          go_[i][k] = live ? go_[i][k] : 0.f;
-        }
-      }
-    }
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
       A[k] = 1.f;
       B[k] = RB[k] = 0.f;
+      if constexpr (!MAPS) h[k] = entering[k];
     }
+    if (resets || !whole) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+      for (int i = 0; i < N; ++i) {
+        const bool live = t + i < live_end, cut = flag(flags, i);
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        B[k] = apply(a[i][k], b[i][k], B[k]);
-        A[k] = decay_of(a[i][k], A[k]);
-        // E through step N - 1 - i: a (g + E)
-        const float aa = a[N - 1 - i][k], sum = go_[N - 1 - i][k] + RB[k];
-        RB[k] = is_reset(aa) ? 0.f : aa * sum;
+        for (int k = 0; k < VW; ++k) {
+          Kept& e = q[i][k];
+          e.a = live ? (cut ? -0.f : e.a) : 1.f;
+          e.b = live ? e.b : 0.f;
+          e.g = live ? e.g : 0.f;
+          B[k] = apply(e.a, e.b, B[k]);
+          A[k] = decay_of(e.a, A[k]);
+        }
       }
 #pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) RB[k] = is_reset(q[i][k].a) ? 0.f : q[i][k].a * (q[i][k].g + RB[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          B[k] = __fmaf_rn(q[i][k].a, B[k], q[i][k].b);
+          A[k] *= q[i][k].a;
+          RB[k] = q[N - 1 - i][k].a * (q[N - 1 - i][k].g + RB[k]);
+        }
+    }
+#pragma unroll
     for (int k = 0; k < VW; ++k) RA[k] = A[k];
-    const int next = t0 - at.tile;
-    if (next >= begin) fetch(set ^ 1, next);
+    if (t0 > begin) fetch(t0 - at.tile);
     const int mine_at = at.wave * LF * VW;
     if constexpr (!MAPS) compose_slots<VW, LF, false>(A, B, at.lane, fwd_a[set] + mine_at, fwd_b[set] + mine_at);
     compose_slots<VW, LF, true>(RA, RB, at.lane, rev_a[set] + mine_at, rev_b[set] + mine_at);
@@ -503,50 +524,52 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
           E[k] = apply(rev_a[set][j], rev_b[set][j], E[k]);
           decay[k] = decay_of(rev_a[set][j], decay[k]);
         }
-      return;
-    }
-    float h[VW], mine[VW], after[VW], before[N][VW];
+    } else {
+      float mine[VW], after[VW], before[N][VW];
+      through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
+      through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
+      if (resets) {
 #pragma unroll
-    for (int k = 0; k < VW; ++k) h[k] = entering[set][k];
-    through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
-    through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+          for (int k = 0; k < VW; ++k) {
+            before[i][k] = is_reset(q[i][k].a) ? 0.f : mine[k];
+            mine[k] = apply(q[i][k].a, q[i][k].b, mine[k]);
+          }
+      } else {
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        before[i][k] = is_reset(a[i][k]) ? 0.f : mine[k];
-        mine[k] = apply(a[i][k], b[i][k], mine[k]);
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int k = 0; k < VW; ++k) {
+            before[i][k] = mine[k];
+            mine[k] = __fmaf_rn(q[i][k].a, mine[k], q[i][k].b);
+          }
       }
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) {
-      const bool live = whole || t + i < live_end;
-      float ox[VW], oi[VW], od[VW];
+      for (int i = N - 1; i >= 0; --i) {
+        const bool live = whole || t + i < live_end;
+        float ox[VW], oi[VW], od[VW];
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const Gates& q = g[i][k];
-        const float D = go_[i][k] + after[k], xv = widen(x[set][i].v[k]);
-        after[k] = is_reset(a[i][k]) ? 0.f : a[i][k] * D;
-        const float dw = D * q.w * q.i;
-        ox[k] = live ? dw : 0.f;
-        oi[k] = live ? dw * xv * q.not_i : 0.f;
-        const float dr = D * (q.a * __fmaf_rn(-q.a * q.over_w, q.i * xv, before[i][k])) * q.r;   // dL r
-        od[k] = live ? -dr * rl[k] * (1.f / LOG2E) * q.not_r : 0.f;
-        drate[k] -= live ? dr : 0.f;
+        for (int k = 0; k < VW; ++k) {
+          const Kept& e = q[i][k];
+          const float D = e.g + after[k];
+          after[k] = resets && is_reset(e.a) ? 0.f : e.a * D;
+          ox[k] = D * e.wi;
+          oi[k] = D * e.b * e.rest;
+          const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
+          od[k] = -dr * rl[k] * (1.f / LOG2E) * e.not_r;
+          if (!whole) {
+            ox[k] = live ? ox[k] : 0.f;
+            oi[k] = live ? oi[k] : 0.f;
+            od[k] = live ? od[k] : 0.f;
+          }
+          drate[k] -= live ? dr : 0.f;
+        }
+        store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
+        store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
+        store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
       }
-      store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
-      store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
-      store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
     }
-  };
-  const int tiles = live_end > begin ? (live_end - begin + at.tile - 1) / at.tile : 0;
-  int t0 = begin + (tiles - 1) * at.tile;
-  if (tiles > 0) fetch(0, t0);
-  while (t0 >= begin) {
-    step_tile(0, t0);
-    t0 -= at.tile;
-    if (t0 < begin) break;
-    step_tile(1, t0);
-    t0 -= at.tile;
   }
   if constexpr (MAPS) {
     if (at.wave == 0 && at.slot == 0) {
@@ -567,9 +590,8 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
       for (int k = 0; k < VW; ++k) p.dcarry[state + k] = E[k];
     }
     if (p.partials) {
-      // the slots' sums, added in their order
+      // the slots' sums, the lanes' by butterflies, the waves' in their order
       float* sums = &fwd_a[0][0];
-      static_assert(sizeof(fwd_a) >= sizeof(float) * MAX_WAVES * LF * VW, "a wave's sums each");
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
         for (int o = LF; o < 64; o <<= 1) drate[k] += __shfl_xor(drate[k], o);
@@ -671,12 +693,15 @@ constexpr int TARGET = 512;   // workgroups that fill the chip
 Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
   Plan s;
   const int N = backward ? BWD_STEPS : FWD_STEPS;
-  s.vw = backward ? 2 : 4;
+  s.vw = LANE;
   if (F < s.vw) s.vw = 1;
-  s.lf = s.vw == 1 ? 8 : 64;
-  while (s.lf > 8 && (s.lf / 2 * s.vw >= F || (int64_t)batch * ceil_div(F, s.lf * s.vw) < TARGET) &&
+  // lanes for the features that are there, of whole cache lines where sequences are few
+  s.lf = 64;
+  const int line = 128 / (s.vw * (dtype == GATE_F32 ? 4 : 2));
+  while (s.lf > 8 && (s.lf / 2 * s.vw >= F || (s.lf > line && (int64_t)batch * ceil_div(F, s.lf * s.vw) < TARGET)) &&
          128 / s.lf * N < 2 * (int64_t)steps)
     s.lf /= 2;
+  if (s.vw == 1) s.lf = 8;
   const int slots = 64 / s.lf;
   s.waves = std::min(MAX_WAVES, ceil_div(steps, slots * N));
   s.blocks = ceil_div(F, s.lf * s.vw);
@@ -731,7 +756,7 @@ void launch_shape(hipStream_t st, const GatedArgs& a, const Plan& s, int batch) 
   }
 }
 template <typename S, bool BWD> void launch(hipStream_t st, GatedArgs a, const Plan& s, int batch) {
-  constexpr int VW = BWD ? 2 : 4;
+  constexpr int VW = LANE;
   a.blocks = s.blocks;
   a.segment = s.segment;
   a.segments = s.segments;
