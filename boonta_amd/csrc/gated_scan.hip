@@ -29,6 +29,7 @@
 #include "row_io.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -39,7 +40,7 @@ enum GateDtype { GATE_F32 = 0, GATE_BF16 = 1 };
 constexpr int MAX_WAVES = 8;
 constexpr int FWD_STEPS = 8, BWD_STEPS = 4;   // of a lane's chunk
 constexpr int LANE = 2;                       // features of a lane
-constexpr float LOG2E = 1.4426950408889634f, LN2_2 = 1.3862943611198906f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
 constexpr int MAX_SEGMENTS = 64;
 
@@ -71,26 +72,32 @@ __device__ __forceinline__ float apply(float a, float b, float h) { return is_re
 __device__ __forceinline__ float decay_of(float later, float earlier) { return is_reset(later) ? later : later * earlier; }
 
 struct Gates {
-  float i, r, a, w, over_w;   // over_w: 1 / w, or 0
-  float not_i, not_r;         // 1 - i, 1 - r
+  float a, wi;                // decay; w i
+  float i, r, not_i, not_r;   // not_: 1 - it
+  float over_w;               // 1 / w, or 0
 };
-// rl = rate log2(e)
-__device__ __forceinline__ Gates gates_of(float input, float decay, float rl) {
+// 1 - a^2 of a = 2^-q.  Below 2 ln(2) q = 1/8 the Chebyshev interpolation of degree 3 of
+// (1 - 2^-2q) / q, within 2^-25 of it; above, what the difference loses is at most 8 times a^2's rounding.
+__device__ __forceinline__ float one_minus_square(float a, float q) {
+  float s = __fmaf_rn(q, -0.1464114f, 0.44361513f);
+  s = __fmaf_rn(q, s, -0.96089852f);
+  s = __fmaf_rn(q, s, 1.38629434f);
+  return q < 0.0901684f ? q * s : __fmaf_rn(-a, a, 1.f);
+}
+// rl = rate log2(e).  BWD: what the gradients need too.
+template <bool BWD> __device__ __forceinline__ Gates gates_of(float input, float decay, float rl) {
   Gates g;
   g.i = sigmoid(input, g.not_i);
   g.r = sigmoid(decay, g.not_r);
   const float q = rl * g.r;
   g.a = __builtin_amdgcn_exp2f(-q);
-  // 1 - a^2 = 1 - e^-z = z - z^2 / 2 + ...: below z = 1/4 the terms left out are under 5e-8 of it
-  const float z = LN2_2 * q;
-  float s = __fmaf_rn(z, -1.f / 720.f, 1.f / 120.f);
-  s = __fmaf_rn(z, s, -1.f / 24.f);
-  s = __fmaf_rn(z, s, 1.f / 6.f);
-  s = __fmaf_rn(z, s, -0.5f);
-  s = __fmaf_rn(z, s, 1.f);
-  const float w2 = z < 0.25f ? z * s : __fmaf_rn(-g.a, g.a, 1.f);
-  g.over_w = w2 > 0.f ? __builtin_amdgcn_rsqf(w2) : w2 * 0.f;   // (NaN of NaN)
-  g.w = w2 * g.over_w;
+  const float w2 = one_minus_square(g.a, q);
+  if constexpr (BWD) {
+    g.over_w = w2 > 0.f ? __builtin_amdgcn_rsqf(w2) : 0.f;
+    g.wi = w2 * g.over_w * g.i;
+  } else {
+    g.wi = __builtin_amdgcn_sqrtf(w2) * g.i;
+  }
   return g;
 }
 
@@ -317,9 +324,9 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
-        const Gates g = gates_of(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const Gates g = gates_of<false>(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
         a[i][k] = g.a;
-        b[i][k] = g.w * g.i * widen(x[i].v[k]);
+        b[i][k] = g.wi * widen(x[i].v[k]);
       }
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
@@ -409,8 +416,8 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
 // What the backward keeps of an element while the maps are composed.
 struct Kept {
   float a, b, g;        // decay (-0 at a reset, 1 past the end), input, cotangent
-  float wi, rest, c;    // w i; 1 - i; a^2 i x / w
-  float r, not_r;       // 1 - r
+  float wi, not_i, c;   // w i; 1 - i; a^2 i x / w
+  float r, not_r;       // and 1 - r
 };
 
 template <typename S, int VW, int LF, bool MAPS>
@@ -424,10 +431,11 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
   const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
   const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
   const int64_t state = (int64_t)at.b * p.F + at.f0;
-  float E[VW], decay[VW], rl[VW], drate[VW];
+  float E[VW], decay[VW], rate[VW], rl[VW], drate[VW];
 #pragma unroll
   for (int k = 0; k < VW; ++k) {
-    rl[k] = p.rate[at.f0 + k] * LOG2E;
+    rate[k] = p.rate[at.f0 + k];
+    rl[k] = rate[k] * LOG2E;
     drate[k] = 0.f;
     decay[k] = 1.f;
     E[k] = 0.f;
@@ -464,13 +472,13 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
         Kept& e = q[i][k];
-        const Gates g = gates_of(MAPS ? 0.f : widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const Gates g = gates_of<true>(MAPS ? 0.f : widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
         const float xv = MAPS ? 0.f : widen(x[i].v[k]);
         e.a = g.a;
         e.g = widen(go[i].v[k]);
-        e.wi = g.w * g.i;
-        e.b = e.wi * xv;
-        e.rest = g.not_i;
+        e.wi = g.wi;
+        e.b = g.wi * xv;
+        e.not_i = g.not_i;
         e.c = g.a * g.over_w * g.a * (g.i * xv);
         e.r = g.r;
         e.not_r = g.not_r;
@@ -545,30 +553,30 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
             mine[k] = __fmaf_rn(q[i][k].a, mine[k], q[i][k].b);
           }
       }
+      auto gradients = [&](auto plain) __attribute__((always_inline)) {   // no resets, a whole tile
+        constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
-      for (int i = N - 1; i >= 0; --i) {
-        const bool live = whole || t + i < live_end;
-        float ox[VW], oi[VW], od[VW];
+        for (int i = N - 1; i >= 0; --i) {
+          const bool live = PLAIN || t + i < live_end;
+          float ox[VW], oi[VW], od[VW];
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          const Kept& e = q[i][k];
-          const float D = e.g + after[k];
-          after[k] = resets && is_reset(e.a) ? 0.f : e.a * D;
-          ox[k] = D * e.wi;
-          oi[k] = D * e.b * e.rest;
-          const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
-          od[k] = -dr * rl[k] * (1.f / LOG2E) * e.not_r;
-          if (!whole) {
-            ox[k] = live ? ox[k] : 0.f;
-            oi[k] = live ? oi[k] : 0.f;
-            od[k] = live ? od[k] : 0.f;
+          for (int k = 0; k < VW; ++k) {
+            const Kept& e = q[i][k];
+            const float D = e.g + after[k];
+            after[k] = !PLAIN && is_reset(e.a) ? 0.f : e.a * D;
+            const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
+            ox[k] = live ? D * e.wi : 0.f;
+            oi[k] = live ? D * e.b * e.not_i : 0.f;
+            od[k] = live ? -dr * rate[k] * e.not_r : 0.f;
+            drate[k] -= live ? dr : 0.f;
           }
-          drate[k] -= live ? dr : 0.f;
+          store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
+          store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
+          store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
         }
-        store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
-        store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
-        store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
-      }
+      };
+      if (resets || !whole) gradients(std::false_type{});
+      else gradients(std::true_type{});
     }
   }
   if constexpr (MAPS) {
@@ -658,8 +666,8 @@ __global__ void __launch_bounds__(256) gated_step_kernel(GatedArgs p, int64_t th
   S* out = static_cast<S*>(p.out) + b * p.F + f0;
   const bool cut = p.done && p.done[b];
   auto step = [&](float xv, float i_, float d, float rate, float h) {
-    const Gates g = gates_of(i_, d, rate * LOG2E);
-    return apply(cut ? -0.f : g.a, g.w * g.i * xv, h);
+    const Gates g = gates_of<false>(i_, d, rate * LOG2E);
+    return apply(cut ? -0.f : g.a, g.wi * xv, h);
   };
   if (left >= VW) {
     Raw<S, VW> rx, ri, rd;
@@ -688,19 +696,23 @@ __global__ void __launch_bounds__(256) gated_step_kernel(GatedArgs p, int64_t th
 struct Plan {
   int vw, lf, waves, blocks, tile, segment, segments;
 };
-constexpr int TARGET = 512;   // workgroups that fill the chip
+constexpr int TARGET = 512, FILL = 192;   // workgroups that fill the chip, and most of it
 
 Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
   Plan s;
   const int N = backward ? BWD_STEPS : FWD_STEPS;
   s.vw = LANE;
   if (F < s.vw) s.vw = 1;
-  // lanes for the features that are there, of whole cache lines where sequences are few
+  // lanes for the features that are there; where those and the sequences do not
+  // fill the chip, fewer side by side, down to a cache line, if that fills most of it
+  // (a segment more reads operands twice)
   s.lf = 64;
-  const int line = 128 / (s.vw * (dtype == GATE_F32 ? 4 : 2));
-  while (s.lf > 8 && (s.lf / 2 * s.vw >= F || (s.lf > line && (int64_t)batch * ceil_div(F, s.lf * s.vw) < TARGET)) &&
-         128 / s.lf * N < 2 * (int64_t)steps)
-    s.lf /= 2;
+  const auto groups_at = [&](int lf) { return (int64_t)batch * ceil_div(F, lf * s.vw); };
+  const auto fits = [&](int lf) { return 64 / lf * N < 2 * (int64_t)steps; };
+  while (s.lf > 8 && s.lf / 2 * s.vw >= F && fits(s.lf / 2)) s.lf /= 2;
+  const int line = std::min(s.lf, 128 / (s.vw * (dtype == GATE_F32 ? 4 : 2)));
+  if (groups_at(line) >= FILL)
+    while (s.lf > line && groups_at(s.lf) < TARGET && fits(s.lf / 2)) s.lf /= 2;
   if (s.vw == 1) s.lf = 8;
   const int slots = 64 / s.lf;
   s.waves = std::min(MAX_WAVES, ceil_div(steps, slots * N));
@@ -709,7 +721,7 @@ Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
   // segments of at least two tiles, as many as fill the chip
   const int64_t groups = (int64_t)batch * s.blocks;
   const int64_t most = std::min<int64_t>(MAX_SEGMENTS, std::max(1, steps / (2 * s.tile)));
-  s.segments = (int)std::max<int64_t>(1, std::min<int64_t>(most, TARGET / std::max<int64_t>(groups, 1)));
+  s.segments = groups >= FILL ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(most, TARGET / groups));
   const int tiles = ceil_div(steps, s.tile);
   const int each = ceil_div(tiles, s.segments);
   s.segment = each * s.tile;
