@@ -171,6 +171,11 @@ template <int VW, int LF, int N> struct Lane {
   __device__ __forceinline__ int chunk_step(int t0) const { return wave_step(t0) + slot * N; }
 };
 
+// In a branch that is seldom taken: at its head, its instructions are not formed
+// beside the other's and selected from (which took a fifth of the loop's); at
+// its end, its loads stay its own (joined with the other's they take 64-bit addresses).
+__device__ __forceinline__ void apart() { asm volatile(""); }
+
 // A tensor's N steps of a lane's chunk: row offsets within 32 bits of the
 // wave's first where the tile is whole, clamped rows of it otherwise.
 template <typename S, int VW, int N, typename L>
@@ -186,6 +191,7 @@ __device__ __forceinline__ void fetch_steps(const void* x, const RowStride& s, c
 #pragma unroll
     for (int i = 0; i < N; ++i)
       v[i] = load_raw<S, VW>(base, (min(at.chunk_step(t0) + i, end - 1) * s.step + at.f0) * (int64_t)sizeof(S));
+    apart();
   }
 }
 // and of an output [batch, steps, F]: steps below `end`.
@@ -334,6 +340,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
       B[k] = 0.f;
     }
     if (resets || !whole) {
+      apart();
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const bool live = t + i < live_end, cut = flag(flags, i);
@@ -374,6 +381,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
         for (int k = 0; k < VW; ++k) s[k] = mine[k];
       }
       if (resets || !whole) {
+      apart();
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           float o[VW];
@@ -490,6 +498,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
       if constexpr (!MAPS) h[k] = entering[k];
     }
     if (resets || !whole) {
+      apart();
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const bool live = t + i < live_end, cut = flag(flags, i);
@@ -537,6 +546,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
       through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
       through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
       if (resets) {
+        apart();
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -555,6 +565,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
       }
       auto gradients = [&](auto plain) __attribute__((always_inline)) {   // no resets, a whole tile
         constexpr bool PLAIN = decltype(plain)::value;
+        if constexpr (!PLAIN) apart();
 #pragma unroll
         for (int i = N - 1; i >= 0; --i) {
           const bool live = PLAIN || t + i < live_end;
