@@ -38,7 +38,7 @@ using namespace ppo;
 enum GateDtype { GATE_F32 = 0, GATE_BF16 = 1 };
 
 constexpr int MAX_WAVES = 8;
-constexpr int FWD_STEPS = 8, BWD_STEPS = 4;   // of a lane's chunk
+constexpr int FWD_STEPS = 8, BWD_STEPS = 4, MAP_STEPS = 4;   // of a lane's chunk
 constexpr int LANE = 2;                       // features of a lane
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
@@ -264,16 +264,38 @@ template <int VW, int LF, bool REVERSE>
 __device__ __forceinline__ void through_waves(float (&h)[VW], float (&mine)[VW], const float (&A)[VW],
                                               const float (&B)[VW], const float* wave_a, const float* wave_b, int lane,
                                               int wave, int waves) {
-  for (int i = 0; i < waves; ++i) {
-    const int w = REVERSE ? waves - 1 - i : i;
-    if (w == wave) {
-#pragma unroll
-      for (int k = 0; k < VW; ++k) mine[k] = h[k];
-    }
+  const auto step = [&](int w, const float (&a)[VW], const float (&b)[VW]) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
-      const int at = (w * LF + lane % LF) * VW + k;
-      h[k] = apply(wave_a[at], wave_b[at], h[k]);
+      mine[k] = w == wave ? h[k] : mine[k];
+      h[k] = apply(a[k], b[k], h[k]);
+    }
+  };
+  const auto read = [&](int w, float (&a)[VW], float (&b)[VW]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      a[k] = wave_a[(w * LF + lane % LF) * VW + k];
+      b[k] = wave_b[(w * LF + lane % LF) * VW + k];
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < VW; ++k) mine[k] = h[k];
+  if (waves == MAX_WAVES) {   // (half of the reads on their way at once)
+    constexpr int H = MAX_WAVES / 2;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float a[H][VW], b[H][VW];
+#pragma unroll
+      for (int i = 0; i < H; ++i) read(REVERSE ? MAX_WAVES - 1 - half * H - i : half * H + i, a[i], b[i]);
+#pragma unroll
+      for (int i = 0; i < H; ++i) step(REVERSE ? MAX_WAVES - 1 - half * H - i : half * H + i, a[i], b[i]);
+    }
+  } else {
+    for (int i = 0; i < waves; ++i) {
+      const int w = REVERSE ? waves - 1 - i : i;
+      float a[VW], b[VW];
+      read(w, a, b);
+      step(w, a, b);
     }
   }
 #pragma unroll
@@ -284,14 +306,142 @@ __device__ __forceinline__ void through_waves(float (&h)[VW], float (&mine)[VW],
 template <int VW, bool REVERSE>
 __device__ __forceinline__ void through_segments(const GatedArgs& p, int64_t b, int f0, int segment, float (&h)[VW]) {
   const int n = REVERSE ? p.segments - 1 - segment : segment;
-  for (int i = 0; i < n; ++i) {
-    const int64_t at = ((b * p.segments + (REVERSE ? p.segments - 1 - i : i)) * 2) * p.F + f0;
+  constexpr int U = 4;   // maps on their way at once
+  for (int i0 = 0; i0 < n; i0 += U) {
+    float a[U][VW], s[U][VW];
 #pragma unroll
-    for (int k = 0; k < VW; ++k) h[k] = apply(p.maps[at + k], p.maps[at + p.F + k], h[k]);
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u, n - 1);
+      const float* m = p.maps + ((b * p.segments + (REVERSE ? p.segments - 1 - i : i)) * 2) * p.F + f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        a[u][k] = m[k];
+        s[u][k] = m[p.F + k];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) h[k] = i0 + u < n ? apply(a[u][k], s[u][k], h[k]) : h[k];
   }
 }
 
-template <typename S, int VW, int LF, bool MAPS>
+// The map of a segment: of the state h (REVERSE: of the cotangent E).  Every
+// slot takes a part of the segment's steps from one end to the other, and the
+// parts are composed at the end.
+template <typename S, int VW, int LF, bool REVERSE>
+__global__ void __launch_bounds__(64 * MAX_WAVES) gated_maps_kernel(GatedArgs p) {
+  constexpr int N = MAP_STEPS;
+  __shared__ float wave_a[MAX_WAVES * LF * VW], wave_b[MAX_WAVES * LF * VW];
+  const Lane<VW, LF, N> at(p);
+  const int segment = blockIdx.y + (REVERSE ? 1 : 0), begin = segment * p.segment;   // (the first, or last, needs none)
+  const int end = min(p.steps, begin + p.segment);
+  const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
+  const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
+  const int part = p.segment / (at.waves * at.SLOTS);   // steps of a slot, a multiple of N
+  const int wave_first = begin + at.wave * at.SLOTS * part, first = wave_first + at.slot * part;
+  const int wave_last = wave_first + (at.SLOTS - 1) * part;
+  float A[VW], B[VW], rl[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    rl[k] = p.rate[at.f0 + k] * LOG2E;
+    A[k] = 1.f;
+    B[k] = 0.f;
+  }
+  Raw<S, VW> x[N], ig[N], dg[N];   // of the next chunk (REVERSE: x the cotangent, no ig)
+  uint64_t flags = 0;
+  auto load = [&](const void* from, const RowStride& s, int c, Raw<S, VW>(&v)[N]) __attribute__((always_inline)) {
+    const char* base = static_cast<const char*>(from) + (int64_t)at.b * s.batch * (int64_t)sizeof(S);
+    const int t = first + c;
+    if (wave_last + c + N <= live_end) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if constexpr (at.SLOTS == 1)
+          v[i] = load_near<S, VW>(base + (wave_first + c + i) * s.step * (int64_t)sizeof(S), (uint32_t)at.f0 * (uint32_t)sizeof(S));
+        else
+          v[i] = load_raw<S, VW>(base, ((t + i) * s.step + at.f0) * (int64_t)sizeof(S));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = load_raw<S, VW>(base, (min(t + i, live_end - 1) * s.step + at.f0) * (int64_t)sizeof(S));
+      apart();
+    }
+  };
+  auto fetch = [&](int c) __attribute__((always_inline)) {
+    load(p.decay_gate, p.decay_s, c, dg);
+    load(REVERSE ? p.dout : p.x, REVERSE ? p.dout_s : p.x_s, c, x);
+    if constexpr (!REVERSE) load(p.input_gate, p.input_s, c, ig);
+    if (done) flags = load_flags<N>(done, first + c, p.steps);
+  };
+  // chunks of the wave's first slot that has the most live steps
+  const int chunks = (max(0, min(part, live_end - wave_first)) + N - 1) / N;
+  if (chunks > 0) fetch(REVERSE ? (chunks - 1) * N : 0);
+  for (int j = 0; j < chunks; ++j) {
+    const int c = (REVERSE ? chunks - 1 - j : j) * N;
+    float a[N][VW], b[N][VW];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates g = gates_of<false>(REVERSE ? 0.f : widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        a[i][k] = g.a;
+        b[i][k] = REVERSE ? widen(x[i].v[k]) : g.wi * widen(x[i].v[k]);
+      }
+    const uint64_t cuts = flags;
+    if (j + 1 < chunks) fetch(REVERSE ? c - N : c + N);
+    if (__any(cuts != 0) || wave_last + c + N > live_end) {
+      apart();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = REVERSE ? N - 1 - i : i;
+        const bool live = first + c + e < live_end, cut = flag(cuts, e);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const float ae = live ? (cut ? -0.f : a[e][k]) : 1.f, be = live ? b[e][k] : 0.f;
+          B[k] = REVERSE ? (is_reset(ae) ? 0.f : ae * (be + B[k])) : apply(ae, be, B[k]);
+          A[k] = decay_of(ae, A[k]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = REVERSE ? N - 1 - i : i;
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          B[k] = REVERSE ? a[e][k] * (b[e][k] + B[k]) : __fmaf_rn(a[e][k], B[k], b[e][k]);
+          A[k] *= a[e][k];
+        }
+      }
+    }
+  }
+  compose_slots<VW, LF, REVERSE>(A, B, at.lane, wave_a + at.wave * LF * VW, wave_b + at.wave * LF * VW);
+  __syncthreads();
+  if (at.wave > 0 || at.slot > 0) return;
+  float decay[VW], sum[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    decay[k] = 1.f;
+    sum[k] = 0.f;
+  }
+  for (int i = 0; i < at.waves; ++i) {
+    const int w = REVERSE ? at.waves - 1 - i : i;
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      const int j = (w * LF + at.lane) * VW + k;
+      sum[k] = apply(wave_a[j], wave_b[j], sum[k]);
+      decay[k] = decay_of(wave_a[j], decay[k]);
+    }
+  }
+  float* m = p.maps + (((int64_t)at.b * p.segments + segment) * 2) * p.F + at.f0;
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    m[k] = decay[k];
+    m[p.F + k] = sum[k];
+  }
+}
+
+template <typename S, int VW, int LF>
 __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) {
   constexpr int N = FWD_STEPS;
   __shared__ float wave_a[2][MAX_WAVES * LF * VW], wave_b[2][MAX_WAVES * LF * VW];
@@ -299,13 +449,9 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
   const int segment = blockIdx.y, begin = segment * p.segment, end = min(p.steps, begin + p.segment);
   const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
   const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
-  float h[VW], decay[VW], rl[VW];
+  float h[VW], rl[VW];
 #pragma unroll
-  for (int k = 0; k < VW; ++k) {
-    rl[k] = p.rate[at.f0 + k] * LOG2E;
-    h[k] = 0.f;
-    decay[k] = 1.f;
-  }
+  for (int k = 0; k < VW; ++k) rl[k] = p.rate[at.f0 + k] * LOG2E;
   Raw<S, VW> x[N], ig[N], dg[N];   // of the next tile
   uint64_t flags = 0;
   auto fetch = [&](int t0) __attribute__((always_inline)) {
@@ -316,10 +462,8 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
     if (done) flags = load_flags<N>(done, at.chunk_step(t0), p.steps);
   };
   if (begin < live_end) fetch(begin);
-  if constexpr (!MAPS) {
-    load_state<VW>(p.carry, (int64_t)at.b * p.F + at.f0, h);
-    through_segments<VW, false>(p, at.b, at.f0, segment, h);
-  }
+  load_state<VW>(p.carry, (int64_t)at.b * p.F + at.f0, h);
+  through_segments<VW, false>(p, at.b, at.f0, segment, h);
   int set = 0, t0 = begin;
   for (; t0 < live_end; t0 += at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
@@ -365,59 +509,38 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
     float *pa = wave_a[set], *pb = wave_b[set];
     compose_slots<VW, LF, false>(A, B, at.lane, pa + at.wave * LF * VW, pb + at.wave * LF * VW);
     lds_barrier();
-    if constexpr (MAPS) {
-      for (int w = 0; w < at.waves; ++w)
+    through_waves<VW, LF, false>(h, mine, A, B, pa, pb, at.lane, at.wave, at.waves);
+    if (p.states && t < live_end && (t & ((1 << p.save_log2) - 1)) == 0) {
+      float* s = p.states + ((int64_t)at.b * p.saved + (t >> p.save_log2)) * p.F + at.f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) s[k] = mine[k];
+    }
+    if (resets || !whole) {
+    apart();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float o[VW];
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
-          const int j = (w * LF + at.lane % LF) * VW + k;
-          h[k] = apply(pa[j], pb[j], h[k]);
-          decay[k] = decay_of(pa[j], decay[k]);
+          mine[k] = apply(a[i][k], b[i][k], mine[k]);
+          o[k] = t + i < live_end ? mine[k] : 0.f;
         }
-    } else {
-      through_waves<VW, LF, false>(h, mine, A, B, pa, pb, at.lane, at.wave, at.waves);
-      if (p.states && t < live_end && (t & ((1 << p.save_log2) - 1)) == 0) {
-        float* s = p.states + ((int64_t)at.b * p.saved + (t >> p.save_log2)) * p.F + at.f0;
-#pragma unroll
-        for (int k = 0; k < VW; ++k) s[k] = mine[k];
+        store_step<S, VW, N>(p.out, p, at, t0, i, end, whole, o);
       }
-      if (resets || !whole) {
-      apart();
+    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          float o[VW];
+      for (int i = 0; i < N; ++i) {
 #pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            mine[k] = apply(a[i][k], b[i][k], mine[k]);
-            o[k] = t + i < live_end ? mine[k] : 0.f;
-          }
-          store_step<S, VW, N>(p.out, p, at, t0, i, end, whole, o);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-#pragma unroll
-          for (int k = 0; k < VW; ++k) mine[k] = __fmaf_rn(a[i][k], mine[k], b[i][k]);
-          store_step<S, VW, N>(p.out, p, at, t0, i, end, true, mine);
-        }
+        for (int k = 0; k < VW; ++k) mine[k] = __fmaf_rn(a[i][k], mine[k], b[i][k]);
+        store_step<S, VW, N>(p.out, p, at, t0, i, end, true, mine);
       }
     }
   }
-  if constexpr (MAPS) {
-    if (at.wave == 0 && at.slot == 0) {
-      float* m = p.maps + (((int64_t)at.b * p.segments + segment) * 2) * p.F + at.f0;
+  clear_steps<S>(p.out, p, at, t0, end);
+  if (segment == p.segments - 1 && at.wave == 0 && at.slot == 0) {
+    float* f = p.final + (int64_t)at.b * p.F + at.f0;
 #pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        m[k] = decay[k];
-        m[p.F + k] = h[k];
-      }
-    }
-  } else {
-    clear_steps<S>(p.out, p, at, t0, end);
-    if (segment == p.segments - 1 && at.wave == 0 && at.slot == 0) {
-      float* f = p.final + (int64_t)at.b * p.F + at.f0;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) f[k] = h[k];
-    }
+    for (int k = 0; k < VW; ++k) f[k] = h[k];
   }
 }
 
@@ -428,25 +551,22 @@ struct Kept {
   float r, not_r;       // and 1 - r
 };
 
-template <typename S, int VW, int LF, bool MAPS>
+template <typename S, int VW, int LF>
 __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) {
   constexpr int N = BWD_STEPS;
   __shared__ float fwd_a[2][MAX_WAVES * LF * VW], fwd_b[2][MAX_WAVES * LF * VW];
   __shared__ float rev_a[2][MAX_WAVES * LF * VW], rev_b[2][MAX_WAVES * LF * VW];
   const Lane<VW, LF, N> at(p);
-  const int segment = blockIdx.y + (MAPS ? 1 : 0), begin = segment * p.segment;   // (of the first no map is needed)
-  const int end = min(p.steps, begin + p.segment);
+  const int segment = blockIdx.y, begin = segment * p.segment, end = min(p.steps, begin + p.segment);
   const int live_end = min(end, p.lengths ? max(0, min(p.lengths[at.b], p.steps)) : p.steps);
   const uint8_t* done = p.done ? p.done + (int64_t)at.b * p.steps : nullptr;
   const int64_t state = (int64_t)at.b * p.F + at.f0;
-  float E[VW], decay[VW], rate[VW], rl[VW], drate[VW];
+  float E[VW], rate[VW], rl[VW], drate[VW];
 #pragma unroll
   for (int k = 0; k < VW; ++k) {
     rate[k] = p.rate[at.f0 + k];
     rl[k] = rate[k] * LOG2E;
     drate[k] = 0.f;
-    decay[k] = 1.f;
-    E[k] = 0.f;
   }
   Raw<S, VW> x[N], ig[N], dg[N], go[N];   // of the tile before
   float entering[VW];
@@ -455,20 +575,16 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
     const bool whole = t0 + at.tile <= live_end;
     fetch_steps<S, VW, N>(p.decay_gate, p.decay_s, at, t0, live_end, whole, dg);
     fetch_steps<S, VW, N>(p.dout, p.dout_s, at, t0, live_end, whole, go);
-    if constexpr (!MAPS) {
-      fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x);
-      fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig);
-      load_state<VW>(p.states, ((int64_t)at.b * p.saved + (t0 >> p.save_log2)) * p.F + at.f0, entering);
-    }
+    fetch_steps<S, VW, N>(p.x, p.x_s, at, t0, live_end, whole, x);
+    fetch_steps<S, VW, N>(p.input_gate, p.input_s, at, t0, live_end, whole, ig);
+    load_state<VW>(p.states, ((int64_t)at.b * p.saved + (t0 >> p.save_log2)) * p.F + at.f0, entering);
     if (done) flags = load_flags<N>(done, at.chunk_step(t0), p.steps);
   };
   const int tiles = live_end > begin ? (live_end - begin + at.tile - 1) / at.tile : 0;
   int set = 0, t0 = begin + (tiles - 1) * at.tile;
   if (tiles > 0) fetch(t0);
-  if constexpr (!MAPS) {
-    load_state<VW>(p.dfinal, state, E);
-    through_segments<VW, true>(p, at.b, at.f0, segment, E);
-  }
+  load_state<VW>(p.dfinal, state, E);
+  through_segments<VW, true>(p, at.b, at.f0, segment, E);
   for (; t0 >= begin; t0 -= at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
     const int t = at.chunk_step(t0);
@@ -480,8 +596,8 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
         Kept& e = q[i][k];
-        const Gates g = gates_of<true>(MAPS ? 0.f : widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
-        const float xv = MAPS ? 0.f : widen(x[i].v[k]);
+        const Gates g = gates_of<true>(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const float xv = widen(x[i].v[k]);
         e.a = g.a;
         e.g = widen(go[i].v[k]);
         e.wi = g.wi;
@@ -495,7 +611,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
     for (int k = 0; k < VW; ++k) {
       A[k] = 1.f;
       B[k] = RB[k] = 0.f;
-      if constexpr (!MAPS) h[k] = entering[k];
+      h[k] = entering[k];
     }
     if (resets || !whole) {
       apart();
@@ -530,105 +646,84 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
     for (int k = 0; k < VW; ++k) RA[k] = A[k];
     if (t0 > begin) fetch(t0 - at.tile);
     const int mine_at = at.wave * LF * VW;
-    if constexpr (!MAPS) compose_slots<VW, LF, false>(A, B, at.lane, fwd_a[set] + mine_at, fwd_b[set] + mine_at);
+    compose_slots<VW, LF, false>(A, B, at.lane, fwd_a[set] + mine_at, fwd_b[set] + mine_at);
     compose_slots<VW, LF, true>(RA, RB, at.lane, rev_a[set] + mine_at, rev_b[set] + mine_at);
     lds_barrier();
-    if constexpr (MAPS) {
-      for (int w = at.waves - 1; w >= 0; --w)
+    float mine[VW], after[VW], before[N][VW];
+    through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
+    through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
+    if (resets) {
+      apart();
+#pragma unroll
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
-          const int j = (w * LF + at.lane % LF) * VW + k;
-          E[k] = apply(rev_a[set][j], rev_b[set][j], E[k]);
-          decay[k] = decay_of(rev_a[set][j], decay[k]);
+          before[i][k] = is_reset(q[i][k].a) ? 0.f : mine[k];
+          mine[k] = apply(q[i][k].a, q[i][k].b, mine[k]);
         }
     } else {
-      float mine[VW], after[VW], before[N][VW];
-      through_waves<VW, LF, false>(h, mine, A, B, fwd_a[set], fwd_b[set], at.lane, at.wave, at.waves);
-      through_waves<VW, LF, true>(E, after, RA, RB, rev_a[set], rev_b[set], at.lane, at.wave, at.waves);
-      if (resets) {
-        apart();
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            before[i][k] = is_reset(q[i][k].a) ? 0.f : mine[k];
-            mine[k] = apply(q[i][k].a, q[i][k].b, mine[k]);
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            before[i][k] = mine[k];
-            mine[k] = __fmaf_rn(q[i][k].a, mine[k], q[i][k].b);
-          }
-      }
-      auto gradients = [&](auto plain) __attribute__((always_inline)) {   // no resets, a whole tile
-        constexpr bool PLAIN = decltype(plain)::value;
-        if constexpr (!PLAIN) apart();
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i) {
-          const bool live = PLAIN || t + i < live_end;
-          float ox[VW], oi[VW], od[VW];
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            const Kept& e = q[i][k];
-            const float D = e.g + after[k];
-            after[k] = !PLAIN && is_reset(e.a) ? 0.f : e.a * D;
-            const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
-            ox[k] = live ? D * e.wi : 0.f;
-            oi[k] = live ? D * e.b * e.not_i : 0.f;
-            od[k] = live ? -dr * rate[k] * e.not_r : 0.f;
-            drate[k] -= live ? dr : 0.f;
-          }
-          store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
-          store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
-          store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
-        }
-      };
-      if (resets || !whole) gradients(std::false_type{});
-      else gradients(std::true_type{});
-    }
-  }
-  if constexpr (MAPS) {
-    if (at.wave == 0 && at.slot == 0) {
-      float* m = p.maps + (((int64_t)at.b * p.segments + segment) * 2) * p.F + at.f0;
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        m[k] = decay[k];
-        m[p.F + k] = E[k];
-      }
-    }
-  } else {
-    const int cleared = begin + tiles * at.tile;
-    clear_steps<S>(p.dx, p, at, cleared, end);
-    clear_steps<S>(p.dinput_gate, p, at, cleared, end);
-    clear_steps<S>(p.ddecay_gate, p, at, cleared, end);
-    if (p.dcarry && segment == 0 && at.wave == 0 && at.slot == 0) {
-#pragma unroll
-      for (int k = 0; k < VW; ++k) p.dcarry[state + k] = E[k];
-    }
-    if (p.partials) {
-      // the slots' sums, the lanes' by butterflies, the waves' in their order
-      float* sums = &fwd_a[0][0];
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        for (int o = LF; o < 64; o <<= 1) drate[k] += __shfl_xor(drate[k], o);
-      }
-      __syncthreads();
-      if (at.slot == 0) {
-#pragma unroll
-        for (int k = 0; k < VW; ++k) sums[(at.wave * LF + at.lane) * VW + k] = drate[k];
-      }
-      __syncthreads();
-      if (at.wave == 0 && at.slot == 0) {
-        float* out = p.partials + ((int64_t)at.b * p.segments + segment) * p.F + at.f0;
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
-          float s = 0.f;
-          for (int w = 0; w < at.waves; ++w) s += sums[(w * LF + at.lane) * VW + k];
-          out[k] = s;
+          before[i][k] = mine[k];
+          mine[k] = __fmaf_rn(q[i][k].a, mine[k], q[i][k].b);
         }
+    }
+    auto gradients = [&](auto plain) __attribute__((always_inline)) {   // no resets, a whole tile
+      constexpr bool PLAIN = decltype(plain)::value;
+      if constexpr (!PLAIN) apart();
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i) {
+        const bool live = PLAIN || t + i < live_end;
+        float ox[VW], oi[VW], od[VW];
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const Kept& e = q[i][k];
+          const float D = e.g + after[k];
+          after[k] = !PLAIN && is_reset(e.a) ? 0.f : e.a * D;
+          const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
+          ox[k] = live ? D * e.wi : 0.f;
+          oi[k] = live ? D * e.b * e.not_i : 0.f;
+          od[k] = live ? -dr * rate[k] * e.not_r : 0.f;
+          drate[k] -= live ? dr : 0.f;
+        }
+        store_step<S, VW, N>(p.dx, p, at, t0, i, end, whole, ox);
+        store_step<S, VW, N>(p.dinput_gate, p, at, t0, i, end, whole, oi);
+        store_step<S, VW, N>(p.ddecay_gate, p, at, t0, i, end, whole, od);
+      }
+    };
+    if (resets || !whole) gradients(std::false_type{});
+    else gradients(std::true_type{});
+  }
+  const int cleared = begin + tiles * at.tile;
+  clear_steps<S>(p.dx, p, at, cleared, end);
+  clear_steps<S>(p.dinput_gate, p, at, cleared, end);
+  clear_steps<S>(p.ddecay_gate, p, at, cleared, end);
+  if (p.dcarry && segment == 0 && at.wave == 0 && at.slot == 0) {
+#pragma unroll
+    for (int k = 0; k < VW; ++k) p.dcarry[state + k] = E[k];
+  }
+  if (p.partials) {
+    // the slots' sums, the lanes' by butterflies, the waves' in their order
+    float* sums = &fwd_a[0][0];
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      for (int o = LF; o < 64; o <<= 1) drate[k] += __shfl_xor(drate[k], o);
+    }
+    __syncthreads();
+    if (at.slot == 0) {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) sums[(at.wave * LF + at.lane) * VW + k] = drate[k];
+    }
+    __syncthreads();
+    if (at.wave == 0 && at.slot == 0) {
+      float* out = p.partials + ((int64_t)at.b * p.segments + segment) * p.F + at.f0;
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        float s = 0.f;
+        for (int w = 0; w < at.waves; ++w) s += sums[(w * LF + at.lane) * VW + k];
+        out[k] = s;
       }
     }
   }
@@ -768,15 +863,10 @@ template <typename S, int VW, int LF, bool BWD>
 void launch_shape(hipStream_t st, const GatedArgs& a, const Plan& s, int batch) {
   const unsigned groups = (unsigned)batch * (unsigned)s.blocks;
   const dim3 t(64 * s.waves);
-  if constexpr (BWD) {
-    if (s.segments > 1)
-      hipLaunchKernelGGL((gated_bwd_kernel<S, VW, LF, true>), dim3(groups, s.segments - 1), t, 0, st, a);
-    hipLaunchKernelGGL((gated_bwd_kernel<S, VW, LF, false>), dim3(groups, s.segments), t, 0, st, a);
-  } else {
-    if (s.segments > 1)
-      hipLaunchKernelGGL((gated_fwd_kernel<S, VW, LF, true>), dim3(groups, s.segments - 1), t, 0, st, a);
-    hipLaunchKernelGGL((gated_fwd_kernel<S, VW, LF, false>), dim3(groups, s.segments), t, 0, st, a);
-  }
+  if (s.segments > 1)
+    hipLaunchKernelGGL((gated_maps_kernel<S, VW, LF, BWD>), dim3(groups, s.segments - 1), t, 0, st, a);
+  if constexpr (BWD) hipLaunchKernelGGL((gated_bwd_kernel<S, VW, LF>), dim3(groups, s.segments), t, 0, st, a);
+  else hipLaunchKernelGGL((gated_fwd_kernel<S, VW, LF>), dim3(groups, s.segments), t, 0, st, a);
 }
 template <typename S, bool BWD> void launch(hipStream_t st, GatedArgs a, const Plan& s, int batch) {
   constexpr int VW = LANE;
