@@ -33,6 +33,20 @@ __device__ __forceinline__ void load_unit(const float* p, int left, Unit8<float>
     for (int j = 0; j < UNIT; ++j) u.w[j] = j < left ? __float_as_uint(p[j]) : 0;
   }
 }
+// A whole unit that is read once: kept out of the caches' way (7.0 TB/s for 6.2 reading 1 GB).
+typedef uint32_t uintx4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load_unit_once(const uint16_t* p, Unit8<uint16_t>& u) {
+  const uintx4u v = __builtin_nontemporal_load(reinterpret_cast<const uintx4u*>(p));
+  u.w[0] = v[0]; u.w[1] = v[1]; u.w[2] = v[2]; u.w[3] = v[3];
+}
+__device__ __forceinline__ void load_unit_once(const float* p, Unit8<float>& u) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uintx4u v = __builtin_nontemporal_load(reinterpret_cast<const uintx4u*>(p + 4 * h));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u.w[4 * h + j] = v[j];
+  }
+}
 __device__ __forceinline__ float value(const Unit8<uint16_t>& u, int j) {
   return __uint_as_float(j & 1 ? u.w[j / 2] & 0xffff0000u : u.w[j / 2] << 16);
 }

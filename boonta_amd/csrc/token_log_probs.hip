@@ -31,6 +31,7 @@ constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of
 constexpr int MAX_SEGMENTS = 256;
 constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
 constexpr int BLOCKS = 4096;            // most workgroups of a launch over narrow rows
+constexpr int AHEAD = 4;                // units of a wide row that a thread has in flight
 constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
 constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
 constexpr float LN2 = 0.6931471805599453f;
@@ -60,25 +61,33 @@ __device__ __forceinline__ int64_t token_of(const TokenArgs& p, uint32_t row) {
   return p.wide_tokens ? static_cast<const int64_t*>(p.tokens)[row] : static_cast<const int32_t*>(p.tokens)[row];
 }
 
-// The 8 values of a unit, -inf where masked or past the row's end.
-template <typename T>
+// The mask's bytes of a unit, 0 past the row's end.
+__device__ __forceinline__ uint64_t read_mask(const uint8_t* mask, int col, int V) {
+  uint64_t allowed = 0;
+  if (col + UNIT <= V) {
+    __builtin_memcpy(&allowed, mask + col, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j)
+      if (col + j < V) allowed |= (uint64_t)mask[col + j] << (8 * j);
+  }
+  return allowed;
+}
+// The 8 values of a unit, -inf where masked or (LAST) past the row's end.
+template <bool MASK, bool LAST, typename T>
+__device__ __forceinline__ void unit_values(const Unit8<T>& raw, uint64_t allowed, int left, float (&v)[UNIT]) {
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) {
+    v[j] = value(raw, j);
+    if constexpr (LAST) v[j] = j < left ? v[j] : -INF;
+    if constexpr (MASK) v[j] = (allowed >> (8 * j)) & 0xff ? v[j] : -INF;
+  }
+}
+template <bool MASK, typename T>
 __device__ __forceinline__ void read_unit(const T* x, const uint8_t* mask, int col, int V, float (&v)[UNIT]) {
   Unit8<T> raw;
-  const int left = V - col;
-  load_unit(x + col, left, raw);
-  uint64_t allowed = ~0ull;
-  if (mask) {
-    if (left >= UNIT) {
-      __builtin_memcpy(&allowed, mask + col, 8);
-    } else {
-      allowed = 0;
-#pragma unroll
-      for (int j = 0; j < UNIT; ++j)
-        if (j < left) allowed |= (uint64_t)mask[col + j] << (8 * j);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < UNIT; ++j) v[j] = j < left && ((allowed >> (8 * j)) & 0xff) ? value(raw, j) : -INF;
+  load_unit(x + col, V - col, raw);
+  unit_values<MASK, true>(raw, MASK ? read_mask(mask, col, V) : 0, V - col, v);
 }
 __device__ __forceinline__ float max8(const float (&v)[UNIT]) {
   return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
@@ -163,7 +172,7 @@ __device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int 
 }
 
 // ---- rows of up to 512 columns: lanes of a wave
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool MASK>
 __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
   const int L = 1 << p.lanes_log2, lane = threadIdx.x & (L - 1), col = lane * UNIT;
   const uint32_t step = (gridDim.x * THREADS) >> p.lanes_log2;
@@ -171,11 +180,11 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
     const bool live = row0 < p.rows;
     const uint32_t row = live ? row0 : p.rows - 1;
     const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
-    const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+    const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
     float v[UNIT];
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) v[j] = -INF;
-    if (col < p.V) read_unit(x, mask, col, p.V, v);
+    if (col < p.V) read_unit<MASK>(x, mask, col, p.V, v);
     Sums a = no_sums();
     add_unit(a, v, max8(v), p.c);
     a = lanes_joined(a, p.lanes_log2, p.c);
@@ -220,28 +229,47 @@ __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n
   return r;
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool MASK>
 __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   __shared__ Sums sums[WAVES];
   __shared__ typename std::conditional<TOP, TopSpace, int>::type space;
   const int tid = threadIdx.x;
   const uint32_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
-  const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+  const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
   const int units = (p.V + UNIT - 1) / UNIT, first = blockIdx.y * p.segment_units;
-  const int end = min(units, first + p.segment_units);
+  const int end = min(units, first + p.segment_units), whole = min(end, p.V / UNIT);
   Sums a = no_sums();
   float best = -INF;
   int best_unit = 0;
-  for (int u = first + tid; u < end; u += THREADS) {
-    float v[UNIT];
-    read_unit(x, mask, u * UNIT, p.V, v);
+  auto add = [&](const float (&v)[UNIT], int u) __attribute__((always_inline)) {
     const float most = max8(v);
     add_unit(a, v, most, p.c);
     if constexpr (TOP) {
       best_unit = most > best ? u : best_unit;
       best = most > best ? most : best;
     }
+  };
+  int u = first + tid;
+  for (; u + (AHEAD - 1) * THREADS < whole; u += AHEAD * THREADS) {
+    Unit8<T> raw[AHEAD];
+    uint64_t allowed[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      load_unit_once(x + (u + k * THREADS) * UNIT, raw[k]);
+      if constexpr (MASK) __builtin_memcpy(&allowed[k], mask + (u + k * THREADS) * UNIT, 8);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      float v[UNIT];
+      unit_values<MASK, false>(raw[k], MASK ? allowed[k] : 0, UNIT, v);
+      add(v, u + k * THREADS);
+    }
+  }
+  for (; u < end; u += THREADS) {
+    float v[UNIT];
+    read_unit<MASK>(x, mask, u * UNIT, p.V, v);
+    add(v, u);
   }
   a = lanes_joined(a, 6, p.c);
   if ((tid & 63) == 0) sums[tid >> 6] = a;
@@ -283,7 +311,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
       const int w = i / each, u = first + (int)space.winners[w] + (i - w * each) * THREADS;
       if (u >= end) continue;
       float v[UNIT];
-      read_unit(x, mask, u * UNIT, p.V, v);
+      read_unit<MASK>(x, mask, u * UNIT, p.V, v);
       const uint64_t key = key_of(max8(v), (uint32_t)u);
       if (key >= least) space.candidates[atomicAdd(&space.count, 1)] = key;
     }
@@ -301,7 +329,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
     if (tid < best_units * UNIT) {
       float v[UNIT];
       const int col = (int)space.winners[tid / UNIT] * UNIT;
-      read_unit(x, mask, col, p.V, v);
+      read_unit<MASK>(x, mask, col, p.V, v);
       float one = -INF;
 #pragma unroll
       for (int j = 0; j < UNIT; ++j) one = tid % UNIT == j ? v[j] : one;
@@ -355,34 +383,96 @@ template <typename T> __global__ void __launch_bounds__(64) token_join_kernel(To
 }
 
 // ---- backward: a workgroup takes `row_block` rows' units, or a segment of one row's
-template <typename T> __global__ void __launch_bounds__(THREADS) token_bwd_kernel(TokenArgs p) {
-  const uint32_t units = p.units.d;
-  const int first = blockIdx.y * p.segment_units, end = min((int)units, first + p.segment_units);
-  for (uint32_t row0 = blockIdx.x * p.row_block; row0 < p.rows; row0 += gridDim.x * p.row_block) {
-    const uint32_t rows = min((uint32_t)p.row_block, p.rows - row0);
-    const uint32_t count = p.row_block > 1 ? rows * units : (uint32_t)(end - first);
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-      const uint32_t r = p.row_block > 1 ? quotient(i, p.units) : 0, row = row0 + r;
-      const int col = (p.row_block > 1 ? (int)(i - r * units) : first + (int)i) * UNIT, left = p.V - col;
-      const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
-      const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
-      const float m = p.stats[2 * (int64_t)row], l = p.stats[2 * (int64_t)row + 1];
-      const int64_t token = token_of(p, row);
-      // a token that is none, or not allowed, passes nothing
-      float g = 0.f;
-      if (p.dlog_prob && token >= 0 && token < p.V && p.log_prob[row] > -INF)
-        g = p.dlog_prob[row_offset(row, p.steps, p.dlog_prob_s)];
-      const float h = p.dentropy ? p.dentropy[row_offset(row, p.steps, p.dentropy_s)] : 0.f, H = p.entropy[row];
-      float v[UNIT];
-      read_unit(x, mask, col, p.V, v);
+// What a row's gradients need: dx = -2^w (hl max(w, .) + gh) with w = (x - m) c - l,
+// hl = h ln(2) / T, gh = (g + h entropy) / T; and g / T at the token.
+struct RowGradient {
+  float m, l, hl, gh, g;
+  int token;   // -1: none
+};
+__device__ __forceinline__ RowGradient row_gradient(const TokenArgs& p, uint32_t row) {
+  RowGradient r;
+  r.m = p.stats[2 * (int64_t)row];
+  r.l = p.stats[2 * (int64_t)row + 1];
+  const int64_t token = token_of(p, row);
+  // a token that is none, or not allowed, passes nothing
+  const bool given = token >= 0 && token < p.V && !(p.log_prob[row] == -INF);
+  r.token = given ? (int)token : -1;
+  r.g = given && p.dlog_prob ? p.dlog_prob[row_offset(row, p.steps, p.dlog_prob_s)] * p.inverse_t : 0.f;
+  const float h = p.dentropy ? p.dentropy[row_offset(row, p.steps, p.dentropy_s)] * p.inverse_t : 0.f;
+  r.hl = h * LN2;
+  r.gh = __fmaf_rn(h, p.entropy[row], r.g);
+  return r;
+}
+__device__ __forceinline__ void unit_gradient(const RowGradient& r, float c, int col, float (&v)[UNIT]) {
+  const bool bad = r.l != r.l;   // a row with an infinity or NaN: NaN, but where the mask allows nothing
+  float d[UNIT];
 #pragma unroll
-      for (int j = 0; j < UNIT; ++j) {
-        const float w = exponent(v[j], m, p.c) - l, e = __builtin_amdgcn_exp2f(w);
-        const float d = -e * __fmaf_rn(h, __fmaf_rn(LN2, fmaxf(w, -1e4f), H), g);
-        v[j] = v[j] == -INF ? 0.f : (col + j == token ? d + g : d) * p.inverse_t;
-      }
-      store_unit(static_cast<T*>(p.dlogits) + (int64_t)row * p.V + col, left, v);
+  for (int j = 0; j < UNIT; ++j) {
+    const float w = __fmaf_rn(v[j] - r.m, c, -r.l), e = __builtin_amdgcn_exp2f(w);
+    d[j] = -e * __fmaf_rn(r.hl, fmaxf(w, -1e4f), r.gh);
+  }
+  if (bad) {
+    asm volatile("");   // (seldom: not selected from beside the others)
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) d[j] = v[j] == -INF ? 0.f : d[j];
+  }
+  const int at = r.token - col;
+  if (at >= 0 && at < UNIT) {
+    asm volatile("");
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) d[j] += j == at ? r.g : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) v[j] = d[j];
+}
+
+template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_bwd_kernel(TokenArgs p) {
+  // rows of few units: several rows side by side
+  const uint32_t units = p.units.d;
+  for (uint32_t row0 = blockIdx.x * p.row_block; row0 < p.rows; row0 += gridDim.x * p.row_block) {
+    const uint32_t count = min((uint32_t)p.row_block, p.rows - row0) * units;
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+      const uint32_t q = quotient(i, p.units), row = row0 + q;
+      const int col = (int)(i - q * units) * UNIT;
+      const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+      float v[UNIT];
+      read_unit<MASK>(x, MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr, col, p.V, v);
+      unit_gradient(row_gradient(p, row), p.c, col, v);
+      store_unit(static_cast<T*>(p.dlogits) + (int64_t)row * p.V + col, p.V - col, v);
     }
+  }
+}
+
+template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_bwd_wide_kernel(TokenArgs p) {
+  const uint32_t row = blockIdx.x;
+  const int first = blockIdx.y * p.segment_units, end = min((int)p.units.d, first + p.segment_units);
+  const int whole = min(end, p.V / UNIT);
+  const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+  const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+  T* out = static_cast<T*>(p.dlogits) + (int64_t)row * p.V;
+  const RowGradient r = row_gradient(p, row);
+  int u = first + threadIdx.x;
+  for (; u + (AHEAD - 1) * THREADS < whole; u += AHEAD * THREADS) {
+    Unit8<T> raw[AHEAD];
+    uint64_t allowed[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      load_unit_once(x + (u + k * THREADS) * UNIT, raw[k]);
+      if constexpr (MASK) __builtin_memcpy(&allowed[k], mask + (u + k * THREADS) * UNIT, 8);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      float v[UNIT];
+      unit_values<MASK, false>(raw[k], MASK ? allowed[k] : 0, UNIT, v);
+      unit_gradient(r, p.c, (u + k * THREADS) * UNIT, v);
+      store_unit(out + (u + k * THREADS) * UNIT, UNIT, v);
+    }
+  }
+  for (; u < end; u += THREADS) {
+    float v[UNIT];
+    read_unit<MASK>(x, mask, u * UNIT, p.V, v);
+    unit_gradient(r, p.c, u * UNIT, v);
+    store_unit(out + u * UNIT, p.V - u * UNIT, v);
   }
 }
 
@@ -425,18 +515,29 @@ TokenArgs common_args(const void* logits, const void* tokens, int wide_tokens, c
   return a;
 }
 
-template <typename T> void launch_fwd(hipStream_t st, TokenArgs& a) {
+template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
   if (a.V <= NARROW) {
     while ((UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
     const unsigned blocks = (unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS));
-    if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true>), dim3(blocks), dim3(THREADS), 0, st, a);
-    else hipLaunchKernelGGL((token_narrow_kernel<T, false>), dim3(blocks), dim3(THREADS), 0, st, a);
+    if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK>), dim3(blocks), dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK>), dim3(blocks), dim3(THREADS), 0, st, a);
     return;
   }
   const dim3 grid(a.rows, a.segments);
-  if (a.top) hipLaunchKernelGGL((token_wide_kernel<T, true>), grid, dim3(THREADS), 0, st, a);
-  else hipLaunchKernelGGL((token_wide_kernel<T, false>), grid, dim3(THREADS), 0, st, a);
+  if (a.top) hipLaunchKernelGGL((token_wide_kernel<T, true, MASK>), grid, dim3(THREADS), 0, st, a);
+  else hipLaunchKernelGGL((token_wide_kernel<T, false, MASK>), grid, dim3(THREADS), 0, st, a);
   if (a.segments > 1) hipLaunchKernelGGL((token_join_kernel<T>), dim3(a.rows), dim3(64), 0, st, a);
+}
+
+template <typename T, bool MASK> void launch_bwd(hipStream_t st, TokenArgs& a) {
+  const int units = (int)a.units.d;
+  a.row_block = std::max(1, 2 * THREADS / units);
+  a.segment_units = std::min(units, 8 * THREADS);
+  if (a.row_block > 1)
+    hipLaunchKernelGGL((token_bwd_kernel<T, MASK>), dim3((unsigned)ceil_div64(a.rows, a.row_block)), dim3(THREADS), 0, st, a);
+  else
+    hipLaunchKernelGGL((token_bwd_wide_kernel<T, MASK>), dim3(a.rows, (unsigned)ceil_div(units, a.segment_units)), dim3(THREADS),
+                       0, st, a);
 }
 
 }  // namespace
@@ -475,8 +576,8 @@ PPO_EXPORT int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logi
   a.partials = static_cast<float*>(workspace);
   a.segments = segments_of(a.rows, vocab);
   a.segment_units = ceil_div(ceil_div(vocab, UNIT), a.segments);
-  if (dtype == TOKEN_F32) launch_fwd<float>(as_stream(stream), a);
-  else launch_fwd<uint16_t>(as_stream(stream), a);
+  if (dtype == TOKEN_F32) mask ? launch_fwd<float, true>(as_stream(stream), a) : launch_fwd<float, false>(as_stream(stream), a);
+  else mask ? launch_fwd<uint16_t, true>(as_stream(stream), a) : launch_fwd<uint16_t, false>(as_stream(stream), a);
   return check_launch(what);
 }
 
@@ -499,11 +600,7 @@ PPO_EXPORT int ppo_token_log_probs_bwd(void* stream, int dtype, const void* logi
   a.dlog_prob_s = RowStride{strides[4], strides[5]};
   a.dentropy_s = RowStride{strides[6], strides[7]};
   a.dlogits = dlogits;
-  const int units = (int)a.units.d;
-  a.row_block = std::max(1, 2 * THREADS / units);
-  a.segment_units = a.row_block > 1 ? units : std::min(units, 8 * THREADS);
-  const dim3 grid((unsigned)ceil_div64(a.rows, a.row_block), (unsigned)ceil_div(units, a.segment_units));
-  if (dtype == TOKEN_F32) hipLaunchKernelGGL((token_bwd_kernel<float>), grid, dim3(THREADS), 0, as_stream(stream), a);
-  else hipLaunchKernelGGL((token_bwd_kernel<uint16_t>), grid, dim3(THREADS), 0, as_stream(stream), a);
+  if (dtype == TOKEN_F32) mask ? launch_bwd<float, true>(as_stream(stream), a) : launch_bwd<float, false>(as_stream(stream), a);
+  else mask ? launch_bwd<uint16_t, true>(as_stream(stream), a) : launch_bwd<uint16_t, false>(as_stream(stream), a);
   return check_launch(what);
 }
