@@ -75,6 +75,30 @@ __device__ __forceinline__ void store_unit(float* p, int left, const float (&v)[
   }
 }
 
+// The columns from `from` to `left` of the unit at p; the others are zeros.
+template <typename S> __device__ __forceinline__ void load_between(const S* p, int from, int left, Unit8<S>& u) {
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) {
+    const bool in = j >= from && j < left;
+    if constexpr (sizeof(S) == 2) {
+      const uint32_t v = in ? p[j] : 0;
+      u.w[j / 2] = j & 1 ? u.w[j / 2] | v << 16 : v;
+    } else {
+      u.w[j] = in ? __float_as_uint(p[j]) : 0;
+    }
+  }
+}
+__device__ __forceinline__ void store_between(uint16_t* p, int from, int left, const float (&v)[UNIT]) {
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j)
+    if (j >= from && j < left) p[j] = (uint16_t)pack_bf16(v[j], v[j]);
+}
+__device__ __forceinline__ void store_between(float* p, int from, int left, const float (&v)[UNIT]) {
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j)
+    if (j >= from && j < left) p[j] = v[j];
+}
+
 // Division of n < 2^31 by a number of 1 .. 2^31 - 1 known on the host: with
 // s = ceil(log2 d) and m = floor(2^(31+s) / d) + 1, m d exceeds 2^(31+s) by at
 // most d <= 2^s, so that n (m d - 2^(31+s)) < 2^(31+s) and the quotient is exact.

@@ -31,7 +31,7 @@ constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of
 constexpr int MAX_SEGMENTS = 256;
 constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
 constexpr int BLOCKS = 4096;            // most workgroups of a launch over narrow rows
-constexpr int AHEAD = 4;                // units of a wide row that a thread has in flight
+constexpr int AHEAD = 4, BWD_AHEAD = 4; // units of a wide row that a thread has in flight
 constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
 constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
 constexpr float LN2 = 0.6931471805599453f;
@@ -61,34 +61,44 @@ __device__ __forceinline__ int64_t token_of(const TokenArgs& p, uint32_t row) {
   return p.wide_tokens ? static_cast<const int64_t*>(p.tokens)[row] : static_cast<const int32_t*>(p.tokens)[row];
 }
 
-// The mask's bytes of a unit, 0 past the row's end.
+// The mask's bytes of a unit at column col, 0 outside the row.
 __device__ __forceinline__ uint64_t read_mask(const uint8_t* mask, int col, int V) {
   uint64_t allowed = 0;
-  if (col + UNIT <= V) {
+  if (col >= 0 && col + UNIT <= V) {
     __builtin_memcpy(&allowed, mask + col, 8);
   } else {
 #pragma unroll
     for (int j = 0; j < UNIT; ++j)
-      if (col + j < V) allowed |= (uint64_t)mask[col + j] << (8 * j);
+      if (col + j >= 0 && col + j < V) allowed |= (uint64_t)mask[col + j] << (8 * j);
   }
   return allowed;
 }
-// The 8 values of a unit, -inf where masked or (LAST) past the row's end.
-template <bool MASK, bool LAST, typename T>
-__device__ __forceinline__ void unit_values(const Unit8<T>& raw, uint64_t allowed, int left, float (&v)[UNIT]) {
+// The 8 values of a unit, -inf where masked.
+template <bool MASK, typename T>
+__device__ __forceinline__ void unit_values(const Unit8<T>& raw, uint64_t allowed, float (&v)[UNIT]) {
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) {
     v[j] = value(raw, j);
-    if constexpr (LAST) v[j] = j < left ? v[j] : -INF;
     if constexpr (MASK) v[j] = (allowed >> (8 * j)) & 0xff ? v[j] : -INF;
   }
 }
+// Those of any unit, -inf outside the row too.
 template <bool MASK, typename T>
 __device__ __forceinline__ void read_unit(const T* x, const uint8_t* mask, int col, int V, float (&v)[UNIT]) {
   Unit8<T> raw;
-  load_unit(x + col, V - col, raw);
-  unit_values<MASK, true>(raw, MASK ? read_mask(mask, col, V) : 0, V - col, v);
+  if (col >= 0) load_unit(x + col, V - col, raw);
+  else load_between(x + col, -col, V - col, raw);
+  unit_values<MASK>(raw, MASK ? read_mask(mask, col, V) : 0, v);
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) v[j] = col + j >= 0 && col + j < V ? v[j] : -INF;
 }
+// Columns before a wide row's start from which its units are counted, so that
+// they begin on a cache line (units that straddle 4-byte words load at 5.0 TB/s for
+// 6.0; a wave's stores are whole lines).
+template <typename T> __device__ __forceinline__ int skew_of(const T* row) {
+  return (int)((reinterpret_cast<uintptr_t>(row) & 127) / sizeof(T));
+}
+constexpr int MAX_SKEW = 63;
 __device__ __forceinline__ float max8(const float (&v)[UNIT]) {
   return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
 }
@@ -216,7 +226,7 @@ __device__ __forceinline__ int64_t partial_floats(int top) { return 4 + 2 * top;
 
 struct TopSpace {
   uint64_t keys[THREADS];
-  uint64_t candidates[MAX_TOP * (SEGMENT / (UNIT * THREADS))];
+  uint64_t candidates[MAX_TOP * (SEGMENT / (UNIT * THREADS) + 1)];
   uint32_t winners[THREADS];
   uint64_t best[MAX_TOP];
   int count;
@@ -237,11 +247,16 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   const uint32_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
   const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
-  const int units = (p.V + UNIT - 1) / UNIT, first = blockIdx.y * p.segment_units;
-  const int end = min(units, first + p.segment_units), whole = min(end, p.V / UNIT);
+  const int skew = skew_of(x), first = blockIdx.y * p.segment_units;
+  const int end = min((p.V + skew + UNIT - 1) / UNIT, first + p.segment_units), whole = min(end, (p.V + skew) / UNIT);
+  x -= skew;   // (columns in the units' count from here on; those before the row are not read)
+  if constexpr (MASK) mask -= skew;
   Sums a = no_sums();
   float best = -INF;
   int best_unit = 0;
+  auto read = [&](int u, float (&v)[UNIT]) __attribute__((always_inline)) {
+    read_unit<MASK>(x + skew, mask + skew, u * UNIT - skew, p.V, v);
+  };
   auto add = [&](const float (&v)[UNIT], int u) __attribute__((always_inline)) {
     const float most = max8(v);
     add_unit(a, v, most, p.c);
@@ -251,6 +266,12 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
     }
   };
   int u = first + tid;
+  if (u * UNIT < skew && u < end) {   // the row's first columns
+    float v[UNIT];
+    read(u, v);
+    add(v, u);
+    u += THREADS;
+  }
   for (; u + (AHEAD - 1) * THREADS < whole; u += AHEAD * THREADS) {
     Unit8<T> raw[AHEAD];
     uint64_t allowed[AHEAD];
@@ -262,13 +283,13 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       float v[UNIT];
-      unit_values<MASK, false>(raw[k], MASK ? allowed[k] : 0, UNIT, v);
+      unit_values<MASK>(raw[k], MASK ? allowed[k] : 0, v);
       add(v, u + k * THREADS);
     }
   }
   for (; u < end; u += THREADS) {
     float v[UNIT];
-    read_unit<MASK>(x, mask, u * UNIT, p.V, v);
+    read(u, v);
     add(v, u);
   }
   a = lanes_joined(a, 6, p.c);
@@ -285,7 +306,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   float* partial = p.partials + ((int64_t)row * p.segments + blockIdx.y) * partial_floats(p.top);
   if (tid == 0) {
     if (p.segments == 1) {
-      finish_row(p, row, a, x, mask);
+      finish_row(p, row, a, x + skew, MASK ? mask + skew : nullptr);
     } else {
       partial[0] = a.m;
       partial[1] = a.s;
@@ -311,7 +332,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
       const int w = i / each, u = first + (int)space.winners[w] + (i - w * each) * THREADS;
       if (u >= end) continue;
       float v[UNIT];
-      read_unit<MASK>(x, mask, u * UNIT, p.V, v);
+      read(u, v);
       const uint64_t key = key_of(max8(v), (uint32_t)u);
       if (key >= least) space.candidates[atomicAdd(&space.count, 1)] = key;
     }
@@ -328,8 +349,8 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
     uint64_t value = 0;
     if (tid < best_units * UNIT) {
       float v[UNIT];
-      const int col = (int)space.winners[tid / UNIT] * UNIT;
-      read_unit<MASK>(x, mask, col, p.V, v);
+      read((int)space.winners[tid / UNIT], v);
+      const int col = (int)space.winners[tid / UNIT] * UNIT - skew;
       float one = -INF;
 #pragma unroll
       for (int j = 0; j < UNIT; ++j) one = tid % UNIT == j ? v[j] : one;
@@ -445,35 +466,50 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) toke
 
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_bwd_wide_kernel(TokenArgs p) {
   const uint32_t row = blockIdx.x;
-  const int first = blockIdx.y * p.segment_units, end = min((int)p.units.d, first + p.segment_units);
-  const int whole = min(end, p.V / UNIT);
   const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
   const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
   T* out = static_cast<T*>(p.dlogits) + (int64_t)row * p.V;
+  const int skew = skew_of(out), first = blockIdx.y * p.segment_units;   // (as the logits where those are contiguous)
+  const int end = min((p.V + skew + UNIT - 1) / UNIT, first + p.segment_units), whole = min(end, (p.V + skew) / UNIT);
   const RowGradient r = row_gradient(p, row);
-  int u = first + threadIdx.x;
-  for (; u + (AHEAD - 1) * THREADS < whole; u += AHEAD * THREADS) {
-    Unit8<T> raw[AHEAD];
-    uint64_t allowed[AHEAD];
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      load_unit_once(x + (u + k * THREADS) * UNIT, raw[k]);
-      if constexpr (MASK) __builtin_memcpy(&allowed[k], mask + (u + k * THREADS) * UNIT, 8);
-    }
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      float v[UNIT];
-      unit_values<MASK, false>(raw[k], MASK ? allowed[k] : 0, UNIT, v);
-      unit_gradient(r, p.c, (u + k * THREADS) * UNIT, v);
-      store_unit(out + (u + k * THREADS) * UNIT, UNIT, v);
-    }
-  }
-  for (; u < end; u += THREADS) {
+  auto one = [&](int u) __attribute__((always_inline)) {
+    const int col = u * UNIT - skew;
     float v[UNIT];
-    read_unit<MASK>(x, mask, u * UNIT, p.V, v);
-    unit_gradient(r, p.c, u * UNIT, v);
-    store_unit(out + u * UNIT, p.V - u * UNIT, v);
+    read_unit<MASK>(x, mask, col, p.V, v);
+    unit_gradient(r, p.c, col, v);
+    store_between(out + col, -col, p.V - col, v);
+  };
+  int u = first + threadIdx.x;
+  if (u * UNIT < skew && u < end) {   // the row's first columns
+    one(u);
+    u += THREADS;
   }
+  for (; u + (BWD_AHEAD - 1) * THREADS < whole; u += BWD_AHEAD * THREADS) {
+    Unit8<T> raw[BWD_AHEAD];
+    uint64_t allowed[BWD_AHEAD];
+#pragma unroll
+    for (int k = 0; k < BWD_AHEAD; ++k) {
+      const int col = (u + k * THREADS) * UNIT - skew;
+      load_unit_once(x + col, raw[k]);
+      if constexpr (MASK) __builtin_memcpy(&allowed[k], mask + col, 8);
+    }
+#pragma unroll
+    for (int k = 0; k < BWD_AHEAD; ++k) {
+      const int col = (u + k * THREADS) * UNIT - skew;
+      float v[UNIT];
+      unit_values<MASK>(raw[k], MASK ? allowed[k] : 0, v);
+      unit_gradient(r, p.c, col, v);
+      store_unit(out + col, UNIT, v);
+    }
+  }
+  for (; u < whole; u += THREADS) {
+    const int col = u * UNIT - skew;
+    float v[UNIT];
+    read_unit<MASK>(x, mask, col, p.V, v);
+    unit_gradient(r, p.c, col, v);
+    store_unit(out + col, UNIT, v);
+  }
+  if (u < end) one(u);   // and its last
 }
 
 // ---- launches
@@ -532,12 +568,14 @@ template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
 template <typename T, bool MASK> void launch_bwd(hipStream_t st, TokenArgs& a) {
   const int units = (int)a.units.d;
   a.row_block = std::max(1, 2 * THREADS / units);
-  a.segment_units = std::min(units, 8 * THREADS);
+  const int most = ceil_div(a.V + MAX_SKEW, UNIT);
+  const int segments = ceil_div(most, 8 * THREADS);
+  a.segment_units = ceil_div(most, segments);
   if (a.row_block > 1)
     hipLaunchKernelGGL((token_bwd_kernel<T, MASK>), dim3((unsigned)ceil_div64(a.rows, a.row_block)), dim3(THREADS), 0, st, a);
   else
-    hipLaunchKernelGGL((token_bwd_wide_kernel<T, MASK>), dim3(a.rows, (unsigned)ceil_div(units, a.segment_units)), dim3(THREADS),
-                       0, st, a);
+    hipLaunchKernelGGL((token_bwd_wide_kernel<T, MASK>), dim3(a.rows, (unsigned)segments), dim3(THREADS), 0, st,
+                       a);
 }
 
 }  // namespace
@@ -575,7 +613,7 @@ PPO_EXPORT int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logi
   a.top_tokens = top_tokens;
   a.partials = static_cast<float*>(workspace);
   a.segments = segments_of(a.rows, vocab);
-  a.segment_units = ceil_div(ceil_div(vocab, UNIT), a.segments);
+  a.segment_units = ceil_div(ceil_div(vocab + MAX_SKEW, UNIT), a.segments);
   if (dtype == TOKEN_F32) mask ? launch_fwd<float, true>(as_stream(stream), a) : launch_fwd<float, false>(as_stream(stream), a);
   else mask ? launch_fwd<uint16_t, true>(as_stream(stream), a) : launch_fwd<uint16_t, false>(as_stream(stream), a);
   return check_launch(what);
