@@ -31,7 +31,7 @@ constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of
 constexpr int MAX_SEGMENTS = 256;
 constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
 constexpr int BLOCKS = 4096;            // most workgroups of a launch over narrow rows
-constexpr int AHEAD = 4, BWD_AHEAD = 4; // units of a wide row that a thread has in flight
+constexpr int AHEAD = 4, BWD_AHEAD = 8; // units of a wide row that a thread has in flight
 constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
 constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
 constexpr float LN2 = 0.6931471805599453f;
@@ -138,22 +138,27 @@ __device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
   return a;
 }
 
-// A row's results from its sums, by one thread.
+// The row's token, read ahead of the sums: its logit where it is one that is allowed.
+struct Given {
+  bool token;
+  float logit;   // -inf: not allowed
+};
 template <typename T>
-__device__ __forceinline__ void finish_row(const TokenArgs& p, uint32_t row, const Sums& a, const T* x,
-                                           const uint8_t* mask) {
+__device__ __forceinline__ Given given_of(const TokenArgs& p, uint32_t row, const T* x, const uint8_t* mask) {
+  const int64_t token = token_of(p, row);
+  Given g{token >= 0 && token < p.V, -INF};
+  if (g.token && !(mask && !mask[token])) {
+    if constexpr (sizeof(T) == 2) g.logit = __uint_as_float((uint32_t)x[token] << 16);
+    else g.logit = x[token];
+  }
+  return g;
+}
+// A row's results from its sums, by one thread.
+__device__ __forceinline__ void finish_row(const TokenArgs& p, uint32_t row, const Sums& a, const Given& g) {
   const bool none = a.s == 0.f;
   const float l = none ? INF : __builtin_amdgcn_logf(a.s);   // log2
   p.entropy[row] = none ? 0.f : LN2 * (l - a.t / a.s);
-  const int64_t token = token_of(p, row);
-  float lp = 0.f;
-  if (token >= 0 && token < p.V) {
-    float v;
-    if constexpr (sizeof(T) == 2) v = __uint_as_float((uint32_t)x[token] << 16);
-    else v = x[token];
-    lp = v == -INF || (mask && !mask[token]) ? -INF : LN2 * (exponent(v, a.m, p.c) - l);
-  }
-  p.log_prob[row] = lp;
+  p.log_prob[row] = !g.token ? 0.f : g.logit == -INF ? -INF : LN2 * (exponent(g.logit, a.m, p.c) - l);
   if (p.stats) {
     p.stats[2 * (int64_t)row] = none ? 0.f : a.m;
     p.stats[2 * (int64_t)row + 1] = l;
@@ -194,11 +199,13 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
     float v[UNIT];
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) v[j] = -INF;
+    Given given{};
+    if (lane == 0) given = given_of(p, row, x, mask);
     if (col < p.V) read_unit<MASK>(x, mask, col, p.V, v);
     Sums a = no_sums();
     add_unit(a, v, max8(v), p.c);
     a = lanes_joined(a, p.lanes_log2, p.c);
-    if (live && lane == 0) finish_row(p, row, a, x, mask);
+    if (live && lane == 0) finish_row(p, row, a, given);
     if constexpr (TOP) {
       const float l = __builtin_amdgcn_logf(a.s);
       uint64_t last = ~0ull;
@@ -224,19 +231,53 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
 // What a segment leaves: its sums, then its best keys.
 __device__ __forceinline__ int64_t partial_floats(int top) { return 4 + 2 * top; }
 
+constexpr int MOST_UNITS = MAX_TOP * (SEGMENT / (UNIT * THREADS) + 1);   // of the best threads
 struct TopSpace {
-  uint64_t keys[THREADS];
-  uint64_t candidates[MAX_TOP * (SEGMENT / (UNIT * THREADS) + 1)];
-  uint32_t winners[THREADS];
-  uint64_t best[MAX_TOP];
+  uint64_t lists[WAVES * MAX_TOP];   // each wave's best keys, in order; 0: none
+  uint64_t best[MAX_TOP];            // and those of all
+  uint64_t candidates[MOST_UNITS];
+  uint64_t values[MAX_TOP * UNIT];
+  uint32_t units[MAX_TOP];
   int count;
 };
 
-// keys' rank: how many of n are better.
+// A key's rank: how many of n are better.
 __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
-  int r = 0;
-  for (int i = 0; i < n; ++i) r += keys[i] > key;
+  int r = 0, i = 0;
+  for (; i + 8 <= n; i += 8) {   // (reads of eight on their way at once)
+    uint64_t k[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = keys[i + j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r += k[j] > key;
+  }
+  for (; i < n; ++i) r += keys[i] > key;
   return r;
+}
+// Among the keys of the wave.
+__device__ __forceinline__ int rank_in_wave(uint64_t key) {
+  int r = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+    r += other > key;
+  }
+  return r;
+}
+// The best keys of lists, `top` of each in order (0: no more), in order; `n` lists of
+// `pitch` keys.  Rooms of the workgroup's; ends with a barrier.
+__device__ __forceinline__ void merge_lists(const uint64_t* lists, int n, int pitch, int top, uint64_t* best) {
+  const int tid = threadIdx.x;
+  if (tid < top) best[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n * top; i += THREADS) {
+    const uint64_t key = lists[(i / top) * pitch + i % top];
+    int r = 0;
+    for (int w = 0; w < n; ++w) r += rank_of(key, lists + w * pitch, top);
+    if (key && r < top) best[r] = key;
+  }
+  __syncthreads();
 }
 
 template <typename T, bool TOP, bool MASK>
@@ -251,6 +292,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   const int end = min((p.V + skew + UNIT - 1) / UNIT, first + p.segment_units), whole = min(end, (p.V + skew) / UNIT);
   x -= skew;   // (columns in the units' count from here on; those before the row are not read)
   if constexpr (MASK) mask -= skew;
+  const Given given = p.segments == 1 ? given_of(p, row, x + skew, MASK ? mask + skew : nullptr) : Given{};
   Sums a = no_sums();
   float best = -INF;
   int best_unit = 0;
@@ -295,9 +337,13 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   a = lanes_joined(a, 6, p.c);
   if ((tid & 63) == 0) sums[tid >> 6] = a;
   if constexpr (TOP) {
-    space.keys[tid] = key_of(best, (uint32_t)best_unit);
+    // the best threads of each wave, in order
+    const uint64_t mine = key_of(best, (uint32_t)best_unit);
+    uint64_t* list = space.lists + (tid >> 6) * MAX_TOP;
+    if ((tid & 63) < MAX_TOP) list[tid & 63] = 0;
+    const int rank = rank_in_wave(mine);
+    if (mine && rank < p.top) list[rank] = mine;
     if (tid == 0) space.count = 0;
-    if (tid < MAX_TOP) space.best[tid] = 0;
   }
   __syncthreads();
   a = sums[0];
@@ -306,7 +352,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   float* partial = p.partials + ((int64_t)row * p.segments + blockIdx.y) * partial_floats(p.top);
   if (tid == 0) {
     if (p.segments == 1) {
-      finish_row(p, row, a, x + skew, MASK ? mask + skew : nullptr);
+      finish_row(p, row, a, given);
     } else {
       partial[0] = a.m;
       partial[1] = a.s;
@@ -314,22 +360,15 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
     }
   }
   if constexpr (TOP) {
-    const uint64_t mine = space.keys[tid];
-    const int rank = rank_of(mine, space.keys, THREADS);
-    if (mine && rank < p.top) {
-      space.winners[rank] = (uint32_t)tid;
-      atomicMax(&space.count, rank + 1);
-    }
-    __syncthreads();
-    // the winners' units that are no worse than the last winner's best
-    const int winners = space.count;
-    const uint64_t least = winners < p.top ? 1 : space.keys[space.winners[winners - 1]];
+    merge_lists(space.lists, WAVES, MAX_TOP, p.top, space.best);
+    // of the best threads' units those no worse than the last thread's best
+    const uint64_t held = (tid & 63) < p.top ? space.best[tid & 63] : 0;
+    const int threads = __popcll(__ballot(held != 0));
+    const uint64_t least = threads < p.top ? 1 : space.best[p.top - 1];
     const int each = (end - first + THREADS - 1) / THREADS;
-    __syncthreads();
-    if (tid == 0) space.count = 0;
-    __syncthreads();
-    for (int i = tid; i < winners * each; i += THREADS) {
-      const int w = i / each, u = first + (int)space.winners[w] + (i - w * each) * THREADS;
+    for (int i = tid; i < threads * each; i += THREADS) {
+      const int w = i / each;
+      const int thread = ((int)index_of(space.best[w]) - first) % THREADS, u = first + thread + (i - w * each) * THREADS;
       if (u >= end) continue;
       float v[UNIT];
       read(u, v);
@@ -337,29 +376,29 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
       if (key >= least) space.candidates[atomicAdd(&space.count, 1)] = key;
     }
     __syncthreads();
-    // the best units among them, and their values
-    const int candidates = space.count;
+    // the best units among them, and of those the best values
+    const int candidates = space.count, units = min(candidates, p.top);
     for (int i = tid; i < candidates; i += THREADS) {
       const uint64_t key = space.candidates[i];
       const int r = rank_of(key, space.candidates, candidates);
-      if (r < p.top) space.winners[r] = index_of(key);
+      if (r < p.top) space.units[r] = index_of(key);
     }
+    if (tid < MAX_TOP) space.best[tid] = 0;
     __syncthreads();
-    const int best_units = min(candidates, p.top);
     uint64_t value = 0;
-    if (tid < best_units * UNIT) {
+    if (tid < units * UNIT) {
       float v[UNIT];
-      read((int)space.winners[tid / UNIT], v);
-      const int col = (int)space.winners[tid / UNIT] * UNIT - skew;
+      const int u = (int)space.units[tid / UNIT];
+      read(u, v);
       float one = -INF;
 #pragma unroll
       for (int j = 0; j < UNIT; ++j) one = tid % UNIT == j ? v[j] : one;
-      value = key_of(one, (uint32_t)(col + tid % UNIT));
+      value = key_of(one, (uint32_t)(u * UNIT - skew + tid % UNIT));
+      space.values[tid] = value;
     }
-    space.keys[tid] = value;
     __syncthreads();
     if (value) {
-      const int r = rank_of(value, space.keys, best_units * UNIT);
+      const int r = rank_of(value, space.values, units * UNIT);
       if (r < p.top) space.best[r] = value;
     }
     __syncthreads();
@@ -370,37 +409,52 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   }
 }
 
-// A row's segments joined, by one wave: the sums in the segments' order, the
-// best of their keys one after the other.
-template <typename T> __global__ void __launch_bounds__(64) token_join_kernel(TokenArgs p) {
+// A row's segments joined: the sums by the first wave; of the segments whose best
+// key is among the `top` best of all segments' the keys, and of those the best.
+template <typename T> __global__ void __launch_bounds__(THREADS) token_join_kernel(TokenArgs p) {
+  __shared__ uint64_t heads[MAX_SEGMENTS], lists[MAX_TOP * MAX_TOP], best[MAX_TOP];
+  __shared__ Sums sums;
+  __shared__ int from[MAX_TOP];
   const uint32_t row = blockIdx.x;
-  const int lane = threadIdx.x;
-  const float* partial = p.partials + (int64_t)row * p.segments * partial_floats(p.top);
-  Sums a = no_sums();
-  for (int s = lane; s < p.segments; s += 64) {
-    const float* q = partial + s * partial_floats(p.top);
-    a = joined(a, Sums{q[0], q[1], q[2]}, p.c);
-  }
-  a = lanes_joined(a, 6, p.c);
-  const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
-  const uint8_t* mask = p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
-  if (lane == 0) finish_row(p, row, a, x, mask);
-  const float l = __builtin_amdgcn_logf(a.s);
-  uint64_t last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    uint64_t best = 0;
-    for (int i = lane; i < p.segments * p.top; i += 64) {
-      uint64_t key;
-      __builtin_memcpy(&key, partial + (i / p.top) * partial_floats(p.top) + 4 + 2 * (i % p.top), 8);
-      best = key < last && key > best ? key : best;
+  const int tid = threadIdx.x, pitch = (int)partial_floats(p.top);
+  const float* partial = p.partials + (int64_t)row * p.segments * pitch;
+  if (tid < 64) {
+    const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+    Given given{};
+    if (tid == 0) given = given_of(p, row, x, p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr);
+    Sums a = no_sums();
+    for (int s = tid; s < p.segments; s += 64) {
+      const float* q = partial + s * pitch;
+      a = joined(a, Sums{q[0], q[1], q[2]}, p.c);
     }
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, o);
-      best = other > best ? other : best;
+    a = lanes_joined(a, 6, p.c);
+    if (tid == 0) {
+      sums = a;
+      finish_row(p, row, a, given);
     }
-    last = best;
-    if (lane == 0) write_top(p, row, k, best, a.m, l);
   }
+  if (p.top == 0) return;
+  auto key_at = [&](int segment, int place) {
+    uint64_t key;
+    __builtin_memcpy(&key, partial + segment * pitch + 4 + 2 * place, 8);
+    return key;
+  };
+  uint64_t mine = 0;
+  if (tid < p.segments) heads[tid] = mine = key_at(tid, 0);
+  if (tid < MAX_TOP) from[tid] = -1;
+  __syncthreads();
+  if (mine) {
+    const int r = rank_of(mine, heads, p.segments);
+    if (r < p.top) from[r] = tid;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.top * p.top; i += THREADS) {
+    const int segment = from[i / p.top];
+    lists[(i / p.top) * MAX_TOP + i % p.top] = segment < 0 ? 0 : key_at(segment, i % p.top);
+  }
+  __syncthreads();
+  merge_lists(lists, p.top, MAX_TOP, p.top, best);
+  if (tid < p.top) write_top(p, row, tid, best[tid], sums.m, __builtin_amdgcn_logf(sums.s));
 }
 
 // ---- backward: a workgroup takes `row_block` rows' units, or a segment of one row's
@@ -525,12 +579,14 @@ int check(const char* what, int dtype, int batch, int steps, int vocab, float te
   return PPO_OK;
 }
 
-// Parts of a wide row: as many as keep every CU busy where rows are few, of at
-// least 4096 columns.
-int segments_of(int64_t rows, int vocab) {
-  if (vocab <= NARROW) return 1;
-  const int64_t fill = std::min(ceil_div64(1024, std::max<int64_t>(rows, 1)), ceil_div64(vocab, 4096));
-  return (int)std::min<int64_t>(MAX_SEGMENTS, std::max(fill, ceil_div64(vocab, SEGMENT)));
+// Parts of a wide row, where rows are few and long: about two for each CU, of at
+// least 8192 columns (32 rows of 131072 bf16 logits, 8 alternatives: 15.7 us for
+// 19.4 in one part; 32768 columns gain nothing, 1 row 11.5 for 12.6 us, and 5000
+// lose the join's 2 to 4 us).  With alternatives no part is longer than SEGMENT.
+int segments_of(int64_t rows, int vocab, int top) {
+  if (vocab <= 32768 || rows == 0) return 1;
+  const int64_t fill = std::min(ceil_div64(512, rows), ceil_div64(vocab, 8192));
+  return (int)std::min<int64_t>(MAX_SEGMENTS, std::max(fill, top ? ceil_div64(vocab, SEGMENT) : 1));
 }
 
 TokenArgs common_args(const void* logits, const void* tokens, int wide_tokens, const uint8_t* mask,
@@ -562,7 +618,7 @@ template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
   const dim3 grid(a.rows, a.segments);
   if (a.top) hipLaunchKernelGGL((token_wide_kernel<T, true, MASK>), grid, dim3(THREADS), 0, st, a);
   else hipLaunchKernelGGL((token_wide_kernel<T, false, MASK>), grid, dim3(THREADS), 0, st, a);
-  if (a.segments > 1) hipLaunchKernelGGL((token_join_kernel<T>), dim3(a.rows), dim3(64), 0, st, a);
+  if (a.segments > 1) hipLaunchKernelGGL((token_join_kernel<T>), dim3(a.rows), dim3(a.top ? THREADS : 64), 0, st, a);
 }
 
 template <typename T, bool MASK> void launch_bwd(hipStream_t st, TokenArgs& a) {
@@ -586,7 +642,7 @@ PPO_EXPORT int ppo_token_log_probs_max_vocab(void) { return MAX_VOCAB; }
 PPO_EXPORT size_t ppo_token_log_probs_workspace(int batch, int steps, int vocab, int top) {
   if (batch <= 0 || steps <= 0 || vocab <= NARROW || vocab > MAX_VOCAB || top < 0 || top > MAX_TOP) return 0;
   const int64_t rows = (int64_t)batch * steps;
-  const int s = segments_of(rows, vocab);
+  const int s = segments_of(rows, vocab, top);
   return s > 1 ? sizeof(float) * (size_t)(4 + 2 * top) * (size_t)rows * s : 0;
 }
 
@@ -612,7 +668,7 @@ PPO_EXPORT int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logi
   a.top_log_probs = top_log_probs;
   a.top_tokens = top_tokens;
   a.partials = static_cast<float*>(workspace);
-  a.segments = segments_of(a.rows, vocab);
+  a.segments = segments_of(a.rows, vocab, top);
   a.segment_units = ceil_div(ceil_div(vocab + MAX_SKEW, UNIT), a.segments);
   if (dtype == TOKEN_F32) mask ? launch_fwd<float, true>(as_stream(stream), a) : launch_fwd<float, false>(as_stream(stream), a);
   else mask ? launch_fwd<uint16_t, true>(as_stream(stream), a) : launch_fwd<uint16_t, false>(as_stream(stream), a);
