@@ -16,8 +16,12 @@
 // mean(f u') is linear in m, so that one exchange of three sums serves both:
 //   mean(f u') = mean((dy + ry e) q post u') - m mean(ry y' q post u').
 //
+// scale and post enter y, dx and du as their product alone, and both their
+// gradients are one sum: with s = sum dx gate u', dscale = post s, dpost = scale s.
+//
 // A thread holds 8 columns of a row and their scales for all its rows; a row is
-// L lanes of a wave (up to 512 columns) or one workgroup.  Sums are float32, the
+// L lanes of a wave (up to 512 columns) or one workgroup, and the next row's
+// operands are on their way while one is formed.  Sums are float32, the
 // lanes' by butterflies, the waves' in order.
 #include "row_io.h"
 
@@ -29,11 +33,13 @@ using namespace ppo;
 
 enum NormDtype { NORM_F32 = 0, NORM_BF16 = 1 };
 
-constexpr int THREADS = 256;               // of a workgroup of narrow rows
+constexpr int THREADS = 256;               // of a workgroup of narrow rows, and of most wide ones
 constexpr int MAX_THREADS = 1024;
 constexpr int NARROW = 64 * UNIT;          // widest row of one wave's lanes
 constexpr int MAX_WIDTH = MAX_THREADS * UNIT;
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;  // most workgroups
+constexpr int FWD_WAVES = 256 * 24, BWD_WAVES = 256 * 12;   // of a launch: what the CUs hold of each
+
+enum Gate { GATE_NONE, GATE_PLAIN, GATE_SIGMOID };
 
 struct ResidualArgs {
   const void* block;
@@ -50,19 +56,14 @@ struct ResidualArgs {
   void* dblock;
   void* dgate;            // or null
   void* dresidual;
-  float* partials;        // [workgroups, 3, D]: dpost, dscale, dpre
+  float* partials;        // [workgroups, 2, D]: sum dx gate u', dpre
   RowStride block_s, gate_s, residual_s, dstream_s, dnormed_s;
   Divisor steps;
   uint32_t rows;
   int D, lanes_log2;
   float eps;
-  bool post_norm, sigmoid_gate;
+  bool post_norm;
 };
-
-__device__ __forceinline__ void load_scales(const float* p, int col, int D, float (&v)[UNIT]) {
-#pragma unroll
-  for (int j = 0; j < UNIT; ++j) v[j] = p && col + j < D ? p[col + j] : 1.f;
-}
 
 // Sums over a row: its lanes (narrow), or the workgroup, whose waves' sums
 // meet in LDS.  `slot`: another at each call until every wave has passed a
@@ -92,72 +93,101 @@ template <bool WIDE, int N> struct RowSum {
   }
 };
 
-// Which rows and columns a thread takes.
+// Which rows and columns a thread takes.  The last columns of a row that 8 does
+// not divide are the row's last 8, some of them another thread's too: those
+// (j < skip), and all of a thread past the row's end, count in no sum over the row.
 struct Place {
   uint32_t row, step;  // its first row, and from one to its next
-  int col, left;       // first column; columns from there to the row's end
+  int col, skip;
+  bool stores;
 };
 template <bool WIDE> __device__ __forceinline__ Place place_of(const ResidualArgs& p) {
   Place r;
+  int col;
   if constexpr (WIDE) {
     r.row = blockIdx.x;
     r.step = gridDim.x;
-    r.col = threadIdx.x * UNIT;
+    col = threadIdx.x * UNIT;
   } else {
     const int L = 1 << p.lanes_log2;
     r.row = (blockIdx.x * THREADS + threadIdx.x) >> p.lanes_log2;
     r.step = (gridDim.x * THREADS) >> p.lanes_log2;
-    r.col = (threadIdx.x & (L - 1)) * UNIT;
+    col = (threadIdx.x & (L - 1)) * UNIT;
   }
-  r.left = p.D - r.col;
+  r.col = max(0, min(col, p.D - UNIT));
+  r.skip = col - r.col;
+  r.stores = col < p.D;
   return r;
 }
+// A unit of a row; of rows of fewer than 8 columns what there is of it.
+template <typename S> __device__ __forceinline__ void load_part(const S* p, int D, Unit8<S>& u) {
+  if (D >= UNIT) __builtin_memcpy(u.w, p, sizeof(u.w));
+  else load_unit(p, D, u);
+}
+template <typename S> __device__ __forceinline__ void store_part(S* p, int D, const float (&v)[UNIT]) {
+  store_unit(p, min(D, UNIT), v);
+}
+__device__ __forceinline__ float scale_of(const float* p, int col, int D) { return p && col < D ? p[col] : 1.f; }
 
 template <typename T, typename R> struct Loaded {
   Unit8<T> u, g, dz;
   Unit8<R> x, dy;
+  float ru, ry;
 };
 
-template <typename T, typename R, bool BWD>
+template <int GATE, bool BWD, typename T, typename R>
 __device__ __forceinline__ void load(const ResidualArgs& p, uint32_t row, const Place& at, Loaded<T, R>& v) {
-  load_unit(static_cast<const T*>(p.block) + row_offset(row, p.steps, p.block_s) + at.col, at.left, v.u);
-  load_unit(static_cast<const R*>(p.residual) + row_offset(row, p.steps, p.residual_s) + at.col, at.left, v.x);
-  if (p.gate) load_unit(static_cast<const T*>(p.gate) + row_offset(row, p.steps, p.gate_s) + at.col, at.left, v.g);
+  load_part(static_cast<const T*>(p.block) + row_offset(row, p.steps, p.block_s) + at.col, p.D, v.u);
+  load_part(static_cast<const R*>(p.residual) + row_offset(row, p.steps, p.residual_s) + at.col, p.D, v.x);
+  if constexpr (GATE != GATE_NONE)
+    load_part(static_cast<const T*>(p.gate) + row_offset(row, p.steps, p.gate_s) + at.col, p.D, v.g);
   if constexpr (BWD) {
-    if (p.dnormed)
-      load_unit(static_cast<const T*>(p.dnormed) + row_offset(row, p.steps, p.dnormed_s) + at.col, at.left, v.dz);
-    if (p.dstream)
-      load_unit(static_cast<const R*>(p.dstream) + row_offset(row, p.steps, p.dstream_s) + at.col, at.left, v.dy);
+    // (a cotangent that is not there: the operand in its place, and zeros selected for it)
+    load_part(static_cast<const T*>(p.dnormed) + row_offset(row, p.steps, p.dnormed_s) + at.col, p.D, v.dz);
+    load_part(static_cast<const R*>(p.dstream) + row_offset(row, p.steps, p.dstream_s) + at.col, p.D, v.dy);
+    v.ru = p.stats[2 * (int64_t)row];
+    v.ry = p.stats[2 * (int64_t)row + 1];
+  }
+}
+// The gate and (sigmoid) its slope.
+template <int GATE, typename T> __device__ __forceinline__ float gate_of(const Unit8<T>& g, int j, float& slope) {
+  slope = 1.f;
+  if constexpr (GATE == GATE_NONE) return 1.f;
+  else if constexpr (GATE == GATE_PLAIN) return value(g, j);
+  else {
+    float rest;
+    const float s = sigmoid(value(g, j), rest);
+    slope = s * rest;
+    return s;
   }
 }
 
-__device__ __forceinline__ float gate_of(const ResidualArgs& p, float g) {
-  return !p.gate ? 1.f : p.sigmoid_gate ? sigmoid(g) : g;
-}
-
-template <typename T, typename R, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_fwd_kernel(ResidualArgs p) {
+template <typename T, typename R, int GATE, bool WIDE, int MOST>
+__global__ void __launch_bounds__(MOST) residual_norm_fwd_kernel(ResidualArgs p) {
   __shared__ float waves[2][MAX_THREADS / 64][1];
   const RowSum<WIDE, 1> row_sum{waves, p.lanes_log2};
   const Place at = place_of<WIDE>(p);
-  float post[UNIT], scale[UNIT], pre[UNIT];
-  load_scales(p.post, at.col, p.D, post);
-  load_scales(p.scale, at.col, p.D, scale);
-  load_scales(p.pre, at.col, p.D, pre);
+  float mix[UNIT], pre[UNIT];   // mix: post scale
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) {
+    mix[j] = scale_of(p.post, at.col + j, p.D) * scale_of(p.scale, at.col + j, p.D);
+    pre[j] = scale_of(p.pre, at.col + j, p.D);
+  }
   const float over_d = 1.f / (float)p.D;
   int slot = 0;
-  for (uint32_t row0 = at.row; __any(row0 < p.rows); row0 += at.step) {
-    const bool live = row0 < p.rows;
-    const uint32_t row = live ? row0 : p.rows - 1;   // (a wave's rows end together)
-    Loaded<T, R> v;
-    load<T, R, false>(p, row, at, v);
-    float u[UNIT], y[UNIT], ru = 1.f, sum[1];
-#pragma unroll
-    for (int j = 0; j < UNIT; ++j) u[j] = value(v.u, j);
+  Loaded<T, R> next;
+  load<GATE, false>(p, min(at.row, p.rows - 1), at, next);
+  for (uint32_t row = at.row; __any(row < p.rows); row += at.step) {   // (a wave's rows end together)
+    const Loaded<T, R> v = next;
+    load<GATE, false>(p, min(row + at.step, p.rows - 1), at, next);
+    float y[UNIT], ru = 1.f, sum[1];
     if (p.post_norm) {
       sum[0] = 0.f;
 #pragma unroll
-      for (int j = 0; j < UNIT; ++j) sum[0] = __fmaf_rn(u[j], u[j], sum[0]);
+      for (int j = 0; j < UNIT; ++j) {
+        const float u = j >= at.skip ? value(v.u, j) : 0.f;
+        sum[0] = __fmaf_rn(u, u, sum[0]);
+      }
       row_sum(sum, slot);
       slot ^= 1;
       ru = rsqrtf(__fmaf_rn(sum[0], over_d, p.eps));
@@ -165,58 +195,61 @@ __global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_fw
     sum[0] = 0.f;
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) {
-      const float q = p.gate ? scale[j] * gate_of(p, value(v.g, j)) : scale[j];
-      y[j] = __fmaf_rn(q, u[j] * ru * post[j], value(v.x, j));   // (past the row's end 0)
-      sum[0] = __fmaf_rn(y[j], y[j], sum[0]);
+      float slope;
+      y[j] = __fmaf_rn(mix[j], gate_of<GATE>(v.g, j, slope) * (value(v.u, j) * ru), value(v.x, j));
+      const float counted = j >= at.skip ? y[j] : 0.f;
+      sum[0] = __fmaf_rn(counted, counted, sum[0]);
     }
     row_sum(sum, slot);
     slot ^= 1;
     const float ry = rsqrtf(__fmaf_rn(sum[0], over_d, p.eps));
-    if (!live) continue;
+    if (row >= p.rows || !at.stores) continue;
     const int64_t out = (int64_t)row * p.D + at.col;
-    store_unit(static_cast<R*>(p.stream) + out, at.left, y);
+    store_part(static_cast<R*>(p.stream) + out, p.D, y);
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) y[j] = y[j] * ry * pre[j];
-    store_unit(static_cast<T*>(p.normed) + out, at.left, y);
-    if (p.stats && at.col == 0) {
+    store_part(static_cast<T*>(p.normed) + out, p.D, y);
+    if (p.stats && at.col + at.skip == 0) {
       p.stats[2 * (int64_t)row] = ru;
       p.stats[2 * (int64_t)row + 1] = ry;
     }
   }
 }
 
-template <typename T, typename R, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_bwd_kernel(ResidualArgs p) {
+template <typename T, typename R, int GATE, bool WIDE, int MOST>
+__global__ void __launch_bounds__(MOST) residual_norm_bwd_kernel(ResidualArgs p, bool has_dstream, bool has_dnormed) {
   __shared__ float waves[2][MAX_THREADS / 64][3];
   const RowSum<WIDE, 3> row_sum{waves, p.lanes_log2};
   const Place at = place_of<WIDE>(p);
-  float post[UNIT], scale[UNIT], pre[UNIT], dpost[UNIT], dscale[UNIT], dpre[UNIT];
-  load_scales(p.post, at.col, p.D, post);
-  load_scales(p.scale, at.col, p.D, scale);
-  load_scales(p.pre, at.col, p.D, pre);
+  float mix[UNIT], pre[UNIT], dmix[UNIT], dpre[UNIT];
 #pragma unroll
-  for (int j = 0; j < UNIT; ++j) dpost[j] = dscale[j] = dpre[j] = 0.f;
+  for (int j = 0; j < UNIT; ++j) {
+    mix[j] = scale_of(p.post, at.col + j, p.D) * scale_of(p.scale, at.col + j, p.D);
+    pre[j] = scale_of(p.pre, at.col + j, p.D);
+    dmix[j] = dpre[j] = 0.f;
+  }
   const float over_d = 1.f / (float)p.D;
   int slot = 0;
-  for (uint32_t row0 = at.row; __any(row0 < p.rows); row0 += at.step) {
-    const bool live = row0 < p.rows;
-    const uint32_t row = live ? row0 : p.rows - 1;
-    Loaded<T, R> v;
-    load<T, R, true>(p, row, at, v);
-    const float ru = p.stats[2 * (int64_t)row], ry = p.stats[2 * (int64_t)row + 1];
-    // (columns past the row's end have u = x = dz = dy = 0)
-    float un[UNIT], q[UNIT], yn[UNIT], e[UNIT], dx[UNIT], sum[3] = {0.f, 0.f, 0.f};
+  Loaded<T, R> next;
+  load<GATE, true>(p, min(at.row, p.rows - 1), at, next);
+  for (uint32_t row = at.row; __any(row < p.rows); row += at.step) {
+    const Loaded<T, R> v = next;
+    load<GATE, true>(p, min(row + at.step, p.rows - 1), at, next);
+    const bool live = row < p.rows;
+    const float ru = v.ru, ry = v.ry;
+    // un = u', gun = gate u', yn = y'
+    float un[UNIT], gun[UNIT], yn[UNIT], dx[UNIT], sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) {
-      q[j] = p.gate ? scale[j] * gate_of(p, value(v.g, j)) : scale[j];
+      float slope;
       un[j] = value(v.u, j) * ru;
-      yn[j] = __fmaf_rn(q[j], un[j] * post[j], value(v.x, j)) * ry;
-      const float dz = p.dnormed ? value(v.dz, j) : 0.f;
-      if (live) dpre[j] = __fmaf_rn(dz, yn[j], dpre[j]);
-      e[j] = dz * pre[j];
-      dx[j] = __fmaf_rn(ry, e[j], p.dstream ? value(v.dy, j) : 0.f);
-      sum[0] = __fmaf_rn(e[j], yn[j], sum[0]);
-      const float k = q[j] * post[j] * un[j];
+      gun[j] = gate_of<GATE>(v.g, j, slope) * un[j];
+      yn[j] = __fmaf_rn(mix[j], gun[j], value(v.x, j)) * ry;
+      const float dz = has_dnormed ? value(v.dz, j) : 0.f, e = dz * pre[j];
+      if (WIDE || live) dpre[j] = __fmaf_rn(dz, yn[j], dpre[j]);
+      dx[j] = __fmaf_rn(ry, e, has_dstream ? value(v.dy, j) : 0.f);
+      const float k = j >= at.skip ? mix[j] * gun[j] : 0.f;
+      sum[0] = __fmaf_rn(j >= at.skip ? e : 0.f, yn[j], sum[0]);
       sum[1] = __fmaf_rn(dx[j], k, sum[1]);
       sum[2] = __fmaf_rn(yn[j], k, sum[2]);
     }
@@ -227,46 +260,45 @@ __global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_bw
     float du[UNIT], dg[UNIT];
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) {
+      float slope;
+      const float gate = gate_of<GATE>(v.g, j, slope);
       dx[j] = __fmaf_rn(-yn[j], m, dx[j]);
-      float rest = 1.f;
-      const float gate = !p.gate ? 1.f : p.sigmoid_gate ? sigmoid(value(v.g, j), rest) : value(v.g, j);
-      const float n = un[j] * post[j], dn = dx[j] * q[j];
-      if (live) {
-        dscale[j] = __fmaf_rn(dx[j], gate * n, dscale[j]);
-        dpost[j] = __fmaf_rn(dn, un[j], dpost[j]);
-      }
-      dg[j] = dx[j] * scale[j] * n * (p.sigmoid_gate ? gate * rest : 1.f);
-      du[j] = ru * __fmaf_rn(-un[j], mu, dn * post[j]);
+      if (WIDE || live) dmix[j] = __fmaf_rn(dx[j], gun[j], dmix[j]);
+      const float dn = dx[j] * mix[j];
+      dg[j] = dn * un[j] * slope;
+      du[j] = ru * __fmaf_rn(-un[j], mu, dn * gate);
     }
-    if (!live) continue;
+    if (!live || !at.stores) continue;
     const int64_t out = (int64_t)row * p.D + at.col;
-    store_unit(static_cast<R*>(p.dresidual) + out, at.left, dx);
-    store_unit(static_cast<T*>(p.dblock) + out, at.left, du);
-    if (p.dgate) store_unit(static_cast<T*>(p.dgate) + out, at.left, dg);
+    store_part(static_cast<R*>(p.dresidual) + out, p.D, dx);
+    store_part(static_cast<T*>(p.dblock) + out, p.D, du);
+    if constexpr (GATE != GATE_NONE) {
+      if (p.dgate) store_part(static_cast<T*>(p.dgate) + out, p.D, dg);
+    }
   }
   if (!p.partials) return;
-  float* mine = p.partials + (int64_t)blockIdx.x * 3 * p.D;
+  float* mine = p.partials + (int64_t)blockIdx.x * 2 * p.D;
   if constexpr (WIDE) {
+    if (!at.stores) return;
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) {
-      if (j >= at.left) break;
-      mine[at.col + j] = dpost[j];
-      mine[p.D + at.col + j] = dscale[j];
-      mine[2 * p.D + at.col + j] = dpre[j];
+      mine[at.col + j] = dmix[j];
+      mine[p.D + at.col + j] = dpre[j];
     }
   } else {
     // the rows of the workgroup side by side, added in their order
     __shared__ float sums[THREADS * UNIT];
     const int L = 1 << p.lanes_log2;
 #pragma unroll
-    for (int w = 0; w < 3; ++w) {
+    for (int w = 0; w < 2; ++w) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < UNIT; ++j) sums[j * THREADS + threadIdx.x] = w == 0 ? dpost[j] : w == 1 ? dscale[j] : dpre[j];
+      for (int j = 0; j < UNIT; ++j) sums[j * THREADS + threadIdx.x] = w == 0 ? dmix[j] : dpre[j];
       __syncthreads();
       for (int c = threadIdx.x; c < p.D; c += THREADS) {
+        const int lane = c / UNIT, place = c - max(0, min(lane * UNIT, p.D - UNIT));
         float s = 0.f;
-        for (int g = c / UNIT; g < THREADS; g += L) s += sums[(c % UNIT) * THREADS + g];
+        for (int g = lane; g < THREADS; g += L) s += sums[place * THREADS + g];
         mine[w * p.D + c] = s;
       }
     }
@@ -276,29 +308,33 @@ __global__ void __launch_bounds__(WIDE ? MAX_THREADS : THREADS) residual_norm_bw
 // The scales' gradients from the workgroups' sums: 64 columns a workgroup, each
 // wave its share of the sums in their order, then the waves'.
 __global__ void __launch_bounds__(1024) residual_norm_scale_kernel(const float* partials, int blocks, int D,
+                                                                   const float* post, const float* scale,
                                                                    float* dpost, float* dscale, float* dpre) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
   const int share = (blocks + 15) / 16, b1 = min(blocks, (wave + 1) * share);
   float s = 0.f;
-  if (i < 3 * D) {
+  if (i < 2 * D) {
     for (int b0 = wave * share; b0 < b1; b0 += 8) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = partials[(int64_t)min(b0 + k, b1 - 1) * 3 * D + i];
+      for (int k = 0; k < 8; ++k) v[k] = partials[(int64_t)min(b0 + k, b1 - 1) * 2 * D + i];
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += b0 + k < b1 ? v[k] : 0.f;
     }
   }
   sums[wave][lane] = s;
   __syncthreads();
-  if (wave > 0 || i >= 3 * D) return;
+  if (wave > 0 || i >= 2 * D) return;
   s = 0.f;
 #pragma unroll
   for (int w = 0; w < 16; ++w) s += sums[w][lane];
-  const int which = i / D, col = i - which * D;
-  float* out = which == 0 ? dpost : which == 1 ? dscale : dpre;
-  if (out) out[col] = s;
+  if (i >= D) {
+    if (dpre) dpre[i - D] = s;
+  } else {
+    if (dpost) dpost[i] = scale ? scale[i] * s : s;
+    if (dscale) dscale[i] = post ? post[i] * s : s;
+  }
 }
 
 // ---- launches
@@ -308,17 +344,17 @@ int lanes_log2_of(int D) {
   return log2;
 }
 
-// Threads and most useful workgroups of a launch.
+// Threads and workgroups of a launch.
 struct Shape {
   bool wide;
   unsigned threads, blocks;
 };
-Shape shape_of(int64_t rows, int D, int most) {
+Shape shape_of(int64_t rows, int D, int waves) {
   Shape s;
   s.wide = D > NARROW;
   s.threads = s.wide ? (unsigned)(64 * ceil_div(D, NARROW)) : THREADS;
   const int64_t at_once = s.wide ? 1 : THREADS >> lanes_log2_of(D);
-  s.blocks = (unsigned)std::min<int64_t>(most, ceil_div64(rows, at_once));
+  s.blocks = (unsigned)std::min<int64_t>(waves * 64 / s.threads, ceil_div64(rows, at_once));
   return s;
 }
 
@@ -334,8 +370,8 @@ int check(const char* what, int dtype, int stream_dtype, int batch, int steps, i
 }
 
 ResidualArgs common_args(const void* block, const void* gate, const void* residual, const int64_t* strides,
-                         const float* post, const float* scale, const float* pre, int post_norm, int gate_sigmoid,
-                         float epsilon, int batch, int steps, int width) {
+                         const float* post, const float* scale, const float* pre, int post_norm, float epsilon, int batch,
+                         int steps, int width) {
   ResidualArgs a{};
   a.block = block;
   a.gate = gate;
@@ -352,25 +388,44 @@ ResidualArgs common_args(const void* block, const void* gate, const void* residu
   a.lanes_log2 = width <= NARROW ? lanes_log2_of(width) : 0;
   a.eps = epsilon;
   a.post_norm = post_norm != 0;
-  a.sigmoid_gate = gate && gate_sigmoid;
   return a;
 }
 
-template <typename T, typename R, bool BWD> void launch(hipStream_t st, const ResidualArgs& a, const Shape& s) {
+template <typename T, typename R, int GATE, bool WIDE, int MOST>
+void launch_shape(hipStream_t st, ResidualArgs a, const Shape& s, bool backward) {
   const dim3 g(s.blocks), t(s.threads);
-  if constexpr (BWD) {
-    if (s.wide) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, R, true>), g, t, 0, st, a);
-    else hipLaunchKernelGGL((residual_norm_bwd_kernel<T, R, false>), g, t, 0, st, a);
+  if (backward) {
+    const bool dstream = a.dstream, dnormed = a.dnormed;
+    if (!dstream) {
+      a.dstream = a.residual;
+      a.dstream_s = a.residual_s;
+    }
+    if (!dnormed) {
+      a.dnormed = a.block;
+      a.dnormed_s = a.block_s;
+    }
+    hipLaunchKernelGGL((residual_norm_bwd_kernel<T, R, GATE, WIDE, MOST>), g, t, 0, st, a, dstream, dnormed);
   } else {
-    if (s.wide) hipLaunchKernelGGL((residual_norm_fwd_kernel<T, R, true>), g, t, 0, st, a);
-    else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, R, false>), g, t, 0, st, a);
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, R, GATE, WIDE, MOST>), g, t, 0, st, a);
   }
 }
-template <bool BWD>
-void launch_typed(hipStream_t st, const ResidualArgs& a, const Shape& s, int dtype, int stream_dtype) {
-  if (dtype == NORM_F32) launch<float, float, BWD>(st, a, s);
-  else if (stream_dtype == NORM_F32) launch<uint16_t, float, BWD>(st, a, s);
-  else launch<uint16_t, uint16_t, BWD>(st, a, s);
+template <typename T, typename R, int GATE>
+void launch_gate(hipStream_t st, const ResidualArgs& a, const Shape& s, bool backward) {
+  if (!s.wide) launch_shape<T, R, GATE, false, THREADS>(st, a, s, backward);
+  else if (s.threads <= THREADS) launch_shape<T, R, GATE, true, THREADS>(st, a, s, backward);
+  else launch_shape<T, R, GATE, true, MAX_THREADS>(st, a, s, backward);
+}
+template <typename T, typename R>
+void launch(hipStream_t st, const ResidualArgs& a, const Shape& s, int gate_sigmoid, bool backward) {
+  if (!a.gate) launch_gate<T, R, GATE_NONE>(st, a, s, backward);
+  else if (gate_sigmoid) launch_gate<T, R, GATE_SIGMOID>(st, a, s, backward);
+  else launch_gate<T, R, GATE_PLAIN>(st, a, s, backward);
+}
+void launch_typed(hipStream_t st, const ResidualArgs& a, const Shape& s, int gate_sigmoid, bool backward, int dtype,
+                  int stream_dtype) {
+  if (dtype == NORM_F32) launch<float, float>(st, a, s, gate_sigmoid, backward);
+  else if (stream_dtype == NORM_F32) launch<uint16_t, float>(st, a, s, gate_sigmoid, backward);
+  else launch<uint16_t, uint16_t>(st, a, s, gate_sigmoid, backward);
 }
 
 }  // namespace
@@ -387,17 +442,17 @@ PPO_EXPORT int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, 
   if ((int64_t)batch * steps == 0 || width == 0) return PPO_OK;
   if (!block || !residual || !strides || !stream_out || !normed) return set_error(PPO_ERR_ARG, "%s: null buffer", what);
   ResidualArgs a = common_args(block, gate, residual, strides, post_scale, residual_scale, pre_scale, post_norm,
-                               gate_sigmoid, epsilon, batch, steps, width);
+                               epsilon, batch, steps, width);
   a.stream = stream_out;
   a.normed = normed;
   a.stats = stats;
-  launch_typed<false>(as_stream(stream), a, shape_of(a.rows, width, FWD_BLOCKS), dtype, stream_dtype);
+  launch_typed(as_stream(stream), a, shape_of(a.rows, width, FWD_WAVES), gate_sigmoid, false, dtype, stream_dtype);
   return check_launch(what);
 }
 
 PPO_EXPORT size_t ppo_residual_norm_bwd_workspace(int batch, int steps, int width) {
   if (batch <= 0 || steps <= 0 || width <= 0 || width > MAX_WIDTH) return 0;
-  return sizeof(float) * 3 * (size_t)width * shape_of((int64_t)batch * steps, width, BWD_BLOCKS).blocks;
+  return sizeof(float) * 2 * (size_t)width * shape_of((int64_t)batch * steps, width, BWD_WAVES).blocks;
 }
 
 PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block,
@@ -419,7 +474,7 @@ PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, 
   unsigned blocks = 0;
   if (!none) {
     ResidualArgs a = common_args(block, gate, residual, strides, post_scale, residual_scale, pre_scale, post_norm,
-                                 gate_sigmoid, 0.f, batch, steps, width);
+                                 0.f, batch, steps, width);
     a.stats = const_cast<float*>(stats);
     a.dstream = dstream;
     a.dnormed = dnormed;
@@ -429,13 +484,13 @@ PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, 
     a.dgate = gate ? dgate : nullptr;
     a.dresidual = dresidual;
     a.partials = scales ? static_cast<float*>(workspace) : nullptr;
-    const Shape s = shape_of(a.rows, width, BWD_BLOCKS);
+    const Shape s = shape_of(a.rows, width, BWD_WAVES);
     blocks = s.blocks;
-    launch_typed<true>(as_stream(stream), a, s, dtype, stream_dtype);
+    launch_typed(as_stream(stream), a, s, gate_sigmoid, true, dtype, stream_dtype);
   }
   if (scales)
-    hipLaunchKernelGGL(residual_norm_scale_kernel, dim3((unsigned)ceil_div(3 * width, 64)), dim3(1024), 0,
-                       as_stream(stream), static_cast<const float*>(workspace), (int)blocks, width, dpost_scale,
-                       dresidual_scale, dpre_scale);
+    hipLaunchKernelGGL(residual_norm_scale_kernel, dim3((unsigned)ceil_div(2 * width, 64)), dim3(1024), 0,
+                       as_stream(stream), static_cast<const float*>(workspace), (int)blocks, width, post_scale,
+                       residual_scale, dpost_scale, dresidual_scale, dpre_scale);
   return check_launch(what);
 }
