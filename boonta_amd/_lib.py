@@ -93,7 +93,7 @@ SIGNATURES = {
     "ppo_qk_norm_rotary_bwd": (I, [P, I, P, P, P, P, P, P, P, P, P, F, I, P, P, P, P, P, SZ, I, I, I, I, I, I]),
     "ppo_residual_norm_max_width": (I, []),
     "ppo_residual_norm_fwd": (I, [P, I, I, P, P, P, P, P, P, P, I, I, F, P, P, P, I, I, I]),
-    "ppo_residual_norm_bwd_workspace": (SZ, [I, I, I]),
+    "ppo_residual_norm_bwd_workspace": (SZ, [I, I, I, I]),
     "ppo_residual_norm_bwd": (I, [P, I, I, P, P, P, P, P, P, P, P, P, I, I, P, P, P, P, P, P, P, P, SZ, I, I, I]),
     "ppo_token_log_probs_max_top": (I, []),
     "ppo_token_log_probs_max_vocab": (I, []),

@@ -37,7 +37,11 @@ constexpr int THREADS = 256;               // of a workgroup of narrow rows, and
 constexpr int MAX_THREADS = 1024;
 constexpr int NARROW = 64 * UNIT;          // widest row of one wave's lanes
 constexpr int MAX_WIDTH = MAX_THREADS * UNIT;
-constexpr int FWD_WAVES = 256 * 24, BWD_WAVES = 256 * 12;   // of a launch: what the CUs hold of each
+// Waves of a launch, a row or part of one each at a time.  The backward's, 67M
+// elements, both passes: 8 a CU for 12, 2048 bf16 columns 357 us for 369, 640 float32
+// 833 for 899, but 640 bf16 404 for 385; 16 and 6 are behind one or the other.
+constexpr int FWD_WAVES = 256 * 24;
+int bwd_waves(int dtype, int D) { return 256 * (dtype == NORM_BF16 && D <= 768 ? 12 : 8); }
 
 enum Gate { GATE_NONE, GATE_PLAIN, GATE_SIGMOID };
 
@@ -230,11 +234,14 @@ __global__ void __launch_bounds__(MOST) residual_norm_bwd_kernel(ResidualArgs p,
   }
   const float over_d = 1.f / (float)p.D;
   int slot = 0;
+  // (16 waves leave no registers for a next row: 8192 bf16 columns 396 us for 512)
+  constexpr bool AHEAD = MOST <= 512;
   Loaded<T, R> next;
-  load<GATE, true>(p, min(at.row, p.rows - 1), at, next);
+  if constexpr (AHEAD) load<GATE, true>(p, min(at.row, p.rows - 1), at, next);
   for (uint32_t row = at.row; __any(row < p.rows); row += at.step) {
+    if constexpr (!AHEAD) load<GATE, true>(p, min(row, p.rows - 1), at, next);
     const Loaded<T, R> v = next;
-    load<GATE, true>(p, min(row + at.step, p.rows - 1), at, next);
+    if constexpr (AHEAD) load<GATE, true>(p, min(row + at.step, p.rows - 1), at, next);
     const bool live = row < p.rows;
     const float ru = v.ru, ry = v.ry;
     // un = u', gun = gate u', yn = y'
@@ -305,17 +312,18 @@ __global__ void __launch_bounds__(MOST) residual_norm_bwd_kernel(ResidualArgs p,
   }
 }
 
-// The scales' gradients from the workgroups' sums: 64 columns a workgroup, each
-// wave its share of the sums in their order, then the waves'.
-__global__ void __launch_bounds__(1024) residual_norm_scale_kernel(const float* partials, int blocks, int D,
-                                                                   const float* post, const float* scale,
-                                                                   float* dpost, float* dscale, float* dpre) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
-  const int share = (blocks + 15) / 16, b1 = min(blocks, (wave + 1) * share);
+// The scales' gradients from the workgroups' sums: 16 columns a workgroup, 64
+// shares of the sums, each in their order, then the shares' by a tree.
+constexpr int SUM_COLUMNS = 16, SUM_SHARES = 64;
+__global__ void __launch_bounds__(SUM_COLUMNS* SUM_SHARES)
+    residual_norm_scale_kernel(const float* partials, int blocks, int D, const float* post, const float* scale,
+                               float* dpost, float* dscale, float* dpre) {
+  __shared__ float sums[SUM_SHARES][SUM_COLUMNS];
+  const int c = threadIdx.x % SUM_COLUMNS, share = threadIdx.x / SUM_COLUMNS, i = blockIdx.x * SUM_COLUMNS + c;
+  const int each = (blocks + SUM_SHARES - 1) / SUM_SHARES, b1 = min(blocks, (share + 1) * each);
   float s = 0.f;
   if (i < 2 * D) {
-    for (int b0 = wave * share; b0 < b1; b0 += 8) {
+    for (int b0 = share * each; b0 < b1; b0 += 8) {
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = partials[(int64_t)min(b0 + k, b1 - 1) * 2 * D + i];
@@ -323,12 +331,13 @@ __global__ void __launch_bounds__(1024) residual_norm_scale_kernel(const float* 
       for (int k = 0; k < 8; ++k) s += b0 + k < b1 ? v[k] : 0.f;
     }
   }
-  sums[wave][lane] = s;
-  __syncthreads();
-  if (wave > 0 || i >= 2 * D) return;
-  s = 0.f;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) s += sums[w][lane];
+  sums[share][c] = s;
+  for (int half = SUM_SHARES / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (share < half) sums[share][c] += sums[share + half][c];
+  }
+  if (share > 0 || i >= 2 * D) return;
+  s = sums[0][c];
   if (i >= D) {
     if (dpre) dpre[i - D] = s;
   } else {
@@ -413,6 +422,7 @@ template <typename T, typename R, int GATE>
 void launch_gate(hipStream_t st, const ResidualArgs& a, const Shape& s, bool backward) {
   if (!s.wide) launch_shape<T, R, GATE, false, THREADS>(st, a, s, backward);
   else if (s.threads <= THREADS) launch_shape<T, R, GATE, true, THREADS>(st, a, s, backward);
+  else if (s.threads <= 512) launch_shape<T, R, GATE, true, 512>(st, a, s, backward);
   else launch_shape<T, R, GATE, true, MAX_THREADS>(st, a, s, backward);
 }
 template <typename T, typename R>
@@ -450,9 +460,9 @@ PPO_EXPORT int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, 
   return check_launch(what);
 }
 
-PPO_EXPORT size_t ppo_residual_norm_bwd_workspace(int batch, int steps, int width) {
+PPO_EXPORT size_t ppo_residual_norm_bwd_workspace(int dtype, int batch, int steps, int width) {
   if (batch <= 0 || steps <= 0 || width <= 0 || width > MAX_WIDTH) return 0;
-  return sizeof(float) * 2 * (size_t)width * shape_of((int64_t)batch * steps, width, BWD_WAVES).blocks;
+  return sizeof(float) * 2 * (size_t)width * shape_of((int64_t)batch * steps, width, bwd_waves(dtype, width)).blocks;
 }
 
 PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block,
@@ -468,7 +478,7 @@ PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, 
   const bool none = (int64_t)batch * steps == 0, scales = dpost_scale || dresidual_scale || dpre_scale;
   if (!none && (!block || !residual || !strides || !stats || !dblock || !dresidual))
     return set_error(PPO_ERR_ARG, "%s: null buffer", what);
-  const size_t need = scales ? ppo_residual_norm_bwd_workspace(batch, steps, width) : 0;
+  const size_t need = scales ? ppo_residual_norm_bwd_workspace(dtype, batch, steps, width) : 0;
   if (need && (!workspace || workspace_bytes < need))
     return set_error(PPO_ERR_SPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   unsigned blocks = 0;
@@ -484,12 +494,13 @@ PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, 
     a.dgate = gate ? dgate : nullptr;
     a.dresidual = dresidual;
     a.partials = scales ? static_cast<float*>(workspace) : nullptr;
-    const Shape s = shape_of(a.rows, width, BWD_WAVES);
+    const Shape s = shape_of(a.rows, width, bwd_waves(dtype, width));
     blocks = s.blocks;
     launch_typed(as_stream(stream), a, s, gate_sigmoid, true, dtype, stream_dtype);
   }
   if (scales)
-    hipLaunchKernelGGL(residual_norm_scale_kernel, dim3((unsigned)ceil_div(2 * width, 64)), dim3(1024), 0,
+    hipLaunchKernelGGL(residual_norm_scale_kernel, dim3((unsigned)ceil_div(2 * width, SUM_COLUMNS)),
+                       dim3(SUM_COLUMNS * SUM_SHARES), 0,
                        as_stream(stream), static_cast<const float*>(workspace), (int)blocks, width, post_scale,
                        residual_scale, dpost_scale, dresidual_scale, dpre_scale);
   return check_launch(what);

@@ -138,7 +138,7 @@ __device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
   return a;
 }
 
-// The row's token, read ahead of the sums: its logit where it is one that is allowed.
+// The row's token: its logit where it is one that is allowed.
 struct Given {
   bool token;
   float logit;   // -inf: not allowed
@@ -292,7 +292,6 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   const int end = min((p.V + skew + UNIT - 1) / UNIT, first + p.segment_units), whole = min(end, (p.V + skew) / UNIT);
   x -= skew;   // (columns in the units' count from here on; those before the row are not read)
   if constexpr (MASK) mask -= skew;
-  const Given given = p.segments == 1 ? given_of(p, row, x + skew, MASK ? mask + skew : nullptr) : Given{};
   Sums a = no_sums();
   float best = -INF;
   int best_unit = 0;
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(THREADS) token_wide_kernel(TokenArgs p) {
   float* partial = p.partials + ((int64_t)row * p.segments + blockIdx.y) * partial_floats(p.top);
   if (tid == 0) {
     if (p.segments == 1) {
-      finish_row(p, row, a, given);
+      finish_row(p, row, a, given_of(p, row, x + skew, MASK ? mask + skew : nullptr));
     } else {
       partial[0] = a.m;
       partial[1] = a.s;

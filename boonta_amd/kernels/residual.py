@@ -66,7 +66,7 @@ class _ResidualNorm(torch.autograd.Function):
                    for x, need in zip(scales, ctx.needs_input_grad[3:6])]
         nbytes, work = 0, None
         if any(x is not None for x in dscales):
-            nbytes = _lib.load().ppo_residual_norm_bwd_workspace(batch, steps, width)
+            nbytes = _lib.load().ppo_residual_norm_bwd_workspace(_DTYPES[block.dtype], batch, steps, width)
             work = torch.empty(nbytes // 4, dtype=torch.float32, device=block.device)
         _launch(block.get_device(), "ppo_residual_norm_bwd", _DTYPES[block.dtype], _DTYPES[residual.dtype],
                 block.data_ptr(), residual.data_ptr(), _ptr(gate), _ptr(dstream), _ptr(dnormed),

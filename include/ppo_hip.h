@@ -496,7 +496,7 @@ int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, const void*
 /* From the cotangents of stream_out and normed (either NULL: zeros; strides: 2
  * more for each): dblock, dresidual and dgate (may be NULL) contiguous, typed as
  * their values; the scales' gradients float [width] (may be NULL). */
-size_t ppo_residual_norm_bwd_workspace(int batch, int steps, int width);
+size_t ppo_residual_norm_bwd_workspace(int dtype, int batch, int steps, int width);
 int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block, const void* residual,
                           const void* gate, const void* dstream, const void* dnormed, const int64_t* strides,
                           const float* post_scale, const float* residual_scale, const float* pre_scale, int post_norm,
