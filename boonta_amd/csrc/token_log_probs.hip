@@ -187,21 +187,44 @@ __device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int 
 }
 
 // ---- rows of up to 512 columns: lanes of a wave
+// Unit u of a narrow row: the row's last 8 columns where it would pass the end,
+// the first `skip` of them in the unit before too (all 8 or more past the end).
+struct Span {
+  int col, skip;
+};
+__device__ __forceinline__ Span span_of(int u, int V) {
+  const int col = max(0, min(u * UNIT, V - UNIT));
+  return Span{col, u * UNIT - col};
+}
+template <bool MASK, typename T>
+__device__ __forceinline__ void read_span(const T* x, const uint8_t* mask, const Span& at, int V, float (&v)[UNIT]) {
+  if (V >= UNIT) {
+    Unit8<T> raw;
+    __builtin_memcpy(raw.w, x + at.col, sizeof(raw.w));
+    uint64_t allowed = 0;
+    if constexpr (MASK) __builtin_memcpy(&allowed, mask + at.col, 8);
+    unit_values<MASK>(raw, allowed, v);
+  } else {
+    read_unit<MASK>(x, mask, 0, V, v);
+  }
+}
+
 template <typename T, bool TOP, bool MASK>
 __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
-  const int L = 1 << p.lanes_log2, lane = threadIdx.x & (L - 1), col = lane * UNIT;
+  const int L = 1 << p.lanes_log2, lane = threadIdx.x & (L - 1);
+  const Span at = span_of(lane, p.V);
   const uint32_t step = (gridDim.x * THREADS) >> p.lanes_log2;
   for (uint32_t row0 = (blockIdx.x * THREADS + threadIdx.x) >> p.lanes_log2; __any(row0 < p.rows); row0 += step) {
     const bool live = row0 < p.rows;
     const uint32_t row = live ? row0 : p.rows - 1;
     const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
     const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
-    float v[UNIT];
-#pragma unroll
-    for (int j = 0; j < UNIT; ++j) v[j] = -INF;
     Given given{};
     if (lane == 0) given = given_of(p, row, x, mask);
-    if (col < p.V) read_unit<MASK>(x, mask, col, p.V, v);
+    float v[UNIT];
+    read_span<MASK>(x, mask, at, p.V, v);
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) v[j] = j >= at.skip ? v[j] : -INF;
     Sums a = no_sums();
     add_unit(a, v, max8(v), p.c);
     a = lanes_joined(a, p.lanes_log2, p.c);
@@ -213,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
         uint64_t best = 0;
 #pragma unroll
         for (int j = 0; j < UNIT; ++j) {
-          const uint64_t key = key_of(v[j], (uint32_t)(col + j));
+          const uint64_t key = key_of(v[j], (uint32_t)(at.col + j));
           best = key < last && key > best ? key : best;
         }
         for (int o = 1; o < L; o <<= 1) {
@@ -500,20 +523,22 @@ __device__ __forceinline__ void unit_gradient(const RowGradient& r, float c, int
   for (int j = 0; j < UNIT; ++j) v[j] = d[j];
 }
 
+// Rows of up to 2048 columns: several side by side, their scalars formed once in LDS.
+constexpr int MAX_ROW_BLOCK = 256;
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_bwd_kernel(TokenArgs p) {
-  // rows of few units: several rows side by side
-  const uint32_t units = p.units.d;
-  for (uint32_t row0 = blockIdx.x * p.row_block; row0 < p.rows; row0 += gridDim.x * p.row_block) {
-    const uint32_t count = min((uint32_t)p.row_block, p.rows - row0) * units;
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-      const uint32_t q = quotient(i, p.units), row = row0 + q;
-      const int col = (int)(i - q * units) * UNIT;
-      const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
-      float v[UNIT];
-      read_unit<MASK>(x, MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr, col, p.V, v);
-      unit_gradient(row_gradient(p, row), p.c, col, v);
-      store_unit(static_cast<T*>(p.dlogits) + (int64_t)row * p.V + col, p.V - col, v);
-    }
+  __shared__ RowGradient scalars[MAX_ROW_BLOCK];
+  const uint32_t units = p.units.d, row0 = blockIdx.x * p.row_block;
+  const uint32_t rows = min((uint32_t)p.row_block, p.rows - row0), count = rows * units;
+  if (threadIdx.x < rows) scalars[threadIdx.x] = row_gradient(p, row0 + threadIdx.x);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+    const uint32_t q = quotient(i, p.units), row = row0 + q;
+    const Span at = span_of((int)(i - q * units), p.V);
+    float v[UNIT];
+    read_span<MASK>(static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s),
+                    MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr, at, p.V, v);
+    unit_gradient(scalars[q], p.c, at.col, v);
+    store_unit(static_cast<T*>(p.dlogits) + (int64_t)row * p.V + at.col, min(p.V, UNIT), v);
   }
 }
 
@@ -622,11 +647,11 @@ template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
 
 template <typename T, bool MASK> void launch_bwd(hipStream_t st, TokenArgs& a) {
   const int units = (int)a.units.d;
-  a.row_block = std::max(1, 2 * THREADS / units);
+  a.row_block = std::min(MAX_ROW_BLOCK, std::max(1, 4 * THREADS / units));
   const int most = ceil_div(a.V + MAX_SKEW, UNIT);
   const int segments = ceil_div(most, 8 * THREADS);
   a.segment_units = ceil_div(most, segments);
-  if (a.row_block > 1)
+  if (units <= THREADS)
     hipLaunchKernelGGL((token_bwd_kernel<T, MASK>), dim3((unsigned)ceil_div64(a.rows, a.row_block)), dim3(THREADS), 0, st, a);
   else
     hipLaunchKernelGGL((token_bwd_wide_kernel<T, MASK>), dim3(a.rows, (unsigned)segments), dim3(THREADS), 0, st,

@@ -29,9 +29,12 @@ from .. import _lib
 from .attention import _DTYPES, _launch, _near_rows, _no_tangents, _on_device, _ptr, _rows
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (3, 6, 8)}
+
+
 def _strides(*tensors):
     flat = [s for x in tensors for s in x.stride()[:-1]]
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
 
 
 def _check(name, x, input_gate, decay_gate, rate, carry, done, dims):

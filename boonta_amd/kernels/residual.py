@@ -26,9 +26,12 @@ from .attention import _DTYPES, _launch, _no_tangents, _on_device, _ptr, _rows
 _max_width = 0
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (6, 10)}
+
+
 def _strides(*tensors):
     flat = [s for x in tensors for s in ((0, 0) if x is None else x.stride()[:2])]
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
 
 
 def _forward(block, residual, gate, post_scale, residual_scale, pre_scale, options, keep):

@@ -34,12 +34,15 @@ class TokenLogProbs(NamedTuple):
     top_tokens: torch.Tensor | None = None
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (4, 8)}
+
+
 def _strides(dims, *tensors):
     flat = []
     for x in tensors:
         s = (0, 0) if x is None else x.stride()[:dims]
         flat += s if dims == 2 else (s[0], 0)
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
 
 
 def _forward(logits, tokens, mask, temperature, top, keep):
