@@ -17,6 +17,7 @@
 #include "row_io.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -25,12 +26,15 @@ using namespace ppo;
 enum TokenDtype { TOKEN_F32 = 0, TOKEN_BF16 = 1 };
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-constexpr int NARROW = 64 * UNIT;       // widest row of one wave's lanes
+// Widest row of one wave's lanes, two units each.  16384 rows of 1000 bf16 logits
+// 12.5 us, a workgroup a row 27.5; of 1500 logits and four units 22 for 31, but 16 such
+// rows with 8 alternatives 11.9 for 8.7, and 3000 logits and eight units 40 for 36.
+constexpr int NARROW = 64 * UNIT * 2;
 constexpr int MAX_TOP = 32;
 constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of a row
 constexpr int MAX_SEGMENTS = 256;
 constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
-constexpr int BLOCKS = 4096;            // most workgroups of a launch over narrow rows
+constexpr int BLOCKS = 8192;            // most workgroups of a launch over narrow rows
 constexpr int AHEAD = 4, BWD_AHEAD = 8; // units of a wide row that a thread has in flight
 constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
 constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
@@ -119,14 +123,17 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
   const Sums x = rescaled(a, m, c), y = rescaled(b, m, c);
   return Sums{m, x.s + y.s, x.t + y.t};
 }
-__device__ __forceinline__ void add_unit(Sums& a, const float (&v)[UNIT], float most, float c) {
-  a = rescaled(a, fmaxf(a.m, most), c);
+__device__ __forceinline__ void add_values(Sums& a, const float (&v)[UNIT], float c) {   // none above a.m
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) {
     const float w = exponent(v[j], a.m, c), e = __builtin_amdgcn_exp2f(w);
     a.s += e;
     a.t = __fmaf_rn(e, fmaxf(w, FAR), a.t);
   }
+}
+__device__ __forceinline__ void add_unit(Sums& a, const float (&v)[UNIT], float most, float c) {
+  a = rescaled(a, fmaxf(a.m, most), c);
+  add_values(a, v, c);
 }
 // Over 2^log2 neighbouring lanes (all active).
 __device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
@@ -186,7 +193,7 @@ __device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int 
   else static_cast<int32_t*>(p.top_tokens)[at] = token;
 }
 
-// ---- rows of up to 512 columns: lanes of a wave
+// ---- rows of up to 1024 columns: lanes of a wave
 // Unit u of a narrow row: the row's last 8 columns where it would pass the end,
 // the first `skip` of them in the unit before too (all 8 or more past the end).
 struct Span {
@@ -209,42 +216,52 @@ __device__ __forceinline__ void read_span(const T* x, const uint8_t* mask, const
   }
 }
 
-template <typename T, bool TOP, bool MASK>
+// U: units of a lane (those of a row's lanes side by side).
+template <typename T, bool TOP, bool MASK, int U>
 __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
-  const int L = 1 << p.lanes_log2, lane = threadIdx.x & (L - 1);
-  const Span at = span_of(lane, p.V);
-  const uint32_t step = (gridDim.x * THREADS) >> p.lanes_log2;
-  for (uint32_t row0 = (blockIdx.x * THREADS + threadIdx.x) >> p.lanes_log2; __any(row0 < p.rows); row0 += step) {
+  const int log2 = U == 1 ? p.lanes_log2 : 6, L = 1 << log2, lane = threadIdx.x & (L - 1);
+  Span at[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) at[k] = span_of(lane + k * L, p.V);
+  const uint32_t step = (gridDim.x * THREADS) >> log2;
+  for (uint32_t row0 = (blockIdx.x * THREADS + threadIdx.x) >> log2; __any(row0 < p.rows); row0 += step) {
     const bool live = row0 < p.rows;
     const uint32_t row = live ? row0 : p.rows - 1;
     const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
     const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
     Given given{};
     if (lane == 0) given = given_of(p, row, x, mask);
-    float v[UNIT];
-    read_span<MASK>(x, mask, at, p.V, v);
+    float v[U][UNIT], most = -INF;
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) v[j] = j >= at.skip ? v[j] : -INF;
-    Sums a = no_sums();
-    add_unit(a, v, max8(v), p.c);
-    a = lanes_joined(a, p.lanes_log2, p.c);
+    for (int k = 0; k < U; ++k) {
+      read_span<MASK>(x, mask, at[k], p.V, v[k]);
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) v[k][j] = j >= at[k].skip ? v[k][j] : -INF;
+      most = fmaxf(most, max8(v[k]));
+    }
+    Sums a{fmaxf(most, LOWEST), 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < U; ++k) add_values(a, v[k], p.c);
+    a = lanes_joined(a, log2, p.c);
     if (live && lane == 0) finish_row(p, row, a, given);
     if constexpr (TOP) {
       const float l = __builtin_amdgcn_logf(a.s);
       uint64_t last = ~0ull;
-      for (int k = 0; k < p.top; ++k) {
+      for (int n = 0; n < p.top; ++n) {
         uint64_t best = 0;
 #pragma unroll
-        for (int j = 0; j < UNIT; ++j) {
-          const uint64_t key = key_of(v[j], (uint32_t)(at.col + j));
-          best = key < last && key > best ? key : best;
-        }
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int j = 0; j < UNIT; ++j) {
+            const uint64_t key = key_of(v[k][j], (uint32_t)(at[k].col + j));
+            best = key < last && key > best ? key : best;
+          }
         for (int o = 1; o < L; o <<= 1) {
           const uint64_t other = __shfl_xor((unsigned long long)best, o);
           best = other > best ? other : best;
         }
         last = best;
-        if (live && lane == (k & (L - 1))) write_top(p, row, k, best, a.m, l);
+        if (live && lane == (n & (L - 1))) write_top(p, row, n, best, a.m, l);
       }
     }
   }
@@ -633,10 +650,15 @@ TokenArgs common_args(const void* logits, const void* tokens, int wide_tokens, c
 
 template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
   if (a.V <= NARROW) {
-    while ((UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
-    const unsigned blocks = (unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS));
-    if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK>), dim3(blocks), dim3(THREADS), 0, st, a);
-    else hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK>), dim3(blocks), dim3(THREADS), 0, st, a);
+    while (a.lanes_log2 < 6 && (UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
+    const dim3 blocks((unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS)));
+    const auto narrow = [&](auto units) {
+      constexpr int U = decltype(units)::value;
+      if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, U>), blocks, dim3(THREADS), 0, st, a);
+      else hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK, U>), blocks, dim3(THREADS), 0, st, a);
+    };
+    if (a.V <= 64 * UNIT) narrow(std::integral_constant<int, 1>{});
+    else narrow(std::integral_constant<int, 2>{});
     return;
   }
   const dim3 grid(a.rows, a.segments);
