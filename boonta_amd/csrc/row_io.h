@@ -134,6 +134,23 @@ __device__ __forceinline__ float lanes_sum(float v, int log2) {
   return v;
 }
 
+// The largest of them (a NaN is none).
+__device__ __forceinline__ float lanes_max(float v, int log2) {
+  if (log2 > 0) v = fmaxf(v, xor16<1>(v));
+  if (log2 > 1) v = fmaxf(v, xor16<2>(v));
+  if (log2 > 2) v = fmaxf(v, xor16<4>(v));
+  if (log2 > 3) v = fmaxf(v, xor16<8>(v));
+  if (log2 > 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if (log2 > 5) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
+}
+
 // A sigmoid from the hardware's exponential and reciprocal (1 ulp each): 0 and
 // 1 at the infinities, NaN of NaN.  And 1 - sigmoid, e / (1 + e) where the
 // difference would cancel (elsewhere e may be infinite).

@@ -135,13 +135,12 @@ __device__ __forceinline__ void add_unit(Sums& a, const float (&v)[UNIT], float 
   a = rescaled(a, fmaxf(a.m, most), c);
   add_values(a, v, c);
 }
-// Over 2^log2 neighbouring lanes (all active).
+// Over 2^log2 neighbouring lanes (all active): one change of the maximum, not one a
+// stage (64 rows of 50000 bf16 logits 8.5 -> 7.9 us).
 __device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
-  for (int i = 0; i < log2; ++i) {
-    const int o = 1 << i;
-    const Sums b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
-    a = joined(a, b, c);
-  }
+  a = rescaled(a, lanes_max(a.m, log2), c);
+  a.s = lanes_sum(a.s, log2);
+  a.t = lanes_sum(a.t, log2);
   return a;
 }
 

@@ -48,7 +48,8 @@ def _strides(dims, *tensors):
 def _forward(logits, tokens, mask, temperature, top, keep):
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     batch, steps = lead if len(lead) == 2 else (lead[0], 1)
-    log_prob, entropy = (torch.empty(lead, dtype=torch.float32, device=logits.device) for _ in range(2))
+    log_prob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(log_prob)
     stats = log_prob.new_empty((*lead, 2)) if keep else None
     top_log_probs = log_prob.new_empty((*lead, top)) if top else None
     top_tokens = tokens.new_empty((*lead, top)) if top else None
