@@ -74,7 +74,7 @@ __device__ __forceinline__ float decay_of(float later, float earlier) { return i
 struct Gates {
   float a, wi;                // decay; w i
   float i, r, not_i, not_r;   // not_: 1 - it
-  float over_w;               // 1 / w, or 0
+  float over_w;               // 1 / w; 0 where w is (the hardware's root of a subnormal number is 0)
 };
 // 1 - a^2 of a = 2^-q.  Below 2 ln(2) q = 1/8 the Chebyshev interpolation of degree 3 of
 // (1 - 2^-2q) / q, within 2^-25 of it; above, what the difference loses is at most 8 times a^2's rounding.
@@ -93,7 +93,7 @@ template <bool BWD> __device__ __forceinline__ Gates gates_of(float input, float
   g.a = __builtin_amdgcn_exp2f(-q);
   const float w2 = one_minus_square(g.a, q);
   if constexpr (BWD) {
-    g.over_w = w2 > 0.f ? __builtin_amdgcn_rsqf(w2) : 0.f;
+    g.over_w = w2 >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(w2) : 0.f;   // (of a subnormal number it is infinite)
     g.wi = w2 * g.over_w * g.i;
   } else {
     g.wi = __builtin_amdgcn_sqrtf(w2) * g.i;

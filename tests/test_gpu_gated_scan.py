@@ -197,6 +197,24 @@ def test_small_and_large_decays():
     assert torch.equal(outs[0], ops["carry"]) and all(torch.isfinite(v).all() for v in grads.values())
 
 
+def test_decays_whose_input_weight_vanishes():
+    """Gates of -60 to -100 and rates down to 1e-6: q = rate r runs from 1e-26 through the subnormal numbers to
+    nothing.  The state stays the carry (w is at most sqrt(2 q) = 1.4e-13 a step), its gradient the sum of the cotangents; what
+    reaches x and the gates is below |D| sqrt(2 q), and the rate below |D| |x| r / w = |D| |x| sqrt(r / (2 rate)) < 1e-9."""
+    B, T, F = 2, 20, 64
+    ops = problem(17, B, T, F, F32)
+    ops["decay_gate"] = torch.linspace(-60, -100, F).repeat(B, T, 1).cuda()
+    ops["rate"] = torch.logspace(0, -6, 7).repeat(10)[:F].cuda()
+    cots = cotangents(18, B, T, F, F32)
+    outs, grads = run(ops, cots)
+    carry, dfinal, dout = np64(ops["carry"]), np64(cots[0]), np64(cots[1])
+    within(outs[0], carry, T * 4 * N * np.abs(carry) + 1e-11)
+    within(outs[1], np.broadcast_to(carry[:, None], (B, T, F)), T * 4 * N * np.abs(carry)[:, None] + 1e-11)
+    within(grads["carry"], dfinal + dout.sum(1), 2 * T * N * (np.abs(dfinal) + np.abs(dout).sum(1)))
+    for n in ("x", "input_gate", "decay_gate", "rate"):
+        within(grads[n], np.zeros(grads[n].shape), 1e-8)
+
+
 @pytest.mark.parametrize("T", [60, 3000])
 def test_bad_steps_reach_what_follows_and_stop_at_a_reset(T):
     for bad in (float("nan"), float("inf")):
