@@ -26,15 +26,26 @@ using namespace ppo;
 enum TokenDtype { TOKEN_F32 = 0, TOKEN_BF16 = 1 };
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-// Widest row of one wave's lanes, two units each.  16384 rows of 1000 bf16 logits
-// 12.5 us, a workgroup a row 27.5; of 1500 logits and four units 22 for 31, but 16 such
-// rows with 8 alternatives 11.9 for 8.7, and 3000 logits and eight units 40 for 36.
-constexpr int NARROW = 64 * UNIT * 2;
+// Rows of up to NARROW logits are a wave's lanes, with alternatives two units each (16384
+// rows of 1000 bf16 logits 12.5 us, a workgroup a row 27.5; 16 rows of 1500 with 8
+// alternatives 11.9 for 8.7).  Without alternatives rows of up to SIDE are so, several
+// a wave, and wider ones a wave each (400M bf16 logits in rows of 1030 241 us, a
+// workgroup a row 680; of 2000 172 for 276, of 8000 150 for 159, but of 20000 151 for
+// 139): up to WAVE_VOCAB, or where rows are few, and a row's time counts, up to FEW_VOCAB
+// (1024 rows of 8000 8.8 us for 7.2 a workgroup a row, 4096 16.3 for 17.5; 64 of
+// 2000 3.5 for 3.5).
+constexpr int NARROW = 64 * UNIT * 2, SIDE = 32 * UNIT;
+constexpr int WAVE_VOCAB = 8192, FEW_VOCAB = 2048, WAVE_ROWS = 2048;
+constexpr int WAVE_UNITS = 2;           // of a lane at a time (3 and 4 are level)
+// Backward: widest row, in units, whose workgroup takes them one after the other, a few
+// rows' together (400M bf16 logits, both passes: rows of 1030 970 us for 1780 a row a
+// workgroup, of 4100 545 for 655, of 8000 440 for 460, but of 12000 462 for 449).
+constexpr int FLAT_UNITS = 1024;
 constexpr int MAX_TOP = 32;
 constexpr int SEGMENT = 65536;          // most columns of a workgroup's part of a row
 constexpr int MAX_SEGMENTS = 256;
 constexpr int MAX_VOCAB = SEGMENT * MAX_SEGMENTS;
-constexpr int BLOCKS = 8192;            // most workgroups of a launch over narrow rows
+constexpr int BLOCKS = 16384;           // most workgroups of a launch over a wave's rows
 constexpr int AHEAD = 4, BWD_AHEAD = 8; // units of a wide row that a thread has in flight
 constexpr float LOWEST = -3.4028234663852886e38f, INF = __builtin_huge_valf();
 constexpr float FAR = -1e30f;           // exponents below: 2^FAR = 0, and 0 FAR is a number
@@ -192,8 +203,8 @@ __device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int 
   else static_cast<int32_t*>(p.top_tokens)[at] = token;
 }
 
-// ---- rows of up to 1024 columns: lanes of a wave
-// Unit u of a narrow row: the row's last 8 columns where it would pass the end,
+// ---- rows of lanes of a wave
+// Unit u of a row: the row's last 8 columns where it would pass the end,
 // the first `skip` of them in the unit before too (all 8 or more past the end).
 struct Span {
   int col, skip;
@@ -215,10 +226,11 @@ __device__ __forceinline__ void read_span(const T* x, const uint8_t* mask, const
   }
 }
 
-// U: units of a lane (those of a row's lanes side by side).
-template <typename T, bool TOP, bool MASK, int U>
+// U: units of a lane (those of a row's lanes side by side).  LOG2: of the lanes, -1: as
+// given (known, 100M bf16 logits in rows of 43 122 -> 89 us).
+template <typename T, bool TOP, bool MASK, int U, int LOG2>
 __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
-  const int log2 = U == 1 ? p.lanes_log2 : 6, L = 1 << log2, lane = threadIdx.x & (L - 1);
+  const int log2 = LOG2 < 0 ? p.lanes_log2 : LOG2, L = 1 << log2, lane = threadIdx.x & (L - 1);
   Span at[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) at[k] = span_of(lane + k * L, p.V);
@@ -263,6 +275,42 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
         if (live && lane == (n & (L - 1))) write_top(p, row, n, best, a.m, l);
       }
     }
+  }
+}
+
+// A wave for each row, WAVE_UNITS of a lane at a time, as many as there are: an empty unit
+// costs the vector work of a full one, which bounds rows of few (1030 logits 299 -> 241 us).
+template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_wave_kernel(TokenArgs p) {
+  const int lane = threadIdx.x & 63, units = (int)p.units.d;
+  for (uint32_t row = blockIdx.x * WAVES + (threadIdx.x >> 6); row < p.rows; row += gridDim.x * WAVES) {
+    const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+    const uint8_t* mask = MASK ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr;
+    Given given{};
+    if (lane == 0) given = given_of(p, row, x, mask);
+    Sums a = no_sums();
+    for (int u0 = 0; u0 < units; u0 += 64 * WAVE_UNITS) {
+      Unit8<T> raw[WAVE_UNITS];
+      uint64_t allowed[WAVE_UNITS];
+#pragma unroll
+      for (int k = 0; k < WAVE_UNITS; ++k) {
+        if (u0 + 64 * k >= units) continue;   // (of the whole wave)
+        const Span at = span_of(u0 + 64 * k + lane, p.V);
+        __builtin_memcpy(raw[k].w, x + at.col, sizeof(raw[k].w));
+        if constexpr (MASK) __builtin_memcpy(&allowed[k], mask + at.col, 8);
+      }
+#pragma unroll
+      for (int k = 0; k < WAVE_UNITS; ++k) {
+        if (u0 + 64 * k >= units) continue;
+        const Span at = span_of(u0 + 64 * k + lane, p.V);
+        float v[UNIT];
+        unit_values<MASK>(raw[k], MASK ? allowed[k] : 0, v);
+#pragma unroll
+        for (int j = 0; j < UNIT; ++j) v[j] = j >= at.skip ? v[j] : -INF;
+        add_unit(a, v, max8(v), p.c);
+      }
+    }
+    a = lanes_joined(a, 6, p.c);
+    if (lane == 0) finish_row(p, row, a, given);
   }
 }
 
@@ -539,7 +587,7 @@ __device__ __forceinline__ void unit_gradient(const RowGradient& r, float c, int
   for (int j = 0; j < UNIT; ++j) v[j] = d[j];
 }
 
-// Rows of up to 2048 columns: several side by side, their scalars formed once in LDS.
+// Rows of up to FLAT_UNITS: several side by side, their scalars formed once in LDS.
 constexpr int MAX_ROW_BLOCK = 256;
 template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) token_bwd_kernel(TokenArgs p) {
   __shared__ RowGradient scalars[MAX_ROW_BLOCK];
@@ -648,16 +696,25 @@ TokenArgs common_args(const void* logits, const void* tokens, int wide_tokens, c
 }
 
 template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
+  if (!a.top && a.V > SIDE && a.V <= (a.rows >= WAVE_ROWS ? WAVE_VOCAB : FEW_VOCAB)) {
+    const dim3 blocks((unsigned)std::min<int64_t>(BLOCKS, ceil_div64(a.rows, WAVES)));
+    hipLaunchKernelGGL((token_wave_kernel<T, MASK>), blocks, dim3(THREADS), 0, st, a);
+    return;
+  }
   if (a.V <= NARROW) {
     while (a.lanes_log2 < 6 && (UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
     const dim3 blocks((unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS)));
-    const auto narrow = [&](auto units) {
-      constexpr int U = decltype(units)::value;
-      if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, U>), blocks, dim3(THREADS), 0, st, a);
-      else hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK, U>), blocks, dim3(THREADS), 0, st, a);
+    const auto lanes = [&](auto log2) {
+      hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK, 1, decltype(log2)::value>), blocks, dim3(THREADS), 0, st, a);
     };
-    if (a.V <= 64 * UNIT) narrow(std::integral_constant<int, 1>{});
-    else narrow(std::integral_constant<int, 2>{});
+    if (a.top && a.V > 64 * UNIT) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 2, 6>), blocks, dim3(THREADS), 0, st, a);
+    else if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 1, -1>), blocks, dim3(THREADS), 0, st, a);
+    else if (a.lanes_log2 == 0) lanes(std::integral_constant<int, 0>{});
+    else if (a.lanes_log2 == 1) lanes(std::integral_constant<int, 1>{});
+    else if (a.lanes_log2 == 2) lanes(std::integral_constant<int, 2>{});
+    else if (a.lanes_log2 == 3) lanes(std::integral_constant<int, 3>{});
+    else if (a.lanes_log2 == 4) lanes(std::integral_constant<int, 4>{});
+    else lanes(std::integral_constant<int, 5>{});
     return;
   }
   const dim3 grid(a.rows, a.segments);
@@ -672,7 +729,7 @@ template <typename T, bool MASK> void launch_bwd(hipStream_t st, TokenArgs& a) {
   const int most = ceil_div(a.V + MAX_SKEW, UNIT);
   const int segments = ceil_div(most, 8 * THREADS);
   a.segment_units = ceil_div(most, segments);
-  if (units <= THREADS)
+  if (units <= FLAT_UNITS)
     hipLaunchKernelGGL((token_bwd_kernel<T, MASK>), dim3((unsigned)ceil_div64(a.rows, a.row_block)), dim3(THREADS), 0, st, a);
   else
     hipLaunchKernelGGL((token_bwd_wide_kernel<T, MASK>), dim3(a.rows, (unsigned)segments), dim3(THREADS), 0, st,

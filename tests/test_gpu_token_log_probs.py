@@ -101,6 +101,15 @@ def test_rows_in_segments_and_many_rows(rows, V):
     check(x, t, m, 0.9, out, 20, grad, g, h)
 
 
+@pytest.mark.parametrize("rows,V,dtype,mask", [(70, 1030, F32, "rows"), (3000, 1025, BF16, None), (9001, 257, F32, "rows"),
+                                               (2047, 2049, BF16, "rows"), (2048, 2049, BF16, "rows"),
+                                               (2050, 4100, F32, None), (2049, 8192, BF16, "one"), (2049, 8193, BF16, None)])
+def test_many_rows_without_alternatives(rows, V, dtype, mask):
+    x, t, m, g, h = problem(rows + V, (rows,), V, dtype, mask)
+    out, grad = run(x, t, m, 1.1, 0, g, h)
+    check(x, t, m, 1.1, out, 0, grad, g, h)
+
+
 @pytest.mark.parametrize("V", [40, 300, 3000, 70000])
 def test_equal_values_go_to_the_lowest_index(V):
     gen = torch.Generator().manual_seed(V)
