@@ -9,11 +9,12 @@
 // grows.  A row that allows nothing has p = 0 and entropy 0.
 // Backward: dx_j = (g (1_{j = token} - p_j) - h p_j (log p_j + entropy)) / T.
 //
-// The `top` largest x, equal ones by index.  A thread also keeps its best unit
-// of 8 columns, by its largest value, then the lowest index.  The units of the
-// `top` best threads hold the `top` best values: every one of those threads
-// has a value that is better than all of any other thread.  So only their units
-// are read again, those worse than the last of them left out, and ranked.
+// The `top` largest x, equal ones by index.  A row held by a wave's lanes gives them one
+// after the other.  Of a wider row a thread also keeps its best unit of 8 columns, by
+// its largest value, then the lowest index.  The units of the `top` best threads hold
+// the `top` best values: every one of those threads has a value that is better than
+// all of any other thread.  So only their units are read again, those worse than the
+// last of them left out, and ranked.
 #include "row_io.h"
 
 #include <algorithm>
@@ -26,15 +27,16 @@ using namespace ppo;
 enum TokenDtype { TOKEN_F32 = 0, TOKEN_BF16 = 1 };
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-// Rows of up to NARROW logits are a wave's lanes, with alternatives two units each (16384
-// rows of 1000 bf16 logits 12.5 us, a workgroup a row 27.5; 16 rows of 1500 with 8
-// alternatives 11.9 for 8.7).  Without alternatives rows of up to SIDE are so, several
-// a wave, and wider ones a wave each (400M bf16 logits in rows of 1030 241 us, a
-// workgroup a row 680; of 2000 172 for 276, of 8000 150 for 159, but of 20000 151 for
-// 139): up to WAVE_VOCAB, or where rows are few, and a row's time counts, up to FEW_VOCAB
-// (1024 rows of 8000 8.8 us for 7.2 a workgroup a row, 4096 16.3 for 17.5; 64 of
-// 2000 3.5 for 3.5).
-constexpr int NARROW = 64 * UNIT * 2, SIDE = 32 * UNIT;
+// With alternatives, rows of up to NARROW logits are a wave's lanes of up to four units (50M
+// bf16 logits in rows of 2000, 8 alternatives 93 us, a workgroup a row 144; 20
+// alternatives 195 for 212); where rows are few and alternatives more than FEW_TOP, of
+// up to two (16 rows of 2000, 1 alternative 4.4 us for 7.1, 8 9.4 for 8.3).
+// Without alternatives rows of up to SIDE are so, several a wave, and wider ones a wave
+// each (400M bf16 logits in rows of 1030 241 us, a workgroup a row 680; of 2000 172 for
+// 276, of 8000 150 for 159, but of 20000 151 for 139): up to WAVE_VOCAB, or where rows are
+// few, and a row's time counts, up to FEW_VOCAB (1024 rows of 8000 8.8 us for 7.2 a
+// workgroup a row, 4096 16.3 for 17.5; 64 of 2000 3.5 for 3.5).
+constexpr int NARROW = 64 * UNIT * 4, SIDE = 32 * UNIT, FEW_TOP = 4;
 constexpr int WAVE_VOCAB = 8192, FEW_VOCAB = 2048, WAVE_ROWS = 2048;
 constexpr int WAVE_UNITS = 2;           // of a lane at a time (3 and 4 are level)
 // Backward: widest row, in units, whose workgroup takes them one after the other, a few
@@ -195,12 +197,14 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int place, uint64_t key, float m, float l) {
+__device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int place, float x, int token, float m, float l) {
   const int64_t at = (int64_t)row * p.top + place;
-  p.top_log_probs[at] = key ? LN2 * (exponent(value_of(key), m, p.c) - l) : -INF;
-  const int32_t token = key ? (int32_t)index_of(key) : -1;
+  p.top_log_probs[at] = token < 0 ? -INF : LN2 * (exponent(x, m, p.c) - l);
   if (p.wide_tokens) static_cast<int64_t*>(p.top_tokens)[at] = token;
   else static_cast<int32_t*>(p.top_tokens)[at] = token;
+}
+__device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int place, uint64_t key, float m, float l) {
+  write_top(p, row, place, value_of(key), key ? (int32_t)index_of(key) : -1, m, l);
 }
 
 // ---- rows of lanes of a wave
@@ -257,22 +261,35 @@ __global__ void __launch_bounds__(THREADS) token_narrow_kernel(TokenArgs p) {
     if (live && lane == 0) finish_row(p, row, a, given);
     if constexpr (TOP) {
       const float l = __builtin_amdgcn_logf(a.s);
-      uint64_t last = ~0ull;
+      // one after the other: the row's largest value, the lowest of its columns (as a
+      // float: below 2^24), and out with it; lane n of the row's keeps the n-th, and
+      // every L of them are written together
+      float kept = -INF;
+      int kept_col = -1;
       for (int n = 0; n < p.top; ++n) {
-        uint64_t best = 0;
+        most = max8(v[0]);
 #pragma unroll
-        for (int k = 0; k < U; ++k)
+        for (int k = 1; k < U; ++k) most = fmaxf(most, max8(v[k]));
+        most = lanes_max(most, log2);
+        float at_most = -INF;   // less its column
 #pragma unroll
-          for (int j = 0; j < UNIT; ++j) {
-            const uint64_t key = key_of(v[k][j], (uint32_t)(at[k].col + j));
-            best = key < last && key > best ? key : best;
-          }
-        for (int o = 1; o < L; o <<= 1) {
-          const uint64_t other = __shfl_xor((unsigned long long)best, o);
-          best = other > best ? other : best;
+        for (int k = U - 1; k >= 0; --k)
+#pragma unroll
+          for (int j = UNIT - 1; j >= 0; --j) at_most = v[k][j] == most ? -(float)(at[k].col + j) : at_most;
+        at_most = lanes_max(at_most, log2);
+        const int col = most > -INF ? (int)-at_most : -1;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int away = col - at[k].col;
+#pragma unroll
+          for (int j = 0; j < UNIT; ++j) v[k][j] = away == j ? -INF : v[k][j];
         }
-        last = best;
-        if (live && lane == (n & (L - 1))) write_top(p, row, n, best, a.m, l);
+        const int place = n & (L - 1);
+        kept = lane == place ? most : kept;
+        kept_col = lane == place ? col : kept_col;
+        if (place == L - 1 || n == p.top - 1) {
+          if (live && lane <= place) write_top(p, row, n - place + lane, kept, kept_col, a.m, l);
+        }
       }
     }
   }
@@ -701,13 +718,14 @@ template <typename T, bool MASK> void launch_fwd(hipStream_t st, TokenArgs& a) {
     hipLaunchKernelGGL((token_wave_kernel<T, MASK>), blocks, dim3(THREADS), 0, st, a);
     return;
   }
-  if (a.V <= NARROW) {
+  if (a.V <= (a.rows >= WAVE_ROWS || a.top <= FEW_TOP ? NARROW : NARROW / 2)) {
     while (a.lanes_log2 < 6 && (UNIT << a.lanes_log2) < a.V) ++a.lanes_log2;
     const dim3 blocks((unsigned)std::min<int64_t>(BLOCKS, ceil_div64((int64_t)a.rows << a.lanes_log2, THREADS)));
     const auto lanes = [&](auto log2) {
       hipLaunchKernelGGL((token_narrow_kernel<T, false, MASK, 1, decltype(log2)::value>), blocks, dim3(THREADS), 0, st, a);
     };
-    if (a.top && a.V > 64 * UNIT) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 2, 6>), blocks, dim3(THREADS), 0, st, a);
+    if (a.top && a.V > 128 * UNIT) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 4, 6>), blocks, dim3(THREADS), 0, st, a);
+    else if (a.top && a.V > 64 * UNIT) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 2, 6>), blocks, dim3(THREADS), 0, st, a);
     else if (a.top) hipLaunchKernelGGL((token_narrow_kernel<T, true, MASK, 1, -1>), blocks, dim3(THREADS), 0, st, a);
     else if (a.lanes_log2 == 0) lanes(std::integral_constant<int, 0>{});
     else if (a.lanes_log2 == 1) lanes(std::integral_constant<int, 1>{});

@@ -110,6 +110,19 @@ def test_many_rows_without_alternatives(rows, V, dtype, mask):
     check(x, t, m, 1.1, out, 0, grad, g, h)
 
 
+@pytest.mark.parametrize("rows,V,top,dtype", [(2048, 1025, 32, F32), (2100, 2048, 7, BF16), (2047, 2047, 5, BF16),
+                                              (30, 1999, 4, F32), (30, 1030, 1, BF16), (70, 5, 5, F32), (70, 9, 9, BF16)])
+def test_many_rows_with_alternatives(rows, V, top, dtype):
+    """Rounded to 8ths, so that many are equal; the last rows' are all one value, or not allowed but for one."""
+    x, t, m, g, h = problem(rows + top, (rows,), V, dtype)
+    x = (8 * x).round() / 8
+    x[-3:] = 1.5
+    m[-1] = False
+    m[-1, V - 1] = True
+    out, grad = run(x, t, m, 0.8, top, g, h)
+    check(x, t, m, 0.8, out, top, grad, g, h)
+
+
 @pytest.mark.parametrize("V", [40, 300, 3000, 70000])
 def test_equal_values_go_to_the_lowest_index(V):
     gen = torch.Generator().manual_seed(V)
