@@ -26,6 +26,13 @@
 //
 // A map's decay is -0 where a step of it starts an episode: then nothing of what
 // enters, an infinity or NaN neither, passes.
+//
+// What bounds it: an element takes some 26 vector and 6 transcendental instructions
+// forward, about as long as its bytes.  65536 steps of 2048 bf16 features: the maps
+// 182 to 195 us (4.1 to 4.4 TB/s), the outputs 219 to 233 (4.6 to 4.9 TB/s; a copy
+// reaches 4.9).  256 x 64 steps of 256 float32 features 19 us, backward 29 (3.6, 4.1
+// TB/s); 24 x 4093 of 640 bf16, ragged, 128 and 288 us (3.3, 2.7 TB/s: the longest
+// sequence's workgroups, one a CU).
 #include "row_io.h"
 
 #include <algorithm>
@@ -42,7 +49,7 @@ constexpr int FWD_STEPS = 8, BWD_STEPS = 4, MAP_STEPS = 4;   // of a lane's chun
 constexpr int LANE = 2;                       // features of a lane
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
-constexpr int MAX_SEGMENTS = 64;
+constexpr int MAX_SEGMENTS = 256;             // (500000 steps of 64 bf16 features: 64 370 us, 256 114, 512 117)
 
 struct GatedArgs {
   const void *x, *input_gate, *decay_gate;
@@ -302,17 +309,30 @@ __device__ __forceinline__ void through_waves(float (&h)[VW], float (&mine)[VW],
   for (int k = 0; k < VW; ++k) mine[k] = apply(A[k], B[k], mine[k]);
 }
 
-// The state entering the segment from those before (REVERSE: after) it.
-template <int VW, bool REVERSE>
-__device__ __forceinline__ void through_segments(const GatedArgs& p, int64_t b, int f0, int segment, float (&h)[VW]) {
-  const int n = REVERSE ? p.segments - 1 - segment : segment;
+// The state h carried through the segments before (REVERSE: after) this one: a run of
+// their maps for each slot, composed as the chunks of a tile are (65536 steps of 64
+// bf16 features in 64 segments 54 us, every lane reading them all 60).  Rooms of LDS
+// that the first tile does not use.
+template <int VW, int LF, bool REVERSE, typename L>
+__device__ __forceinline__ void through_segments(const GatedArgs& p, const L& at, int segment, float (&h)[VW],
+                                                 float* wave_a, float* wave_b) {
+  if (p.segments == 1) return;
+  const int n = REVERSE ? p.segments - 1 - segment : segment, slots = at.waves * at.SLOTS;
+  const int slot = at.wave * at.SLOTS + at.slot, each = (n + slots - 1) / slots;
+  const int first = (REVERSE ? slots - 1 - slot : slot) * each;
+  float A[VW], B[VW], mine[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    A[k] = 1.f;
+    B[k] = 0.f;
+  }
   constexpr int U = 4;   // maps on their way at once
-  for (int i0 = 0; i0 < n; i0 += U) {
+  for (int i0 = 0; i0 < each; i0 += U) {
     float a[U][VW], s[U][VW];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = min(i0 + u, n - 1);
-      const float* m = p.maps + ((b * p.segments + (REVERSE ? p.segments - 1 - i : i)) * 2) * p.F + f0;
+      const int i = min(first + i0 + u, n - 1);
+      const float* m = p.maps + (((int64_t)at.b * p.segments + (REVERSE ? p.segments - 1 - i : i)) * 2) * p.F + at.f0;
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
         a[u][k] = m[k];
@@ -320,10 +340,18 @@ __device__ __forceinline__ void through_segments(const GatedArgs& p, int64_t b, 
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const bool there = i0 + u < each && first + i0 + u < n;
 #pragma unroll
-      for (int k = 0; k < VW; ++k) h[k] = i0 + u < n ? apply(a[u][k], s[u][k], h[k]) : h[k];
+      for (int k = 0; k < VW; ++k) {
+        B[k] = there ? apply(a[u][k], s[u][k], B[k]) : B[k];
+        A[k] = there ? decay_of(a[u][k], A[k]) : A[k];
+      }
+    }
   }
+  compose_slots<VW, LF, REVERSE>(A, B, at.lane, wave_a + at.wave * LF * VW, wave_b + at.wave * LF * VW);
+  lds_barrier();
+  through_waves<VW, LF, REVERSE>(h, mine, A, B, wave_a, wave_b, at.lane, at.wave, at.waves);
 }
 
 // The map of a segment: of the state h (REVERSE: of the cotangent E).  Every
@@ -463,7 +491,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_fwd_kernel(GatedArgs p) 
   };
   if (begin < live_end) fetch(begin);
   load_state<VW>(p.carry, (int64_t)at.b * p.F + at.f0, h);
-  through_segments<VW, false>(p, at.b, at.f0, segment, h);
+  through_segments<VW, LF, false>(p, at, segment, h, wave_a[1], wave_b[1]);
   int set = 0, t0 = begin;
   for (; t0 < live_end; t0 += at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
@@ -584,7 +612,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
   int set = 0, t0 = begin + (tiles - 1) * at.tile;
   if (tiles > 0) fetch(t0);
   load_state<VW>(p.dfinal, state, E);
-  through_segments<VW, true>(p, at.b, at.f0, segment, E);
+  through_segments<VW, LF, true>(p, at, segment, E, rev_a[1], rev_b[1]);
   for (; t0 >= begin; t0 -= at.tile, set ^= 1) {
     const bool whole = t0 + at.tile <= live_end;
     const int t = at.chunk_step(t0);
@@ -809,9 +837,11 @@ Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
   const int N = backward ? BWD_STEPS : FWD_STEPS;
   s.vw = LANE;
   if (F < s.vw) s.vw = 1;
-  // lanes for the features that are there; where those and the sequences do not
-  // fill the chip, fewer side by side, down to a cache line, if that fills most of it
-  // (a segment more reads operands twice)
+  // lanes for the features that are there (2048 x 500 steps of 16 bf16 features, both
+  // passes: 154 us, 64 lanes 584); where those and the sequences do not fill the chip,
+  // fewer side by side, down to a cache line, if that fills most of it (a segment more
+  // reads operands twice: 24 x 4093 steps of 640 features 413 us, in segments 491; 24
+  // of 256, which it does not fill, 202 in segments, 352 without)
   s.lf = 64;
   const auto groups_at = [&](int lf) { return (int64_t)batch * ceil_div(F, lf * s.vw); };
   const auto fits = [&](int lf) { return 64 / lf * N < 2 * (int64_t)steps; };

@@ -128,7 +128,7 @@ def test_sequences_match_the_recurrence(case, dtype):
             assert all(torch.equal(a, b) for a, b in zip(gated_scan(*ops.values()), outs))
 
 
-@pytest.mark.parametrize("case", [(1, 9000, 16), (1, 2100, 520), (3, 3000, 40), (2, 8191, 3)])
+@pytest.mark.parametrize("case", [(1, 9000, 16), (1, 2100, 520), (3, 3000, 40), (2, 8191, 3), (1, 4200, 100)])
 def test_long_sequences_in_segments(case):
     B, T, F = case
     for dtype, ragged in ((F32, False), (BF16, True)):
