@@ -176,7 +176,7 @@ __device__ __forceinline__ Given given_of(const TokenArgs& p, uint32_t row, cons
 __device__ __forceinline__ void finish_row(const TokenArgs& p, uint32_t row, const Sums& a, const Given& g) {
   const bool none = a.s == 0.f;
   const float l = none ? INF : __builtin_amdgcn_logf(a.s);   // log2
-  p.entropy[row] = none ? 0.f : LN2 * (l - a.t / a.s);
+  p.entropy[row] = none ? 0.f : LN2 * (l - a.t * __builtin_amdgcn_rcpf(a.s));   // (S from 1 to 2^24)
   p.log_prob[row] = !g.token ? 0.f : g.logit == -INF ? -INF : LN2 * (exponent(g.logit, a.m, p.c) - l);
   if (p.stats) {
     p.stats[2 * (int64_t)row] = none ? 0.f : a.m;
