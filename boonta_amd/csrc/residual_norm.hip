@@ -23,6 +23,11 @@
 // L lanes of a wave (up to 512 columns) or one workgroup, and the next row's
 // operands are on their way while one is formed.  Sums are float32, the
 // lanes' by butterflies, the waves' in order.
+//
+// What bounds it is HBM: 65536 rows of 2048 bf16 columns with a float32 stream 323 us
+// (5.0 TB/s); 128000 of 640 bf16 with gates 175 us, backward 277 (4.7, 4.8 TB/s) and
+// 7 for the scales; 15984 of 1333 float32 100 and 166 us (4.4, 4.2 TB/s).  64 rows of
+// 1000 take 4.5 us: a launch, and a row's two sums one after the other.
 #include "row_io.h"
 
 #include <algorithm>
