@@ -12,7 +12,8 @@
 // 1 - a^2 = -expm1(-2 rate r) is a series where it is small: a^2 rounds away
 // there.  A rate of 0 keeps the state: w = 0, and the term through 1 / w is taken as 0.
 //
-// Both directions compose affine maps.  A lane holds a chunk of steps of VW
+// Sequences of up to SHORT steps are stepped through, a thread for each sequence's
+// features.  Else both directions compose affine maps.  A lane holds a chunk of steps of VW
 // features in registers, LF lanes stand side by side over the features and the
 // rest of the workgroup over the time: a chunk's map, composed with those of the
 // chunks before it (lanes by shuffles, waves through LDS), gives the state that
@@ -49,6 +50,8 @@ constexpr int FWD_STEPS = 8, BWD_STEPS = 4, MAP_STEPS = 4;   // of a lane's chun
 constexpr int LANE = 2;                       // features of a lane
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t MAX_STRIDE = 1 << 23;       // of a step, in elements: a wave's steps are told apart in 32 bits
+constexpr int SHORT = 8;                      // most steps of a short sequence
+constexpr int SHORT_THREADS = 256;
 constexpr int MAX_SEGMENTS = 256;             // (500000 steps of 64 bf16 features: 64 370 us, 256 114, 512 117)
 
 struct GatedArgs {
@@ -578,6 +581,9 @@ struct Kept {
   float wi, not_i, c;   // w i; 1 - i; a^2 i x / w
   float r, not_r;       // and 1 - r
 };
+__device__ __forceinline__ Kept kept_of(const Gates& g, float x, float cotangent) {
+  return Kept{g.a, g.wi * x, cotangent, g.wi, g.not_i, g.a * g.over_w * g.a * (g.i * x), g.r, g.not_r};
+}
 
 template <typename S, int VW, int LF>
 __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) {
@@ -623,17 +629,8 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < VW; ++k) {
-        Kept& e = q[i][k];
         const Gates g = gates_of<true>(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
-        const float xv = widen(x[i].v[k]);
-        e.a = g.a;
-        e.g = widen(go[i].v[k]);
-        e.wi = g.wi;
-        e.b = g.wi * xv;
-        e.not_i = g.not_i;
-        e.c = g.a * g.over_w * g.a * (g.i * xv);
-        e.r = g.r;
-        e.not_r = g.not_r;
+        q[i][k] = kept_of(g, widen(x[i].v[k]), widen(go[i].v[k]));
       }
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
@@ -757,6 +754,148 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
   }
 }
 
+// ---- short sequences: a thread takes VW features through all steps of a sequence and
+// goes on to the next, with no exchange, and is bound by HBM: 33M bf16 elements in
+// sequences of one step take 106 us (5.0 TB/s), in chunks 484; of four 66 for 133, of
+// eight 57 for 65; both passes 312, 197, 195 us (4.5 to 4.2 TB/s) for 1583, 410, 228.
+// Its lanes stand side by side over the features, the rest of the workgroup over
+// the sequences.
+template <int VW> struct ShortLane {
+  int lane, row, rows, f0;
+  __device__ __forceinline__ ShortLane(const GatedArgs& p, int lanes_log2) {
+    lane = threadIdx.x & ((1 << lanes_log2) - 1);
+    row = threadIdx.x >> lanes_log2;
+    rows = SHORT_THREADS >> lanes_log2;
+    // (lanes past the row's end repeat its last features: they read and write the same values)
+    f0 = min((int)((blockIdx.x << lanes_log2) + lane) * VW, p.F - VW);
+  }
+};
+// A sequence's steps of an operand, the last again where there are fewer than N.
+template <typename S, int VW, int N>
+__device__ __forceinline__ void fetch_short(const void* x, const RowStride& s, const GatedArgs& p, int64_t b, int f0,
+                                            Raw<S, VW> (&v)[N]) {
+  const char* base = static_cast<const char*>(x);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = load_raw<S, VW>(base, (b * s.batch + min(i, p.steps - 1) * s.step + f0) * (int64_t)sizeof(S));
+}
+template <int N> __device__ __forceinline__ uint32_t short_flags(const GatedArgs& p, int64_t b) {
+  uint32_t cuts = 0;
+  if (p.done) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) cuts |= (p.done[b * p.steps + min(i, p.steps - 1)] ? 1u : 0u) << i;
+  }
+  return cuts;
+}
+template <typename S, int VW> __device__ __forceinline__ void store_short(void* out, int64_t at, const float (&v)[VW]) {
+  store_near<VW>(static_cast<S*>(out) + at, 0, v);
+}
+
+template <typename S, int VW, int N>
+__global__ void __launch_bounds__(SHORT_THREADS) gated_short_fwd_kernel(GatedArgs p, int batch, int lanes_log2) {
+  const ShortLane<VW> at(p, lanes_log2);
+  float rl[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) rl[k] = p.rate[at.f0 + k] * LOG2E;
+  for (int64_t b = (int64_t)blockIdx.y * at.rows + at.row; b < batch; b += (int64_t)gridDim.y * at.rows) {
+    Raw<S, VW> x[N], ig[N], dg[N];
+    fetch_short<S, VW, N>(p.x, p.x_s, p, b, at.f0, x);
+    fetch_short<S, VW, N>(p.input_gate, p.input_s, p, b, at.f0, ig);
+    fetch_short<S, VW, N>(p.decay_gate, p.decay_s, p, b, at.f0, dg);
+    const uint32_t cuts = short_flags<N>(p, b);
+    const int live_end = p.lengths ? max(0, min(p.lengths[b], p.steps)) : p.steps;
+    float h[VW];
+    load_state<VW>(p.carry, b * p.F + at.f0, h);
+    if (p.states) store_near<VW>(p.states + b * p.F + at.f0, 0, h);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i >= p.steps) break;
+      const bool live = i < live_end, cut = cuts >> i & 1;
+      float o[VW];
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates g = gates_of<false>(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const float next = apply(cut ? -0.f : g.a, g.wi * widen(x[i].v[k]), h[k]);
+        h[k] = live ? next : h[k];
+        o[k] = live ? next : 0.f;
+      }
+      store_short<S, VW>(p.out, (b * p.steps + i) * p.F + at.f0, o);
+    }
+    store_near<VW>(p.final + b * p.F + at.f0, 0, h);
+  }
+}
+
+template <typename S, int VW, int N>
+__global__ void __launch_bounds__(SHORT_THREADS) gated_short_bwd_kernel(GatedArgs p, int batch, int lanes_log2) {
+  __shared__ float sums[SHORT_THREADS * VW];
+  const ShortLane<VW> at(p, lanes_log2);
+  float rate[VW], rl[VW], drate[VW];
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    rate[k] = p.rate[at.f0 + k];
+    rl[k] = rate[k] * LOG2E;
+    drate[k] = 0.f;
+  }
+  for (int64_t b = (int64_t)blockIdx.y * at.rows + at.row; b < batch; b += (int64_t)gridDim.y * at.rows) {
+    Raw<S, VW> x[N], ig[N], dg[N], go[N];
+    fetch_short<S, VW, N>(p.x, p.x_s, p, b, at.f0, x);
+    fetch_short<S, VW, N>(p.input_gate, p.input_s, p, b, at.f0, ig);
+    fetch_short<S, VW, N>(p.decay_gate, p.decay_s, p, b, at.f0, dg);
+    fetch_short<S, VW, N>(p.dout, p.dout_s, p, b, at.f0, go);
+    const uint32_t cuts = short_flags<N>(p, b);
+    const int live_end = p.lengths ? max(0, min(p.lengths[b], p.steps)) : p.steps;
+    float h[VW], E[VW], before[N][VW];
+    load_state<VW>(p.states, b * p.F + at.f0, h);
+    load_state<VW>(p.dfinal, b * p.F + at.f0, E);
+    Kept q[N][VW];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Gates g = gates_of<true>(widen(ig[i].v[k]), widen(dg[i].v[k]), rl[k]);
+        const float xv = widen(x[i].v[k]);
+        const bool cut = cuts >> i & 1;
+        q[i][k] = kept_of(g, xv, widen(go[i].v[k]));
+        if (cut) q[i][k].a = -0.f;
+        before[i][k] = cut ? 0.f : h[k];
+        h[k] = i < live_end ? apply(q[i][k].a, q[i][k].b, h[k]) : h[k];
+      }
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) {
+      if (i >= p.steps) continue;
+      const bool live = i < live_end;
+      float ox[VW], oi[VW], od[VW];
+#pragma unroll
+      for (int k = 0; k < VW; ++k) {
+        const Kept& e = q[i][k];
+        const float D = e.g + E[k];
+        const float dr = D * __fmaf_rn(e.a, before[i][k], -e.c) * e.r;   // dL r
+        E[k] = live ? (is_reset(e.a) ? 0.f : e.a * D) : E[k];
+        ox[k] = live ? D * e.wi : 0.f;
+        oi[k] = live ? D * e.b * e.not_i : 0.f;
+        od[k] = live ? -dr * rate[k] * e.not_r : 0.f;
+        drate[k] -= live ? dr : 0.f;
+      }
+      const int64_t to = (b * p.steps + i) * p.F + at.f0;
+      store_short<S, VW>(p.dx, to, ox);
+      store_short<S, VW>(p.dinput_gate, to, oi);
+      store_short<S, VW>(p.ddecay_gate, to, od);
+    }
+    if (p.dcarry) store_near<VW>(p.dcarry + b * p.F + at.f0, 0, E);
+  }
+  if (!p.partials) return;
+#pragma unroll
+  for (int k = 0; k < VW; ++k) sums[k * SHORT_THREADS + threadIdx.x] = drate[k];
+  __syncthreads();
+  if (at.row > 0) return;
+#pragma unroll
+  for (int k = 0; k < VW; ++k) {
+    float s = 0.f;
+    for (int r = 0; r < at.rows; ++r) s += sums[k * SHORT_THREADS + (r << lanes_log2) + at.lane];
+    p.partials[(int64_t)blockIdx.y * p.F + at.f0 + k] = s;
+  }
+}
+
 // Sums over rows [from, from + each) of parts [rows, F]: 64 columns a workgroup,
 // each wave its share of the rows in their order, then the waves'.
 __global__ void __launch_bounds__(1024) gated_rate_kernel(const float* parts, int64_t rows, int each, int F, float* out) {
@@ -832,6 +971,7 @@ struct Plan {
   int vw, lf, waves, blocks, tile, segment, segments;
 };
 constexpr int TARGET = 512, FILL = 192;   // workgroups that fill the chip, and most of it
+constexpr int SHORT_GROUPS = 4096;        // most workgroups of a launch over short sequences
 
 Plan plan_of(int dtype, bool backward, int batch, int steps, int F) {
   Plan s;
@@ -911,7 +1051,53 @@ template <typename S, bool BWD> void launch(hipStream_t st, GatedArgs a, const P
   else launch_shape<S, VW, 8, BWD>(st, a, s, batch);
 }
 
+// Short sequences (up to SHORT steps): lanes over the features, workgroups over those
+// and the sequences.
+struct ShortPlan {
+  int vw, lanes_log2;
+  unsigned blocks, groups;
+};
+ShortPlan short_plan_of(bool backward, int batch, int steps, int F) {
+  ShortPlan s;
+  // (backward, four features of four steps take 256 registers)
+  s.vw = F < 4 ? 1 : steps <= 2 ? 4 : steps <= 4 || !backward ? 2 : 1;
+  s.lanes_log2 = 0;
+  while (s.lanes_log2 < 8 && (s.vw << s.lanes_log2) < F) ++s.lanes_log2;
+  s.blocks = (unsigned)ceil_div(F, s.vw << s.lanes_log2);
+  s.groups = (unsigned)std::min<int64_t>(ceil_div64(batch, SHORT_THREADS >> s.lanes_log2),
+                                         std::max<int64_t>(1, SHORT_GROUPS / s.blocks));
+  return s;
+}
+template <typename S, int VW, int N, bool BWD>
+void launch_short_steps(hipStream_t st, const GatedArgs& a, const ShortPlan& s, int batch) {
+  const dim3 grid(s.blocks, s.groups), block(SHORT_THREADS);
+  if constexpr (BWD) hipLaunchKernelGGL((gated_short_bwd_kernel<S, VW, N>), grid, block, 0, st, a, batch, s.lanes_log2);
+  else hipLaunchKernelGGL((gated_short_fwd_kernel<S, VW, N>), grid, block, 0, st, a, batch, s.lanes_log2);
+}
+template <typename S, int VW, bool BWD>
+void launch_short_width(hipStream_t st, const GatedArgs& a, const ShortPlan& s, int batch) {
+  if constexpr (VW != 2) {
+    if (a.steps == 1) return launch_short_steps<S, VW, 1, BWD>(st, a, s, batch);
+    if (a.steps == 2) return launch_short_steps<S, VW, 2, BWD>(st, a, s, batch);
+  }
+  if constexpr (VW != 4) {
+    if (a.steps <= 4) return launch_short_steps<S, VW, 4, BWD>(st, a, s, batch);
+  }
+  if constexpr (VW == 1 || (VW == 2 && !BWD)) launch_short_steps<S, VW, SHORT, BWD>(st, a, s, batch);
+}
+template <typename S, bool BWD> void launch_short(hipStream_t st, const GatedArgs& a, int batch) {
+  const ShortPlan s = short_plan_of(BWD, batch, a.steps, a.F);
+  if (s.vw == 4) launch_short_width<S, 4, BWD>(st, a, s, batch);
+  else if (s.vw == 2) launch_short_width<S, 2, BWD>(st, a, s, batch);
+  else launch_short_width<S, 1, BWD>(st, a, s, batch);
+}
+
 constexpr int RATE_ROWS = 512;   // of partial sums that a workgroup adds
+
+// Rows of a rate's partial sums.
+int64_t rate_rows(const Plan& s, int batch, int steps, int F) {
+  return steps <= SHORT ? (int64_t)short_plan_of(true, batch, steps, F).groups : (int64_t)batch * s.segments;
+}
 
 size_t maps_floats(const Plan& s, int batch, int F) { return s.segments > 1 ? 2 * (size_t)batch * s.segments * F : 0; }
 
@@ -962,6 +1148,11 @@ PPO_EXPORT int ppo_gated_scan_fwd(void* stream, int dtype, const void* x, const 
   a.save_log2 = save_log2_of(plan_of(dtype, true, batch, steps, features));
   a.saved = (int)ceil_div64(steps, 1ll << a.save_log2);
   const Plan s = plan_of(dtype, false, batch, steps, features);
+  if (steps <= SHORT) {
+    if (dtype == GATE_F32) launch_short<float, false>(as_stream(stream), a, batch);
+    else launch_short<uint16_t, false>(as_stream(stream), a, batch);
+    return check_launch(what);
+  }
   if (dtype == GATE_F32) launch<float, false>(as_stream(stream), a, s, batch);
   else launch<uint16_t, false>(as_stream(stream), a, s, batch);
   return check_launch(what);
@@ -970,7 +1161,7 @@ PPO_EXPORT int ppo_gated_scan_fwd(void* stream, int dtype, const void* x, const 
 PPO_EXPORT size_t ppo_gated_scan_bwd_workspace(int dtype, int batch, int steps, int features) {
   if (batch <= 0 || steps <= 0 || features <= 0) return 0;
   const Plan s = plan_of(dtype, true, batch, steps, features);
-  const int64_t rows = (int64_t)batch * s.segments;
+  const int64_t rows = rate_rows(s, batch, steps, features);
   const int64_t sums = rows + (rows > RATE_ROWS ? ceil_div64(rows, RATE_ROWS) : 0);
   return sizeof(float) * (maps_floats(s, batch, features) + (size_t)sums * features);
 }
@@ -1016,10 +1207,12 @@ PPO_EXPORT int ppo_gated_scan_bwd(void* stream, int dtype, const void* x, const 
   a.F = features;
   a.save_log2 = save_log2_of(s);
   a.saved = (int)ceil_div64(steps, 1ll << a.save_log2);
-  if (dtype == GATE_F32) launch<float, true>(as_stream(stream), a, s, batch);
+  if (steps <= SHORT && dtype == GATE_F32) launch_short<float, true>(as_stream(stream), a, batch);
+  else if (steps <= SHORT) launch_short<uint16_t, true>(as_stream(stream), a, batch);
+  else if (dtype == GATE_F32) launch<float, true>(as_stream(stream), a, s, batch);
   else launch<uint16_t, true>(as_stream(stream), a, s, batch);
   if (drate) {
-    const int64_t rows = (int64_t)batch * s.segments;
+    const int64_t rows = rate_rows(s, batch, steps, features);
     const unsigned columns = (unsigned)ceil_div(features, 64);
     if (rows > RATE_ROWS) {
       const int64_t some = ceil_div64(rows, RATE_ROWS);

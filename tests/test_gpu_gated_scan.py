@@ -128,6 +128,22 @@ def test_sequences_match_the_recurrence(case, dtype):
             assert all(torch.equal(a, b) for a, b in zip(gated_scan(*ops.values()), outs))
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("F", [1, 2, 3, 4, 5, 17, 130, 1027])
+def test_short_sequences(T, F):
+    """Many of few steps: every form of them, with resets and sequences of no steps, and without a carry."""
+    for B, dtype, packed, ragged, carry in ((70, F32, True, True, True), (301, BF16, False, False, False)):
+        ops = problem(F * 8 + T, B, T, F, dtype, packed, 0.3, ragged, carry)
+        cots = cotangents(F, B, T, F, dtype)
+        outs, grads = run(ops, cots)
+        check(ops, cots, outs, grads)
+        again = run(ops, cots)
+        assert all(torch.equal(a, b) for a, b in zip((*outs, *grads.values()), (*again[0], *again[1].values())))
+        with torch.no_grad():
+            alone = gated_scan(*(ops[n] for n in NAMES), ops["done"], ops["lengths"])
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+
+
 @pytest.mark.parametrize("case", [(1, 9000, 16), (1, 2100, 520), (3, 3000, 40), (2, 8191, 3), (1, 4200, 100)])
 def test_long_sequences_in_segments(case):
     B, T, F = case
