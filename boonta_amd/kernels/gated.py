@@ -121,7 +121,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     keeps the state, and the gradient through its input weight, which has no
     bound there, is taken as 0).  done: bool [batch, steps], the step starts an
     episode: nothing from before it passes, an infinity or NaN neither.  lengths:
-    int32 [batch], steps of each sequence: what follows is not read, and its
+    int32 [batch], steps of each sequence: what follows counts nowhere, and its
     outputs and gradients are zeros.  What the recurrence gives an infinity may
     come out as NaN."""
     shape = _check("gated_scan", x, input_gate, decay_gate, rate, carry, done, 3)

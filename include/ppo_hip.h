@@ -367,7 +367,7 @@ int ppo_ssm_scan_bwd(void* stream, int dtype, const void* a, const void* h, cons
  * Per feature f, with r = sigmoid(decay_gate), i = sigmoid(input_gate),
  * a = exp(-rate[f] r), w = sqrt(1 - a^2):
  *   h_t = a_t (done_t ? 0 : h_{t-1}) + w_t i_t x_t,  h_{-1} = carry
- * for t < lengths[b]; later rows are not read, and theirs of the outputs and
+ * for t < lengths[b]; later rows count nowhere, and theirs of the outputs and
  * gradients are zeros.  dtype 0 = float32, 1 = bf16 storage of x, the gates, out
  * and their gradients; states are float32.
  *   x, input_gate, decay_gate [batch, steps, features]: columns side by side,

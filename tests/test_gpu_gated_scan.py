@@ -301,7 +301,7 @@ def test_the_same_twice():
     check(ops, cots, *a)
 
 
-@pytest.mark.parametrize("size", [(2, 50, 32), (1, 3000, 24)])
+@pytest.mark.parametrize("size", [(2, 50, 32), (1, 3000, 24), (400, 3, 24), (5000, 8, 130)])
 def test_a_captured_pass_replays(size):
     sets = [problem(10 + k, *size, BF16, done=0.05) for k in range(3)]
     cots = cotangents(1, *size, BF16)
