@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
       }
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
-      A[k] = 1.f;
+      A[k] = RA[k] = 1.f;
       B[k] = RB[k] = 0.f;
       h[k] = entering[k];
     }
@@ -653,10 +653,14 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
           A[k] = decay_of(e.a, A[k]);
         }
       }
+      // (the cotangents' map in its own order: a NaN decay behind a reset, multiplied to it, is no reset)
 #pragma unroll
       for (int i = N - 1; i >= 0; --i)
 #pragma unroll
-        for (int k = 0; k < VW; ++k) RB[k] = is_reset(q[i][k].a) ? 0.f : q[i][k].a * (q[i][k].g + RB[k]);
+        for (int k = 0; k < VW; ++k) {
+          RB[k] = is_reset(q[i][k].a) ? 0.f : q[i][k].a * (q[i][k].g + RB[k]);
+          RA[k] = decay_of(q[i][k].a, RA[k]);
+        }
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -666,9 +670,9 @@ __global__ void __launch_bounds__(64 * MAX_WAVES) gated_bwd_kernel(GatedArgs p) 
           A[k] *= q[i][k].a;
           RB[k] = q[N - 1 - i][k].a * (q[N - 1 - i][k].g + RB[k]);
         }
-    }
 #pragma unroll
-    for (int k = 0; k < VW; ++k) RA[k] = A[k];
+      for (int k = 0; k < VW; ++k) RA[k] = A[k];
+    }
     if (t0 > begin) fetch(t0 - at.tile);
     const int mine_at = at.wave * LF * VW;
     compose_slots<VW, LF, false>(A, B, at.lane, fwd_a[set] + mine_at, fwd_b[set] + mine_at);
