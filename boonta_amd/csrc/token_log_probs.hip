@@ -164,6 +164,12 @@ __device__ __forceinline__ Sums lanes_joined(Sums a, int log2, float c) {
   return a;
 }
 
+// log p of a logit, l = log2 S: from halves, whose difference every pair of float32 numbers has (-3e38 less 3e38, or
+// the type's lowest value as a mask), times 1 / T at once.
+__device__ __forceinline__ float log_p(const TokenArgs& p, float x, float m, float l) {
+  return __fmaf_rn(0.5f * x - 0.5f * m, 2.f * p.inverse_t, -LN2 * l);
+}
+
 // The row's token: its logit where it is one that is allowed.
 struct Given {
   bool token;
@@ -184,7 +190,7 @@ __device__ __forceinline__ void finish_row(const TokenArgs& p, uint32_t row, con
   const bool none = a.s == 0.f;
   const float l = none ? INF : __builtin_amdgcn_logf(a.s);   // log2
   p.entropy[row] = none ? 0.f : LN2 * (l - a.t * __builtin_amdgcn_rcpf(a.s));   // (S from 1 to 2^24)
-  p.log_prob[row] = !g.token ? 0.f : g.logit == -INF ? -INF : LN2 * (exponent(g.logit, a.m, p.c) - l);
+  p.log_prob[row] = !g.token ? 0.f : g.logit == -INF ? -INF : log_p(p, g.logit, a.m, l);
   if (p.stats) {
     p.stats[2 * (int64_t)row] = none ? 0.f : a.m;
     p.stats[2 * (int64_t)row + 1] = l;
@@ -206,7 +212,7 @@ __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)k
 
 __device__ __forceinline__ void write_top(const TokenArgs& p, uint32_t row, int place, float x, int token, float m, float l) {
   const int64_t at = (int64_t)row * p.top + place;
-  p.top_log_probs[at] = token < 0 ? -INF : LN2 * (exponent(x, m, p.c) - l);
+  p.top_log_probs[at] = token < 0 ? -INF : log_p(p, x, m, l);
   if (p.wide_tokens) static_cast<int64_t*>(p.top_tokens)[at] = token;
   else static_cast<int32_t*>(p.top_tokens)[at] = token;
 }
@@ -574,13 +580,17 @@ struct RowGradient {
   float m, l, hl, gh, g;
   int token;   // -1: none
 };
-__device__ __forceinline__ RowGradient row_gradient(const TokenArgs& p, uint32_t row) {
+template <typename T> __device__ __forceinline__ RowGradient row_gradient(const TokenArgs& p, uint32_t row) {
   RowGradient r;
   r.m = p.stats[2 * (int64_t)row];
   r.l = p.stats[2 * (int64_t)row + 1];
   const int64_t token = token_of(p, row);
-  // a token that is none, or not allowed, passes nothing
-  const bool given = token >= 0 && token < p.V && !(p.log_prob[row] == -INF);
+  // a token that is none, or not allowed, passes nothing (its log probability is -inf, which an allowed one's may be)
+  bool given = token >= 0 && token < p.V;
+  if (given && p.log_prob[row] == -INF) {
+    const T* x = static_cast<const T*>(p.logits) + row_offset(row, p.steps, p.logits_s);
+    given = given_of(p, row, x, p.mask ? p.mask + row_offset(row, p.steps, p.mask_s) : nullptr).logit > -INF;
+  }
   r.token = given ? (int)token : -1;
   r.g = given && p.dlog_prob ? p.dlog_prob[row_offset(row, p.steps, p.dlog_prob_s)] * p.inverse_t : 0.f;
   const float h = p.dentropy ? p.dentropy[row_offset(row, p.steps, p.dentropy_s)] * p.inverse_t : 0.f;
@@ -617,7 +627,7 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) toke
   __shared__ RowGradient scalars[MAX_ROW_BLOCK];
   const uint32_t units = p.units.d, row0 = blockIdx.x * p.row_block;
   const uint32_t rows = min((uint32_t)p.row_block, p.rows - row0), count = rows * units;
-  if (threadIdx.x < rows) scalars[threadIdx.x] = row_gradient(p, row0 + threadIdx.x);
+  if (threadIdx.x < rows) scalars[threadIdx.x] = row_gradient<T>(p, row0 + threadIdx.x);
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
     const uint32_t q = quotient(i, p.units), row = row0 + q;
@@ -637,7 +647,7 @@ template <typename T, bool MASK> __global__ void __launch_bounds__(THREADS) toke
   T* out = static_cast<T*>(p.dlogits) + (int64_t)row * p.V;
   const int skew = skew_of(out), first = blockIdx.y * p.segment_units;   // (as the logits where those are contiguous)
   const int end = min((p.V + skew + UNIT - 1) / UNIT, first + p.segment_units), whole = min(end, (p.V + skew) / UNIT);
-  const RowGradient r = row_gradient(p, row);
+  const RowGradient r = row_gradient<T>(p, row);
   auto one = [&](int u) __attribute__((always_inline)) {
     const int col = u * UNIT - skew;
     float v[UNIT];

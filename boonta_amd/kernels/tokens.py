@@ -95,9 +95,10 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tens
                     temperature: float = 1.0, top: int = 0) -> TokenLogProbs:
     """Of the categorical distributions softmax(logits / temperature) over the last axis:
 
-    - log_prob: of ``tokens``, -inf where the token is not allowed; a token
-      outside the vocabulary (-1, say) is none: its log_prob is 0 and passes no
-      gradient;
+    - log_prob: of ``tokens``, -inf where the token is not allowed (or where the
+      value of an allowed one is below float32's range: its gradient is that of
+      any other); a token outside the vocabulary (-1, say) is none: its log_prob
+      is 0 and passes no gradient;
     - entropy (0 where nothing is allowed);
     - top_log_probs, top_tokens: the ``top`` most probable tokens in falling
       order, equal ones by index, without gradients; past the allowed ones -inf
