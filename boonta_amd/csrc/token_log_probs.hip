@@ -579,7 +579,9 @@ template <typename T> __global__ void __launch_bounds__(THREADS) token_join_kern
 struct RowGradient {
   float m, l, hl, gh, g;
   int token;   // -1: none
+  bool bad;    // a logit or cotangent that is not finite: NaN, but where the mask allows nothing
 };
+constexpr float LEAST = -200.f;   // exponents below: 2^LEAST = 0
 template <typename T> __device__ __forceinline__ RowGradient row_gradient(const TokenArgs& p, uint32_t row) {
   RowGradient r;
   r.m = p.stats[2 * (int64_t)row];
@@ -596,17 +598,17 @@ template <typename T> __device__ __forceinline__ RowGradient row_gradient(const 
   const float h = p.dentropy ? p.dentropy[row_offset(row, p.steps, p.dentropy_s)] * p.inverse_t : 0.f;
   r.hl = h * LN2;
   r.gh = __fmaf_rn(h, p.entropy[row], r.g);
+  r.bad = r.l != r.l || !(__fmaf_rn(fabsf(r.hl), -LEAST, fabsf(r.gh)) < INF);
   return r;
 }
 __device__ __forceinline__ void unit_gradient(const RowGradient& r, float c, int col, float (&v)[UNIT]) {
-  const bool bad = r.l != r.l;   // a row with an infinity or NaN: NaN, but where the mask allows nothing
   float d[UNIT];
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) {
     const float w = __fmaf_rn(v[j] - r.m, c, -r.l), e = __builtin_amdgcn_exp2f(w);
-    d[j] = -e * __fmaf_rn(r.hl, fmaxf(w, -1e4f), r.gh);
+    d[j] = -e * __fmaf_rn(r.hl, fmaxf(w, LEAST), r.gh);
   }
-  if (bad) {
+  if (r.bad) {
     asm volatile("");   // (seldom: not selected from beside the others)
 #pragma unroll
     for (int j = 0; j < UNIT; ++j) d[j] = v[j] == -INF ? 0.f : d[j];
