@@ -42,11 +42,16 @@ constexpr int THREADS = 256;               // of a workgroup of narrow rows, and
 constexpr int MAX_THREADS = 1024;
 constexpr int NARROW = 64 * UNIT;          // widest row of one wave's lanes
 constexpr int MAX_WIDTH = MAX_THREADS * UNIT;
-// Waves of a launch, a row or part of one each at a time.  The backward's, 67M
-// elements, both passes: 8 a CU for 12, 2048 bf16 columns 357 us for 369, 640 float32
-// 833 for 899, but 640 bf16 404 for 385; 16 and 6 are behind one or the other.
-constexpr int FWD_WAVES = 256 * 24;
-int bwd_waves(int dtype, int D) { return 256 * (dtype == NORM_BF16 && D <= 768 ? 12 : 8); }
+// Workgroups a CU, of `waves` waves each: whole numbers, or some CUs hold one more than others and the launch takes as
+// long as they do (67M elements, both passes, for as many waves spread unevenly: rows of 3000 bf16 columns 375 us for 456,
+// 8192 381 for 469, 8192 float32 781 for 1079; forward alone, 134M, 5632 bf16 275 for 331, 8192 float32 511 for 613).
+constexpr int CUS = 256;
+// Forward at most 24 waves (rows of 2304 bf16 columns, five waves: 286 us, with 25 309).
+int fwd_groups(int waves) { return std::max(1, 24 / waves); }
+// Backward at least 8, and 12 for narrow bf16 rows: those whose last lanes are idle have too little on its way with 8
+// (both passes, 67M elements: rows of 40 385 us for 428, 136 429 for 489, 300 422 for 469, 640 386 for 405, 768 370 for 371;
+// but full ones lose, of 16 to 512 columns 1 to 3 %, and wider ones, 700 413 for 403, 800 392 for 374, 1024 368 for 353).
+int bwd_groups(int dtype, int D, int waves) { return ceil_div(dtype == NORM_BF16 && D <= 768 ? 12 : 8, waves); }
 
 enum Gate { GATE_NONE, GATE_PLAIN, GATE_SIGMOID };
 
@@ -363,12 +368,13 @@ struct Shape {
   bool wide;
   unsigned threads, blocks;
 };
-Shape shape_of(int64_t rows, int D, int waves) {
+Shape shape_of(int64_t rows, int D, int dtype, bool backward) {
   Shape s;
   s.wide = D > NARROW;
   s.threads = s.wide ? (unsigned)(64 * ceil_div(D, NARROW)) : THREADS;
   const int64_t at_once = s.wide ? 1 : THREADS >> lanes_log2_of(D);
-  s.blocks = (unsigned)std::min<int64_t>(waves * 64 / s.threads, ceil_div64(rows, at_once));
+  const int waves = (int)s.threads / 64, groups = backward ? bwd_groups(dtype, D, waves) : fwd_groups(waves);
+  s.blocks = (unsigned)std::min<int64_t>(CUS * groups, ceil_div64(rows, at_once));
   return s;
 }
 
@@ -461,13 +467,13 @@ PPO_EXPORT int ppo_residual_norm_fwd(void* stream, int dtype, int stream_dtype, 
   a.stream = stream_out;
   a.normed = normed;
   a.stats = stats;
-  launch_typed(as_stream(stream), a, shape_of(a.rows, width, FWD_WAVES), gate_sigmoid, false, dtype, stream_dtype);
+  launch_typed(as_stream(stream), a, shape_of(a.rows, width, dtype, false), gate_sigmoid, false, dtype, stream_dtype);
   return check_launch(what);
 }
 
 PPO_EXPORT size_t ppo_residual_norm_bwd_workspace(int dtype, int batch, int steps, int width) {
   if (batch <= 0 || steps <= 0 || width <= 0 || width > MAX_WIDTH) return 0;
-  return sizeof(float) * 2 * (size_t)width * shape_of((int64_t)batch * steps, width, bwd_waves(dtype, width)).blocks;
+  return sizeof(float) * 2 * (size_t)width * shape_of((int64_t)batch * steps, width, dtype, true).blocks;
 }
 
 PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void* block,
@@ -499,7 +505,7 @@ PPO_EXPORT int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, 
     a.dgate = gate ? dgate : nullptr;
     a.dresidual = dresidual;
     a.partials = scales ? static_cast<float*>(workspace) : nullptr;
-    const Shape s = shape_of(a.rows, width, bwd_waves(dtype, width));
+    const Shape s = shape_of(a.rows, width, dtype, true);
     blocks = s.blocks;
     launch_typed(as_stream(stream), a, s, gate_sigmoid, true, dtype, stream_dtype);
   }
