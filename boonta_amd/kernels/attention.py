@@ -52,8 +52,11 @@ def _no_tangents(name, *tensors):
 
 
 def _on_device(name, *tensors):
-    """The index of the device that all of them (None aside) are on."""
+    """The index of the device that all of them (None aside) are on; the first two have the operator's sizes."""
     _no_tangents(name, *tensors)
+    for x in tensors[:2]:
+        if x.numel() > 0x7fffffff and max(x.shape) > 0x7fffffff:   # (a C int keeps the low 32 bits)
+            raise ValueError(f"{name} takes sizes up to 2^31 - 1, not {tuple(x.shape)}")
     index = tensors[0].get_device()   # (-1: the host)
     for x in tensors:
         if x is not None and x.get_device() != index:
