@@ -143,13 +143,17 @@ __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
   const Sums x = rescaled(a, m, c), y = rescaled(b, m, c);
   return Sums{m, x.s + y.s, x.t + y.t};
 }
+// The unit's own sums first: a thread's are of an eighth of the terms, which a far larger one would each round.
 __device__ __forceinline__ void add_values(Sums& a, const float (&v)[UNIT], float c) {   // none above a.m
+  float s = 0.f, t = 0.f;
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) {
     const float w = exponent(v[j], a.m, c), e = __builtin_amdgcn_exp2f(w);
-    a.s += e;
-    a.t = __fmaf_rn(e, fmaxf(w, FAR), a.t);
+    s += e;
+    t = __fmaf_rn(e, fmaxf(w, FAR), t);
   }
+  a.s += s;
+  a.t += t;
 }
 __device__ __forceinline__ void add_unit(Sums& a, const float (&v)[UNIT], float most, float c) {
   a = rescaled(a, fmaxf(a.m, most), c);
