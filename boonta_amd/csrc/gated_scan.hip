@@ -29,11 +29,11 @@
 // enters, an infinity or NaN neither, passes.
 //
 // What bounds it: an element takes some 26 vector and 6 transcendental instructions
-// forward, about as long as its bytes.  65536 steps of 2048 bf16 features: the maps
-// 182 to 195 us (4.1 to 4.4 TB/s), the outputs 219 to 233 (4.6 to 4.9 TB/s; a copy
-// reaches 4.9).  256 x 64 steps of 256 float32 features 19 us, backward 29 (3.6, 4.1
-// TB/s); 24 x 4093 of 640 bf16, ragged, 128 and 288 us (3.3, 2.7 TB/s: the longest
-// sequence's workgroups, one a CU).
+// forward, about as long as its bytes.  As traced, a launch at a time: 65536 steps of
+// 2048 bf16 features, the maps 188 us (4.2 TB/s), the outputs 223 (4.8 TB/s; a copy
+// reaches 4.9; untraced both take 388 us together); 256 x 64 steps of 256 float32 features
+// 19 us, backward 29 (3.5, 4.0 TB/s); 24 x 4093 of 640 bf16, ragged, 127 and 289 us (3.3, 2.7
+// TB/s: the longest sequence's workgroups, one a CU).
 #include "row_io.h"
 
 #include <algorithm>

@@ -24,9 +24,9 @@
 // operands are on their way while one is formed.  Sums are float32, the
 // lanes' by butterflies, the waves' in order.
 //
-// What bounds it is HBM: 65536 rows of 2048 bf16 columns with a float32 stream 323 us
-// (5.0 TB/s); 128000 of 640 bf16 with gates 175 us, backward 277 (4.7, 4.8 TB/s) and
-// 7 for the scales; 15984 of 1333 float32 100 and 166 us (4.4, 4.2 TB/s).  64 rows of
+// What bounds it is HBM: 65536 rows of 2048 bf16 columns with a float32 stream 322 us
+// (5.0 TB/s); 128000 of 640 bf16 with gates 174 us, backward 277 (4.7 TB/s both) and
+// 7 for the scales; 15984 of 1333 float32 101 and 153 us (4.2, 4.5 TB/s).  64 rows of
 // 1000 take 4.5 us: a launch, and a row's two sums one after the other.
 #include "row_io.h"
 
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(MOST) residual_norm_bwd_kernel(ResidualArgs p,
   }
   const float over_d = 1.f / (float)p.D;
   int slot = 0;
-  // (16 waves leave no registers for a next row: 8192 bf16 columns 396 us for 512)
+  // (9 to 16 waves leave no registers for a next row: 67M elements in rows of 8192 bf16 columns, both passes, 358 us for 432)
   constexpr bool AHEAD = MOST <= 512;
   Loaded<T, R> next;
   if constexpr (AHEAD) load<GATE, true>(p, min(at.row, p.rows - 1), at, next);

@@ -16,10 +16,10 @@
 // all of any other thread.  So only their units are read again, those worse than the
 // last of them left out, and ranked.
 //
-// What bounds it: HBM where rows are wide (8192 rows of 50001 bf16 logits 152 us, 5.4
-// TB/s, backward 343, 4.9 TB/s), the vector work where they are short, a dozen
+// What bounds it: HBM where rows are wide (8192 rows of 50001 bf16 logits 151 us, 5.4
+// TB/s, backward 342, 4.8 TB/s), the vector work where they are short, a dozen
 // instructions a column of a lane, there or not, and a hundred a row (262144 rows of
-// 43 float32 logits with a mask 16 us, 4.0 TB/s, backward 21, 5.4 TB/s).  32 rows of
+// 43 float32 logits with a mask 16 us, 3.8 TB/s, backward 21, 5.1 TB/s).  32 rows of
 // 131072 with 8 alternatives take 12 us in 16 parts and 4 to join them, half of it the
 // search.
 #include "row_io.h"

@@ -107,9 +107,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tens
     logits [batch, steps, vocab] or [batch, vocab] in any strides, float32 or
     bfloat16; tokens int32 or int64 of the leading shape; mask: bool, broadcast to
     the logits, False (as a logit of -inf) where a token is not allowed: what is
-    there, NaN among it, counts nowhere, and gets no gradient.  A token that is
-    not allowed passes no gradient.  An infinity or NaN among the allowed makes
-    its row's results NaN.  Results are float32 of the leading shape, top_tokens
+    there, NaN among it, counts nowhere, and gets no gradient, whatever the
+    cotangents.  A token that is not allowed passes no gradient.  +inf or NaN
+    among the allowed makes its row's results NaN.  Results are float32 of the leading shape, top_tokens
     of the tokens' type.  Vocabularies up to 2^24, ``top`` up to 32 and the vocabulary,
     2^24 - 1 rows."""
     global _limits

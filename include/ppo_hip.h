@@ -508,7 +508,8 @@ int ppo_residual_norm_bwd(void* stream, int dtype, int stream_dtype, const void*
  * of rows of logits (boonta/networks/distributions.py:8-38 for any vocabulary,
  * with a mask).  Per row of `vocab` logits over `temperature`, -inf where the
  * mask does not allow: log_prob float [batch x steps] of the row's token (-inf
- * where it is not allowed; a token outside 0 .. vocab - 1 is none: 0), entropy
+ * where it is not allowed or its value is below float's range; a token outside
+ * 0 .. vocab - 1 is none: 0; NaN in a row of an allowed NaN or +inf), entropy
  * float [batch x steps] (0 where nothing is allowed), top_log_probs float and
  * top_tokens [batch x steps, top] in falling order, equal ones by index (-inf
  * and -1 past the allowed ones; a NaN is none).  dtype 0 = float32, 1 = bf16
@@ -527,7 +528,8 @@ int ppo_token_log_probs_fwd(void* stream, int dtype, const void* logits, const v
                             size_t workspace_bytes, int batch, int steps, int vocab);
 /* dlogits contiguous, of the logits' type, from the cotangents of log_prob and
  * entropy (either NULL: zeros; strides: 2 more for each).  A token that is none
- * or not allowed passes none, and logits that are not allowed get 0. */
+ * or not allowed passes none, and logits that are not allowed get 0, whatever
+ * the cotangents. */
 int ppo_token_log_probs_bwd(void* stream, int dtype, const void* logits, const void* tokens, int wide_tokens,
                             const uint8_t* mask, const int64_t* strides, float temperature, const float* log_prob,
                             const float* entropy, const float* stats, const float* dlog_prob, const float* dentropy,
