@@ -621,7 +621,7 @@ __device__ __forceinline__ void unit_gradient(const RowGradient& r, float c, int
   if (at >= 0 && at < UNIT) {
     asm volatile("");
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) d[j] += j == at ? r.g : 0.f;
+    for (int j = 0; j < UNIT; ++j) d[j] = j == at ? d[j] + r.g : d[j];   // (-0 stays: a unit that overlaps this one writes it)
   }
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) v[j] = d[j];
