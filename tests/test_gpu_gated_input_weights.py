@@ -22,8 +22,8 @@ N = 2.0 ** -24
 
 
 def rates():
-    """Of 2 q where the decay gate is 8 (r = 0.99966): 4096 about 1/8, and from 1e-6 to 30."""
-    about = torch.linspace(0.0620, 0.0631, 3072)
+    """q where the decay gate is 8 (r = 0.99966): 3000 about 1/16, and from 1e-6 to 30."""
+    about = torch.linspace(0.0620, 0.0631, 3000)
     wide = torch.logspace(-6, math.log10(30.0), 1024)
     return torch.cat([about, wide])
 
